@@ -575,6 +575,146 @@ int praghip_frame_encode(const praghip_frame_header *header, uint8_t *out);
 int praghip_frame_decode(const uint8_t *in, praghip_frame_header *header);
 int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
 
+/* ------------------------------------------------- serving: paged attention */
+/* No counterpart in the reference, whose attention is a two-party protocol: these
+ * serve a model in the clear beside it.  All pointers are device memory, all calls
+ * asynchronous on `stream`; 16-bit data of PRAGHIP_BF16 or PRAGHIP_F16. */
+#define PRAGHIP_BF16 0
+#define PRAGHIP_F16 1
+
+/* One layer's keys and values in pages: position p of sequence s is token p %
+ * page_size of page tables[s][p / page_size].  k and v are [pages][kv_heads]
+ * [page_size][head_dim] by strides in elements {page, head, token}; a row of
+ * head_dim values is contiguous.  An entry of `tables` outside 0 .. pages - 1 is no
+ * page: its positions are seen by no query.  Memory that no position below a
+ * sequence's length names is never used, whatever it holds.
+ *
+ * page_size is a power of two of 16 .. 32768, head_dim a multiple of 8 up to 256
+ * (E_ATTENTION_SHAPE); base addresses are 16-byte aligned and strides multiples of 8
+ * (E_ATTENTION_ALIGNMENT).  A length outside 0 .. table_width * page_size is taken
+ * as the nearer end. */
+typedef struct praghip_cache {
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  size_t pages, kv_heads, page_size, head_dim;
+  int type;
+  const int32_t *tables; /* [seqs][table_width] */
+  int64_t table_stride;
+  size_t table_width;
+  const int32_t *lengths; /* [seqs] */
+  size_t seqs;
+} praghip_cache;
+
+/* Attention of the newest token of every sequence, at position lengths[s] - 1, whose
+ * key and value the cache holds already: out[s][h] = sum_j p_j v_j, p = softmax over
+ * the visible keys of scale q[s][h].k_j, with head h reading key/value head h /
+ * (heads / kv_heads).  With a window > 0 the query at position p sees key j where j >
+ * p - window or j < sinks; window 0 is no window.  lse (or NULL) [seqs][heads] gets
+ * the logarithm of the softmax's sum.  A sequence that sees nothing gets zeros, and
+ * -infinity.  q and out are [seqs][heads][head_dim] by strides {sequence, head}, 16-byte
+ * aligned, strides multiples of 8.  max_length is a bound of the lengths, used for the
+ * launch's size alone (0: the tables' width); results hold without it, and a given size
+ * of it gives the same bits each time.  work: 16-byte aligned, at least
+ * praghip_paged_decode_workspace(...) bytes (E_ATTENTION_WORKSPACE), not used by another
+ * call until this one is done. */
+size_t praghip_paged_decode_workspace(const praghip_cache *cache, size_t heads, size_t max_length);
+int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,
+                         void *out, const int64_t *out_strides, float *lse, float scale, size_t window, size_t sinks,
+                         size_t max_length, void *work, size_t work_bytes, void *stream);
+
+/* The same for many tokens per sequence: rows starts[s] .. starts[s + 1] - 1 of q
+ * [tokens][heads][head_dim] (strides {token, head}) are the newest tokens of sequence
+ * s, the last of them at position lengths[s] - 1; the cache holds their keys and values
+ * already.  Causal, with window and sinks as above; a row whose position is below 0 sees
+ * nothing.  max_rows is at least the longest of these stretches; rows beyond it are not
+ * computed.  lse: [tokens][heads]. */
+size_t praghip_paged_prompt_workspace(const praghip_cache *cache, size_t heads, size_t max_rows, size_t window,
+                                      size_t sinks, size_t max_length);
+int praghip_paged_prompt(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,
+                         const int32_t *starts, size_t tokens, size_t max_rows, void *out, const int64_t *out_strides,
+                         float *lse, float scale, size_t window, size_t sinks, size_t max_length, void *work,
+                         size_t work_bytes, void *stream);
+
+/* ----------------------------------------------------- serving: cache pages */
+/* Who holds which page, on the device: tables (-1: no page), lengths, and refs, the
+ * number of table entries that name each page.  A page with refs 0 is free; new pages
+ * are the free ones of the lowest index, given in the order of the call's list.  A list
+ * names rows of the tables, each once (at most 8192 names, 131072 rows).
+ *
+ * The calls check their lists on the device.  One that is refused changes nothing and,
+ * where status (device, or NULL) is 0, sets it to a PRAGHIP_PAGES_* code; a later call
+ * does not clear it. */
+#define PRAGHIP_PAGES_SEQUENCE 1  /* a name out of range or twice; a child that is not empty or is a parent */
+#define PRAGHIP_PAGES_CAPACITY 2  /* a negative count, or more tokens than a row of the tables holds */
+#define PRAGHIP_PAGES_EXHAUSTED 3 /* fewer free pages than the call needs */
+typedef struct praghip_page_table {
+  int32_t *tables; /* [seqs][width] */
+  int64_t stride;
+  size_t width, seqs;
+  int32_t *lengths; /* [seqs] */
+  int32_t *refs;    /* [pages] */
+  size_t pages, page_size;
+  int32_t *status;
+} praghip_page_table;
+/* Planes (layers, keys and values) of pages of page_bytes (a multiple of 16), page i of
+ * plane p at base + p plane_bytes + i page_bytes. */
+typedef struct praghip_page_pool {
+  void *base;
+  int64_t plane_bytes;
+  size_t page_bytes, planes, pages;
+} praghip_page_pool;
+
+/* counts[i] more tokens for sequence list[i]: its new pages and its length. */
+int praghip_page_reserve(int device, const praghip_page_table *t, const int32_t *list, const int32_t *counts, size_t n,
+                         void *stream);
+/* Empties sequences: their pages lose a reference, their rows become -1, lengths 0. */
+int praghip_page_free(int device, const praghip_page_table *t, const int32_t *list, size_t n, void *stream);
+/* Gives back the pages that no token after the sequence's last one can see through
+ * this window (> 0) and these sinks. */
+int praghip_page_trim(int device, const praghip_page_table *t, const int32_t *list, size_t n, size_t window,
+                      size_t sinks, void *stream);
+/* children[i], an empty sequence, becomes a copy of parents[i]: full pages are shared, a
+ * last page that is not full is copied (in every plane) to a new page.  A parent may
+ * have several children. */
+size_t praghip_page_fork_workspace(size_t n);
+int praghip_page_fork(int device, const praghip_page_table *t, const praghip_page_pool *pool, const int32_t *parents,
+                      const int32_t *children, size_t n, void *work, size_t work_bytes, void *stream);
+/* Moves pages so that the held ones are 0 .. count - 1: held pages above move into the
+ * holes below, both in rising order, and the tables follow. */
+size_t praghip_page_compact_workspace(size_t pages);
+int praghip_page_compact(int device, const praghip_page_table *t, const praghip_page_pool *pool, void *work,
+                         size_t work_bytes, void *stream);
+/* Page from[i] of every plane over page to[i], for the i whose indexes are pages; no
+ * page is both copied from and copied to, and none copied to twice. */
+int praghip_page_copy(int device, const praghip_page_pool *pool, const int32_t *from, const int32_t *to, size_t n,
+                      void *stream);
+/* Rows starts[s] .. starts[s + 1] - 1 of k and v ([tokens][kv_heads][head_dim], strides
+ * {token, head}) into the cache as the newest tokens of sequence s, the last at position
+ * lengths[s] - 1.  Tokens at a position below 0, beyond the tables or without a page are
+ * dropped. */
+int praghip_page_write(int device, const praghip_cache *cache, const void *k, const int64_t *k_strides, const void *v,
+                       const int64_t *v_strides, const int32_t *starts, size_t tokens, void *stream);
+
+/* ------------------------------------------------- serving: 4-bit products */
+/* y[m][n] = sum_k x[m][k] (w[n][k] - z[n][k / group]) s[n][k / group]: x [m][k], y [m][n]
+ * and scales [n][groups] of `type`, w [n][width] bytes of two 4-bit values each, the lower
+ * bits first (width >= (k + 1) / 2), zeros [n][groups] bytes (NULL: 8 everywhere); groups =
+ * ceil(k / group), group a multiple of 32 (E_W4_SHAPE).  Strides in elements of a row each;
+ * rows at odd addresses are read as they are, more slowly.  k 0 gives zeros.  Sums are 32-bit,
+ * rounded once.  An infinity or NaN in a row of x makes that row of y NaN. */
+typedef struct praghip_w4 {
+  const uint8_t *w;
+  int64_t w_stride;
+  const void *scales;
+  int64_t scale_stride;
+  const uint8_t *zeros;
+  int64_t zero_stride;
+  size_t n, k, width, group;
+  int type;
+} praghip_w4;
+int praghip_matvec_w4(int device, const praghip_w4 *weights, const void *x, int64_t x_stride, size_t m, void *y,
+                      int64_t y_stride, void *stream);
+
 /* ------------------------------------------------------ synthetic inputs */
 /* Seeded counter-based inputs (no counterpart in the reference, whose probes
  * draw from mt19937_64, check_resident.cpp:26): element i of the buffer is

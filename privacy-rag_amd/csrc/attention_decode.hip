@@ -1,0 +1,400 @@
+// Attention of one new token per sequence over a paged key/value cache:
+//   s_j = scale q.k_j over the visible keys j,  m = max s_j,  l = sum 2^(s_j - m),
+//   o = sum 2^(s_j - m) v_j / l,   lse = (m + log2 l) ln 2
+// in one pass over the cache with a running m and l (the scale holds log2 e).
+//
+// The work is read once: 4 dim bytes of K and V per key and key/value head, for
+// 4 dim group operations, so the bytes bound it.  What decides is that every CU
+// always has loads under way, whatever the lengths are: the blocks of 32 keys of
+// all sequences and heads stand in one row, and every wave of the grid takes an
+// equal stretch of it, across heads and sequences.
+//
+// A wave works by itself, with no LDS in its loop:
+// * S^T = K Q^T by 16x16x32 products, 16 keys a tile: a lane's 8 values of a key
+//   are contiguous in the page, so K goes from memory into the operand;
+// * the products' layout leaves a lane with query column lane % 16 and the four
+//   keys 4 (lane / 16) + 0..3 of both tiles.  Taking these eight as the lane's
+//   slots of the second product's sum needs no exchange for P; V is loaded by
+//   whole rows (dim / 16 values of each of the lane's eight keys), and byte
+//   permutes turn 8 keys x dim / 16 values into the operand of O^T = V^T P^T;
+// * 16 query columns are the heads of one key/value head (groups above 16 take
+//   several turns), so m, l and the factor of O are one value per lane.
+// P goes into the product as a sum of two 16-bit values: 8 more of 24 products per
+// block, which the loads hide, and the rounding of P drops out of the error.
+//
+// A stretch that holds a head's blocks from first to last writes the output.
+// Else its m, l and o go to LDS, where the workgroup merges neighbours, and what a
+// workgroup holds in part goes to the workspace, at most two pieces of it; the
+// join kernel adds the pieces in order, so results do not depend on timing.
+#include "attention.hpp"
+
+namespace praghip {
+namespace {
+
+constexpr int kWaves = 4;
+
+template <typename T, int D>
+struct DecodeShape {
+  static constexpr int steps = D / 32;       // of the first product
+  static constexpr int per = D / 16;         // values of a key's row that a lane holds
+  static constexpr int words = per / 2;
+  static constexpr int tiles16 = (per + 7) / 8;
+};
+
+// Blocks of all heads over the grid's waves, one block or more to each of the first
+// `waves`: a workgroup with a later neighbour that has blocks has blocks itself.
+struct Range {
+  int64_t total;
+  unsigned waves;
+  __device__ __forceinline__ Range(int64_t blocks, unsigned grid)
+      : total(blocks), waves(unsigned(min(max(blocks, int64_t(1)), int64_t(grid)))) {}
+  __device__ __forceinline__ int64_t begin(unsigned w) const { return total * min(w, waves) / waves; }
+  // the wave whose stretch holds block u
+  __device__ __forceinline__ unsigned of(int64_t u) const {
+    return unsigned(((u + 1) * waves + total - 1) / total) - 1;
+  }
+};
+
+// pieces of the workspace: [workgroup][2] of rows x (dim + 2)
+__device__ __forceinline__ size_t piece_floats(int rows, int D) { return size_t(rows) * (D + 2); }
+
+template <typename T, int D, bool EXACT>
+__global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a) {
+  using S = DecodeShape<T, D>;
+  extern __shared__ float lds[];
+  __shared__ int64_t before[kWaves * 64 + 1];
+  __shared__ int piece_id[2 * kWaves], piece_flags[2 * kWaves];
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int qtiles = (c.group + 15) >> 4, heads = c.kv_heads * qtiles, rows = min(c.group, 16);
+
+  // key blocks before each stretch of sequences, one stretch per thread
+  const int per = (c.seqs + kWaves * 64 - 1) / (kWaves * 64);
+  {
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int s = int(threadIdx.x) * per + i;
+      if (s < c.seqs) {
+        const int n = length_of(c, s);
+        mine += visible_blocks(c, n - 1, n - 1, 5).count();
+      }
+    }
+    int64_t sum = mine;  // inclusive over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t up = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += up;
+    }
+    before[threadIdx.x + 1] = sum;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    int64_t add = 0;
+    for (int w = 0; w < wave; ++w) add += before[w * 64 + 64];
+    __syncthreads();
+    before[threadIdx.x + 1] = sum + add;
+    if (threadIdx.x < 2 * kWaves) piece_id[threadIdx.x] = -1;
+    __syncthreads();
+    if (blockIdx.x == 0) {  // for the join
+      int64_t at = sum + add - mine;
+      for (int i = 0; i < per; ++i) {
+        const int s = int(threadIdx.x) * per + i;
+        if (s >= c.seqs) break;
+        a.base[s] = at;
+        const int n = length_of(c, s);
+        at += visible_blocks(c, n - 1, n - 1, 5).count();
+        if (s == c.seqs - 1) a.base[c.seqs] = at;
+      }
+    }
+  }
+  const Range range(before[kWaves * 64] * heads, gridDim.x * kWaves);
+  const int64_t wg_begin = range.begin(blockIdx.x * kWaves), wg_end = range.begin(blockIdx.x * kWaves + kWaves);
+  int64_t u = range.begin(blockIdx.x * kWaves + wave);
+  const int64_t u_end = range.begin(blockIdx.x * kWaves + wave + 1), u_begin = u;
+
+  if (u < u_end) {
+    // the sequence of block u: its thread's stretch, then along the stretch
+    int lo = 0, hi = kWaves * 64 - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before[mid] * heads <= u)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    int s = lo * per;
+    int64_t base = before[lo] * heads;
+    while (u < u_end) {
+      const int len = length_of(c, s);
+      const Blocks blocks = visible_blocks(c, len - 1, len - 1, 5);
+      const int nb = blocks.count();
+      if (u >= base + int64_t(nb) * heads) {
+        base += int64_t(nb) * heads;
+        ++s;
+        continue;
+      }
+      const int h = int((u - base) / nb), first = int((u - base) - int64_t(h) * nb);
+      const int count = int(min(int64_t(nb - first), u_end - u));
+      const int kvh = h / qtiles, head0 = kvh * c.group + (h - kvh * qtiles) * 16;
+      const bool has = (h - kvh * qtiles) * 16 + col < c.group;
+
+      u32x4 q[S::steps];
+#pragma unroll
+      for (int i = 0; i < S::steps; ++i) {
+        q[i] = u32x4{0, 0, 0, 0};
+        const int d = 32 * i + 8 * quad;
+        if (has && (EXACT || d < c.dim))
+          q[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + s * a.q_seq + (head0 + col) * a.q_head + d);
+      }
+      f32x4 o[S::per];
+#pragma unroll
+      for (int j = 0; j < S::per; ++j) o[j] = f32x4{0, 0, 0, 0};
+      float m = kNegInf, l = 0;
+
+      const int from = c.window > 0 ? len - c.window : 0;  // first position of the window
+      for (int i = first; i < first + count; ++i) {
+        const int kb = blocks.at(i) << 5;
+        u32x4 kf[2][S::steps];
+        uint32_t vr[8][S::words];
+        bool page_ok[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int at = (kb + 16 * t) >> c.page_shift;
+          int page = at < int((c.capacity) >> c.page_shift) ? c.tables[s * c.table_stride + at] : -1;
+          page_ok[t] = page >= 0 && page < c.pages;
+          page = page_ok[t] ? page : 0;
+          const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
+          const T* kp = static_cast<const T*>(c.k) + page * c.k_page + kvh * c.k_head + (row + col) * c.k_token + 8 * quad;
+#pragma unroll
+          for (int n = 0; n < S::steps; ++n) {
+            kf[t][n] = u32x4{0, 0, 0, 0};
+            if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
+          }
+          const T* vp = static_cast<const T*>(c.v) + page * c.v_page + kvh * c.v_head + (row + 4 * quad) * c.v_token + S::per * col;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int w = 0; w < S::words; ++w) vr[4 * t + e][w] = 0;
+            if (EXACT || S::per * col < c.dim) {
+              if constexpr (S::words == 2) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(vp + e * c.v_token);
+                vr[4 * t + e][0] = x[0];
+                vr[4 * t + e][1] = x[1];
+              } else {
+#pragma unroll
+                for (int w = 0; w < S::words; w += 4) {
+                  if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
+                  const u32x4 x = *reinterpret_cast<const u32x4*>(vp + e * c.v_token + 2 * w);
+#pragma unroll
+                  for (int b = 0; b < 4; ++b) vr[4 * t + e][w + b] = x[b];
+                }
+              }
+            }
+          }
+        }
+        f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int n = 0; n < S::steps; ++n) {
+          st[0] = Half<T>::mma16(kf[0][n], q[n], st[0]);
+          st[1] = Half<T>::mma16(kf[1][n], q[n], st[1]);
+        }
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * c.scale;
+        const bool whole = page_ok[0] && page_ok[1] && kb + 32 <= len && (kb >= from || kb + 32 <= c.sinks);
+        if (!whole) {  // keys that the query does not see count as nothing, whatever their page holds
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = kb + 16 * (e >> 2) + 4 * quad + (e & 3);
+            const bool sees = bool(page_ok[e >> 2]) & (at < len) & ((at >= from) | (at < c.sinks));
+            x[e] = sees ? x[e] : kNegInf;
+#pragma unroll
+            for (int w = 0; w < S::words; ++w) vr[e][w] = sees ? vr[e][w] : 0;
+          }
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        top = fmaxf(m, max32(max16(top)));
+        if (__any(top > m)) {
+          const float f = __builtin_amdgcn_exp2f(m - origin(top));
+          l *= f;
+#pragma unroll
+          for (int j = 0; j < S::per; ++j) o[j] *= f;
+          m = top;
+        }
+        uint32_t hi[4], rest[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(x[e] - origin(m)), p1 = __builtin_amdgcn_exp2f(x[e + 1] - origin(m));
+          l += p0 + p1;
+          hi[e / 2] = pack2<T>(p0, p1);
+          rest[e / 2] = pack2<T>(p0 - low<T>(hi[e / 2]), p1 - high<T>(hi[e / 2]));
+        }
+        const u32x4 ph = {hi[0], hi[1], hi[2], hi[3]}, pl = {rest[0], rest[1], rest[2], rest[3]};
+#pragma unroll
+        for (int j = 0; j < S::per; ++j) {
+          u32x4 vt;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            vt[p] = __builtin_amdgcn_perm(vr[2 * p + 1][j / 2], vr[2 * p][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+          o[j] = Half<T>::mma16(vt, ph, o[j]);
+          o[j] = Half<T>::mma16(vt, pl, o[j]);
+        }
+      }
+      l = sum32(sum16(l));
+
+      if (first == 0 && count == nb) {
+        if (has) {
+          const float r = l > 0 || l != l ? 1.f / l : 0.f;
+          T* out = static_cast<T*>(a.out) + s * a.out_seq + (head0 + col) * a.out_head;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = (4 * quad + e) * S::per;
+#pragma unroll
+            for (int j = 0; j < S::per; j += 2)
+              if (EXACT || d + j < c.dim)
+                *reinterpret_cast<uint32_t*>(out + d + j) = pack2<T>(o[j][e] * r, o[j + 1][e] * r);
+          }
+          if (a.lse && quad == 0)
+            a.lse[int64_t(s) * c.kv_heads * c.group + head0 + col] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+        }
+      } else {
+        const int slot = 2 * wave + (u != u_begin);
+        float* to = lds + slot * piece_floats(rows, D);
+        if (col < rows) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < S::per; ++j) to[col * D + (4 * quad + e) * S::per + j] = o[j][e];
+          if (quad == 0) {
+            to[rows * D + col] = m;
+            to[rows * D + rows + col] = l;
+          }
+        }
+        if (lane == 0) {
+          const int64_t b = base + int64_t(h) * nb;
+          piece_id[slot] = s * heads + h;
+          piece_flags[slot] = (b >= wg_begin && b + nb <= wg_end ? 1 : 0) | (b > wg_begin ? 2 : 0);
+        }
+      }
+      u += count;
+    }
+  }
+  __syncthreads();
+  // neighbouring pieces of one head, merged in order
+  for (int e = 0; e < 2 * kWaves; ++e) {
+    const int id = piece_id[e];
+    if (id < 0) continue;
+    int last = e;
+    for (int n = e + 1; n < 2 * kWaves; ++n)
+      if (piece_id[n] == id)
+        last = n;
+      else if (piece_id[n] >= 0)
+        break;
+    const int s = id / heads, h = id - s * heads, kvh = h / qtiles, head0 = kvh * c.group + (h - kvh * qtiles) * 16;
+    const bool complete = piece_flags[e] & 1;
+    float* to = a.work + (size_t(blockIdx.x) * 2 + (piece_flags[e] >> 1)) * piece_floats(rows, D);
+    const int have = min(16, c.group - (h - kvh * qtiles) * 16);
+    for (int i = threadIdx.x; i < have * D; i += kWaves * 64) {
+      const int r = i / D, d = i - r * D;
+      float m = kNegInf;
+      for (int n = e; n <= last; ++n)
+        if (piece_id[n] >= 0) m = fmaxf(m, lds[n * piece_floats(rows, D) + rows * D + r]);
+      float sum = 0, l = 0;
+      for (int n = e; n <= last; ++n) {
+        if (piece_id[n] < 0) continue;
+        const float* p = lds + n * piece_floats(rows, D);
+        const float f = __builtin_amdgcn_exp2f(p[rows * D + r] - origin(m));
+        sum += f * p[i];
+        l += f * p[rows * D + rows + r];
+      }
+      if (complete) {
+        const float inv = l > 0 || l != l ? 1.f / l : 0.f;
+        if (EXACT || d < c.dim) static_cast<T*>(a.out)[s * a.out_seq + (head0 + r) * a.out_head + d] = T(sum * inv);
+        if (a.lse && d == 0)
+          a.lse[int64_t(s) * c.kv_heads * c.group + head0 + r] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+      } else {
+        to[i] = sum;
+        if (d == 0) {
+          to[rows * D + r] = m;
+          to[rows * D + rows + r] = l;
+        }
+      }
+    }
+    e = last;
+  }
+}
+
+// One workgroup per sequence and head: the pieces of a head that workgroups share,
+// and rows that see nothing.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) decode_join_kernel(DecodeArgs a, unsigned workgroups) {
+  const CacheArgs& c = a.c;
+  const int qtiles = (c.group + 15) >> 4, heads = c.kv_heads * qtiles, rows = min(c.group, 16);
+  const int s = blockIdx.x / heads, h = blockIdx.x - s * heads, kvh = h / qtiles;
+  const int head0 = kvh * c.group + (h - kvh * qtiles) * 16, have = min(16, c.group - (h - kvh * qtiles) * 16);
+  const int64_t nb = a.base[s + 1] - a.base[s], b = a.base[s] * heads + h * nb;
+  T* out = static_cast<T*>(a.out) + s * a.out_seq + head0 * a.out_head;
+  float* lse = a.lse ? a.lse + int64_t(s) * c.kv_heads * c.group + head0 : nullptr;
+  if (nb == 0) {
+    for (int i = threadIdx.x; i < have * c.dim; i += 256) out[(i / c.dim) * a.out_head + i % c.dim] = T(0.f);
+    if (lse && int(threadIdx.x) < have) lse[threadIdx.x] = kNegInf;
+    return;
+  }
+  const Range range(a.base[c.seqs] * heads, workgroups * kWaves);
+  const unsigned w0 = range.of(b) / kWaves, w1 = range.of(b + nb - 1) / kWaves;
+  if (w0 == w1) return;
+  const size_t piece = piece_floats(rows, D);
+  const float* first = a.work + (size_t(w0) * 2 + (b > range.begin(w0 * kWaves))) * piece;
+  const float* rest = a.work + size_t(w0) * 2 * piece;  // piece 0 of the others
+  for (int i = threadIdx.x; i < have * D; i += 256) {
+    const int r = i / D, d = i - r * D;
+    float m = first[rows * D + r];
+    for (unsigned w = w0 + 1; w <= w1; ++w) m = fmaxf(m, rest[(w - w0) * 2 * piece + rows * D + r]);
+    float sum = 0, l = 0;
+    for (unsigned w = w0; w <= w1; ++w) {
+      const float* p = w == w0 ? first : rest + (w - w0) * 2 * piece;
+      const float f = __builtin_amdgcn_exp2f(p[rows * D + r] - origin(m));
+      sum += f * p[i];
+      l += f * p[rows * D + rows + r];
+    }
+    const float inv = l > 0 || l != l ? 1.f / l : 0.f;
+    if (d < c.dim) out[r * a.out_head + d] = T(sum * inv);
+    if (lse && d == 0) lse[r] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch(const DecodeArgs& a, unsigned workgroups, hipStream_t s) {
+  const int rows = std::min(a.c.group, 16), heads = a.c.kv_heads * ((a.c.group + 15) / 16);
+  const size_t lds = 2 * kWaves * size_t(rows) * (D + 2) * sizeof(float);
+  const auto kernel = a.c.dim == D ? paged_decode_kernel<T, D, true> : paged_decode_kernel<T, D, false>;
+  hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kWaves * 64), lds, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((decode_join_kernel<T, D>), dim3(unsigned(a.c.seqs) * heads), dim3(256), 0, s, a, workgroups);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_dim(const DecodeArgs& a, unsigned workgroups, hipStream_t s) {
+  return a.c.dim <= 64 ? launch<T, 64>(a, workgroups, s) : a.c.dim <= 128 ? launch<T, 128>(a, workgroups, s) : launch<T, 256>(a, workgroups, s);
+}
+
+}  // namespace
+
+// As many workgroups as the chip holds at three a CU, and no more than there are
+// blocks for their waves.
+unsigned decode_workgroups(size_t seqs, size_t kv_heads, size_t group, size_t keys) {
+  const size_t blocks = seqs * kv_heads * ((group + 15) / 16) * ((keys + 31) / 32 + 1);
+  return unsigned(std::max<size_t>(1, std::min<size_t>((blocks + kWaves - 1) / kWaves, 256 * 3)));
+}
+size_t decode_work_floats(unsigned workgroups, size_t group, size_t dim) {
+  const size_t D = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  return size_t(workgroups) * 2 * std::min<size_t>(group, 16) * (D + 2);
+}
+
+hipError_t launch_paged_decode(const DecodeArgs& a, int type, unsigned workgroups, hipStream_t s) {
+  return type == PRAGHIP_F16 ? launch_dim<_Float16>(a, workgroups, s) : launch_dim<__bf16>(a, workgroups, s);
+}
+
+}  // namespace praghip

@@ -18,6 +18,10 @@ libpraghip.so:
   (resident.hpp:20-45) and the acyclic packing tree (bfv_gpu_packing.hpp:10-45)
 * :class:`Qwen3LocalGemms` - the local products of a Qwen3 forward
   (model.hpp:66-126) as one batched call
+* :func:`paged_decode`, :func:`paged_prompt`, the ``page_*`` calls and
+  :func:`matvec_w4` - serving a model in the clear beside the protocol (no
+  counterpart in the reference): attention over a paged cache, its pages, and
+  few-row products with 4-bit weights
 
 Device data is handed over as torch tensors on the GPU (int64 or uint64 with
 u64 bit patterns); torch is used only for memory and streams.
@@ -34,6 +38,10 @@ from .weights import MappedWeights  # noqa: F401
 from .qwen3 import QWEN3_0_6B, Qwen3LocalGemms, Qwen3Shape  # noqa: F401
 from .matrix import Matrix, MatrixPacking, PublicZero, matrix_packing  # noqa: F401
 from .token import DeviceCipherBatch, Packing, TokenWeights, packed_target  # noqa: F401
+from .attention import page_write, paged_decode, paged_prompt  # noqa: F401
+from .pages import (page_check, page_compact, page_copy, page_fork, page_free, page_reserve,  # noqa: F401
+                    page_trim)
+from .matvec import matvec_w4, quantize_w4  # noqa: F401
 from . import frames, synth  # noqa: F401
 
 

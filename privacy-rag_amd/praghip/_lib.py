@@ -69,7 +69,33 @@ class FrameHeaderT(ctypes.Structure):
                 ("size", ctypes.c_uint64), ("stage", ctypes.c_uint64), ("operation", ctypes.c_uint64)]
 
 
+class Cache(ctypes.Structure):
+    """praghip_cache: one layer's keys and values in pages."""
+    _fields_ = [("k", vp), ("v", vp), ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3),
+                ("pages", sz), ("kv_heads", sz), ("page_size", sz), ("head_dim", sz), ("type", i32), ("tables", vp),
+                ("table_stride", ctypes.c_int64), ("table_width", sz), ("lengths", vp), ("seqs", sz)]
+
+
+class PageTable(ctypes.Structure):
+    """praghip_page_table: who holds which page."""
+    _fields_ = [("tables", vp), ("stride", ctypes.c_int64), ("width", sz), ("seqs", sz), ("lengths", vp),
+                ("refs", vp), ("pages", sz), ("page_size", sz), ("status", vp)]
+
+
+class PagePool(ctypes.Structure):
+    """praghip_page_pool: planes of pages."""
+    _fields_ = [("base", vp), ("plane_bytes", ctypes.c_int64), ("page_bytes", sz), ("planes", sz), ("pages", sz)]
+
+
+class W4(ctypes.Structure):
+    """praghip_w4: 4-bit weights with group scales."""
+    _fields_ = [("w", vp), ("w_stride", ctypes.c_int64), ("scales", vp), ("scale_stride", ctypes.c_int64),
+                ("zeros", vp), ("zero_stride", ctypes.c_int64), ("n", sz), ("k", sz), ("width", sz), ("group", sz),
+                ("type", i32)]
+
+
 pp = ctypes.POINTER(ctypes.c_void_p)
+f32, i64 = ctypes.c_float, ctypes.c_int64
 
 SIGNATURES = {
     "praghip_last_error": (ctypes.c_char_p, []),
@@ -176,6 +202,20 @@ SIGNATURES = {
     "praghip_fill_i8": (i32, [i32, vp, sz, u64, vp]),
     "praghip_fill_shift": (i32, [i32, vp, sz, u64, vp]),
     "praghip_share_gemm_batch": (i32, [i32, vp, sz, vp]),
+    "praghip_paged_decode_workspace": (sz, [vp, sz, sz]),
+    "praghip_paged_decode": (i32, [i32, vp, vp, vp, sz, vp, vp, vp, f32, sz, sz, sz, vp, sz, vp]),
+    "praghip_paged_prompt_workspace": (sz, [vp, sz, sz, sz, sz, sz]),
+    "praghip_paged_prompt": (i32, [i32, vp, vp, vp, sz, vp, sz, sz, vp, vp, vp, f32, sz, sz, sz, vp, sz, vp]),
+    "praghip_page_reserve": (i32, [i32, vp, vp, vp, sz, vp]),
+    "praghip_page_free": (i32, [i32, vp, vp, sz, vp]),
+    "praghip_page_trim": (i32, [i32, vp, vp, sz, sz, sz, vp]),
+    "praghip_page_fork_workspace": (sz, [sz]),
+    "praghip_page_fork": (i32, [i32, vp, vp, vp, vp, sz, vp, sz, vp]),
+    "praghip_page_compact_workspace": (sz, [sz]),
+    "praghip_page_compact": (i32, [i32, vp, vp, vp, sz, vp]),
+    "praghip_page_copy": (i32, [i32, vp, vp, vp, sz, vp]),
+    "praghip_page_write": (i32, [i32, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "praghip_matvec_w4": (i32, [i32, vp, vp, i64, sz, vp, i64, vp]),
 }
 
 _lib = None

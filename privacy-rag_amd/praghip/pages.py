@@ -1,0 +1,135 @@
+"""The pages of a key/value cache: who holds them, and their copies.
+
+``tables`` int32 [seqs][width] names each sequence's pages (-1: none), ``lengths``
+int32 [seqs] counts its tokens and ``refs`` int32 [pages] the table entries that name
+a page (0: free).  All three are on the GPU and change in place; new pages are the
+free ones of the lowest index, in the order of the call's list.  A pool is a
+contiguous tensor [...planes][pages][kv_heads][page_size][dim], one plane per layer
+and keys or values.
+
+The lists (int32 on the GPU, each sequence at most once) are checked there: a call
+that is refused changes nothing and leaves a code in ``status`` (int32 [1], if given,
+while it is 0), which :func:`page_check` turns into an error.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from ._lib import E_STATE, PageTable, PagePool, PraghipError, check, lib, shape_error
+from .attention import _stream, _torch, _type_error, _work
+
+_REFUSED = {1: "E_PAGES_SEQUENCE", 2: "E_PAGES_CAPACITY", 3: "E_PAGES_EXHAUSTED"}
+
+
+def _ints(t, dims: int, index: int) -> int:
+    if t.dtype is not _torch().int32 or t.get_device() != index or index < 0:
+        raise _type_error("E_PAGES_INTS")
+    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise shape_error("E_PAGES_SHAPE")
+    return t.data_ptr()
+
+
+def _table(tables, lengths, refs, page_size: int, status, index: int) -> PageTable:
+    at, held, counts = _ints(tables, 2, index), _ints(lengths, 1, index), _ints(refs, 1, index)
+    if lengths.shape[0] != tables.shape[0]:
+        raise shape_error("E_PAGES_SHAPE")
+    return PageTable(at, tables.stride(0), tables.shape[1], lengths.shape[0], held, counts, refs.shape[0], page_size,
+                     None if status is None else _ints(status, 1, index))
+
+
+def _pool(pool, index: int) -> PagePool:
+    if pool.dim() < 4 or not pool.is_contiguous():
+        raise shape_error("E_PAGES_POOL")
+    if pool.get_device() != index or index < 0:
+        raise _type_error("E_PAGES_DEVICE")
+    shape, size = pool.shape, pool.element_size()
+    page = math.prod(shape[-3:]) * size
+    return PagePool(pool.data_ptr(), shape[-4] * page, page, math.prod(shape[:-4]), shape[-4])
+
+
+def _list(t, n: int | None, index: int) -> int:
+    at = _ints(t, 1, index)
+    if n is not None and t.shape[0] != n:
+        raise shape_error("E_PAGES_SHAPE")
+    return at
+
+
+def page_reserve(tables, lengths, refs, page_size: int, sequences, counts, status=None, stream=None) -> None:
+    """counts[i] more tokens for sequences[i]: its new pages, and its length."""
+    index = tables.get_device()
+    t = _table(tables, lengths, refs, page_size, status, index)
+    n = sequences.shape[0]
+    check(lib().praghip_page_reserve(index, ctypes.byref(t), _list(sequences, None, index), _list(counts, n, index), n,
+                                     _stream(index, stream)))
+
+
+def page_free(tables, lengths, refs, sequences, status=None, stream=None) -> None:
+    """Empties sequences: their pages lose a reference, their rows become -1, their lengths 0."""
+    index = tables.get_device()
+    t = _table(tables, lengths, refs, 1, status, index)
+    check(lib().praghip_page_free(index, ctypes.byref(t), _list(sequences, None, index), sequences.shape[0],
+                                  _stream(index, stream)))
+
+
+def page_trim(tables, lengths, refs, page_size: int, sequences, window: int, sinks: int = 0, status=None,
+              stream=None) -> None:
+    """Gives back the pages that no token after a sequence's last one sees through this window and these sinks."""
+    index = tables.get_device()
+    t = _table(tables, lengths, refs, page_size, status, index)
+    if window < 0 or sinks < 0:
+        raise shape_error("E_PAGES_WINDOW")
+    check(lib().praghip_page_trim(index, ctypes.byref(t), _list(sequences, None, index), sequences.shape[0], window,
+                                  sinks, _stream(index, stream)))
+
+
+def page_fork(pool, tables, lengths, refs, parents, children, status=None, stream=None) -> None:
+    """children[i], an empty sequence, becomes a copy of parents[i] (which may have several).
+
+    Full pages are shared; a last page that is not full is copied in every plane of
+    the pool to a new page.
+    """
+    index = tables.get_device()
+    p = _pool(pool, index)
+    t = _table(tables, lengths, refs, pool.shape[-2], status, index)
+    n = parents.shape[0]
+    of, to = _list(parents, None, index), _list(children, n, index)
+    if n:
+        L = lib()
+        size = L.praghip_page_fork_workspace(n)
+        work = _work(size, tables, stream)
+        check(L.praghip_page_fork(index, ctypes.byref(t), ctypes.byref(p), of, to, n, work.data_ptr(), size,
+                                  _stream(index, stream)))
+
+
+def page_compact(pool, tables, refs, stream=None) -> None:
+    """Moves pages so that the held ones are 0 .. count - 1: held pages above move into
+    the holes below, both in rising order, and the tables follow."""
+    index = tables.get_device()
+    p = _pool(pool, index)
+    at, counts = _ints(tables, 2, index), _ints(refs, 1, index)
+    t = PageTable(at, tables.stride(0), tables.shape[1], tables.shape[0], at, counts, refs.shape[0], pool.shape[-2],
+                  None)
+    L = lib()
+    size = L.praghip_page_compact_workspace(t.pages)
+    work = _work(size, tables, stream)
+    check(L.praghip_page_compact(index, ctypes.byref(t), ctypes.byref(p), work.data_ptr(), size,
+                                 _stream(index, stream)))
+
+
+def page_copy(pool, sources, targets, stream=None) -> None:
+    """Page sources[i] of every plane over page targets[i]; indexes that are no pages are
+    skipped.  No page may be both a source and a target, or a target twice."""
+    index = pool.get_device()
+    p = _pool(pool, index)
+    n = sources.shape[0]
+    check(lib().praghip_page_copy(index, ctypes.byref(p), _list(sources, None, index), _list(targets, n, index), n,
+                                  _stream(index, stream)))
+
+
+def page_check(status) -> None:
+    """Waits for the GPU; raises where a call was refused since `status` was 0, and clears it."""
+    code = int(status.item())
+    if code:
+        status.zero_()
+        raise PraghipError(E_STATE, _REFUSED.get(code, f"E_PAGES_{code}"))
