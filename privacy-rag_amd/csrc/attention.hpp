@@ -24,7 +24,8 @@ struct CacheArgs {
   int pages, page_shift, seqs, kv_heads, group, dim;
   int64_t capacity;  // positions that a row of the table has room for
   int window, sinks;
-  float scale;       // of q.k, times log2 e: the kernels work in powers of two
+  float scale;       // of q.k, times log2 e (the kernels work in powers of two), positive:
+  uint32_t flip;     // its sign is in the bits that q's values are flipped by
 };
 
 struct DecodeArgs {

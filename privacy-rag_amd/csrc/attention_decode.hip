@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
         const int d = 32 * i + 8 * quad;
         if (has && (EXACT || d < c.dim))
           q[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + s * a.q_seq + (head0 + col) * a.q_head + d);
+        q[i] ^= c.flip;
       }
       f32x4 o[S::per];
 #pragma unroll

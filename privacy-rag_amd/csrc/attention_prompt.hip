@@ -30,9 +30,47 @@ namespace {
 
 constexpr int kTile = 64;  // keys of a tile
 
+// 16 bytes a lane from memory into LDS at M0 + 16 lane (global_load_lds_dwordx4).  The
+// compiler adds no wait of its own for an asm, so the caller waits before it reads; the
+// asm starts with the wait state that the DMA needs after the write of M0.
+__device__ __forceinline__ void dma16(const void* src, void* lds_wave_base) {
+  const unsigned at = unsigned(reinterpret_cast<uintptr_t>((void __attribute__((address_space(3)))*)(lds_wave_base)));
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(__builtin_amdgcn_readfirstlane(at))
+               : "memory");
+}
+
+// One tile's scores, 16 of 32 keys in st[t] for the lane's query, into P: the running
+// maximum, the sum of P and O's factor.  Within 2^kSlack of it the old maximum stays in
+// use: P may then be up to 2^kSlack, with the same relative rounding, and the dim / 2
+// products with the factor are left out.
+constexpr float kSlack = 8;
+template <typename T, int B>
+__device__ __forceinline__ void soften(const f32x16 (&st)[2], u32x4 (&p)[4], f32x16 (&o)[B], float& m, float& l, float scale) {
+  float x[32], top = m;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) x[r] = st[r >> 4][r & 15] * scale;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) top = fmaxf(top, x[r]);
+  top = max32(top);
+  if (__any(top > m + kSlack)) {
+    const float f = __builtin_amdgcn_exp2f(m - origin(top));
+    l *= f;
+#pragma unroll
+    for (int b = 0; b < B; ++b) o[b] *= f;
+    m = top;
+  }
+  const float base = origin(m);
+#pragma unroll
+  for (int r = 0; r < 32; r += 2) {
+    const float p0 = __builtin_amdgcn_exp2f(x[r] - base), p1 = __builtin_amdgcn_exp2f(x[r + 1] - base);
+    l += p0 + p1;
+    p[r >> 3][(r & 7) >> 1] = pack2<T>(p0, p1);
+  }
+}
+
 template <typename T, int D, int NW, bool EXACT>
 __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArgs a, int ntile) {
-  constexpr int ROWS = 32 * NW, CPR = D / 8, PER = kTile * CPR / (NW * 64);  // chunks of a row, of a thread
+  constexpr int ROWS = 32 * NW, CPR = D / 8;  // 16-byte chunks of a row
   constexpr int steps = D / 16, blocks32 = D / 32;
   extern __shared__ uint32_t lds[];
   T* const kbuf = reinterpret_cast<T*>(lds);            // [2][64][D]
@@ -72,6 +110,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     const int d = 16 * n + 8 * half;
     if (has && (EXACT || d < c.dim))
       q[n] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (begin + token) * a.q_token + head * a.q_head + d);
+    q[n] ^= c.flip;
   }
   f32x16 o[blocks32];
 #pragma unroll
@@ -80,93 +119,96 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     for (int r = 0; r < 16; ++r) o[b][r] = 0;
   float m = kNegInf, l = 0;
 
+  // tiles come by DMA, 1 KiB an instruction: RPI rows, whose page is one, and 16 bytes
+  // a lane, which takes the chunk that belongs at its place
+  constexpr int RPI = 64 / CPR, PER = kTile / RPI / NW;
   const auto fk = [](int r) { return D == 64 ? (r >> 1) & 7 : r & 15; };
   const auto fv = [](int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; };
-  const int width = int(c.capacity >> c.page_shift);
-
-  u32x4 kx[PER], vx[PER];
-  uint32_t pages_ok = 0;  // groups of 16 keys of the tile in registers that have a page
-  const auto load = [&](int kb) {
-    uint32_t ok = 0;
-    {
-      const int at = (kb + 16 * (lane & 3)) >> c.page_shift;
-      const int page = at < width ? c.tables[s * c.table_stride + at] : -1;
-      ok = uint32_t(__ballot(page >= 0 && page < c.pages)) & 15;
-    }
-    pages_ok = ok;
+  const int width = int(c.capacity >> c.page_shift), inrow = lane / CPR;
+  const int32_t* const table = c.tables + s * c.table_stride;
+  // lane x % 4 holds the page of the tile's keys 16 x .. 16 x + 15; -1: none
+  const auto pages_of = [&](int kb) {
+    const int at = (kb + 16 * (lane & 3)) >> c.page_shift;
+    const int page = at < width ? table[at] : -1;
+    return page < c.pages ? page : -1;
+  };
+  const auto load = [&](int kb, int pages, int buf) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int chunk = threadIdx.x + i * NW * 64, r = chunk / CPR, x = chunk % CPR, at = kb + r;
-      kx[i] = vx[i] = u32x4{0, 0, 0, 0};
-      if (at < len && (ok >> (r >> 4) & 1) && (EXACT || 8 * x < c.dim)) {
-        const int64_t page = c.tables[s * c.table_stride + (at >> c.page_shift)];
-        const int in = at & ((1 << c.page_shift) - 1);
-        kx[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(c.k) + page * c.k_page + kvh * c.k_head + in * c.k_token + 8 * x);
-        vx[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(c.v) + page * c.v_page + kvh * c.v_head + in * c.v_token + 8 * x);
+      const int r0 = RPI * (wave + NW * i), r = r0 + inrow;
+      const int page = max(0, __builtin_amdgcn_readlane(pages, r0 >> 4)), in = (kb + r0) & ((1 << c.page_shift) - 1);
+      const T* const kp = static_cast<const T*>(c.k) + page * c.k_page + kvh * c.k_head + in * c.k_token;
+      const T* const vp = static_cast<const T*>(c.v) + page * c.v_page + kvh * c.v_head + in * c.v_token;
+      const int xk = (lane % CPR) ^ fk(r), xv = (lane % CPR) ^ fv(r);
+      if (EXACT || 8 * xk < c.dim) dma16(kp + inrow * c.k_token + 8 * xk, kbuf + (buf * kTile + r0) * D);
+      if (EXACT || 8 * xv < c.dim) dma16(vp + inrow * c.v_token + 8 * xv, vbuf + (buf * kTile + r0) * D);
+    }
+  };
+  // the wave's own loads have arrived; rows of V that are no key of the sequence's hold
+  // whatever their page does, and P's zeros would not silence a NaN there
+  const auto arrived = [&](int kb, uint32_t ok, int buf) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (ok != 15 || kb + kTile > len) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r0 = RPI * (wave + NW * i), r = r0 + inrow;
+        if (kb + r >= len || !(ok >> (r0 >> 4) & 1))
+          *reinterpret_cast<u32x4*>(vbuf + (buf * kTile + r0) * D + 8 * lane) = u32x4{0, 0, 0, 0};
       }
     }
+    __syncthreads();
   };
-  const auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int chunk = threadIdx.x + i * NW * 64, r = chunk / CPR, x = chunk % CPR;
-      *reinterpret_cast<u32x4*>(kbuf + buf * kTile * D + r * D + 8 * (x ^ fk(r))) = kx[i];
-      *reinterpret_cast<u32x4*>(vbuf + buf * kTile * D + r * D + 8 * (x ^ fv(r))) = vx[i];
-    }
-  };
-
-  if (i0 < i1) {
-    load(blocks.at(i0) * kTile);
-    store(0);
+  if (!EXACT) {  // columns beyond dim are never loaded
+    for (int i = threadIdx.x; i < 4 * kTile * CPR; i += NW * 64) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    __syncthreads();
   }
-  __syncthreads();
-  for (int i = i0; i < i1; ++i) {
-    const int kb = blocks.at(i) * kTile, buf = (i - i0) & 1;
-    const uint32_t ok = pages_ok;
-    if (i + 1 < i1) load(blocks.at(i + 1) * kTile);
+
+  int kb = 0, next = 0, pages = -1;
+  uint32_t ok = 0, next_ok = 0;
+  if (i0 < i1) {
+    kb = blocks.at(i0) * kTile;
+    const int mine = pages_of(kb);
+    ok = uint32_t(__ballot(mine >= 0)) & 15;
+    if (i0 + 1 < i1) pages = pages_of(blocks.at(i0 + 1) * kTile);
+    load(kb, mine, 0);
+    arrived(kb, ok, 0);
+  }
+  for (int i = i0; i < i1; ++i, kb = next, ok = next_ok) {
+    const int buf = (i - i0) & 1;
+    if (i + 1 < i1) {
+      next = blocks.at(i + 1) * kTile;
+      const int mine = pages;
+      next_ok = uint32_t(__ballot(mine >= 0)) & 15;
+      if (i + 2 < i1) pages = pages_of(blocks.at(i + 2) * kTile);
+      load(next, mine, buf ^ 1);
+    }
     const bool any = kb <= wmax && (c.window == 0 || kb + kTile > wmin - c.window + 1 || kb < c.sinks);
     if (any) {
       f32x16 st[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[t][r] = 0;
 #pragma unroll
-        for (int n = 0; n < steps; ++n) {
+      for (int n = 0; n < steps; ++n)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
           const int r = 32 * t + col;
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + buf * kTile * D + r * D + 8 * ((2 * n + half) ^ fk(r)));
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + (buf * kTile + r) * D + 8 * ((2 * n + half) ^ fk(r)));
           st[t] = Half<T>::mma32(kf, q[n], st[t]);
         }
-      }
       const bool whole = ok == 15 && kb + kTile - 1 <= wmin && (c.window == 0 || kb > wmax - c.window || kb + kTile <= c.sinks);
-      float top = m, x[32];
-#pragma unroll
-      for (int r = 0; r < 32; ++r) x[r] = st[r >> 4][r & 15] * c.scale;
-      if (!whole) {
+      u32x4 p[4];
+      if (!whole) {  // before the scale, which is positive: the compiler would canonicalise
+                     // each of the values that pass a join of branches into a maximum
 #pragma unroll
         for (int r = 0; r < 32; ++r) {
           const int key = 8 * (r >> 2) + 4 * half + (r & 3), at = kb + key;
           const bool sees = (at <= place) & ((at > from) | (at < c.sinks)) & bool(ok >> (key >> 4) & 1);
-          x[r] = sees ? x[r] : kNegInf;
+          st[r >> 4][r & 15] = sees ? st[r >> 4][r & 15] : kNegInf;
         }
       }
-#pragma unroll
-      for (int r = 0; r < 32; ++r) top = fmaxf(top, x[r]);
-      top = max32(top);
-      if (__any(top > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - origin(top));
-        l *= f;
-#pragma unroll
-        for (int b = 0; b < blocks32; ++b) o[b] *= f;
-        m = top;
-      }
-      u32x4 p[4];
-#pragma unroll
-      for (int r = 0; r < 32; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(x[r] - origin(m)), p1 = __builtin_amdgcn_exp2f(x[r + 1] - origin(m));
-        l += p0 + p1;
-        p[r >> 3][(r & 7) >> 1] = pack2<T>(p0, p1);
-      }
+      soften<T, blocks32>(st, p, o, m, l, c.scale);
       const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -179,15 +221,14 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             const auto x = __builtin_bit_cast(
                 u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                           vbuf + buf * kTile * D + r * D + 8 * ((d >> 3) ^ fv(r)) + (d & 7))));
+                           vbuf + (buf * kTile + r) * D + 8 * ((d >> 3) ^ fv(r)) + (d & 7))));
             vt[2 * e] = x[0];
             vt[2 * e + 1] = x[1];
           }
           o[b] = Half<T>::mma32(vt, p[t], o[b]);
         }
     }
-    if (i + 1 < i1) store(buf ^ 1);
-    __syncthreads();
+    if (i + 1 < i1) arrived(next, next_ok, buf ^ 1);
   }
   l = sum32(l);
 

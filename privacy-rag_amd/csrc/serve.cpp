@@ -61,7 +61,9 @@ CacheArgs cache_args(const praghip_cache& c, size_t heads, float scale, size_t w
   // a window that every position fits in is none
   a.window = window >= size_t(a.capacity) ? 0 : int(window);
   a.sinks = int(std::min(sinks, size_t(a.capacity)));
-  a.scale = scale * 1.4426950408889634f;
+  // a scale of 0 as one that leaves no score above rounding: -inf times it stays -inf
+  a.scale = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  a.flip = scale < 0 ? 0x80008000u : 0;
   return a;
 }
 

@@ -252,6 +252,24 @@ def test_prompt_strides(gpu):
     assert not room[:, :, 64:].any()
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0])
+def test_scales(gpu, scale):
+    """Negative scales turn the order of the scores; with 0 all visible keys weigh the same."""
+    say("scale", scale)
+    c = plain.make([150, 41], 8, 4, 64, 16, BF16, seed=28)
+    q = (torch.randn((60, 8, 64), generator=c["g"]) * (0.1 if scale == 1.0 else 1)).to(BF16)
+    starts = [0, 40, 60]
+    want, wlse, size = plain.attention(c, q, starts, scale=scale, window=50, sinks=3)
+    out, lse = praghip.paged_prompt(q.to("cuda"), *to_gpu(c), torch.tensor(starts, dtype=torch.int32, device="cuda"), 40,
+                                    scale=scale, window=50, sinks=3, lse=True)
+    plain.check(out, want, size, BF16, rounded=True)
+    plain.check_lse(lse, wlse)
+    want, wlse, size = plain.attention(c, q[:2], [0, 1, 2], scale=scale, window=50, sinks=3)
+    out, lse = decode(c, q[:2], scale=scale, window=50, sinks=3)
+    plain.check(out, want, size, BF16, rounded=False)
+    plain.check_lse(lse, wlse)
+
+
 def test_zero_sequences_and_rows(gpu):
     c = plain.make([20], 4, 2, 64, 16, BF16, seed=24)
     k, v, tables, lengths = to_gpu(c)
