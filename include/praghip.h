@@ -590,8 +590,8 @@ int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
  * sequence's length names is never used, whatever it holds.
  *
  * page_size is a power of two of 16 .. 32768, head_dim a multiple of 8 up to 256
- * (E_ATTENTION_SHAPE); base addresses are 16-byte aligned and strides multiples of 8
- * (E_ATTENTION_ALIGNMENT).  A length outside 0 .. table_width * page_size is taken
+ * and the cache's strides are below 2^31, a token's below 2^26 (E_ATTENTION_SHAPE); base addresses are 16-byte
+ * aligned and strides multiples of 8 (E_ATTENTION_ALIGNMENT).  A length outside 0 .. table_width * page_size is taken
  * as the nearer end. */
 typedef struct praghip_cache {
   void *k, *v;

@@ -17,7 +17,7 @@ namespace praghip {
 struct CacheArgs {
   const void* k;
   const void* v;
-  int64_t k_page, k_head, k_token, v_page, v_head, v_token;
+  uint32_t k_page, k_head, k_token, v_page, v_head, v_token;
   const int32_t* tables;
   int64_t table_stride;
   const int32_t* lengths;

@@ -165,27 +165,27 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
           page_ok[t] = page >= 0 && page < c.pages;
           page = page_ok[t] ? page : 0;
           const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
-          const T* kp = static_cast<const T*>(c.k) + page * c.k_page + kvh * c.k_head + (row + col) * c.k_token + 8 * quad;
+          const T* kp = static_cast<const T*>(c.k) + uint64_t(page) * c.k_page + uint64_t(kvh) * c.k_head + uint64_t(row + col) * c.k_token + 8 * quad;
 #pragma unroll
           for (int n = 0; n < S::steps; ++n) {
             kf[t][n] = u32x4{0, 0, 0, 0};
             if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
           }
-          const T* vp = static_cast<const T*>(c.v) + page * c.v_page + kvh * c.v_head + (row + 4 * quad) * c.v_token + S::per * col;
+          const T* vp = static_cast<const T*>(c.v) + uint64_t(page) * c.v_page + uint64_t(kvh) * c.v_head + uint64_t(row + 4 * quad) * c.v_token + S::per * col;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
 #pragma unroll
             for (int w = 0; w < S::words; ++w) vr[4 * t + e][w] = 0;
             if (EXACT || S::per * col < c.dim) {
               if constexpr (S::words == 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(vp + e * c.v_token);
+                const u32x2 x = *reinterpret_cast<const u32x2*>(vp + uint64_t(e) * c.v_token);
                 vr[4 * t + e][0] = x[0];
                 vr[4 * t + e][1] = x[1];
               } else {
 #pragma unroll
                 for (int w = 0; w < S::words; w += 4) {
                   if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
-                  const u32x4 x = *reinterpret_cast<const u32x4*>(vp + e * c.v_token + 2 * w);
+                  const u32x4 x = *reinterpret_cast<const u32x4*>(vp + uint64_t(e) * c.v_token + 2 * w);
 #pragma unroll
                   for (int b = 0; b < 4; ++b) vr[4 * t + e][w + b] = x[b];
                 }

@@ -28,14 +28,28 @@
 namespace praghip {
 namespace {
 
-constexpr int kTile = 64;  // keys of a tile
+constexpr int kRing = 4;      // tiles of K, and of V, in LDS
+constexpr int kGroups = 512;  // groups of 16 keys whose addresses are in LDS, by halves
+constexpr int kFlags = 64;    // bytes of LDS beside them
+// keys of a tile
+template <int D>
+constexpr int tile_keys() {
+  return D == 256 ? 32 : 64;
+}
 
-// 16 bytes a lane from memory into LDS at M0 + 16 lane (global_load_lds_dwordx4).  The
-// compiler adds no wait of its own for an asm, so the caller waits before it reads; the
-// asm starts with the wait state that the DMA needs after the write of M0.
-__device__ __forceinline__ void dma16(const void* src, void* lds_wave_base) {
-  const unsigned at = unsigned(reinterpret_cast<uintptr_t>((void __attribute__((address_space(3)))*)(lds_wave_base)));
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(__builtin_amdgcn_readfirstlane(at))
+// LDS addresses as they are: through generic pointers every access would test for null
+typedef __attribute__((address_space(3))) char* Lds;
+template <typename V>
+__device__ __forceinline__ __attribute__((address_space(3))) V* lds_at(Lds p) {
+  return (__attribute__((address_space(3))) V*)p;
+}
+
+// 16 bytes a lane, from base + its offset, into LDS at M0 + 16 lane.  The
+// compiler adds no wait of its own for an asm, so the caller waits before it reads; and
+// the asm starts with the wait states that the DMA needs after the writes of M0 (one) and,
+// by a VALU, of the base (five).
+__device__ __forceinline__ void dma16(uint64_t base, uint32_t offset, Lds to) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(uint32_t(uintptr_t(to))))
                : "memory");
 }
 
@@ -44,25 +58,27 @@ __device__ __forceinline__ void dma16(const void* src, void* lds_wave_base) {
 // use: P may then be up to 2^kSlack, with the same relative rounding, and the dim / 2
 // products with the factor are left out.
 constexpr float kSlack = 8;
-template <typename T, int B>
-__device__ __forceinline__ void soften(const f32x16 (&st)[2], u32x4 (&p)[4], f32x16 (&o)[B], float& m, float& l, float scale) {
-  float x[32], top = m;
+template <int B>
+__device__ __forceinline__ void top_of(const f32x16& st, f32x16 (&o)[B], float& m, float& l, float scale) {
+  float top = m;  // (a maximum that keeps NaN takes its operands as they are)
 #pragma unroll
-  for (int r = 0; r < 32; ++r) x[r] = st[r >> 4][r & 15] * scale;
-#pragma unroll
-  for (int r = 0; r < 32; ++r) top = fmaxf(top, x[r]);
-  top = max32(top);
-  if (__any(top > m + kSlack)) {
-    const float f = __builtin_amdgcn_exp2f(m - origin(top));
+  for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, st[r]);
+  const Two both = swap32(top);
+  top = __builtin_elementwise_maximum(both.a, both.b);
+  if (__any((top - m) * scale > kSlack)) {
+    const float f = __builtin_amdgcn_exp2f((m - origin(top)) * scale);
     l *= f;
 #pragma unroll
     for (int b = 0; b < B; ++b) o[b] *= f;
     m = top;
   }
-  const float base = origin(m);
+}
+template <typename T>
+__device__ __forceinline__ void soften(const f32x16& st, u32x4 (&p)[2], float m, float& l, float scale) {
+  const float base = -origin(m) * scale;
 #pragma unroll
-  for (int r = 0; r < 32; r += 2) {
-    const float p0 = __builtin_amdgcn_exp2f(x[r] - base), p1 = __builtin_amdgcn_exp2f(x[r + 1] - base);
+  for (int r = 0; r < 16; r += 2) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(st[r], scale, base)), p1 = __builtin_amdgcn_exp2f(fmaf(st[r + 1], scale, base));
     l += p0 + p1;
     p[r >> 3][(r & 7) >> 1] = pack2<T>(p0, p1);
   }
@@ -73,8 +89,9 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   constexpr int ROWS = 32 * NW, CPR = D / 8;  // 16-byte chunks of a row
   constexpr int steps = D / 16, blocks32 = D / 32;
   extern __shared__ uint32_t lds[];
-  T* const kbuf = reinterpret_cast<T*>(lds);            // [2][64][D]
-  T* const vbuf = kbuf + 2 * kTile * D;                 // [2][64][D]
+    constexpr int TK = tile_keys<D>(), ROW = 2 * D, TILE = TK * ROW;  // bytes
+  const Lds kbuf = (Lds)lds, vbuf = kbuf + kRing * TILE;  // [kRing][TK][D] each
+  const Lds list = vbuf + kRing * TILE, flags = list + 16 * kGroups;
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -100,7 +117,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   const int wmin = row0 + wave * 32 < nrow ? int((row0 + wave * 32) / c.group) + shift : 0;
   const int wmax = row0 + wave * 32 < nrow ? int(wlast / c.group) + shift : -1;
 
-  const Blocks blocks = visible_blocks(c, max(0, int(row0 / c.group) + shift), int((min(row0 + ROWS, nrow) - 1) / c.group) + shift, 6);
+  const Blocks blocks = visible_blocks(c, max(0, int(row0 / c.group) + shift), int((min(row0 + ROWS, nrow) - 1) / c.group) + shift, TK == 32 ? 5 : 6);
   const int nb = blocks.count(), i0 = int(int64_t(nb) * split / a.splits), i1 = int(int64_t(nb) * (split + 1) / a.splits);
 
   u32x4 q[steps];
@@ -121,116 +138,187 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
 
   // tiles come by DMA, 1 KiB an instruction: RPI rows, whose page is one, and 16 bytes
   // a lane, which takes the chunk that belongs at its place
-  constexpr int RPI = 64 / CPR, PER = kTile / RPI / NW;
+  constexpr int RPI = 64 / CPR, PER = TK / RPI / NW, GROUPS = TK / 16, TURNS = 64 / GROUPS;
   const auto fk = [](int r) { return D == 64 ? (r >> 1) & 7 : r & 15; };
   const auto fv = [](int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; };
   const int width = int(c.capacity >> c.page_shift), inrow = lane / CPR;
-  const int32_t* const table = c.tables + s * c.table_stride;
-  // lane x % 4 holds the page of the tile's keys 16 x .. 16 x + 15; -1: none
-  const auto pages_of = [&](int kb) {
-    const int at = (kb + 16 * (lane & 3)) >> c.page_shift;
-    const int page = at < width ? table[at] : -1;
-    return page < c.pages ? page : -1;
+  // Where 16 keys begin in memory, kGroups / 2 groups at a time in LDS: the addresses of K
+  // and V; the top bit of V's says that they have no page (they read page 0's).
+  const auto fill_list = [&](int i) {
+    const int at = (i - i0) * GROUPS;
+    for (int x = threadIdx.x; x < min(kGroups / 2, (i1 - i) * GROUPS); x += NW * 64) {
+      const int key = blocks.at(i + x / GROUPS) * TK + 16 * (x % GROUPS), entry = key >> c.page_shift;
+      int page = entry < width ? c.tables[s * c.table_stride + entry] : -1;
+      const bool none = page < 0 || page >= c.pages;
+      if (none & (key < len)) *lds_at<int>(flags) = 1;
+      page = none ? 0 : page;
+      const uint32_t in = key & ((1 << c.page_shift) - 1);
+      const uint64_t ka = uint64_t(uintptr_t(static_cast<const T*>(c.k) + uint64_t(kvh) * c.k_head + uint64_t(uint32_t(page)) * c.k_page + uint64_t(in) * c.k_token));
+      const uint64_t va = uint64_t(uintptr_t(static_cast<const T*>(c.v) + uint64_t(kvh) * c.v_head + uint64_t(uint32_t(page)) * c.v_page + uint64_t(in) * c.v_token));
+      *lds_at<u32x4>(list + 16 * (at % kGroups + x)) = u32x4{uint32_t(ka), uint32_t(ka >> 32), uint32_t(va), uint32_t(va >> 32) | (none ? 1u << 31 : 0)};
+    }
+    __syncthreads();
   };
-  const auto load = [&](int kb, int pages, int buf) {
+  // Of these a wave holds 64 in its lanes, one instruction away: an LDS read's latency and
+  // a product for each address before each load cost more than the products of a tile.
+  uint32_t klow = 0, khigh = 0, vlow = 0, vhigh = 0, koff[PER], voff[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int r0 = RPI * (wave + NW * i), r = r0 + inrow;
-      const int page = max(0, __builtin_amdgcn_readlane(pages, r0 >> 4)), in = (kb + r0) & ((1 << c.page_shift) - 1);
-      const T* const kp = static_cast<const T*>(c.k) + page * c.k_page + kvh * c.k_head + in * c.k_token;
-      const T* const vp = static_cast<const T*>(c.v) + page * c.v_page + kvh * c.v_head + in * c.v_token;
-      const int xk = (lane % CPR) ^ fk(r), xv = (lane % CPR) ^ fv(r);
-      if (EXACT || 8 * xk < c.dim) dma16(kp + inrow * c.k_token + 8 * xk, kbuf + (buf * kTile + r0) * D);
-      if (EXACT || 8 * xv < c.dim) dma16(vp + inrow * c.v_token + 8 * xv, vbuf + (buf * kTile + r0) * D);
+  for (int n = 0; n < PER; ++n) {  // a wave's rows start at a multiple of RPI within 16 keys
+    const int r0 = RPI * (wave + NW * n), r = r0 + inrow;
+    koff[n] = 2 * ((r & 15) * c.k_token + 8 * ((lane % CPR) ^ fk(r)));
+    voff[n] = 2 * ((r & 15) * c.v_token + 8 * ((lane % CPR) ^ fv(r)));
+  }
+  bool missing = false;  // some key has no page: no tile is taken as seen whole
+  const auto lane_of = [](uint32_t lo, uint32_t hi, int x) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(hi, x))) << 32 | uint32_t(__builtin_amdgcn_readlane(lo, x));
+  };
+  const auto load_k = [&](int at) {  // `at` counts the tiles from i0
+    if (at % TURNS == 0) {
+      const u32x2 x = *lds_at<u32x2>(list + 16 * (at * GROUPS % kGroups + lane));
+      klow = x[0], khigh = x[1];
+    }
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int r0 = RPI * (wave + NW * n);
+      if (EXACT || 8 * ((lane % CPR) ^ fk(r0 + inrow)) < c.dim)
+        dma16(lane_of(klow, khigh, at % TURNS * GROUPS + (r0 >> 4)), koff[n], kbuf + at % kRing * TILE + r0 * ROW);
     }
   };
-  // the wave's own loads have arrived; rows of V that are no key of the sequence's hold
-  // whatever their page does, and P's zeros would not silence a NaN there
-  const auto arrived = [&](int kb, uint32_t ok, int buf) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (ok != 15 || kb + kTile > len) {
+  const auto load_v = [&](int at) {
+    if (at % TURNS == 0) {
+      const u32x2 x = *lds_at<u32x2>(list + 16 * (at * GROUPS % kGroups + lane) + 8);
+      vlow = x[0], vhigh = x[1] & 0x7fffffffu;
+    }
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int r0 = RPI * (wave + NW * i), r = r0 + inrow;
-        if (kb + r >= len || !(ok >> (r0 >> 4) & 1))
-          *reinterpret_cast<u32x4*>(vbuf + (buf * kTile + r0) * D + 8 * lane) = u32x4{0, 0, 0, 0};
+    for (int n = 0; n < PER; ++n) {
+      const int r0 = RPI * (wave + NW * n);
+      if (EXACT || 8 * ((lane % CPR) ^ fv(r0 + inrow)) < c.dim)
+        dma16(lane_of(vlow, vhigh, at % TURNS * GROUPS + (r0 >> 4)), voff[n], vbuf + at % kRing * TILE + r0 * ROW);
+    }
+  };
+  // which groups of 16 keys of a tile have a page
+  const auto groups_of = [&](int at) {
+    uint32_t none = 0;
+#pragma unroll
+    for (int x = 0; x < GROUPS; ++x) none |= *lds_at<uint32_t>(list + 16 * ((at * GROUPS + x) % kGroups) + 12) >> 31 << x;
+    return ~uint32_t(__builtin_amdgcn_readfirstlane(none));
+  };
+  // The wave's own loads of V's tile and K's after it have arrived, a turn's of later ones
+  // are under way; rows of V that are no key of the sequence's hold whatever their page
+  // does, and P's zeros would not silence a NaN there.
+  const auto arrived = [&](int i, bool more) {
+    if (more)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int kb = blocks.at(i) * TK;
+    if (missing || kb + TK > len) {
+      const uint32_t held = groups_of(i - i0);
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        const int r0 = RPI * (wave + NW * n);
+        if (kb + r0 + inrow >= len || !(held >> (r0 >> 4) & 1))
+          *lds_at<u32x4>(vbuf + (i - i0) % kRing * TILE + r0 * ROW + 16 * lane) = u32x4{0, 0, 0, 0};
       }
     }
     __syncthreads();
   };
   if (!EXACT) {  // columns beyond dim are never loaded
-    for (int i = threadIdx.x; i < 4 * kTile * CPR; i += NW * 64) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
-    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * kRing * TK * CPR; i += NW * 64) *lds_at<u32x4>(kbuf + 16 * i) = u32x4{0, 0, 0, 0};
   }
+  if (threadIdx.x == 0) *lds_at<int>(flags) = 0;
+  __syncthreads();
 
-  int kb = 0, next = 0, pages = -1;
-  uint32_t ok = 0, next_ok = 0;
-  if (i0 < i1) {
-    kb = blocks.at(i0) * kTile;
-    const int mine = pages_of(kb);
-    ok = uint32_t(__ballot(mine >= 0)) & 15;
-    if (i0 + 1 < i1) pages = pages_of(blocks.at(i0 + 1) * kTile);
-    load(kb, mine, 0);
-    arrived(kb, ok, 0);
-  }
-  for (int i = i0; i < i1; ++i, kb = next, ok = next_ok) {
-    const int buf = (i - i0) & 1;
-    if (i + 1 < i1) {
-      next = blocks.at(i + 1) * kTile;
-      const int mine = pages;
-      next_ok = uint32_t(__ballot(mine >= 0)) & 15;
-      if (i + 2 < i1) pages = pages_of(blocks.at(i + 2) * kTile);
-      load(next, mine, buf ^ 1);
-    }
-    const bool any = kb <= wmax && (c.window == 0 || kb + kTile > wmin - c.window + 1 || kb < c.sinks);
-    if (any) {
-      f32x16 st[2];
+  // S^T = K Q^T of keys 32 t .. of a tile
+  const auto score = [&](int at, int t, f32x16& st) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int r = 0; r < 16; ++r) st[r] = 0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[t][r] = 0;
+    for (int n = 0; n < steps; ++n)
+      st = Half<T>::mma32(*lds_at<u32x4>(kbuf + at % kRing * TILE + (32 * t + col) * ROW + 16 * ((2 * n + half) ^ fk(col))), q[n], st);
+  };
+  // O^T += V^T P^T of the same keys
+  const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const auto weigh = [&](int at, int t, const u32x4 (&p)[2]) {
 #pragma unroll
-      for (int n = 0; n < steps; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int r = 32 * t + col;
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kbuf + (buf * kTile + r) * D + 8 * ((2 * n + half) ^ fk(r)));
-          st[t] = Half<T>::mma32(kf, q[n], st[t]);
+      for (int b = 0; b < blocks32; ++b) {
+        u32x4 vt;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 32 * t + 16 * n + 8 * e + trow, d = 32 * b + tcol;
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          const auto x = __builtin_bit_cast(
+              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(vbuf + at % kRing * TILE + r * ROW + 16 * ((d >> 3) ^ fv(trow)) + 2 * (d & 7))));
+          vt[2 * e] = x[0];
+          vt[2 * e + 1] = x[1];
         }
-      const bool whole = ok == 15 && kb + kTile - 1 <= wmin && (c.window == 0 || kb > wmax - c.window || kb + kTile <= c.sinks);
-      u32x4 p[4];
-      if (!whole) {  // before the scale, which is positive: the compiler would canonicalise
-                     // each of the values that pass a join of branches into a maximum
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-          const int key = 8 * (r >> 2) + 4 * half + (r & 3), at = kb + key;
-          const bool sees = (at <= place) & ((at > from) | (at < c.sinks)) & bool(ok >> (key >> 4) & 1);
-          st[r >> 4][r & 15] = sees ? st[r >> 4][r & 15] : kNegInf;
-        }
+        o[b] = Half<T>::mma32(vt, p[n], o[b]);
       }
-      soften<T, blocks32>(st, p, o, m, l, c.scale);
-      const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  };
+
+  // Turn i takes tile i through the softmax and into O, 32 keys at a time, each beside the
+  // products of the next 32 keys' scores, which depend on nothing in it: the matrix cores
+  // run while the exponentials do.  Loads go two tiles ahead for V, three for K.
+  //
+  // Tiles lo .. hi - 1 are seen whole by all of the wave's rows, none of tile `stop` and
+  // later.
+  int lo = i0, hi = blocks.first + (wmin + 1) / TK - blocks.second;
+  if (c.window > 0) lo = max(blocks.first, blocks.first + (max(0, wmax - c.window + 1) + TK - 1) / TK - blocks.second);
+  const int stop = wmax < 0 ? 0 : min(i1, blocks.first + wmax / TK + 1 - blocks.second);
+  f32x16 st;
+  if (i0 < i1) {
+    fill_list(i0);
+    missing = *lds_at<int>(flags);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int b = 0; b < blocks32; ++b) {
-          u32x4 vt;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = 16 * t + 8 * e + trow, d = 32 * b + tcol;
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const auto x = __builtin_bit_cast(
-                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                           vbuf + (buf * kTile + r) * D + 8 * ((d >> 3) ^ fv(r)) + (d & 7))));
-            vt[2 * e] = x[0];
-            vt[2 * e + 1] = x[1];
-          }
-          o[b] = Half<T>::mma32(vt, p[t], o[b]);
-        }
+    for (int x = 0; x < 3; ++x) {
+      if (x < 2 && i0 + x < i1) load_v(x);
+      if (i0 + x < i1) load_k(x);
     }
-    if (i + 1 < i1) arrived(next, next_ok, buf ^ 1);
+    arrived(i0, false);
+    score(0, 0, st);
+  }
+  for (int i = i0; i < i1; ++i) {
+    const int at = i - i0;
+    if (i + 2 < i1) load_v(at + 2);
+    if (i + 3 < i1) {
+      if ((at + 3) * GROUPS % (kGroups / 2) == 0) {
+        fill_list(i + 3);  // over groups that are long done
+        missing = *lds_at<int>(flags);
+      }
+      load_k(at + 3);
+    }
+    if (i < stop) {
+      const bool whole = i >= lo && i < hi && !missing;
+#pragma unroll
+      for (int t = 0; t < TK / 32; ++t) {
+        if (!whole) {
+          const int kb = blocks.at(i) * TK + 32 * t;
+          const uint32_t held = groups_of(at) >> 2 * t;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = 8 * (r >> 2) + 4 * half + (r & 3), j = kb + key;
+            const bool sees = (j <= place) & ((j > from) | (j < c.sinks)) & bool(held >> (key >> 4) & 1);
+            st[r] = sees ? st[r] : kNegInf;
+          }
+        }
+        top_of<blocks32>(st, o, m, l, c.scale);
+        f32x16 after;  // of the last turn: of what LDS holds, unused
+        if (t + 1 < TK / 32)
+          score(at, t + 1, after);
+        else
+          score(at + 1, 0, after);
+        u32x4 p[2];
+        soften<T>(st, p, m, l, c.scale);
+        weigh(at, t, p);
+        st = after;
+      }
+    }
+    if (i + 1 < i1) arrived(i + 1, i + 3 < i1);
   }
   l = sum32(l);
+  m *= c.scale;
 
   if (a.splits == 1) {
     if (!has) return;
@@ -305,7 +393,7 @@ int tiles_of(size_t max_rows, size_t group, size_t dim) {
 template <typename T, int D, int NW>
 hipError_t launch(const PromptArgs& a, hipStream_t s) {
   const int ntile = tiles_of(a.max_rows, a.c.group, a.c.dim);
-  const size_t lds = size_t(4) * kTile * D * sizeof(T);
+  const size_t lds = size_t(2) * kRing * tile_keys<D>() * D * sizeof(T) + 16 * kGroups + kFlags;
   const auto kernel = a.c.dim == D ? paged_prompt_kernel<T, D, NW, true> : paged_prompt_kernel<T, D, NW, false>;
   const unsigned groups = unsigned(ntile) * a.c.seqs * a.c.kv_heads;
   hipLaunchKernelGGL(kernel, dim3(groups * a.splits), dim3(NW * 64), lds, s, a, ntile);
@@ -325,7 +413,7 @@ hipError_t launch_dim(const PromptArgs& a, hipStream_t s) {
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys) {
   const size_t tiles = size_t(tiles_of(max_rows, group, dim)) * seqs * kv_heads;
   if (!tiles || tiles > 128) return 1;
-  return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, keys / (4 * kTile))));
+  return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, keys / 256)));
 }
 size_t prompt_work_floats(int splits, size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows) {
   if (splits <= 1) return 0;

@@ -25,6 +25,10 @@ bool eights(const int64_t* s, int n) {
     if (s[i] % 8) return false;
   return true;
 }
+// strides that the kernels hold in 32 bits: 16 tokens' bytes in one number
+bool words(const int64_t* s) {
+  return s[0] >= 0 && s[0] <= INT_MAX && s[1] >= 0 && s[1] <= INT_MAX && s[2] >= 0 && s[2] < (1 << 26);
+}
 int log2_of(size_t n) { return 63 - __builtin_clzll(n); }
 
 // positions that a row of the tables holds, as the kernels count them (32 bits, and
@@ -38,7 +42,7 @@ int check_cache(const praghip_cache* c) {
   if (c->type != PRAGHIP_BF16 && c->type != PRAGHIP_F16) return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_TYPE");
   if (!power_of_two(c->page_size) || c->page_size < 16 || c->page_size > 32768 || !c->head_dim || c->head_dim % 8 ||
       c->head_dim > 256 || !c->pages || c->pages > INT_MAX || !c->kv_heads || c->kv_heads > 65536 || c->seqs > (1u << 20) ||
-      !c->table_width || c->table_width > INT_MAX)
+      !c->table_width || c->table_width > INT_MAX || !words(c->k_strides) || !words(c->v_strides))
     return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
   if (!aligned16(c->k) || !aligned16(c->v) || !eights(c->k_strides, 3) || !eights(c->v_strides, 3) || !aligned4(c->tables) ||
       !aligned4(c->lengths))
@@ -50,8 +54,8 @@ CacheArgs cache_args(const praghip_cache& c, size_t heads, float scale, size_t w
   CacheArgs a{};
   a.k = c.k;
   a.v = c.v;
-  a.k_page = c.k_strides[0], a.k_head = c.k_strides[1], a.k_token = c.k_strides[2];
-  a.v_page = c.v_strides[0], a.v_head = c.v_strides[1], a.v_token = c.v_strides[2];
+  a.k_page = uint32_t(c.k_strides[0]), a.k_head = uint32_t(c.k_strides[1]), a.k_token = uint32_t(c.k_strides[2]);
+  a.v_page = uint32_t(c.v_strides[0]), a.v_head = uint32_t(c.v_strides[1]), a.v_token = uint32_t(c.v_strides[2]);
   a.tables = c.tables;
   a.table_stride = c.table_stride;
   a.lengths = c.lengths;

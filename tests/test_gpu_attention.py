@@ -270,6 +270,25 @@ def test_scales(gpu, scale):
     plain.check_lse(lse, wlse)
 
 
+def test_prompt_over_a_long_cache(gpu):
+    """More tiles than a workgroup keeps the pages of; few of the rows, by their definition."""
+    say("long cache")
+    n, rows = 70000, 300
+    g = torch.Generator(device="cuda").manual_seed(29)
+    k, v = (torch.randn((n // 16 + 2, 1, 16, 64), generator=g, device="cuda").to(F16) for _ in range(2))
+    tables = torch.randperm(n // 16 + 2, generator=g, device="cuda").to(torch.int32)[None]
+    q = torch.randn((rows, 1, 64), generator=g, device="cuda").to(F16)
+    lengths, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([n], [0, rows]))
+    c = {"k": k.cpu(), "v": v.cpu(), "tables": tables.cpu(), "lengths": lengths.cpu(), "page": 16, "kv": 1}
+    for window, sinks in ((0, 0), (40000, 3)):
+        out = praghip.paged_prompt(q.repeat(1, 32, 1), k, v, tables, lengths, starts, rows, window=window, sinks=sinks)
+        for row in (0, 150, 299):
+            part = dict(c, lengths=torch.tensor([n - rows + row + 1]))
+            want, _, size = plain.attention(part, q[row:row + 1].cpu(), [0, 1], window=window, sinks=sinks)
+            for head in (0, 31):
+                plain.check(out[row:row + 1, head:head + 1], want, size, F16, rounded=True)
+
+
 def test_zero_sequences_and_rows(gpu):
     c = plain.make([20], 4, 2, 64, 16, BF16, seed=24)
     k, v, tables, lengths = to_gpu(c)
