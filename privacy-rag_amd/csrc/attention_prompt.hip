@@ -25,6 +25,8 @@
 // order.
 #include "attention.hpp"
 
+#include <type_traits>
+
 namespace praghip {
 namespace {
 
@@ -53,34 +55,29 @@ __device__ __forceinline__ void dma16(uint64_t base, uint32_t offset, Lds to) {
                : "memory");
 }
 
-// One tile's scores, 16 of 32 keys in st[t] for the lane's query, into P: the running
-// maximum, the sum of P and O's factor.  Within 2^kSlack of it the old maximum stays in
-// use: P may then be up to 2^kSlack, with the same relative rounding, and the dim / 2
-// products with the factor are left out.
-constexpr float kSlack = 8;
-template <int B>
-__device__ __forceinline__ void top_of(const f32x16& st, f32x16 (&o)[B], float& m, float& l, float scale) {
-  float top = m;  // (a maximum that keeps NaN takes its operands as they are)
+// (a maximum that keeps NaN takes its operands as they are, with no instructions to
+// canonicalise them)
+__device__ __forceinline__ float top_of(const f32x16& st) {
+  float top = kNegInf;
 #pragma unroll
   for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, st[r]);
+  return top;
+}
+// The running maximum, and with it l's and O's factor, where the lane's half of the keys
+// has `top`.  Within 2^kSlack of it the old maximum stays in use: P may then be up to
+// 2^kSlack, with the same relative rounding, and the products with the factor are left out.
+constexpr float kSlack = 8;
+template <int B>
+__device__ __forceinline__ void raise(float top, f32x16 (&o)[B], float& m, float& l, float scale) {
   const Two both = swap32(top);
   top = __builtin_elementwise_maximum(both.a, both.b);
   if (__any((top - m) * scale > kSlack)) {
+    top = __builtin_elementwise_maximum(top, m);
     const float f = __builtin_amdgcn_exp2f((m - origin(top)) * scale);
     l *= f;
 #pragma unroll
     for (int b = 0; b < B; ++b) o[b] *= f;
     m = top;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void soften(const f32x16& st, u32x4 (&p)[2], float m, float& l, float scale) {
-  const float base = -origin(m) * scale;
-#pragma unroll
-  for (int r = 0; r < 16; r += 2) {
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(st[r], scale, base)), p1 = __builtin_amdgcn_exp2f(fmaf(st[r + 1], scale, base));
-    l += p0 + p1;
-    p[r >> 3][(r & 7) >> 1] = pack2<T>(p0, p1);
   }
 }
 
@@ -139,6 +136,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   // tiles come by DMA, 1 KiB an instruction: RPI rows, whose page is one, and 16 bytes
   // a lane, which takes the chunk that belongs at its place
   constexpr int RPI = 64 / CPR, PER = TK / RPI / NW, GROUPS = TK / 16, TURNS = 64 / GROUPS;
+  constexpr int AHEAD = TK == 64 ? 3 : 4;  // tiles that K's loads go ahead (the keys of 64 after a turn's are read in it)
   const auto fk = [](int r) { return D == 64 ? (r >> 1) & 7 : r & 15; };
   const auto fv = [](int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; };
   const int width = int(c.capacity >> c.page_shift), inrow = lane / CPR;
@@ -172,7 +170,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   const auto lane_of = [](uint32_t lo, uint32_t hi, int x) {
     return uint64_t(uint32_t(__builtin_amdgcn_readlane(hi, x))) << 32 | uint32_t(__builtin_amdgcn_readlane(lo, x));
   };
-  const auto load_k = [&](int at) {  // `at` counts the tiles from i0
+  const auto load_k = [&](int at, int slot) {  // `at` counts the tiles from i0
     if (at % TURNS == 0) {
       const u32x2 x = *lds_at<u32x2>(list + 16 * (at * GROUPS % kGroups + lane));
       klow = x[0], khigh = x[1];
@@ -181,10 +179,10 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     for (int n = 0; n < PER; ++n) {
       const int r0 = RPI * (wave + NW * n);
       if (EXACT || 8 * ((lane % CPR) ^ fk(r0 + inrow)) < c.dim)
-        dma16(lane_of(klow, khigh, at % TURNS * GROUPS + (r0 >> 4)), koff[n], kbuf + at % kRing * TILE + r0 * ROW);
+        dma16(lane_of(klow, khigh, at % TURNS * GROUPS + (r0 >> 4)), koff[n], kbuf + slot * TILE + r0 * ROW);
     }
   };
-  const auto load_v = [&](int at) {
+  const auto load_v = [&](int at, int slot) {
     if (at % TURNS == 0) {
       const u32x2 x = *lds_at<u32x2>(list + 16 * (at * GROUPS % kGroups + lane) + 8);
       vlow = x[0], vhigh = x[1] & 0x7fffffffu;
@@ -193,7 +191,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     for (int n = 0; n < PER; ++n) {
       const int r0 = RPI * (wave + NW * n);
       if (EXACT || 8 * ((lane % CPR) ^ fv(r0 + inrow)) < c.dim)
-        dma16(lane_of(vlow, vhigh, at % TURNS * GROUPS + (r0 >> 4)), voff[n], vbuf + at % kRing * TILE + r0 * ROW);
+        dma16(lane_of(vlow, vhigh, at % TURNS * GROUPS + (r0 >> 4)), voff[n], vbuf + slot * TILE + r0 * ROW);
     }
   };
   // which groups of 16 keys of a tile have a page
@@ -229,33 +227,17 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   if (threadIdx.x == 0) *lds_at<int>(flags) = 0;
   __syncthreads();
 
-  // S^T = K Q^T of keys 32 t .. of a tile
-  const auto score = [&](int at, int t, f32x16& st) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) st[r] = 0;
-#pragma unroll
-    for (int n = 0; n < steps; ++n)
-      st = Half<T>::mma32(*lds_at<u32x4>(kbuf + at % kRing * TILE + (32 * t + col) * ROW + 16 * ((2 * n + half) ^ fk(col))), q[n], st);
+  // Fragments of 32 keys: of K, rows for S^T = K Q^T, and of V, by transposed reads for
+  // O^T = V^T P^T.  `slot` and t are constants, and so all but a few addresses.
+  const auto read_k = [&](int slot, int t, int n) {
+    return *lds_at<u32x4>(kbuf + slot * TILE + (32 * t + col) * ROW + 16 * ((2 * n + half) ^ fk(col)));
   };
-  // O^T += V^T P^T of the same keys
   const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  const auto weigh = [&](int at, int t, const u32x4 (&p)[2]) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int b = 0; b < blocks32; ++b) {
-        u32x4 vt;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 32 * t + 16 * n + 8 * e + trow, d = 32 * b + tcol;
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          const auto x = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(vbuf + at % kRing * TILE + r * ROW + 16 * ((d >> 3) ^ fv(trow)) + 2 * (d & 7))));
-          vt[2 * e] = x[0];
-          vt[2 * e + 1] = x[1];
-        }
-        o[b] = Half<T>::mma32(vt, p[n], o[b]);
-      }
+  const auto read_v = [&](int slot, int t, int n, int b, int e) {
+    const int r = 32 * t + 16 * n + 8 * e + trow, d = 32 * b + tcol;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(
+                                         vbuf + slot * TILE + r * ROW + 16 * ((d >> 3) ^ fv(trow)) + 2 * (d & 7))));
   };
 
   // Turn i takes tile i through the softmax and into O, 32 keys at a time, each beside the
@@ -267,27 +249,38 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   int lo = i0, hi = blocks.first + (wmin + 1) / TK - blocks.second;
   if (c.window > 0) lo = max(blocks.first, blocks.first + (max(0, wmax - c.window + 1) + TK - 1) / TK - blocks.second);
   const int stop = wmax < 0 ? 0 : min(i1, blocks.first + wmax / TK + 1 - blocks.second);
-  f32x16 st;
+  f32x16 st;           // a turn's first scores,
+  float top = kNegInf;  // their maximum before masks,
+  u32x4 kf[steps];      // and the next keys
   if (i0 < i1) {
     fill_list(i0);
     missing = *lds_at<int>(flags);
 #pragma unroll
-    for (int x = 0; x < 3; ++x) {
-      if (x < 2 && i0 + x < i1) load_v(x);
-      if (i0 + x < i1) load_k(x);
+    for (int x = 0; x < AHEAD; ++x) {
+      if (x < 2 && i0 + x < i1) load_v(x, x);
+      if (i0 + x < i1) load_k(x, x);
     }
     arrived(i0, false);
-    score(0, 0, st);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = 0;
+#pragma unroll
+    for (int n = 0; n < steps; ++n) st = Half<T>::mma32(read_k(0, 0, n), q[n], st);
+#pragma unroll
+    for (int n = 0; n < steps; ++n) kf[n] = read_k(TK == 64 ? 0 : 1, TK == 64 ? 1 : 0, n);
+    top = top_of(st);
   }
-  for (int i = i0; i < i1; ++i) {
+  const auto turn = [&](int i, auto slot_constant) {
+    constexpr int slot = decltype(slot_constant)::value;  // of tile i
     const int at = i - i0;
-    if (i + 2 < i1) load_v(at + 2);
-    if (i + 3 < i1) {
-      if ((at + 3) * GROUPS % (kGroups / 2) == 0) {
-        fill_list(i + 3);  // over groups that are long done
-        missing = *lds_at<int>(flags);
-      }
-      load_k(at + 3);
+    const auto more_v = [&] {
+      if (i + 2 < i1) load_v(at + 2, (slot + 2) % kRing);
+    };
+    const auto more_k = [&] {
+      if (i + AHEAD < i1) load_k(at + AHEAD, (slot + AHEAD) % kRing);
+    };
+    if (i + AHEAD < i1 && (at + AHEAD) * GROUPS % (kGroups / 2) == 0) {
+      fill_list(i + AHEAD);  // over groups that are long done
+      missing = *lds_at<int>(flags);
     }
     if (i < stop) {
       const bool whole = i >= lo && i < hi && !missing;
@@ -302,20 +295,64 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
             const bool sees = (j <= place) & ((j > from) | (j < c.sinks)) & bool(held >> (key >> 4) & 1);
             st[r] = sees ? st[r] : kNegInf;
           }
+          top = top_of(st);
         }
-        top_of<blocks32>(st, o, m, l, c.scale);
-        f32x16 after;  // of the last turn: of what LDS holds, unused
-        if (t + 1 < TK / 32)
-          score(at, t + 1, after);
-        else
-          score(at + 1, 0, after);
-        u32x4 p[2];
-        soften<T>(st, p, m, l, c.scale);
-        weigh(at, t, p);
+        raise<blocks32>(top, o, m, l, c.scale);
+        // What follows runs as it stands, each product with what fills its time: the next
+        // scores' with exponentials of these, reads of V and the loads; O's with the next
+        // scores' maximum and reads of the keys after them.  (The last turn's next keys are
+        // what LDS holds, and their scores unused.)
+        f32x16 after;
+        u32x4 p[2], vf[2][blocks32];
+        const float base = -origin(m) * c.scale;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) after[r] = 0;
+#pragma unroll
+        for (int n = 0; n < steps; ++n) {
+          after = Half<T>::mma32(kf[n], q[n], after);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const u32x2 x = read_v(slot, t, n / blocks32, n % blocks32, e);
+            vf[n / blocks32][n % blocks32][2 * e] = x[0];
+            vf[n / blocks32][n % blocks32][2 * e + 1] = x[1];
+          }
+#pragma unroll
+          for (int r = 16 * n / steps & ~1; r + 1 < 16 * (n + 1) / steps; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[r], c.scale, base)), p1 = __builtin_amdgcn_exp2f(fmaf(st[r + 1], c.scale, base));
+            l += p0 + p1;
+            p[r >> 3][(r & 7) >> 1] = pack2<T>(p0, p1);
+          }
+          if (t == 0 && n == 0) more_v();
+          if (t == 0 && n == steps / 2) more_k();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        top = kNegInf;
+#pragma unroll
+        for (int n = 0; n < 2 * blocks32; ++n) {
+          o[n % blocks32] = Half<T>::mma32(vf[n / blocks32][n % blocks32], p[n / blocks32], o[n % blocks32]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (TK == 64)
+            kf[n] = t == 0 ? read_k((slot + 1) % kRing, 0, n) : read_k((slot + 1) % kRing, 1, n);
+          else
+            kf[n] = read_k((slot + 2) % kRing, 0, n);
+#pragma unroll
+          for (int r = 8 * n / blocks32; r < 8 * (n + 1) / blocks32; ++r) top = __builtin_elementwise_maximum(top, after[r]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         st = after;
       }
+    } else {
+      more_v();
+      more_k();
     }
-    if (i + 1 < i1) arrived(i + 1, i + 3 < i1);
+    if (i + 1 < i1) arrived(i + 1, i + AHEAD < i1);
+  };
+  for (int i = i0; i < i1; i += kRing) {
+    turn(i, std::integral_constant<int, 0>{});
+    if (i + 1 < i1) turn(i + 1, std::integral_constant<int, 1>{});
+    if (i + 2 < i1) turn(i + 2, std::integral_constant<int, 2>{});
+    if (i + 3 < i1) turn(i + 3, std::integral_constant<int, 3>{});
   }
   l = sum32(l);
   m *= c.scale;
