@@ -87,7 +87,59 @@ __device__ __forceinline__ u32x4 load_w(const uint8_t* row, int at, int width) {
   return w;
 }
 
-// MT tiles of 16 rows of x, NT tiles of 16 columns a wave, KW waves along K
+// The sums of the waves along K, in order, and y's values.
+template <typename T, int MT, int NT>
+__device__ __forceinline__ void finish_rows(const MatvecArgs& a, f32x4 (&y)[NT][MT], float* sums, int kw, int part, int wave,
+                                            int lane, int tile, int m0) {
+  const int col = lane & 15, quad = lane >> 4;
+  if (kw > 1) {
+    float* mine = sums + wave * NT * MT * 256 + lane * 4;
+    if (part) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(mine + (t * MT + i) * 256) = y[t][i];
+    }
+    __syncthreads();
+    if (part) return;
+    for (int p = 1; p < kw; ++p)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) y[t][i] += *reinterpret_cast<const f32x4*>(mine + (p * NT * MT + t * MT + i) * 256);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = (tile + t) * 16 + col;
+    if (n >= a.n) continue;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + 16 * i + 4 * quad + r;
+        if (m < a.m) static_cast<T*>(a.y)[m * a.y_stride + n] = T(y[t][i][r]);
+      }
+  }
+}
+
+// the words of the four lanes of a column, turned: word s of quad g is word g of quad s
+__device__ __forceinline__ u32x4 turned(u32x4 w) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(w[i], w[i + 2], false, false);
+    w[i] = r[0];
+    w[i + 2] = r[1];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(w[i], w[i + 1], false, false);
+    w[i] = r[0];
+    w[i + 1] = r[1];
+  }
+  return w;
+}
+
+// MT tiles of 16 rows of x, NT tiles of 16 columns a wave, kw waves along K: any group
 template <typename T, int MT, int NT, bool ALIGNED, bool ZEROS>
 __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
   extern __shared__ float sums[];
@@ -146,20 +198,7 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) w[t] = load_w<ALIGNED>(row[t], kb / 2 + 16 * quad, a.width);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {  // the words of four lanes of a column, turned
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const auto r = __builtin_amdgcn_permlane32_swap(w[t][i], w[t][i + 2], false, false);
-          w[t][i] = r[0];
-          w[t][i + 2] = r[1];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const auto r = __builtin_amdgcn_permlane16_swap(w[t][i], w[t][i + 1], false, false);
-          w[t][i] = r[0];
-          w[t][i + 1] = r[1];
-        }
-      }
+      for (int t = 0; t < NT; ++t) w[t] = turned(w[t]);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const int k = kb + 32 * st;
@@ -181,53 +220,169 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
     }
     if (kw == 1) finish((a.k - 1) / a.group);
   }
-  if (kw > 1) {
-    float* mine = sums + wave * NT * MT * 256 + lane * 4;
-    if (part) {
+  finish_rows<T, MT, NT>(a, y, sums, kw, part, wave, lane, tile, m0);
+}
+
+// For groups of 32 S, S = 1, 2 or 4, many columns and whole turns.  A turn is eight groups, 2 S blocks
+// of 128: their weights are under way together (a row's bytes one after the other: with
+// one block at a time all waves of the chip asked for the same 64 of every K / 2 bytes, and
+// so of the same memory channels), and their scales and zero points come as one load of 16
+// and of 8 bytes a column (a load for each of them took more of the memory path than the
+// weights).  x stands in LDS, `part` values of k at a time, in the order that the weights pair
+// up in.  A workgroup stays
+// and takes tiles of columns in turn, and the next turn's weights are under way beside a
+// turn's products (no load stands behind a condition: at the join the compiler would wait
+// for it).
+template <typename T, int NT, int S>
+struct Turn {
+  u32x4 w[2 * S][NT], sc[NT];
+  u32x2 zc[NT];
+};
+template <typename T, int MT, int NT, int S, bool ZEROS>
+__global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int part) {
+  constexpr int kTurn = 256 * S;
+  extern __shared__ float lds[];
+  uint16_t* const xs = reinterpret_cast<uint16_t*>(lds);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4, row_step = part + 8;  // a row in LDS: 16 bytes more than its data
+  const int m0 = blockIdx.y * 16 * MT, turns = a.k / kTurn;
+  const int sets = (a.n + 64 * NT - 1) / (64 * NT);  // of a workgroup's tiles
+
+  const auto load = [&](Turn<T, NT, S>& u, int set, int turn) {
+    const int k0 = turn * kTurn, g0 = 8 * turn;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      const int n = min(((set * 4 + wave) * NT + t) * 16 + col, a.n - 1);
+      const uint8_t* const row = a.w + n * a.w_stride + 16 * quad + k0 / 2;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(mine + (t * MT + i) * 256) = y[t][i];
+      for (int b = 0; b < 2 * S; ++b) u.w[b][t] = *reinterpret_cast<const u32x4*>(row + 64 * b);
+      u.sc[t] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.scales) + n * a.scale_stride + g0);
+      if (ZEROS) u.zc[t] = *reinterpret_cast<const u32x2*>(a.zeros + n * a.zero_stride + g0);
+    }
+  };
+  const auto stage = [&](int from) {
+    const int chunks = part / 8;
+    for (int c = threadIdx.x; c < 16 * MT * chunks; c += 256) {
+      const int r = c / chunks, k = (c - r * chunks) * 8;
+      const bool has = m0 + r < a.m;
+      *reinterpret_cast<u32x4*>(xs + r * row_step + k) =
+          load_x<T, true>(static_cast<const T*>(a.x) + (has ? m0 + r : 0) * a.x_stride, has, from + k, a.k);
     }
     __syncthreads();
-    if (part) return;
-    for (int p = 1; p < kw; ++p)
+  };
+  f32x4 y[NT][MT];
+  const u32x4 one = {Nibble<T>::one, Nibble<T>::one, Nibble<T>::one, Nibble<T>::one};
+  const auto multiply = [&](const Turn<T, NT, S>& u, int at) {  // `at`: the turn's place in LDS
+    f32x4 acc[NT][MT], ones[MT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int b = 0; b < 2 * S; ++b) {
+      u32x4 v[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) y[t][i] += *reinterpret_cast<const f32x4*>(mine + (p * NT * MT + t * MT + i) * 256);
-  }
+      for (int t = 0; t < NT; ++t) v[t] = turned(u.w[b][t]);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int n = (tile + t) * 16 + col;
-    if (n >= a.n) continue;
+      for (int st = 0; st < 4; ++st) {
+        const bool first = (4 * b + st) % S == 0;
+        const f32x4 none = {0, 0, 0, 0};
+        u32x4 xf[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i) {
+          xf[i] = *reinterpret_cast<const u32x4*>(xs + (16 * i + col) * row_step + at + kBlockK * b + 32 * st + 8 * quad);
+          ones[i] = Half<T>::mma16(xf[i], one, first ? none : ones[i]);
+        }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = m0 + 16 * i + 4 * quad + r;
-        if (m < a.m) static_cast<T*>(a.y)[m * a.y_stride + n] = T(y[t][i][r]);
+        for (int t = 0; t < NT; ++t) {
+          const u32x4 wf = widen<T>(v[t][st]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[t][i] = Half<T>::mma16(xf[i], wf, first ? none : acc[t][i]);
+        }
+        if ((4 * b + st + 1) % S == 0) {
+          const int g = (4 * b + st) / S;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float s = g & 1 ? high<T>(u.sc[t][g / 2]) : low<T>(u.sc[t][g / 2]);
+            const float c = 16.f + (ZEROS ? float(u.zc[t][g / 4] >> (8 * (g & 3)) & 255) : 8.f);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) y[t][i][r] += s * (acc[t][i][r] - c * ones[i][r]);
+          }
+        }
       }
+    }
+  };
+  const auto clear = [&] {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) y[t][i] = f32x4{0, 0, 0, 0};
+  };
+
+  Turn<T, NT, S> u[2];
+  clear();
+  int set = blockIdx.x, turn = 0, staged = -1;
+  load(u[0], set, 0);
+  while (set < sets) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      int next = turn + 1, next_set = set;
+      if (next == turns) next = 0, next_set += gridDim.x;
+      load(u[b ^ 1], min(next_set, sets - 1), next);
+      const int from = turn * kTurn / part * part;
+      if (from != staged) {
+        if (staged >= 0) __syncthreads();  // the part before has been read
+        stage(from);
+        staged = from;
+      }
+      multiply(u[b], turn * kTurn - from);
+      if (next == 0) {
+        finish_rows<T, MT, NT>(a, y, nullptr, 1, 0, wave, lane, (set * 4 + wave) * NT, m0);
+        clear();
+        if (next_set >= sets) return;
+      }
+      turn = next, set = next_set;
+    }
   }
 }
 
-template <typename T, int MT, int NT>
+template <typename T, int MT, int NT, int S>
+hipError_t launch_groups(const MatvecArgs& a, hipStream_t s) {
+  const auto kernel = a.zeros ? matvec_w4_groups_kernel<T, MT, NT, S, true> : matvec_w4_groups_kernel<T, MT, NT, S, false>;
+  // x in LDS as a whole up to 64 KiB, two workgroups of a CU; three where there is room for four
+  // (155,648 columns of K = 1024 and one row: 20.9 us, four 22.8)
+  const int whole = a.k, part = MT * whole <= 2048 ? whole : 2048 / MT;
+  const unsigned sets = unsigned((a.n + 64 * NT - 1) / (64 * NT)), most = MT * whole <= 1024 ? 768 : 512;
+  hipLaunchKernelGGL(kernel, dim3(std::min(sets, most), (a.m + 16 * MT - 1) / (16 * MT)), dim3(256),
+                     size_t(16) * MT * (part + 8) * 2, s, a, part);
+  return hipGetLastError();
+}
+template <typename T, int S>
+hipError_t launch_groups(const MatvecArgs& a, hipStream_t s) {
+  return a.m <= 16 ? launch_groups<T, 1, 1, S>(a, s) : launch_groups<T, 2, 1, S>(a, s);
+}
+
+template <typename T, int MT>
 hipError_t launch(const MatvecArgs& a, int kw, hipStream_t s) {
   const bool z = a.zeros != nullptr;
-  const auto kernel = a.aligned ? (z ? matvec_w4_kernel<T, MT, NT, true, true> : matvec_w4_kernel<T, MT, NT, true, false>)
-                                : (z ? matvec_w4_kernel<T, MT, NT, false, true> : matvec_w4_kernel<T, MT, NT, false, false>);
-  const unsigned tiles = unsigned((a.n + 16 * NT - 1) / (16 * NT)), per = 4 / kw;
+  const auto kernel = a.aligned ? (z ? matvec_w4_kernel<T, MT, 1, true, true> : matvec_w4_kernel<T, MT, 1, true, false>)
+                                : (z ? matvec_w4_kernel<T, MT, 1, false, true> : matvec_w4_kernel<T, MT, 1, false, false>);
+  const unsigned tiles = unsigned((a.n + 15) / 16), per = 4 / kw;
   hipLaunchKernelGGL(kernel, dim3((tiles + per - 1) / per, (a.m + 16 * MT - 1) / (16 * MT)), dim3(256),
-                     kw > 1 ? 4 * NT * MT * 256 * sizeof(float) : 0, s, a, kw);
+                     kw > 1 ? 4 * MT * 256 * sizeof(float) : 0, s, a, kw);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch_type(const MatvecArgs& a, hipStream_t s) {
-  const int tiles = (a.n + 15) / 16, blocks = (a.k + kBlockK - 1) / kBlockK;
-  if (tiles >= 4096) return a.m <= 16 ? launch<T, 1, 4>(a, 1, s) : launch<T, 2, 4>(a, 1, s);
+  const int blocks = (a.k + kBlockK - 1) / kBlockK;
+  // where there are columns enough for a wave of each SIMD: its turn of eight groups is a
+  // long piece of K
+  if (a.aligned && a.vector_scales && a.n >= 16384 && a.k % (8 * a.group) == 0) {
+    if (a.group == 32) return launch_groups<T, 1>(a, s);
+    if (a.group == 64) return launch_groups<T, 2>(a, s);
+    if (a.group == 128) return launch_groups<T, 4>(a, s);
+  }
   const int kw = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
-  return a.m <= 16 ? launch<T, 1, 1>(a, kw, s) : launch<T, 2, 1>(a, kw, s);
+  return a.m <= 16 ? launch<T, 1>(a, kw, s) : launch<T, 2>(a, kw, s);
 }
 
 }  // namespace

@@ -18,7 +18,8 @@ struct MatvecArgs {
   void* y;  // [m][n]
   int64_t y_stride;
   int m, k, n, group, width;
-  bool aligned;  // 16-byte loads of x and w stay within their rows
+  bool aligned;        // 16-byte loads of x and w stay within their rows
+  bool vector_scales;  // eight scales, and eight zero points, are one aligned load
 };
 
 hipError_t launch_matvec_w4(const MatvecArgs& a, int type, hipStream_t s);

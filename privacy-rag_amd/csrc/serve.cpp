@@ -314,6 +314,8 @@ int praghip_matvec_w4(int device, const praghip_w4* w, const void* x, int64_t x_
   a.y = y, a.y_stride = y_stride;
   a.m = int(m), a.k = int(w->k), a.n = int(w->n), a.group = int(w->group), a.width = int(w->width);
   a.aligned = aligned16(x) && x_stride % 8 == 0 && aligned16(w->w) && w->w_stride % 16 == 0 && w->width % 16 == 0;
+  a.vector_scales = aligned16(w->scales) && w->scale_stride % 8 == 0 &&
+                    (!w->zeros || ((reinterpret_cast<uintptr_t>(w->zeros) & 7) == 0 && w->zero_stride % 8 == 0));
   DeviceScope scope(device);
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_matvec_w4(a, w->type, pick(stream));

@@ -47,6 +47,11 @@ SIZES = [
     (17, 1000, 100, 96, True, BF16), (5, 535, 521, 32, True, F16), (33, 257, 48, 256, False, BF16),
     (64, 2048, 33, 64, True, BF16), (70, 4097, 40, 1024, False, F16), (8, 130, 31, 160, True, BF16),
     (16, 256, 65600, 64, True, F16), (20, 96, 65700, 32, False, BF16), (4, 8192, 50, 128, True, F16),
+    (1, 8192, 4099, 128, True, BF16), (7, 4096, 2050, 64, False, F16), (18, 2048, 2100, 32, True, BF16),
+    # many columns: whole turns of eight groups, in LDS as a whole or in parts, and others
+    (1, 1024, 16400, 128, False, BF16), (16, 512, 16385, 64, True, F16), (18, 768, 16390, 32, True, BF16),
+    (40, 4096, 16384, 128, True, F16), (3, 8192, 16400, 128, False, BF16), (17, 3072, 65540, 64, False, F16),
+    (2, 256, 70001, 32, True, BF16), (33, 1184, 16400, 32, True, F16), (2, 1600, 65600, 64, False, BF16),
 ]
 
 
