@@ -7,89 +7,85 @@ are asynchronous on ``stream`` (the tensors' device's current stream by default)
 """
 from __future__ import annotations
 
-import ctypes
-import functools
+import struct
 
-from ._lib import E_ARGUMENT, Cache, PraghipError, check, lib, shape_error
+from ._lib import E_ARGUMENT, PraghipError, check, lib, shape_error
+
+# A call's checks and packing are a few microseconds, as long as a small kernel: they
+# read each attribute of a tensor once, and structures go to the library as packed bytes.
+_torch = _int32 = _uint8 = _current = None
+_kinds: dict = {}                     # torch dtype -> type code
+_CACHE = struct.Struct("2P6q4Qi4xPqQPQ")  # praghip_cache
+_two = struct.Struct("2q").pack
 
 
-@functools.lru_cache(maxsize=None)
-def _types():
+def _load():
+    global _torch, _int32, _uint8, _current
     import torch
-    return {torch.bfloat16: 0, torch.float16: 1}
-
-
-@functools.lru_cache(maxsize=None)
-def _torch():
-    import torch
-    return torch
-
-
-@functools.lru_cache(maxsize=None)
-def _raw_stream():
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _torch, _int32, _uint8 = torch, torch.int32, torch.uint8
+    _kinds.update({torch.bfloat16: 0, torch.float16: 1})
+    _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _stream(index: int, stream):
     """hipStream_t of a call on device `index`: the given stream, or the device's current one."""
-    return (_raw_stream()(index) if stream is None else stream.cuda_stream) or None
+    if _current is None:
+        _load()
+    return (_current(index) if stream is None else stream.cuda_stream) or None
 
 
 def _type_error(text: str) -> PraghipError:
     return PraghipError(E_ARGUMENT, text)
 
 
-def _ints(t, shape, index: int):
-    """Address of an int32 tensor of this shape (None: any size) with contiguous rows."""
-    if t.dtype is not _torch().int32 or t.get_device() != index:
+def _kind(t, text: str) -> int:
+    code = _kinds.get(t.dtype)
+    if code is None:
+        _load()
+        code = _kinds.get(t.dtype)
+        if code is None:
+            raise _type_error(text)
+    return code
+
+
+def _cache(k, v, tables, lengths, like, kind: int, index: int):
+    """(praghip_cache as bytes, pages' shape, sequences) of one layer's pages, tables and lengths."""
+    if not k.get_device() == v.get_device() == index >= 0:
+        raise _type_error("E_ATTENTION_DEVICE")
+    if not k.dtype is v.dtype is like.dtype:
+        raise _type_error("E_ATTENTION_TYPE")
+    if not tables.dtype is lengths.dtype is _int32 or not tables.get_device() == lengths.get_device() == index:
         raise _type_error("E_ATTENTION_INTS")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) or \
-            (t.shape[-1] > 1 and t.stride(-1) != 1):
+    shape, held, named = k.shape, lengths.shape, tables.shape
+    ks, vs, ts = k.stride(), v.stride(), tables.stride()
+    if len(shape) != 4 or v.shape != shape or ks[3] != 1 or vs[3] != 1 or len(held) != 1 or len(named) != 2 or \
+            named[0] != held[0] or (ts[1] != 1 and named[1] > 1) or (held[0] > 1 and lengths.stride(0) != 1):
+        raise shape_error("E_ATTENTION_SHAPE")
+    return _CACHE.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], *shape, kind,
+                       tables.data_ptr(), ts[0], named[1], lengths.data_ptr(), held[0]), shape, held[0]
+
+
+def _starts(t, seqs: int, index: int) -> int:
+    if t.dtype is not _int32 or t.get_device() != index:
+        raise _type_error("E_ATTENTION_INTS")
+    if t.shape != (seqs + 1,) or (seqs and t.stride(0) != 1):
         raise shape_error("E_ATTENTION_SHAPE")
     return t.data_ptr()
 
 
-def _cache(k, v, tables, lengths, type_of, index: int) -> Cache:
-    if k.get_device() != index or v.get_device() != index or index < 0:
-        raise _type_error("E_ATTENTION_DEVICE")
-    if k.dtype is not type_of or v.dtype is not type_of:
-        raise _type_error("E_ATTENTION_TYPE")
-    pages, kv, size, dim = k.shape
-    ks, vs = k.stride(), v.stride()
-    if v.shape != k.shape or ks[3] != 1 or vs[3] != 1:
-        raise shape_error("E_ATTENTION_SHAPE")
-    seqs = lengths.shape[0]
-    at = _ints(tables, (seqs, None), index)
-    held = _ints(lengths, (seqs,), index)
-    return Cache(k.data_ptr(), v.data_ptr(), ks[:3], vs[:3], pages, kv, size, dim, _types()[type_of], at,
-                 tables.stride(0), tables.shape[1], held, seqs)
-
-
-def _outputs(q, out, lse):
-    torch = _torch()
+def _output(q, shape, out, index: int):
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != q.get_device() or \
-            (out.shape[2] > 1 and out.stride(2) != 1):
+        return _torch.empty_like(q)
+    if out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or \
+            (shape[2] > 1 and out.stride(2) != 1):
         raise shape_error("E_ATTENTION_OUT")
-    return out, torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if lse else None
+    return out
 
 
-def _queries(q):
-    if q.dtype not in _types():
-        raise _type_error("E_ATTENTION_TYPE")
-    if q.dim() != 3 or (q.shape[2] > 1 and q.stride(2) != 1):
-        raise shape_error("E_ATTENTION_SHAPE")
-
-
-_Two = ctypes.c_int64 * 2
-
-
-def _work(size: int, q, stream):
+def _work(size: int, like, stream):
     """Workspace of one call; torch's allocator keeps it until `stream` is done with it."""
-    work = _torch().empty(size, dtype=_torch().uint8, device=q.device)
+    work = _torch.empty(size, dtype=_uint8, device=like.device)
     if stream is not None:
         work.record_stream(stream)
     return work
@@ -112,21 +108,20 @@ def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = 
     logarithm of each softmax's sum, float32 [seqs][heads]; a sequence that sees
     nothing gets zeros and -inf.
     """
-    _queries(q)
-    index = q.get_device()
-    cache = _cache(k_pages, v_pages, tables, lengths, q.dtype, index)
-    seqs, heads, dim = q.shape
-    if cache.seqs != seqs or cache.head_dim != dim or not cache.kv_heads or heads % cache.kv_heads or window < 0 or \
-            sinks < 0 or max_length < 0:
+    kind, index, shape, qs = _kind(q, "E_ATTENTION_TYPE"), q.get_device(), q.shape, q.stride()
+    cache, pages, seqs = _cache(k_pages, v_pages, tables, lengths, q, kind, index)
+    if len(shape) != 3 or shape[0] != seqs or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
+            shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0:
         raise shape_error("E_ATTENTION_SHAPE")
-    out, sums = _outputs(q, out, lse)
+    out = _output(q, shape, out, index)
+    sums = _torch.empty(shape[:2], dtype=_torch.float32, device=q.device) if lse else None
     if seqs:
-        L, c = lib(), ctypes.byref(cache)
-        size = L.praghip_paged_decode_workspace(c, heads, max_length)
+        L, heads, to = lib(), shape[1], out.stride()
+        size = L.praghip_paged_decode_workspace(cache, heads, max_length)
         work = _work(size, q, stream)
-        check(L.praghip_paged_decode(index, c, q.data_ptr(), _Two(q.stride(0), q.stride(1)), heads, out.data_ptr(),
-                                     _Two(out.stride(0), out.stride(1)), sums.data_ptr() if lse else None,
-                                     dim ** -0.5 if scale is None else scale, window, sinks, max_length,
+        check(L.praghip_paged_decode(index, cache, q.data_ptr(), _two(qs[0], qs[1]), heads, out.data_ptr(),
+                                     _two(to[0], to[1]), sums.data_ptr() if lse else None,
+                                     shape[2] ** -0.5 if scale is None else scale, window, sinks, max_length,
                                      work.data_ptr(), size, _stream(index, stream)))
     return (out, sums) if lse else out
 
@@ -142,25 +137,24 @@ def paged_prompt(q, k_pages, v_pages, tables, lengths, starts, max_rows: int, *,
     sees key j where j <= p and, with a window, j > p - window or j < sinks.  The rest
     is as in :func:`paged_decode`.
     """
-    _queries(q)
-    index = q.get_device()
-    cache = _cache(k_pages, v_pages, tables, lengths, q.dtype, index)
-    tokens, heads, dim = q.shape
-    if cache.head_dim != dim or not cache.kv_heads or heads % cache.kv_heads or window < 0 or sinks < 0 or \
-            max_length < 0 or max_rows < 0:
+    kind, index, shape, qs = _kind(q, "E_ATTENTION_TYPE"), q.get_device(), q.shape, q.stride()
+    cache, pages, seqs = _cache(k_pages, v_pages, tables, lengths, q, kind, index)
+    if len(shape) != 3 or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
+            shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0 or max_rows < 0:
         raise shape_error("E_ATTENTION_SHAPE")
-    first = _ints(starts, (cache.seqs + 1,), index)
-    out, sums = _outputs(q, out, lse)
-    if tokens and cache.seqs:
-        L, c = lib(), ctypes.byref(cache)
+    first = _starts(starts, seqs, index)
+    out = _output(q, shape, out, index)
+    sums = _torch.empty(shape[:2], dtype=_torch.float32, device=q.device) if lse else None
+    tokens, heads = shape[0], shape[1]
+    if tokens and seqs:
+        L, to = lib(), out.stride()
         max_rows = min(max_rows, tokens)
-        size = L.praghip_paged_prompt_workspace(c, heads, max_rows, window, sinks, max_length)
+        size = L.praghip_paged_prompt_workspace(cache, heads, max_rows, window, sinks, max_length)
         work = _work(size, q, stream) if size else None
-        check(L.praghip_paged_prompt(index, c, q.data_ptr(), _Two(q.stride(0), q.stride(1)), heads, first, tokens,
-                                     max_rows, out.data_ptr(), _Two(out.stride(0), out.stride(1)),
-                                     sums.data_ptr() if lse else None, dim ** -0.5 if scale is None else scale, window,
-                                     sinks, max_length, work.data_ptr() if size else None, size,
-                                     _stream(index, stream)))
+        check(L.praghip_paged_prompt(index, cache, q.data_ptr(), _two(qs[0], qs[1]), heads, first, tokens, max_rows,
+                                     out.data_ptr(), _two(to[0], to[1]), sums.data_ptr() if lse else None,
+                                     shape[2] ** -0.5 if scale is None else scale, window, sinks, max_length,
+                                     work.data_ptr() if size else None, size, _stream(index, stream)))
     return (out, sums) if lse else out
 
 
@@ -171,16 +165,12 @@ def page_write(k, v, k_pages, v_pages, tables, lengths, starts, stream=None) -> 
     tokens of sequence s, the last at position lengths[s] - 1 (so the lengths, and the
     pages, are those after :func:`page_reserve`).  Tokens without a page are dropped.
     """
-    if k.dtype not in _types():
-        raise _type_error("E_ATTENTION_TYPE")
-    index = k.get_device()
-    cache = _cache(k_pages, v_pages, tables, lengths, k.dtype, index)
-    if k.dim() != 3 or v.shape != k.shape or k.shape[1] != cache.kv_heads or k.shape[2] != cache.head_dim or \
-            k.stride(2) != 1 or v.stride(2) != 1:
-        raise shape_error("E_ATTENTION_SHAPE")
+    kind, index, shape = _kind(k, "E_ATTENTION_TYPE"), k.get_device(), k.shape
+    cache, pages, seqs = _cache(k_pages, v_pages, tables, lengths, k, kind, index)
     if v.dtype is not k.dtype or v.get_device() != index:
         raise _type_error("E_ATTENTION_TYPE")
-    first = _ints(starts, (cache.seqs + 1,), index)
-    check(lib().praghip_page_write(index, ctypes.byref(cache), k.data_ptr(), _Two(k.stride(0), k.stride(1)),
-                                   v.data_ptr(), _Two(v.stride(0), v.stride(1)), first, k.shape[0],
-                                   _stream(index, stream)))
+    ks, vs = k.stride(), v.stride()
+    if len(shape) != 3 or v.shape != shape or shape[1] != pages[1] or shape[2] != pages[3] or ks[2] != 1 or vs[2] != 1:
+        raise shape_error("E_ATTENTION_SHAPE")
+    check(lib().praghip_page_write(index, cache, k.data_ptr(), _two(ks[0], ks[1]), v.data_ptr(), _two(vs[0], vs[1]),
+                                   _starts(starts, seqs, index), shape[0], _stream(index, stream)))

@@ -1,10 +1,13 @@
 """Products of a few rows with 4-bit weights and group scales."""
 from __future__ import annotations
 
-import ctypes
+import struct
 
-from ._lib import W4, check, lib, shape_error
-from .attention import _stream, _torch, _type_error, _types
+from . import attention
+from ._lib import check, lib, shape_error
+from .attention import _kind, _stream, _type_error
+
+_W4 = struct.Struct("PqPqPq4Qi4x").pack  # praghip_w4
 
 
 def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, stream=None):
@@ -16,31 +19,30 @@ def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, str
     group may be short.  Sums are 32-bit, rounded once to x's type.  Reads the weights
     once per 32 rows: meant for few rows.
     """
-    torch = _torch()
-    if x.dtype not in _types() or weights.dtype is not torch.uint8 or scales.dtype is not x.dtype or \
-            (zeros is not None and zeros.dtype is not torch.uint8):
+    kind, index = _kind(x, "E_W4_TYPE"), x.get_device()
+    if weights.dtype is not attention._uint8 or scales.dtype is not x.dtype or \
+            (zeros is not None and zeros.dtype is not weights.dtype):
         raise _type_error("E_W4_TYPE")
-    index = x.get_device()
-    if index < 0 or weights.get_device() != index or scales.get_device() != index or \
+    if not weights.get_device() == scales.get_device() == index >= 0 or \
             (zeros is not None and zeros.get_device() != index):
         raise _type_error("E_W4_DEVICE")
-    m, k = x.shape
-    n, width = weights.shape
-    if group <= 0 or group % 32 or width < (k + 1) // 2 or tuple(scales.shape) != (n, -(-k // group)) or \
-            (zeros is not None and zeros.shape != scales.shape):
+    xs, ws, ss = x.stride(), weights.stride(), scales.stride()
+    (m, k), (n, width) = x.shape, weights.shape
+    if group <= 0 or group % 32 or width < (k + 1) // 2 or scales.shape != (n, -(-k // group)) or \
+            (xs[1] != 1 and k > 1) or (ws[1] != 1 and width > 1) or (ss[1] != 1 and k > group):
         raise shape_error("E_W4_SHAPE")
-    for t in (x, weights, scales) + (() if zeros is None else (zeros,)):
-        if t.shape[1] > 1 and t.stride(1) != 1:
+    zero, zs = 0, 0
+    if zeros is not None:
+        if zeros.shape != scales.shape or (zeros.stride(1) != 1 and k > group):
             raise shape_error("E_W4_SHAPE")
+        zero, zs = zeros.data_ptr(), zeros.stride(0)
     if out is None:
-        out = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    elif tuple(out.shape) != (m, n) or out.dtype is not x.dtype or out.get_device() != index or \
+        out = x.new_empty((m, n))
+    elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != index or \
             (n > 1 and out.stride(1) != 1):
         raise shape_error("E_W4_OUT")
-    w = W4(weights.data_ptr(), weights.stride(0), scales.data_ptr(), scales.stride(0),
-           None if zeros is None else zeros.data_ptr(), 0 if zeros is None else zeros.stride(0), n, k, width, group,
-           _types()[x.dtype])
-    check(lib().praghip_matvec_w4(index, ctypes.byref(w), x.data_ptr(), x.stride(0), m, out.data_ptr(), out.stride(0),
+    w = _W4(weights.data_ptr(), ws[0], scales.data_ptr(), ss[0], zero, zs, n, k, width, group, kind)
+    check(lib().praghip_matvec_w4(index, w, x.data_ptr(), xs[0], m, out.data_ptr(), out.stride(0),
                                   _stream(index, stream)))
     return out
 
@@ -53,9 +55,10 @@ def quantize_w4(weight, group: int = 128, *, zeros: bool = False):
     zero points a group spans -8 .. 7 times its scale, with them 0 .. 15 from its
     smallest value on (0 included, so that a weight of 0 stays 0).
     """
-    torch = _torch()
-    if weight.dtype not in _types() or weight.dim() != 2 or group <= 0 or group % 32:
-        raise _type_error("E_W4_TYPE")
+    import torch
+    _kind(weight, "E_W4_TYPE")
+    if weight.dim() != 2 or group <= 0 or group % 32:
+        raise shape_error("E_W4_SHAPE")
     n, k = weight.shape
     groups, width = -(-k // group), -(-k // 32) * 16
     w = torch.zeros((n, groups * group), dtype=torch.float32, device=weight.device)

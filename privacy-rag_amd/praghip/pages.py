@@ -13,46 +13,52 @@ while it is 0), which :func:`page_check` turns into an error.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
-from ._lib import E_STATE, PageTable, PagePool, PraghipError, check, lib, shape_error
-from .attention import _stream, _torch, _type_error, _work
+from . import attention
+from ._lib import E_STATE, PraghipError, check, lib, shape_error
+from .attention import _stream, _type_error, _work
 
 _REFUSED = {1: "E_PAGES_SEQUENCE", 2: "E_PAGES_CAPACITY", 3: "E_PAGES_EXHAUSTED"}
+_TABLE = struct.Struct("Pq2Q2P2QP").pack  # praghip_page_table
+_POOL = struct.Struct("Pq3Q").pack        # praghip_page_pool
 
 
-def _ints(t, dims: int, index: int) -> int:
-    if t.dtype is not _torch().int32 or t.get_device() != index or index < 0:
+def _table(tables, lengths, refs, page_size: int, status, index: int) -> bytes:
+    if attention._int32 is None:
+        attention._load()
+    int32 = attention._int32
+    if not tables.dtype is refs.dtype is int32 or not tables.get_device() == refs.get_device() == index >= 0:
         raise _type_error("E_PAGES_INTS")
-    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    shape, ts, pages = tables.shape, tables.stride(), refs.shape
+    if len(shape) != 2 or (ts[1] != 1 and shape[1] > 1) or len(pages) != 1 or \
+            (pages[0] > 1 and refs.stride(0) != 1) or page_size < 0:
         raise shape_error("E_PAGES_SHAPE")
-    return t.data_ptr()
+    # (a compaction has no use for lengths: any address stands for them)
+    held = refs.data_ptr() if lengths is None else _list(lengths, shape[0], index)
+    return _TABLE(tables.data_ptr(), ts[0], shape[1], shape[0], held, refs.data_ptr(), pages[0], page_size,
+                  0 if status is None else _list(status, 1, index))
 
 
-def _table(tables, lengths, refs, page_size: int, status, index: int) -> PageTable:
-    at, held, counts = _ints(tables, 2, index), _ints(lengths, 1, index), _ints(refs, 1, index)
-    if lengths.shape[0] != tables.shape[0]:
-        raise shape_error("E_PAGES_SHAPE")
-    return PageTable(at, tables.stride(0), tables.shape[1], lengths.shape[0], held, counts, refs.shape[0], page_size,
-                     None if status is None else _ints(status, 1, index))
-
-
-def _pool(pool, index: int) -> PagePool:
-    if pool.dim() < 4 or not pool.is_contiguous():
+def _pool(pool, index: int) -> bytes:
+    shape = pool.shape
+    if len(shape) < 4 or not pool.is_contiguous():
         raise shape_error("E_PAGES_POOL")
     if pool.get_device() != index or index < 0:
         raise _type_error("E_PAGES_DEVICE")
-    shape, size = pool.shape, pool.element_size()
-    page = math.prod(shape[-3:]) * size
-    return PagePool(pool.data_ptr(), shape[-4] * page, page, math.prod(shape[:-4]), shape[-4])
+    page = math.prod(shape[-3:]) * pool.element_size()
+    return _POOL(pool.data_ptr(), shape[-4] * page, page, math.prod(shape[:-4]), shape[-4])
 
 
-def _list(t, n: int | None, index: int) -> int:
-    at = _ints(t, 1, index)
-    if n is not None and t.shape[0] != n:
+def _list(t, n: int, index: int) -> int:
+    if attention._int32 is None:
+        attention._load()
+    if t.dtype is not attention._int32 or t.get_device() != index or index < 0:
+        raise _type_error("E_PAGES_INTS")
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise shape_error("E_PAGES_SHAPE")
-    return at
+    return t.data_ptr()
 
 
 def page_reserve(tables, lengths, refs, page_size: int, sequences, counts, status=None, stream=None) -> None:
@@ -60,7 +66,7 @@ def page_reserve(tables, lengths, refs, page_size: int, sequences, counts, statu
     index = tables.get_device()
     t = _table(tables, lengths, refs, page_size, status, index)
     n = sequences.shape[0]
-    check(lib().praghip_page_reserve(index, ctypes.byref(t), _list(sequences, None, index), _list(counts, n, index), n,
+    check(lib().praghip_page_reserve(index, t, _list(sequences, sequences.shape[0], index), _list(counts, n, index), n,
                                      _stream(index, stream)))
 
 
@@ -68,7 +74,7 @@ def page_free(tables, lengths, refs, sequences, status=None, stream=None) -> Non
     """Empties sequences: their pages lose a reference, their rows become -1, their lengths 0."""
     index = tables.get_device()
     t = _table(tables, lengths, refs, 1, status, index)
-    check(lib().praghip_page_free(index, ctypes.byref(t), _list(sequences, None, index), sequences.shape[0],
+    check(lib().praghip_page_free(index, t, _list(sequences, sequences.shape[0], index), sequences.shape[0],
                                   _stream(index, stream)))
 
 
@@ -79,7 +85,7 @@ def page_trim(tables, lengths, refs, page_size: int, sequences, window: int, sin
     t = _table(tables, lengths, refs, page_size, status, index)
     if window < 0 or sinks < 0:
         raise shape_error("E_PAGES_WINDOW")
-    check(lib().praghip_page_trim(index, ctypes.byref(t), _list(sequences, None, index), sequences.shape[0], window,
+    check(lib().praghip_page_trim(index, t, _list(sequences, sequences.shape[0], index), sequences.shape[0], window,
                                   sinks, _stream(index, stream)))
 
 
@@ -93,12 +99,12 @@ def page_fork(pool, tables, lengths, refs, parents, children, status=None, strea
     p = _pool(pool, index)
     t = _table(tables, lengths, refs, pool.shape[-2], status, index)
     n = parents.shape[0]
-    of, to = _list(parents, None, index), _list(children, n, index)
+    of, to = _list(parents, n, index), _list(children, n, index)
     if n:
         L = lib()
         size = L.praghip_page_fork_workspace(n)
         work = _work(size, tables, stream)
-        check(L.praghip_page_fork(index, ctypes.byref(t), ctypes.byref(p), of, to, n, work.data_ptr(), size,
+        check(L.praghip_page_fork(index, t, p, of, to, n, work.data_ptr(), size,
                                   _stream(index, stream)))
 
 
@@ -107,13 +113,12 @@ def page_compact(pool, tables, refs, stream=None) -> None:
     the holes below, both in rising order, and the tables follow."""
     index = tables.get_device()
     p = _pool(pool, index)
-    at, counts = _ints(tables, 2, index), _ints(refs, 1, index)
-    t = PageTable(at, tables.stride(0), tables.shape[1], tables.shape[0], at, counts, refs.shape[0], pool.shape[-2],
-                  None)
+    pages = refs.shape[0]
+    t = _table(tables, None, refs, pool.shape[-2], None, index)
     L = lib()
-    size = L.praghip_page_compact_workspace(t.pages)
+    size = L.praghip_page_compact_workspace(pages)
     work = _work(size, tables, stream)
-    check(L.praghip_page_compact(index, ctypes.byref(t), ctypes.byref(p), work.data_ptr(), size,
+    check(L.praghip_page_compact(index, t, p, work.data_ptr(), size,
                                  _stream(index, stream)))
 
 
@@ -123,7 +128,7 @@ def page_copy(pool, sources, targets, stream=None) -> None:
     index = pool.get_device()
     p = _pool(pool, index)
     n = sources.shape[0]
-    check(lib().praghip_page_copy(index, ctypes.byref(p), _list(sources, None, index), _list(targets, n, index), n,
+    check(lib().praghip_page_copy(index, p, _list(sources, n, index), _list(targets, n, index), n,
                                   _stream(index, stream)))
 
 
