@@ -614,7 +614,8 @@ typedef struct praghip_cache {
  * -infinity.  q and out are [seqs][heads][head_dim] by strides {sequence, head}, 16-byte
  * aligned, strides multiples of 8.  max_length is a bound of the lengths, used for the
  * launch's size alone (0: the tables' width); results hold without it, and a given size
- * of it gives the same bits each time.  work: 16-byte aligned, at least
+ * of it gives the same bits each time.  The blocks of 32 positions of all sequences' tables and
+ * key/value heads are at most 2^31 (E_ATTENTION_SHAPE).  work: 16-byte aligned, at least
  * praghip_paged_decode_workspace(...) bytes (E_ATTENTION_WORKSPACE), not used by another
  * call until this one is done. */
 size_t praghip_paged_decode_workspace(const praghip_cache *cache, size_t heads, size_t max_length);

@@ -36,7 +36,7 @@ struct DecodeArgs {
   int64_t out_seq, out_head;
   float* lse;  // [seqs][heads] or null
   float* work;
-  int64_t* base;  // [seqs + 1] key blocks before each sequence
+  uint32_t* base;  // [seqs + 1] key blocks before each sequence
 };
 
 struct PromptArgs {

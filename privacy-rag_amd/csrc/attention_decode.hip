@@ -41,100 +41,85 @@ struct DecodeShape {
   static constexpr int tiles16 = (per + 7) / 8;
 };
 
-// Blocks of all heads over the grid's waves, one block or more to each of the first
-// `waves`: a workgroup with a later neighbour that has blocks has blocks itself.
+// Blocks of all heads over the grid's waves: each of the first `extra` has one more than
+// the others, so a workgroup with a later neighbour that has blocks has blocks itself.
 struct Range {
-  int64_t total;
-  unsigned waves;
-  __device__ __forceinline__ Range(int64_t blocks, unsigned grid)
-      : total(blocks), waves(unsigned(min(max(blocks, int64_t(1)), int64_t(grid)))) {}
-  __device__ __forceinline__ int64_t begin(unsigned w) const { return total * min(w, waves) / waves; }
+  uint32_t each, extra;
+  __device__ __forceinline__ Range(uint32_t blocks, uint32_t waves) : each(blocks / waves), extra(blocks - each * waves) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t w) const { return each * w + min(w, extra); }
   // the wave whose stretch holds block u
-  __device__ __forceinline__ unsigned of(int64_t u) const {
-    return unsigned(((u + 1) * waves + total - 1) / total) - 1;
+  __device__ __forceinline__ uint32_t of(uint32_t u) const {
+    const uint32_t longer = extra * (each + 1);
+    return u < longer ? u / (each + 1) : extra + (u - longer) / each;
   }
 };
 
 // pieces of the workspace: [workgroup][2] of rows x (dim + 2)
-__device__ __forceinline__ size_t piece_floats(int rows, int D) { return size_t(rows) * (D + 2); }
+// (a multiple of four floats, which the join loads together)
+__host__ __device__ __forceinline__ size_t piece_floats(int rows, int D) { return size_t(rows) * D + (2 * rows + 3) / 4 * 4; }
 
 template <typename T, int D, bool EXACT>
 __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a) {
   using S = DecodeShape<T, D>;
   extern __shared__ float lds[];
-  __shared__ int64_t before[kWaves * 64 + 1];
   __shared__ int piece_id[2 * kWaves], piece_flags[2 * kWaves];
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int qtiles = (c.group + 15) >> 4, heads = c.kv_heads * qtiles, rows = min(c.group, 16);
+  if (threadIdx.x < 2 * kWaves) piece_id[threadIdx.x] = -1;
+  __syncthreads();
 
-  // key blocks before each stretch of sequences, one stretch per thread
-  const int per = (c.seqs + kWaves * 64 - 1) / (kWaves * 64);
-  {
-    int64_t mine = 0;
-    for (int i = 0; i < per; ++i) {
-      const int s = int(threadIdx.x) * per + i;
-      if (s < c.seqs) {
-        const int n = length_of(c, s);
-        mine += visible_blocks(c, n - 1, n - 1, 5).count();
-      }
-    }
-    int64_t sum = mine;  // inclusive over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t up = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += up;
-    }
-    before[threadIdx.x + 1] = sum;
-    if (threadIdx.x == 0) before[0] = 0;
-    __syncthreads();
-    int64_t add = 0;
-    for (int w = 0; w < wave; ++w) add += before[w * 64 + 64];
-    __syncthreads();
-    before[threadIdx.x + 1] = sum + add;
-    if (threadIdx.x < 2 * kWaves) piece_id[threadIdx.x] = -1;
-    __syncthreads();
-    if (blockIdx.x == 0) {  // for the join
-      int64_t at = sum + add - mine;
-      for (int i = 0; i < per; ++i) {
-        const int s = int(threadIdx.x) * per + i;
-        if (s >= c.seqs) break;
-        a.base[s] = at;
-        const int n = length_of(c, s);
-        at += visible_blocks(c, n - 1, n - 1, 5).count();
-        if (s == c.seqs - 1) a.base[c.seqs] = at;
-      }
+  // key blocks before each stretch of sequences, one stretch per lane; every wave counts
+  // for itself, which takes no exchange with the others
+  const int per = (c.seqs + 63) >> 6;
+  uint32_t mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int s = lane * per + i;
+    if (s < c.seqs) {
+      const int n = length_of(c, s);
+      mine += visible_blocks(c, n - 1, n - 1, 5).count();
     }
   }
-  const Range range(before[kWaves * 64] * heads, gridDim.x * kWaves);
-  const int64_t wg_begin = range.begin(blockIdx.x * kWaves), wg_end = range.begin(blockIdx.x * kWaves + kWaves);
-  int64_t u = range.begin(blockIdx.x * kWaves + wave);
-  const int64_t u_end = range.begin(blockIdx.x * kWaves + wave + 1), u_begin = u;
+  uint32_t sum = mine;  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += up;
+  }
+  if (blockIdx.x == 0 && wave == 0) {  // for the join
+    uint32_t at = sum - mine;
+    for (int i = 0; i < per; ++i) {
+      const int s = lane * per + i;
+      if (s >= c.seqs) break;
+      a.base[s] = at;
+      const int n = length_of(c, s);
+      at += visible_blocks(c, n - 1, n - 1, 5).count();
+      if (s == c.seqs - 1) a.base[c.seqs] = at;
+    }
+  }
+  const Range range(uint32_t(__builtin_amdgcn_readlane(int(sum), 63)) * heads, gridDim.x * kWaves);
+  const uint32_t wg_begin = range.begin(blockIdx.x * kWaves), wg_end = range.begin(blockIdx.x * kWaves + kWaves);
+  const uint32_t u_begin = range.begin(blockIdx.x * kWaves + wave), u_end = range.begin(blockIdx.x * kWaves + wave + 1);
+  uint32_t u = u_begin;
 
   if (u < u_end) {
-    // the sequence of block u: its thread's stretch, then along the stretch
-    int lo = 0, hi = kWaves * 64 - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (before[mid] * heads <= u)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    int s = lo * per;
-    int64_t base = before[lo] * heads;
+    // the sequence of block u: its lane's stretch (the stretches before it end at or before
+    // u), then along the stretch
+    const int from_lane = __popcll(__ballot(sum * heads <= u));
+    int s = from_lane * per;
+    uint32_t base = uint32_t(__builtin_amdgcn_readlane(int(sum - mine), from_lane)) * heads;
     while (u < u_end) {
       const int len = length_of(c, s);
       const Blocks blocks = visible_blocks(c, len - 1, len - 1, 5);
       const int nb = blocks.count();
-      if (u >= base + int64_t(nb) * heads) {
-        base += int64_t(nb) * heads;
+      if (u >= base + uint32_t(nb) * heads) {
+        base += uint32_t(nb) * heads;
         ++s;
         continue;
       }
-      const int h = int((u - base) / nb), first = int((u - base) - int64_t(h) * nb);
-      const int count = int(min(int64_t(nb - first), u_end - u));
+      const int h = int((u - base) / uint32_t(nb)), first = int(u - base) - h * nb;
+      const int count = min(nb - first, int(u_end - u));
       const int kvh = h / qtiles, head0 = kvh * c.group + (h - kvh * qtiles) * 16;
       const bool has = (h - kvh * qtiles) * 16 + col < c.group;
 
@@ -272,7 +257,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
           }
         }
         if (lane == 0) {
-          const int64_t b = base + int64_t(h) * nb;
+          const uint32_t b = base + uint32_t(h) * nb;
           piece_id[slot] = s * heads + h;
           piece_flags[slot] = (b >= wg_begin && b + nb <= wg_end ? 1 : 0) | (b > wg_begin ? 2 : 0);
         }
@@ -325,54 +310,71 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
   }
 }
 
-// One workgroup per sequence and head: the pieces of a head that workgroups share,
-// and rows that see nothing.
+// One workgroup per sequence and query head, for heads that workgroups share and rows that
+// see nothing.  Each D / 4 threads merge every (1024 / D)-th piece, with the next pieces'
+// loads under way, and LDS the results, all in a fixed order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) decode_join_kernel(DecodeArgs a, unsigned workgroups) {
+  constexpr int per = D / 4, sets = 256 / per;
+  __shared__ __attribute__((aligned(16))) float part[sets][D];
+  __shared__ float tops[sets], sums[sets];
   const CacheArgs& c = a.c;
+  const int all = c.kv_heads * c.group, s = blockIdx.x / all, head = blockIdx.x - s * all, kvh = head / c.group;
   const int qtiles = (c.group + 15) >> 4, heads = c.kv_heads * qtiles, rows = min(c.group, 16);
-  const int s = blockIdx.x / heads, h = blockIdx.x - s * heads, kvh = h / qtiles;
-  const int head0 = kvh * c.group + (h - kvh * qtiles) * 16, have = min(16, c.group - (h - kvh * qtiles) * 16);
-  const int64_t nb = a.base[s + 1] - a.base[s], b = a.base[s] * heads + h * nb;
-  T* out = static_cast<T*>(a.out) + s * a.out_seq + head0 * a.out_head;
-  float* lse = a.lse ? a.lse + int64_t(s) * c.kv_heads * c.group + head0 : nullptr;
-  if (nb == 0) {
-    for (int i = threadIdx.x; i < have * c.dim; i += 256) out[(i / c.dim) * a.out_head + i % c.dim] = T(0.f);
-    if (lse && int(threadIdx.x) < have) lse[threadIdx.x] = kNegInf;
-    return;
-  }
-  const Range range(a.base[c.seqs] * heads, workgroups * kWaves);
-  const unsigned w0 = range.of(b) / kWaves, w1 = range.of(b + nb - 1) / kWaves;
-  if (w0 == w1) return;
-  const size_t piece = piece_floats(rows, D);
-  const float* first = a.work + (size_t(w0) * 2 + (b > range.begin(w0 * kWaves))) * piece;
-  const float* rest = a.work + size_t(w0) * 2 * piece;  // piece 0 of the others
-  for (int i = threadIdx.x; i < have * D; i += 256) {
-    const int r = i / D, d = i - r * D;
-    float m = first[rows * D + r];
-    for (unsigned w = w0 + 1; w <= w1; ++w) m = fmaxf(m, rest[(w - w0) * 2 * piece + rows * D + r]);
-    float sum = 0, l = 0;
-    for (unsigned w = w0; w <= w1; ++w) {
-      const float* p = w == w0 ? first : rest + (w - w0) * 2 * piece;
-      const float f = __builtin_amdgcn_exp2f(p[rows * D + r] - origin(m));
-      sum += f * p[i];
-      l += f * p[rows * D + rows + r];
+  const int g = head - kvh * c.group, h = kvh * qtiles + (g >> 4), r = g & 15;
+  const uint32_t b0 = a.base[s], nb = a.base[s + 1] - b0, b = b0 * heads + h * nb, total = a.base[c.seqs] * heads;
+  const int set = threadIdx.x / per, d = threadIdx.x % per * 4;
+  T* const out = static_cast<T*>(a.out) + s * a.out_seq + head * a.out_head;
+  float m = kNegInf, l = 0;
+  f32x4 o = {0, 0, 0, 0};
+  if (nb) {
+    const Range range(total, workgroups * kWaves);
+    const uint32_t w0 = range.of(b) / kWaves, w1 = range.of(b + nb - 1) / kWaves;
+    if (w0 == w1) return;
+    const size_t piece = piece_floats(rows, D);
+    const uint32_t second = b > range.begin(w0 * kWaves);  // the first workgroup's other piece
+    for (uint32_t w = w0 + set; w <= w1; w += sets) {
+      const float* const p = a.work + (size_t(w) * 2 + (w == w0 ? second : 0)) * piece;
+      const f32x4 po = *reinterpret_cast<const f32x4*>(p + r * D + d);
+      const float pm = p[rows * D + r], pl = p[rows * D + rows + r], top = fmaxf(m, pm);
+      const float f = __builtin_amdgcn_exp2f(m - origin(top)), pf = __builtin_amdgcn_exp2f(pm - origin(top));
+      o = o * f + po * pf;
+      l = l * f + pl * pf;
+      m = top;
     }
-    const float inv = l > 0 || l != l ? 1.f / l : 0.f;
-    if (d < c.dim) out[r * a.out_head + d] = T(sum * inv);
-    if (lse && d == 0) lse[r] = (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
+  *reinterpret_cast<f32x4*>(&part[set][d]) = o;
+  if (d == 0) {
+    tops[set] = m;
+    sums[set] = l;
+  }
+  __syncthreads();
+  if (int(threadIdx.x) >= D) return;
+  m = kNegInf;
+#pragma unroll
+  for (int i = 0; i < sets; ++i) m = fmaxf(m, tops[i]);
+  float sum = 0;
+  l = 0;
+#pragma unroll
+  for (int i = 0; i < sets; ++i) {
+    const float f = __builtin_amdgcn_exp2f(tops[i] - origin(m));
+    sum += f * part[i][threadIdx.x];
+    l += f * sums[i];
+  }
+  const float inv = l > 0 || l != l ? 1.f / l : 0.f;
+  if (int(threadIdx.x) < c.dim) out[threadIdx.x] = T(sum * inv);
+  if (a.lse && threadIdx.x == 0) a.lse[int64_t(s) * all + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <typename T, int D>
 hipError_t launch(const DecodeArgs& a, unsigned workgroups, hipStream_t s) {
-  const int rows = std::min(a.c.group, 16), heads = a.c.kv_heads * ((a.c.group + 15) / 16);
-  const size_t lds = 2 * kWaves * size_t(rows) * (D + 2) * sizeof(float);
+  const int rows = std::min(a.c.group, 16);
+  const size_t lds = 2 * kWaves * piece_floats(rows, D) * sizeof(float);
   const auto kernel = a.c.dim == D ? paged_decode_kernel<T, D, true> : paged_decode_kernel<T, D, false>;
   hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kWaves * 64), lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((decode_join_kernel<T, D>), dim3(unsigned(a.c.seqs) * heads), dim3(256), 0, s, a, workgroups);
+  hipLaunchKernelGGL((decode_join_kernel<T, D>), dim3(unsigned(a.c.seqs) * a.c.kv_heads * a.c.group), dim3(256), 0, s, a, workgroups);
   return hipGetLastError();
 }
 
@@ -391,7 +393,7 @@ unsigned decode_workgroups(size_t seqs, size_t kv_heads, size_t group, size_t ke
 }
 size_t decode_work_floats(unsigned workgroups, size_t group, size_t dim) {
   const size_t D = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  return size_t(workgroups) * 2 * std::min<size_t>(group, 16) * (D + 2);
+  return size_t(workgroups) * 2 * piece_floats(int(std::min<size_t>(group, 16)), int(D));
 }
 
 hipError_t launch_paged_decode(const DecodeArgs& a, int type, unsigned workgroups, hipStream_t s) {

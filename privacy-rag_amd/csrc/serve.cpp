@@ -78,6 +78,11 @@ size_t bound_of(const praghip_cache& c, size_t max_length) {
   const size_t most = size_t(capacity_of(c.table_width, c.page_size));
   return max_length ? std::min(max_length, most) : most;
 }
+// the decode counts blocks of 32 keys over all sequences and heads in 32 bits
+bool blocks_fit(const praghip_cache& c, size_t heads) {
+  const size_t blocks = size_t(capacity_of(c.table_width, c.page_size)) / 32 + 1;
+  return c.seqs * c.kv_heads * ((heads / c.kv_heads + 15) / 16) <= (size_t(1) << 31) / blocks;
+}
 // keys that a query, or the queries of `rows` neighbours, can see at most
 size_t keys_of(size_t bound, size_t rows, size_t window, size_t sinks) {
   return window && window < bound ? std::min(bound, window + std::min(sinks, bound) + rows) : bound;
@@ -92,7 +97,7 @@ DecodePlan decode_plan(const praghip_cache& c, size_t heads, size_t max_length) 
   DecodePlan p;
   const size_t group = heads / c.kv_heads;
   p.workgroups = decode_workgroups(c.seqs, c.kv_heads, group, bound_of(c, max_length));
-  p.base_bytes = ((c.seqs + 1) * sizeof(int64_t) + 15) / 16 * 16;
+  p.base_bytes = ((c.seqs + 1) * sizeof(uint32_t) + 15) / 16 * 16;
   p.bytes = p.base_bytes + decode_work_floats(p.workgroups, group, c.head_dim) * sizeof(float);
   return p;
 }
@@ -138,7 +143,7 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
   if (c && c->seqs == 0) return PRAGHIP_OK;
   if (const int rc = check_cache(c)) return rc;
   if (!q || !q_strides || !out || !out_strides || !work) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
-  if (!heads_fit(*c, heads) || !std::isfinite(scale)) return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
+  if (!heads_fit(*c, heads) || !blocks_fit(*c, heads) || !std::isfinite(scale)) return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
   if (!aligned16(q) || !aligned16(out) || !aligned16(work) || !aligned4(lse) || !eights(q_strides, 2) || !eights(out_strides, 2))
     return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_ALIGNMENT");
   const DecodePlan p = decode_plan(*c, heads, max_length);
@@ -148,7 +153,7 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
   a.q = q, a.q_seq = q_strides[0], a.q_head = q_strides[1];
   a.out = out, a.out_seq = out_strides[0], a.out_head = out_strides[1];
   a.lse = lse;
-  a.base = static_cast<int64_t*>(work);
+  a.base = static_cast<uint32_t*>(work);
   a.work = reinterpret_cast<float*>(static_cast<char*>(work) + p.base_bytes);
   DeviceScope scope(device);
   hipError_t e = scope.status();
