@@ -198,8 +198,8 @@ __device__ __forceinline__ void copy_pages(const PoolArgs& p, const int32_t* fro
     uint4 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t at = turn * kTurn + (j * 256 + threadIdx.x) * 16;
-      if (at < p.page_bytes) x[j] = *reinterpret_cast<const uint4*>(a + at);
+      // (no load behind a condition: the compiler would keep x in LDS)
+      x[j] = *reinterpret_cast<const uint4*>(a + min(turn * kTurn + (j * 256 + int64_t(threadIdx.x)) * 16, p.page_bytes - 16));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -270,6 +270,34 @@ def test_scales(gpu, scale):
     plain.check_lse(lse, wlse)
 
 
+@pytest.mark.parametrize("dim,type", [(64, BF16), (128, F16), (96, BF16), (256, F16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_prompt_masked_keys_may_hold_anything(gpu, dim, type, window, sinks):
+    """NaN and infinities in keys and values reach the rows that see them and no others:
+    later rows of the same tile, earlier ones, and those whose window has moved on."""
+    say("poisoned prompt", dim, type, window, sinks)
+    n, rows, heads, kv = 230, 150, 4, 2
+    c = plain.make([n], heads, kv, dim, 16, type, seed=dim + window)
+    q = torch.randn((rows, heads, dim), generator=c["g"]).to(type)
+    want, _, size = plain.attention(c, q, [0, rows], window=window, sinks=sinks)
+    bad = {100: ("v", math.nan), 171: ("k", math.nan), 190: ("v", math.inf), 207: ("v", -math.inf)}
+    for at, (x, value) in bad.items():
+        c[x][c["tables"][0, at // 16], 1, at % 16, 5] = value
+    out = praghip.paged_prompt(q.to("cuda"), *to_gpu(c), torch.tensor([0, rows], dtype=torch.int32, device="cuda"), rows,
+                               window=window, sinks=sinks).cpu()
+    place = torch.arange(n - rows, n)
+    hit = torch.zeros(rows, dtype=torch.bool)
+    for at in bad:
+        hit |= (at <= place) & ((place - at < window) if window else torch.ones(rows, dtype=torch.bool))
+    clean = torch.ones(rows, heads, dtype=torch.bool)
+    clean[hit, 2:] = False  # the heads of key/value head 1
+    assert bool(hit.any()) and not bool(hit.all())
+    assert torch.isfinite(out[clean]).all()
+    plain.check(out[clean], want[clean], size[clean], type, rounded=True)
+    # column 5 of the rows that see a bad value is not finite
+    assert not torch.isfinite(out[hit][:, 2:, 5].float()).any()
+
+
 def test_prompt_over_a_long_cache(gpu):
     """More tiles than a workgroup keeps the pages of; few of the rows, by their definition."""
     say("long cache")
