@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   constexpr int ROWS = 32 * NW, CPR = D / 8;  // 16-byte chunks of a row
   constexpr int steps = D / 16, blocks32 = D / 32;
   extern __shared__ uint32_t lds[];
-    constexpr int TK = tile_keys<D>(), ROW = 2 * D, TILE = TK * ROW;  // bytes
+  constexpr int TK = tile_keys<D>(), ROW = 2 * D, TILE = TK * ROW;  // bytes
   const Lds kbuf = (Lds)lds, vbuf = kbuf + kRing * TILE;  // [kRing][TK][D] each
   const Lds list = vbuf + kRing * TILE, flags = list + 16 * kGroups;
   const CacheArgs& c = a.c;
@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     voff[n] = 2 * ((r & 15) * c.v_token + 8 * ((lane % CPR) ^ fv(r)));
   }
   bool missing = false;  // some key has no page: no tile is taken as seen whole
+  // (taken where all lanes are active: what moves klow elsewhere and back then moves all of it)
   const auto lane_of = [](uint32_t lo, uint32_t hi, int x) {
     return uint64_t(uint32_t(__builtin_amdgcn_readlane(hi, x))) << 32 | uint32_t(__builtin_amdgcn_readlane(lo, x));
   };
@@ -178,8 +179,8 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       const int r0 = RPI * (wave + NW * n);
-      if (EXACT || 8 * ((lane % CPR) ^ fk(r0 + inrow)) < c.dim)
-        dma16(lane_of(klow, khigh, at % TURNS * GROUPS + (r0 >> 4)), koff[n], kbuf + slot * TILE + r0 * ROW);
+      const uint64_t base = lane_of(klow, khigh, at % TURNS * GROUPS + (r0 >> 4));
+      if (EXACT || 8 * ((lane % CPR) ^ fk(r0 + inrow)) < c.dim) dma16(base, koff[n], kbuf + slot * TILE + r0 * ROW);
     }
   };
   const auto load_v = [&](int at, int slot) {
@@ -190,8 +191,8 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       const int r0 = RPI * (wave + NW * n);
-      if (EXACT || 8 * ((lane % CPR) ^ fv(r0 + inrow)) < c.dim)
-        dma16(lane_of(vlow, vhigh, at % TURNS * GROUPS + (r0 >> 4)), voff[n], vbuf + slot * TILE + r0 * ROW);
+      const uint64_t base = lane_of(vlow, vhigh, at % TURNS * GROUPS + (r0 >> 4));
+      if (EXACT || 8 * ((lane % CPR) ^ fv(r0 + inrow)) < c.dim) dma16(base, voff[n], vbuf + slot * TILE + r0 * ROW);
     }
   };
   // which groups of 16 keys of a tile have a page
@@ -353,6 +354,97 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     if (i + 1 < i1) turn(i + 1, std::integral_constant<int, 1>{});
     if (i + 2 < i1) turn(i + 2, std::integral_constant<int, 2>{});
     if (i + 3 < i1) turn(i + 3, std::integral_constant<int, 3>{});
+  }
+  // V may hold values that are not finite, and of keys that only some rows of a tile see the
+  // others' P of 0 makes NaN.  Where O is not finite it is formed again from the cache, with
+  // the maximum known: 32 keys at a time, those with such values one by one, each added where
+  // the row sees it.  (In the loop above the same test took 3% of a long prompt's time.)
+  bool finite = true;
+#pragma unroll
+  for (int b = 0; b < blocks32; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) finite &= __builtin_fabsf(o[b][r]) < __builtin_inff();
+  if (__any(!finite)) {
+#pragma unroll
+    for (int b = 0; b < blocks32; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] = 0;
+    const float base = -origin(m) * c.scale;
+#pragma unroll 1
+    for (int x = i0 * (TK / 32); x < i1 * (TK / 32); ++x) {
+      const int kb = blocks.at(x / (TK / 32)) * TK + 32 * (x % (TK / 32));
+      const T *kp[2], *vp[2];  // of either 16 keys
+      uint32_t held = 0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = kb + 16 * n, entry = key >> c.page_shift;
+        const int page = entry < width ? c.tables[s * c.table_stride + entry] : -1;
+        const bool none = page < 0 || page >= c.pages;
+        const uint64_t at = none ? 0 : page, in = key & ((1 << c.page_shift) - 1);
+        held |= uint32_t(!none) << n;
+        kp[n] = static_cast<const T*>(c.k) + uint64_t(kvh) * c.k_head + at * c.k_page + in * c.k_token;
+        vp[n] = static_cast<const T*>(c.v) + uint64_t(kvh) * c.v_head + at * c.v_page + in * c.v_token;
+      }
+      const auto seen = [&](int key) {
+        const int j = kb + key;
+        return bool((j <= place) & ((j > from) | (j < c.sinks)) & bool(held >> (key >> 4) & 1));
+      };
+      f32x16 score;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) score[r] = 0;
+#pragma unroll
+      for (int n = 0; n < steps; ++n) {
+        u32x4 k = {0, 0, 0, 0};
+        const int d = 16 * n + 8 * half;
+        if (EXACT || d < c.dim) k = *reinterpret_cast<const u32x4*>((col < 16 ? kp[0] : kp[1]) + uint64_t(col & 15) * c.k_token + d);
+        score = Half<T>::mma32(k, q[n], score);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool sees = seen(8 * (r >> 2) + 4 * half + (r & 3));
+        score[r] = sees ? __builtin_amdgcn_exp2f(fmaf(score[r], c.scale, base)) : 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        u32x4 p;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) p[w] = pack2<T>(score[8 * n + 2 * w], score[8 * n + 2 * w + 1]);
+#pragma unroll
+        for (int b = 0; b < blocks32; ++b) {
+          const int d = 32 * b + col;
+          u32x4 v = {0, 0, 0, 0};
+          bool apart = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = 8 * (e >> 2) + 4 * half + (e & 3);
+            uint32_t bits = 0;
+            if ((EXACT || d < c.dim) && (held >> n & 1) && kb + 16 * n + key < len)
+              bits = *reinterpret_cast<const uint16_t*>(vp[n] + uint64_t(key) * c.v_token + d);
+            constexpr uint32_t exponent = std::is_same<T, __bf16>::value ? 0x7f80 : 0x7c00;
+            apart |= (bits & exponent) == exponent;
+            v[e >> 1] |= bits << 16 * (e & 1);
+          }
+          if (!__any(apart)) {
+            o[b] = Half<T>::mma32(v, p, o[b]);
+            continue;
+          }
+#pragma unroll 1
+          for (int y = 0; y < 16; ++y) {  // key y is slot 4 (y / 8) + y % 4 of half y / 4 % 2
+            const int e = (y >> 3) * 4 + (y & 3);
+            const bool sees = seen(16 * n + y);
+            u32x4 pick;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) pick[w] = ((half == (y >> 2 & 1)) & (w == e >> 1)) ? 0xffffu << 16 * (e & 1) : 0;
+            f32x16 add;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add[r] = 0;
+            add = Half<T>::mma32(v & pick, p & pick, add);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[b][r] += sees ? add[r] : 0.f;
+          }
+        }
+      }
+    }
   }
   l = sum32(l);
   m *= c.scale;

@@ -51,3 +51,30 @@ def test_m0_before_the_prompt_attention_dma(machine_code):
             dmas += 1
             bad += w[0] < 1
     assert dmas > 0 and bad == 0
+
+
+def test_addresses_come_from_lanes_that_are_on(machine_code):
+    """The prompt attention keeps 64 addresses across a wave's lanes.  Loaded where some lanes
+    are off (as when a compiler moves them to memory and back inside a branch), the others'
+    would be taken from whatever the register held before."""
+    taken = 0
+    bad = []
+    for i, (op, ops, line) in enumerate(machine_code):
+        if not op.startswith("v_readlane"):
+            continue
+        taken += 1
+        source, load = ops[1], None
+        for k in range(i - 1, max(0, i - 200), -1):
+            o, p, text = machine_code[k]
+            if o == "FUNC":
+                break
+            if load is None:
+                if p and p[0].split()[0] == source:
+                    if not (MEMORY.match(o) and "load" in o):
+                        break
+                    load = text
+            elif "saveexec" in o or (p and p[0] == "exec"):
+                if o.startswith(("s_and_saveexec", "s_andn2_saveexec")):
+                    bad.append((load, line))
+                break
+    assert taken > 0 and not bad, bad[:5]
