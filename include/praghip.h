@@ -11,7 +11,9 @@
  * [batch][component][prime][N] for ciphertexts (ntt.hpp:20, switch.cu:65,71),
  * [digit][component][key prime][N] NTT-form keys (keyswitch/seal_adapter.cpp:37-39),
  * [prime][N][2] (operand, quotient) NTT tables (seal_tables.cpp:22-33) and
- * [out][in] weights (bfv_matrix.inc:101-105, artifacts.hpp:86-92).
+ * [out][in] weights (bfv_matrix.inc:101-105, artifacts.hpp:86-92).  All of that is exact
+ * integer arithmetic; the "serving" sections (attention over a paged cache, its pages,
+ * 4-bit products) have no counterpart there and work on 16-bit floating point.
  *
  * Pointers documented "device" are HIP device pointers on the plan's device;
  * "host" pointers are ordinary host memory.  `stream` is a hipStream_t used as
@@ -589,10 +591,12 @@ int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
  * page: its positions are seen by no query.  Memory that no position below a
  * sequence's length names is never used, whatever it holds.
  *
- * page_size is a power of two of 16 .. 32768, head_dim a multiple of 8 up to 256
- * and the cache's strides are below 2^31, a token's below 2^26 (E_ATTENTION_SHAPE); base addresses are 16-byte
- * aligned and strides multiples of 8 (E_ATTENTION_ALIGNMENT).  A length outside 0 .. table_width * page_size is taken
- * as the nearer end. */
+ * page_size is a power of two of 16 .. 32768, head_dim a multiple of 8 up to 256 and
+ * the cache's strides are below 2^31, a token's below 2^26 (E_ATTENTION_SHAPE); base
+ * addresses are 16-byte aligned and strides multiples of 8 (E_ATTENTION_ALIGNMENT).  A
+ * length outside 0 .. table_width * page_size is taken as the nearer end.  A key or
+ * value that is not finite makes the outputs of the queries that see it NaN or
+ * infinite, and no others'. */
 typedef struct praghip_cache {
   void *k, *v;
   int64_t k_strides[3], v_strides[3];
@@ -614,8 +618,9 @@ typedef struct praghip_cache {
  * -infinity.  q and out are [seqs][heads][head_dim] by strides {sequence, head}, 16-byte
  * aligned, strides multiples of 8.  max_length is a bound of the lengths, used for the
  * launch's size alone (0: the tables' width); results hold without it, and a given size
- * of it gives the same bits each time.  The blocks of 32 positions of all sequences' tables and
- * key/value heads are at most 2^31 (E_ATTENTION_SHAPE).  work: 16-byte aligned, at least
+ * of it gives the same bits each time.  seqs x heads is below 2^24, the blocks of 32
+ * positions of all sequences' tables and key/value heads are at most 2^31
+ * (E_ATTENTION_SHAPE).  work: 16-byte aligned, at least
  * praghip_paged_decode_workspace(...) bytes (E_ATTENTION_WORKSPACE), not used by another
  * call until this one is done. */
 size_t praghip_paged_decode_workspace(const praghip_cache *cache, size_t heads, size_t max_length);
@@ -628,7 +633,8 @@ int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, 
  * s, the last of them at position lengths[s] - 1; the cache holds their keys and values
  * already.  Causal, with window and sinks as above; a row whose position is below 0 sees
  * nothing.  max_rows is at least the longest of these stretches; rows beyond it are not
- * computed.  lse: [tokens][heads]. */
+ * computed.  seqs x kv_heads x (max_rows x group / 128 + 1) is below 2^23
+ * (E_ATTENTION_SHAPE).  lse: [tokens][heads]. */
 size_t praghip_paged_prompt_workspace(const praghip_cache *cache, size_t heads, size_t max_rows, size_t window,
                                       size_t sinks, size_t max_length);
 int praghip_paged_prompt(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,
@@ -700,7 +706,7 @@ int praghip_page_write(int device, const praghip_cache *cache, const void *k, co
 /* y[m][n] = sum_k x[m][k] (w[n][k] - z[n][k / group]) s[n][k / group]: x [m][k], y [m][n]
  * and scales [n][groups] of `type`, w [n][width] bytes of two 4-bit values each, the lower
  * bits first (width >= (k + 1) / 2), zeros [n][groups] bytes (NULL: 8 everywhere); groups =
- * ceil(k / group), group a multiple of 32 (E_W4_SHAPE).  Strides in elements of a row each;
+ * ceil(k / group), group a multiple of 32, n up to 2^27, m up to 2^20 (E_W4_SHAPE).  Strides in elements of a row each;
  * rows at odd addresses are read as they are, more slowly.  k 0 gives zeros.  Sums are 32-bit,
  * rounded once.  An infinity or NaN in a row of x makes that row of y NaN. */
 typedef struct praghip_w4 {

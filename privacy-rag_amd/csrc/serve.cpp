@@ -71,8 +71,14 @@ CacheArgs cache_args(const praghip_cache& c, size_t heads, float scale, size_t w
   return a;
 }
 
+// (a launch's threads are counted in 32 bits: 256 for a sequence's head, 512 for a
+// prompt's tile)
 bool heads_fit(const praghip_cache& c, size_t heads) {
-  return heads && heads % c.kv_heads == 0 && heads <= 65536 && c.seqs * heads < (1ull << 30);
+  return heads && heads % c.kv_heads == 0 && heads <= 65536 && c.seqs * heads < (size_t(1) << 24);
+}
+bool tiles_fit(const praghip_cache& c, size_t heads, size_t max_rows) {
+  const size_t group = heads / c.kv_heads;
+  return max_rows <= INT_MAX && max_rows * group / 128 + 1 <= ((size_t(1) << 23) - 1) / std::max<size_t>(1, c.seqs * c.kv_heads);
 }
 size_t bound_of(const praghip_cache& c, size_t max_length) {
   const size_t most = size_t(capacity_of(c.table_width, c.page_size));
@@ -163,7 +169,7 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
 
 size_t praghip_paged_prompt_workspace(const praghip_cache* c, size_t heads, size_t max_rows, size_t window, size_t sinks,
                                       size_t max_length) {
-  if (!c || check_cache(c) || !heads_fit(*c, heads) || max_rows > INT_MAX) return 0;
+  if (!c || check_cache(c) || !heads_fit(*c, heads) || !tiles_fit(*c, heads, max_rows)) return 0;
   const size_t group = heads / c->kv_heads;
   const int splits = prompt_splits(c->seqs, c->kv_heads, group, c->head_dim, max_rows,
                                    keys_of(bound_of(*c, max_length), max_rows, window, sinks));
@@ -177,12 +183,12 @@ int praghip_paged_prompt(int device, const praghip_cache* c, const void* q, cons
   if (tokens == 0 || max_rows == 0 || (c && c->seqs == 0)) return PRAGHIP_OK;
   if (const int rc = check_cache(c)) return rc;
   if (!q || !q_strides || !starts || !out || !out_strides) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
-  if (!heads_fit(*c, heads) || !std::isfinite(scale) || tokens > INT_MAX || max_rows > INT_MAX)
+  max_rows = std::min(max_rows, tokens);
+  if (!heads_fit(*c, heads) || !tiles_fit(*c, heads, max_rows) || !std::isfinite(scale) || tokens > INT_MAX)
     return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
   if (!aligned16(q) || !aligned16(out) || !aligned16(work) || !aligned4(lse) || !aligned4(starts) || !eights(q_strides, 2) ||
       !eights(out_strides, 2))
     return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_ALIGNMENT");
-  max_rows = std::min(max_rows, tokens);
   const size_t group = heads / c->kv_heads;
   PromptArgs a{};
   a.splits = prompt_splits(c->seqs, c->kv_heads, group, c->head_dim, max_rows,
@@ -306,7 +312,7 @@ int praghip_matvec_w4(int device, const praghip_w4* w, const void* x, int64_t x_
   if (m == 0 || (w && w->n == 0)) return PRAGHIP_OK;
   if (!w || !y || (w->k && (!w->w || !w->scales || !x))) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
   if (w->type != PRAGHIP_BF16 && w->type != PRAGHIP_F16) return fail(PRAGHIP_E_ARGUMENT, "E_W4_TYPE");
-  if (!w->group || w->group % 32 || w->group > (1u << 30) || w->k > (1u << 30) || w->n > (1u << 30) || m > (1u << 20) ||
+  if (!w->group || w->group % 32 || w->group > (1u << 30) || w->k > (1u << 30) || w->n > (1u << 27) || m > (1u << 20) ||
       w->width > (1u << 30) || w->width < (w->k + 1) / 2)
     return fail(PRAGHIP_E_SHAPE, "E_W4_SHAPE");
   const auto odd = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & 1; };
