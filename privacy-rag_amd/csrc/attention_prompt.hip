@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     for (int b = 0; b < blocks32; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f32x4*>(to + r * D + 32 * b + 8 * e + 4 * half) = f32x4{o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]};
+        *reinterpret_cast<f32x4*>(to + ((8 * b + 2 * e + half) * ROWS + r) * 4) = f32x4{o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]};
     if (half == 0) {
       to[ROWS * D + r] = m;
       to[ROWS * D + ROWS + r] = l;
@@ -478,15 +478,17 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   }
 }
 
-// One wave per row: the splits' m, l and o in order.
+// The splits' m, l and o in order, four values of a row a thread: with the next splits'
+// loads under way, and rows side by side as the workspace has them.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a, int ntile) {
+  constexpr int WG = 1024 / D;  // rows of a workgroup
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63;
-  int64_t index = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int r = int(index % ROWS);
+  int64_t index = int64_t(blockIdx.x) * WG;
+  const int chunk = threadIdx.x / WG, r = int(index % ROWS) + threadIdx.x % WG;
   index /= ROWS;
-  const float* from = a.work + index * a.splits * ROWS * (D + 2);
+  const size_t piece = size_t(ROWS) * (D + 2);
+  const float* const from = a.work + index * a.splits * piece;
   const int kvh = int(index % c.kv_heads);
   index /= c.kv_heads;
   const int tile = int(index % ntile), s = int(index / ntile);
@@ -494,22 +496,33 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptArgs a, int ntil
   const int64_t row = int64_t(tile) * ROWS + r;
   if (row >= int64_t(count) * c.group) return;
   const int token = int(row / c.group), head = kvh * c.group + int(row - int64_t(token) * c.group);
-  float m = kNegInf, l = 0, sum[D / 64] = {};
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, from[int64_t(i) * ROWS * (D + 2) + ROWS * D + r]);
-  for (int i = 0; i < a.splits; ++i) {
-    const float* p = from + int64_t(i) * ROWS * (D + 2);
-    const float f = __builtin_amdgcn_exp2f(p[ROWS * D + r] - origin(m));
-    l += f * p[ROWS * D + ROWS + r];
+  float m = kNegInf, l = 0;
+  f32x4 o = {0, 0, 0, 0};
+  constexpr int AT_ONCE = 4;
+  for (int i = 0; i < a.splits; i += AT_ONCE) {
+    f32x4 po[AT_ONCE];
+    float pm[AT_ONCE], pl[AT_ONCE];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) sum[j] += f * p[r * D + lane + 64 * j];
+    for (int j = 0; j < AT_ONCE; ++j) {  // (of the last split again where there are no more, as nothing)
+      const float* const p = from + size_t(min(i + j, a.splits - 1)) * piece;
+      po[j] = *reinterpret_cast<const f32x4*>(p + (size_t(chunk) * ROWS + r) * 4);
+      pm[j] = i + j < a.splits ? p[ROWS * D + r] : kNegInf;
+      pl[j] = p[ROWS * D + ROWS + r];
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (i + j >= a.splits) break;
+      const float top = fmaxf(m, pm[j]);
+      const float f = __builtin_amdgcn_exp2f(m - origin(top)), pf = __builtin_amdgcn_exp2f(pm[j] - origin(top));
+      o = o * f + po[j] * pf;
+      l = l * f + pl[j] * pf;
+      m = top;
+    }
   }
   const float inv = l > 0 || l != l ? 1.f / l : 0.f;
-#pragma unroll
-  for (int j = 0; j < D / 64; ++j) {
-    const int d = lane + 64 * j;
-    if (d < c.dim) static_cast<T*>(a.out)[(begin + token) * a.out_token + head * a.out_head + d] = T(sum[j] * inv);
-  }
-  if (a.lse && lane == 0) a.lse[int64_t(begin + token) * c.kv_heads * c.group + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  T* const out = static_cast<T*>(a.out) + (begin + token) * a.out_token + head * a.out_head;
+  if (4 * chunk < c.dim) *reinterpret_cast<u32x2*>(out + 4 * chunk) = u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+  if (a.lse && chunk == 0) a.lse[int64_t(begin + token) * c.kv_heads * c.group + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // rows of a workgroup: eight waves of 32, four where a row of 256 values takes the
@@ -528,7 +541,7 @@ hipError_t launch(const PromptArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(kernel, dim3(groups * a.splits), dim3(NW * 64), lds, s, a, ntile);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((prompt_join_kernel<T, D, 32 * NW>), dim3(groups * (32 * NW / 4)), dim3(256), 0, s, a, ntile);
+  hipLaunchKernelGGL((prompt_join_kernel<T, D, 32 * NW>), dim3(groups * (32 * NW * D / 1024)), dim3(256), 0, s, a, ntile);
   return hipGetLastError();
 }
 
@@ -541,8 +554,13 @@ hipError_t launch_dim(const PromptArgs& a, hipStream_t s) {
 
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys) {
   const size_t tiles = size_t(tiles_of(max_rows, group, dim)) * seqs * kv_heads;
+  // One tile alone has a CU; more than one of them there gained nothing (16 query heads of
+  // 128 over 8, 512 rows after 4000 keys: 40.5 us, with twice the splits 54.9, with none 130).
+  // Shorter stretches than 256 keys cost the join more than they save (16 rows after 300:
+  // 13.4, of 128 keys 14.7), in rows of 256 values, whose tiles take longer, than 128 (64
+  // rows after 1000: 25.1, of 256 keys 30.4).
   if (!tiles || tiles > 128) return 1;
-  return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, keys / 256)));
+  return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, keys / (dim > 128 ? 128 : 256))));
 }
 size_t prompt_work_floats(int splits, size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows) {
   if (splits <= 1) return 0;
