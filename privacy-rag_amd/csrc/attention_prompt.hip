@@ -360,6 +360,11 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
     if (i + 2 < i1) turn(i + 2, std::integral_constant<int, 2>{});
     if (i + 3 < i1) turn(i + 3, std::integral_constant<int, 3>{});
   }
+  // The arguments once more: held across the loop they cost registers that it lacks, and a
+  // kernel with anything in scratch memory starts later.
+  typedef const __attribute__((address_space(4))) PromptArgs* Again;
+  Again again = (Again)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(again));
   // V may hold values that are not finite, and of keys that only some rows of a tile see the
   // others' P of 0 makes NaN.  Where O is not finite it is formed again from the cache, with
   // the maximum known: 32 keys at a time, those with such values one by one, each added where
@@ -382,17 +387,17 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
       uint32_t held = 0;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int key = kb + 16 * n, entry = key >> c.page_shift;
-        const int page = entry < width ? c.tables[s * c.table_stride + entry] : -1;
-        const bool none = page < 0 || page >= c.pages;
-        const uint64_t at = none ? 0 : page, in = key & ((1 << c.page_shift) - 1);
+        const int key = kb + 16 * n, entry = key >> again->c.page_shift;
+        const int page = entry < width ? again->c.tables[s * again->c.table_stride + entry] : -1;
+        const bool none = page < 0 || page >= again->c.pages;
+        const uint64_t at = none ? 0 : page, in = key & ((1 << again->c.page_shift) - 1);
         held |= uint32_t(!none) << n;
-        kp[n] = static_cast<const T*>(c.k) + uint64_t(kvh) * c.k_head + at * c.k_page + in * c.k_token;
-        vp[n] = static_cast<const T*>(c.v) + uint64_t(kvh) * c.v_head + at * c.v_page + in * c.v_token;
+        kp[n] = static_cast<const T*>(again->c.k) + uint64_t(kvh) * again->c.k_head + at * again->c.k_page + in * again->c.k_token;
+        vp[n] = static_cast<const T*>(again->c.v) + uint64_t(kvh) * again->c.v_head + at * again->c.v_page + in * again->c.v_token;
       }
       const auto seen = [&](int key) {
         const int j = kb + key;
-        return bool((j <= place) & ((j > from) | (j < c.sinks)) & bool(held >> (key >> 4) & 1));
+        return bool((j <= place) & ((j > from) | (j < again->c.sinks)) & bool(held >> (key >> 4) & 1));
       };
       f32x16 score;
 #pragma unroll
@@ -401,7 +406,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
       for (int n = 0; n < steps; ++n) {
         u32x4 k = {0, 0, 0, 0};
         const int d = 16 * n + 8 * half;
-        if (EXACT || d < c.dim) k = *reinterpret_cast<const u32x4*>((col < 16 ? kp[0] : kp[1]) + uint64_t(col & 15) * c.k_token + d);
+        if (EXACT || d < again->c.dim) k = *reinterpret_cast<const u32x4*>((col < 16 ? kp[0] : kp[1]) + uint64_t(col & 15) * again->c.k_token + d);
         score = Half<T>::mma32(k, q[n], score);
       }
 #pragma unroll
@@ -423,8 +428,8 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
           for (int e = 0; e < 8; ++e) {
             const int key = 8 * (e >> 2) + 4 * half + (e & 3);
             uint32_t bits = 0;
-            if ((EXACT || d < c.dim) && (held >> n & 1) && kb + 16 * n + key < len)
-              bits = *reinterpret_cast<const uint16_t*>(vp[n] + uint64_t(key) * c.v_token + d);
+            if ((EXACT || d < again->c.dim) && (held >> n & 1) && kb + 16 * n + key < len)
+              bits = *reinterpret_cast<const uint16_t*>(vp[n] + uint64_t(key) * again->c.v_token + d);
             constexpr uint32_t exponent = std::is_same<T, __bf16>::value ? 0x7f80 : 0x7c00;
             apart |= (bits & exponent) == exponent;
             v[e >> 1] |= bits << 16 * (e & 1);
@@ -454,22 +459,26 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   l = sum32(l);
   m *= c.scale;
 
-  if (a.splits == 1) {
-    if (!has) return;
+  int place_in = lane;  // (the row's place in the output is found again, too)
+  asm volatile("" : "+v"(place_in));
+  const int64_t out_row = row0 + wave * 32 + (place_in & 31);
+  if (out_row >= nrow) return;
+  if (again->splits == 1) {
+    const int out_token = int(out_row / again->c.group), out_head = kvh * again->c.group + int(out_row - int64_t(out_token) * again->c.group);
     const float r = l > 0 || l != l ? 1.f / l : 0.f;
-    T* out = static_cast<T*>(a.out) + (begin + token) * a.out_token + head * a.out_head;
+    T* out = static_cast<T*>(again->out) + (begin + out_token) * again->out_token + out_head * again->out_head;
 #pragma unroll
     for (int b = 0; b < blocks32; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = 32 * b + 8 * e + 4 * half;
-        if (EXACT || d < c.dim)
+        if (EXACT || d < again->c.dim)
           *reinterpret_cast<u32x2*>(out + d) = u32x2{pack2<T>(o[b][4 * e] * r, o[b][4 * e + 1] * r), pack2<T>(o[b][4 * e + 2] * r, o[b][4 * e + 3] * r)};
       }
-    if (a.lse && half == 0)
-      a.lse[int64_t(begin + token) * c.kv_heads * c.group + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-  } else if (has) {
-    float* to = a.work + (((int64_t(s) * ntile + tile) * c.kv_heads + kvh) * a.splits + split) * ROWS * (D + 2);
+    if (again->lse && half == 0)
+      again->lse[int64_t(begin + out_token) * again->c.kv_heads * again->c.group + out_head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  } else {
+    float* to = again->work + (((int64_t(s) * ntile + tile) * again->c.kv_heads + kvh) * again->splits + split) * ROWS * (D + 2);
     const int r = wave * 32 + col;
 #pragma unroll
     for (int b = 0; b < blocks32; ++b)
