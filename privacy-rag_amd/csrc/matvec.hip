@@ -20,7 +20,7 @@
 //   that keeps all 16 values in one binade, so the difference loses at most two bits
 //   of the 32-bit sum.
 // Waves of a workgroup take K blocks of 128 in turn and add their sums through LDS in
-// order.
+// order.  1024 x 4096, one row: the kernel takes 5.3 us, the host's call 8.1.
 #include "matvec.hpp"
 
 #include <algorithm>
@@ -229,10 +229,10 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
 // so of the same memory channels), and their scales and zero points come as one load of 16
 // and of 8 bytes a column (a load for each of them took more of the memory path than the
 // weights).  x stands in LDS, `part` values of k at a time, in the order that the weights pair
-// up in.  A workgroup stays
-// and takes tiles of columns in turn, and the next turn's weights are under way beside a
-// turn's products (no load stands behind a condition: at the join the compiler would wait
-// for it).
+// up in.  A workgroup stays and takes tiles of columns in turn, and the next turn's weights
+// are under way beside a turn's products (no load stands behind a condition: at the join the
+// compiler would wait for it).  16 rows, K = 1024, 155,648 columns: 24.8 us, 3.7 TB/s of the
+// 5.1 of a large copy.
 template <typename T, int NT, int S>
 struct Turn {
   u32x4 w[2 * S][NT], sc[NT];
@@ -375,12 +375,14 @@ template <typename T>
 hipError_t launch_type(const MatvecArgs& a, hipStream_t s) {
   const int blocks = (a.k + kBlockK - 1) / kBlockK;
   // where there are columns enough for a wave of each SIMD: its turn of eight groups is a
-  // long piece of K
+  // long piece of K (K = 4096, one row: 16384 columns 17.6 us against 26.1, 8192 15.8 against
+  // 16.2; K = 1024, 16 rows: 32768 columns 9.8 against 17.2)
   if (a.aligned && a.vector_scales && a.n >= 16384 && a.k % (8 * a.group) == 0) {
     if (a.group == 32) return launch_groups<T, 1>(a, s);
     if (a.group == 64) return launch_groups<T, 2>(a, s);
     if (a.group == 128) return launch_groups<T, 4>(a, s);
   }
+  // else the waves of a workgroup share K (1024 x 4096, one row: 8.5 us, by one wave a tile 11.9)
   const int kw = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
   return a.m <= 16 ? launch<T, 1>(a, kw, s) : launch<T, 2>(a, kw, s);
 }
