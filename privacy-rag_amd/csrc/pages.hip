@@ -21,6 +21,8 @@
 namespace praghip {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
 __device__ __forceinline__ void refuse(int32_t* status, int code) {
@@ -185,6 +187,19 @@ __global__ void __launch_bounds__(kThreads) page_reserve_kernel(TableArgs t, con
   for (int i = threadIdx.x; i < n; i += kThreads) t.lengths[list[i]] += counts[i];
 }
 
+// i / by and i % by of an i below `most`, in 32 bits where that holds all (a division in 64
+// takes some hundred instructions).
+struct Parts {
+  int64_t whole, rest;
+};
+__device__ __forceinline__ Parts parts(int64_t i, int64_t by, int64_t most) {
+  if (most >> 32 == 0) {
+    const uint32_t q = uint32_t(i) / uint32_t(by);
+    return {q, uint32_t(i) - q * uint32_t(by)};
+  }
+  return {i / by, i % by};
+}
+
 // ----------------------------------------------------------------------- copy
 // moves[i] of all planes, 16 KiB a turn of a workgroup
 __device__ __forceinline__ void copy_pages(const PoolArgs& p, const int32_t* from, const int32_t* to, int moves, unsigned block,
@@ -192,21 +207,22 @@ __device__ __forceinline__ void copy_pages(const PoolArgs& p, const int32_t* fro
   constexpr int kTurn = 256 * 64;
   const int64_t turns = (p.page_bytes + kTurn - 1) / kTurn, items = turns * p.planes * moves;
   for (int64_t i = block; i < items; i += blocks) {
-    const int64_t turn = i % turns, rest = i / turns;
-    const int move = int(rest % moves), plane = int(rest / moves), src = from[move], dst = to[move];
+    const Parts x0 = parts(i, turns, items), x1 = parts(x0.whole, moves, items);
+    const int64_t turn = x0.rest;
+    const int move = int(x1.rest), plane = int(x1.whole), src = from[move], dst = to[move];
     if (src < 0 || src >= p.pages || dst < 0 || dst >= p.pages || src == dst) continue;
     const char* a = p.base + plane * p.plane_bytes + src * p.page_bytes;
     char* b = p.base + plane * p.plane_bytes + dst * p.page_bytes;
-    uint4 x[4];
+    u32x4 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // (no load behind a condition: the compiler would keep x in LDS)
-      x[j] = *reinterpret_cast<const uint4*>(a + min(turn * kTurn + (j * 256 + int64_t(threadIdx.x)) * 16, p.page_bytes - 16));
+      x[j] = *reinterpret_cast<const u32x4*>(a + min(turn * kTurn + (j * 256 + int64_t(threadIdx.x)) * 16, p.page_bytes - 16));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t at = turn * kTurn + (j * 256 + threadIdx.x) * 16;
-      if (at < p.page_bytes) *reinterpret_cast<uint4*>(b + at) = x[j];
+      if (at < p.page_bytes) __builtin_nontemporal_store(x[j], reinterpret_cast<u32x4*>(b + at));
     }
   }
 }
@@ -275,12 +291,14 @@ __global__ void __launch_bounds__(kThreads) fork_plan_kernel(TableArgs t, const 
 }
 
 __global__ void __launch_bounds__(256) fork_apply_kernel(TableArgs t, PoolArgs p, const int32_t* parents,
-                                                         const int32_t* children, int n, const int32_t* work) {
+                                                         const int32_t* children, int n, const int32_t* work, unsigned table_blocks) {
   if (!work[kPlanAllowed]) return;
   const int32_t *from = work + kPlanHead, *to = from + n;
-  const int64_t items = int64_t(n) * t.width, step = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += step) {
-    const int child = int(i / t.width), at = int(i % t.width), s = parents[child], len = t.lengths[s];
+  const int64_t items = int64_t(n) * t.width;
+  if (blockIdx.x >= table_blocks) return copy_pages(p, from, to, n, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += int64_t(table_blocks) * blockDim.x) {
+    const Parts x = parts(i, t.width, items);
+    const int child = int(x.whole), at = int(x.rest), s = parents[child], len = t.lengths[s];
     const int count = pages_for(len, t.page_shift);
     int page = at < count ? t.tables[s * t.stride + at] : -1;
     if (at == count - 1 && to[child] >= 0)
@@ -290,7 +308,6 @@ __global__ void __launch_bounds__(256) fork_apply_kernel(TableArgs t, PoolArgs p
     t.tables[children[child] * t.stride + at] = page;
     if (at == 0) t.lengths[children[child]] = len;
   }
-  copy_pages(p, from, to, n, blockIdx.x, gridDim.x);
 }
 
 // -------------------------------------------------------------------- compact
@@ -337,7 +354,8 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(TableArgs t, PoolArg
   const int32_t *from = work + kPlanHead, *to = from + most, *place = to + most;
   const int64_t items = int64_t(t.seqs) * t.width, step = int64_t(gridDim.x) * blockDim.x;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += step) {
-    int32_t* entry = t.tables + (i / t.width) * t.stride + i % t.width;
+    const Parts x = parts(i, t.width, items);
+    int32_t* entry = t.tables + x.whole * t.stride + x.rest;
     const int page = *entry;
     if (page >= live && page < t.pages) *entry = place[page];
   }
@@ -350,7 +368,8 @@ __global__ void __launch_bounds__(256) page_write_kernel(WriteArgs a) {
   const int chunks = a.row_bytes / 16;
   const int64_t items = int64_t(a.tokens) * a.kv_heads * chunks, step = int64_t(gridDim.x) * blockDim.x;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += step) {
-    const int x = int(i % chunks), h = int(i / chunks % a.kv_heads), token = int(i / chunks / a.kv_heads);
+    const Parts x0 = parts(i, chunks, items), x1 = parts(x0.whole, a.kv_heads, items);
+    const int x = int(x0.rest), h = int(x1.rest), token = int(x1.whole);
     int lo = 0, hi = a.seqs - 1;  // the last sequence that starts at or before the token
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -394,8 +413,9 @@ hipError_t launch_page_fork(const TableArgs& t, const PoolArgs& p, const int32_t
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kThreads), 0, s, t, parents, children, n, work);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(fork_apply_kernel, dim3(grid_of(std::max(copy_items(p, n), int64_t(n) * t.width / 256 + 1), 1)), dim3(256), 0, s, t, p,
-                     parents, children, n, work);
+  // the tables by workgroups of their own, whose chain of reads is as long as a copy's
+  const unsigned tables = std::min(grid_of(int64_t(n) * t.width, 256), 256u);
+  hipLaunchKernelGGL(fork_apply_kernel, dim3(tables + grid_of(copy_items(p, n), 1)), dim3(256), 0, s, t, p, parents, children, n, work, tables);
   return hipGetLastError();
 }
 hipError_t launch_page_compact(const TableArgs& t, const PoolArgs& p, int32_t* work, hipStream_t s) {
