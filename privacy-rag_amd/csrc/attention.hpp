@@ -37,6 +37,7 @@ struct DecodeArgs {
   float* lse;  // [seqs][heads] or null
   float* work;
   uint32_t* base;  // [seqs + 1] key blocks before each sequence
+  bool past;       // whether keys and values are read past the caches
 };
 
 struct PromptArgs {

@@ -27,8 +27,8 @@
 // workgroup holds in part goes to the workspace, at most two pieces of it; the
 // join kernel adds the pieces in order, so results do not depend on timing.
 //
-// 64 sequences of 0 to 8192 tokens, 16 heads of 128 over 8 (627 MB): 131 us, 4.8 TB/s where
-// a large copy has 5.1.  Four through a window of 32768, 32 heads of 64 over 4 (134 MB): 37
+// 64 sequences of 0 to 8192 tokens, 16 heads of 128 over 8 (627 MB): 120 us, 5.2 TB/s where
+// a large copy has 5.1.  Four through a window of 32768, 32 heads of 64 over 4 (134 MB): 35.5
 // us of the copy's 26.  One of 2049 tokens (8 MB): 13.8 us, a chain of dependent reads
 // (lengths, tables, keys) in 10 us and the join's launch in 3.9.
 #include "attention.hpp"
@@ -63,7 +63,14 @@ struct Range {
 // (a multiple of four floats, which the join loads together)
 __host__ __device__ __forceinline__ size_t piece_floats(int rows, int D) { return size_t(rows) * D + (2 * rows + 3) / 4 * 4; }
 
-template <typename T, int D, bool EXACT>
+// a load of the cache, past the caches or not
+template <bool PAST, typename V>
+__device__ __forceinline__ V fetch(const V* p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
+template <typename T, int D, bool EXACT, bool PAST>
 __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a) {
   using S = DecodeShape<T, D>;
   extern __shared__ float lds[];
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
 #pragma unroll
           for (int n = 0; n < S::steps; ++n) {
             kf[t][n] = u32x4{0, 0, 0, 0};
-            if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
+            if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = fetch<PAST>(reinterpret_cast<const u32x4*>(kp + 32 * n));
           }
           const T* vp = static_cast<const T*>(c.v) + uint64_t(page) * c.v_page + uint64_t(kvh) * c.v_head + uint64_t(row + 4 * quad) * c.v_token + S::per * col;
 #pragma unroll
@@ -168,14 +175,14 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
             for (int w = 0; w < S::words; ++w) vr[4 * t + e][w] = 0;
             if (EXACT || S::per * col < c.dim) {
               if constexpr (S::words == 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(vp + uint64_t(e) * c.v_token);
+                const u32x2 x = fetch<PAST>(reinterpret_cast<const u32x2*>(vp + uint64_t(e) * c.v_token));
                 vr[4 * t + e][0] = x[0];
                 vr[4 * t + e][1] = x[1];
               } else {
 #pragma unroll
                 for (int w = 0; w < S::words; w += 4) {
                   if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
-                  const u32x4 x = *reinterpret_cast<const u32x4*>(vp + uint64_t(e) * c.v_token + 2 * w);
+                  const u32x4 x = fetch<PAST>(reinterpret_cast<const u32x4*>(vp + uint64_t(e) * c.v_token + 2 * w));
 #pragma unroll
                   for (int b = 0; b < 4; ++b) vr[4 * t + e][w + b] = x[b];
                 }
@@ -375,7 +382,9 @@ template <typename T, int D>
 hipError_t launch(const DecodeArgs& a, unsigned workgroups, hipStream_t s) {
   const int rows = std::min(a.c.group, 16);
   const size_t lds = 2 * kWaves * piece_floats(rows, D) * sizeof(float);
-  const auto kernel = a.c.dim == D ? paged_decode_kernel<T, D, true> : paged_decode_kernel<T, D, false>;
+  const bool exact = a.c.dim == D;
+  const auto kernel = a.past ? (exact ? paged_decode_kernel<T, D, true, true> : paged_decode_kernel<T, D, false, true>)
+                             : (exact ? paged_decode_kernel<T, D, true, false> : paged_decode_kernel<T, D, false, false>);
   hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kWaves * 64), lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -390,7 +399,7 @@ hipError_t launch_dim(const DecodeArgs& a, unsigned workgroups, hipStream_t s) {
 
 }  // namespace
 
-// As many workgroups as the chip holds at three a CU (two: 140 us where three take 131), and
+// As many workgroups as the chip holds at three a CU (two: 140 us where three took 131), and
 // no more than there are blocks for their waves.
 unsigned decode_workgroups(size_t seqs, size_t kv_heads, size_t group, size_t keys) {
   const size_t blocks = seqs * kv_heads * ((group + 15) / 16) * ((keys + 31) / 32 + 1);

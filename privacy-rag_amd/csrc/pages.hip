@@ -9,9 +9,11 @@
 // its code in `status`.
 //
 // Moving pages is bound by memory: 2 bytes of traffic a byte, 16-byte accesses, four
-// loads of a thread under way.  A compaction that moves 293 MB takes 121 us (4.9 TB/s, a large
-// copy 5.1), a fork's copies of 29 MB 21 us after 5 of plan, 34 MB of new tokens 12.4 us
-// (5.4 TB/s), one token of 64 sequences 4.1 us of the host's 9.9.
+// loads of a thread under way.  Their stores pass the caches by: a kernel's end waits for
+// the dirty lines of all L2s (a fork's 29 MB of copies: 8.1 us, through the caches 21).  A
+// fork takes 5 us of plan before its copies, a compaction's 92 us and 5 of plan.  New tokens
+// go through the caches, where the attention finds them: 34 MB in 12.4 us (5.4 TB/s with
+// their reads), one token of 64 sequences in 4.1 of the host's 9.9.
 #include "pages.hpp"
 
 #include <algorithm>

@@ -46,6 +46,23 @@ def test_forms(gpu, type, dim, window, sinks):
         plain.check_lse(lse[see], wlse)
 
 
+@pytest.mark.parametrize("type", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 56, 128, 120, 256, 248])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 5)])
+def test_decode_of_wide_tables(gpu, type, dim, window, sinks):
+    """Tables with room for a cache that is read past the caches, and short sequences in them;
+    with a window through the caches.  Poison in what no query sees."""
+    print("[forms] wide tables", type, dim, window, sinks, flush=True)
+    width = (64 << 20) // (2 * 2 * dim * 4) // 32 + 2
+    c = plain.make([730, 331], 6, 2, dim, 32, type, seed=dim + window + 1, width=width)
+    q = torch.randn((2, 6, dim), generator=c["g"]).to(type)
+    want, wlse, size = plain.attention(c, q, [0, 1, 2], window=window, sinks=sinks)
+    out, lse = praghip.paged_decode(q.to("cuda"), *to_gpu(c), window=window, sinks=sinks, lse=True)
+    torch.cuda.synchronize()
+    plain.check(out, want, size, type, rounded=False)
+    plain.check_lse(lse, wlse)
+
+
 def rows_of(c, q, starts, see, window, sinks):
     """attention() of some of the rows, each with its keys at once."""
     heads, dim = q.shape[1:]
