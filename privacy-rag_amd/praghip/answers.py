@@ -18,7 +18,8 @@ from .qwen3 import QWEN3_0_6B, Qwen3Shape
 
 
 class Qwen3Answers:
-    """Weights, a cache of `pages` pages for every layer, and up to `slots` sequences.
+    """Weights, a cache of `pages` pages for every layer, and up to `slots` sequences of
+    `capacity` tokens, rounded up to whole pages.
 
     weights: {"embed": [vocab][hidden], "norm": [hidden], "layers": [{"qkv", "o",
     "gate_up", "down": [out][in], "attention_norm", "mlp_norm": [hidden], "q_norm",
@@ -45,7 +46,8 @@ class Qwen3Answers:
         self.status = torch.zeros(1, **ints)
         self.held = [0] * slots  # the lengths, as the host knows them
         half = torch.arange(0, shape.head_dim, 2, dtype=torch.float64, device=self.device)
-        angle = torch.arange(capacity, dtype=torch.float64, device=self.device)[:, None] * theta ** (-half / shape.head_dim)
+        angle = torch.arange(self.tables.shape[1] * page_size, dtype=torch.float64, device=self.device)[:, None] * \
+            theta ** (-half / shape.head_dim)
         self.cos, self.sin = angle.cos().float(), angle.sin().float()
 
     def _ints(self, values):
@@ -101,6 +103,8 @@ class Qwen3Answers:
         sequences, rows = list(sequences), [list(r) for r in rows]
         if len(sequences) != len(rows) or not rows or not all(rows):
             raise ValueError("each sequence takes one token or more")
+        if any(not 0 <= t < self.embed.shape[0] for r in rows for t in r):
+            raise ValueError("a token outside the vocabulary")
         listed = self._ints(sequences)
         page_reserve(self.tables, self.lengths, self.refs, self.page_size, listed, self._ints(map(len, rows)), self.status)
         page_check(self.status)

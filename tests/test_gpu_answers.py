@@ -116,3 +116,22 @@ def test_pages_that_do_not_suffice(gpu):
         m.extend([0], [[1] * 99])
     assert m.held == [30, 0] == m.lengths.tolist()
     near(m.extend([1], [[5, 6, 7]])[0], plain(m, [5, 6, 7]), torch.float16)
+
+
+def test_the_last_position_and_what_is_refused(gpu):
+    """A capacity that is no whole number of pages is rounded up, and its last position used."""
+    m = model(torch.float16, slots=2, pages=8, capacity=20)
+    tokens = [(7 * i) % VOCAB for i in range(32)]
+    m.extend([0], [tokens[:31]])
+    near(m.extend([0], [tokens[31:]])[0], plain(m, tokens), torch.float16)
+    with pytest.raises(praghip.PraghipError, match="E_PAGES_CAPACITY"):
+        m.extend([0], [[1]])
+    for bad in ([[]], [[VOCAB]], [[-1]], [[1], [2]]):
+        with pytest.raises(ValueError):
+            m.extend([1], bad)
+    for sequences in ([1, 1], [2], [-1]):
+        with pytest.raises(praghip.PraghipError, match="E_PAGES_SEQUENCE"):
+            m.extend(sequences, [[1]] * len(sequences))
+    with pytest.raises(praghip.PraghipError, match="E_PAGES_SEQUENCE"):
+        m.fork(0, [0])
+    assert m.held == [32, 0] == m.lengths.tolist()
