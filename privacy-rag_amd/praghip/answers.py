@@ -69,17 +69,20 @@ class Qwen3Answers:
 
     def _forward(self, sequences, rows):
         """Logits after the newest tokens, rows[i] of sequences[i], which have their pages already."""
+        at = self._ints(sequences).long()
+        ends = [sum(len(r) for r in rows[: i + 1]) for i in range(len(rows))]
+        places = self._ints(self.held[s] - len(r) + i for s, r in zip(sequences, rows) for i in range(len(r))).long()
+        x = self._layers(self._ints(t for r in rows for t in r).long(), places, self.tables[at], self.lengths[at],
+                         self._ints([0] + ends), max(len(r) for r in rows), max(self.held[s] for s in sequences))
+        return self._logits(x[self._ints(e - 1 for e in ends).long()])
+
+    def _layers(self, tokens, places, tables, lengths, starts, most: int, longest: int):
+        """The last layer's output of tokens at `places`, rows starts[s] .. of the sequences whose tables these are."""
         import torch
         shape = self.shape
-        at = self._ints(sequences).long()
-        tables, lengths = self.tables[at], self.lengths[at]
-        ends = [sum(len(r) for r in rows[: i + 1]) for i in range(len(rows))]
-        starts = self._ints([0] + ends)
-        places = self._ints(self.held[s] - len(r) + i for s, r in zip(sequences, rows) for i in range(len(r))).long()
-        longest, most = max(self.held[s] for s in sequences), max(len(r) for r in rows)
         see = dict(window=self.window, sinks=self.sinks, max_length=longest)
         q_out, kv_out = shape.q_heads * shape.head_dim, shape.kv_heads * shape.head_dim
-        x = self.embed[self._ints(t for r in rows for t in r).long()]
+        x = self.embed[tokens]
         for layer, (keys, values) in zip(self.layers, self.pool):
             qkv = self._product(self._normed(x, layer["attention_norm"]), layer["qkv"])
             q, k, v = (t.unflatten(1, (-1, shape.head_dim)) for t in qkv.split((q_out, kv_out, kv_out), 1))
@@ -93,8 +96,10 @@ class Qwen3Answers:
             x = x + self._product(o.flatten(1), layer["o"])
             gate, up = self._product(self._normed(x, layer["mlp_norm"]), layer["gate_up"]).chunk(2, 1)
             x = x + self._product((torch.nn.functional.silu(gate.float()) * up.float()).to(self.type), layer["down"])
-        last = self._normed(x[self._ints(e - 1 for e in ends).long()], self.norm)
-        return self._product(last, self.head)
+        return x
+
+    def _logits(self, x):
+        return self._product(self._normed(x, self.norm), self.head)
 
     def extend(self, sequences, rows):
         """Appends rows[i], a list of one token or more, to sequences[i]; returns the logits
@@ -106,14 +111,63 @@ class Qwen3Answers:
         if any(not 0 <= t < self.embed.shape[0] for r in rows for t in r):
             raise ValueError("a token outside the vocabulary")
         listed = self._ints(sequences)
-        page_reserve(self.tables, self.lengths, self.refs, self.page_size, listed, self._ints(map(len, rows)), self.status)
-        page_check(self.status)
-        for s, r in zip(sequences, rows):
-            self.held[s] += len(r)
+        self._reserve(sequences, listed, self._ints(map(len, rows)), [len(r) for r in rows])
         logits = self._forward(sequences, rows)
+        self._trim(listed)
+        return logits
+
+    def _reserve(self, sequences, listed, counts, more):
+        page_reserve(self.tables, self.lengths, self.refs, self.page_size, listed, counts, self.status)
+        page_check(self.status)
+        for s, n in zip(sequences, more):
+            self.held[s] += n
+
+    def _trim(self, listed):
         if self.window:
             page_trim(self.tables, self.lengths, self.refs, self.page_size, listed, self.window, self.sinks, self.status)
-        return logits
+
+    def steps(self, sequences):
+        """A function that appends one token to each of these sequences, given as a list or an
+        int64 tensor (whose values outside the vocabulary count as its nearest), and returns
+        the logits after them (in the same memory each time): the layers' calls, some 30 a
+        layer, as one captured graph.  The sequences may be forked, ended and extended between
+        its calls."""
+        import torch
+        sequences = list(sequences)
+        if not sequences or any(not 0 <= s < len(self.held) for s in sequences):
+            raise ValueError("no such sequence")
+        n, capacity = len(sequences), self.tables.shape[1] * self.page_size
+        listed, ones = self._ints(sequences), self._ints([1] * n)
+        at, starts = listed.long(), self._ints(range(n + 1))
+        tokens = torch.zeros(n, dtype=torch.int64, device=self.device)
+
+        def forward():
+            lengths = self.lengths[at]
+            places = (lengths - 1).clamp(min=0).long()
+            return self._logits(self._layers(tokens.clamp(0, self.embed.shape[0] - 1), places, self.tables[at], lengths,
+                                             starts, 1, capacity))
+
+        held = self.lengths.clone()
+        self.lengths.zero_()  # (a first time outside, which loads code and writes nothing)
+        forward()
+        self.lengths.copy_(held)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = forward()
+
+        def step(new):
+            if not isinstance(new, torch.Tensor):
+                if len(new) != n or any(not 0 <= t < self.embed.shape[0] for t in new):
+                    raise ValueError("one token of the vocabulary for each sequence")
+                new = torch.tensor(new)
+            self._reserve(sequences, listed, ones, [1] * n)
+            tokens.copy_(new)
+            graph.replay()
+            self._trim(listed)
+            return logits
+
+        step.reads = at, starts  # (the graph's addresses: they live as long as it does)
+        return step
 
     def fork(self, parent: int, children) -> None:
         """The empty sequences `children` go on from the parent's tokens, whose full pages they share."""
@@ -187,8 +241,9 @@ def main() -> None:
         timed("fork", lambda: model.fork(0, answers))
         tokens = logits[0].topk(args.answers).indices.tolist()
         said = [[t] for t in tokens]
+        step = timed("capture", lambda: model.steps(answers))
         for _ in range(args.tokens - 1):
-            tokens = timed("token", lambda: model.extend(answers, [[t] for t in tokens]).argmax(-1).tolist())
+            tokens = timed("token", lambda: step(tokens).argmax(-1).tolist())
             for s, t in zip(said, tokens):
                 s.append(t)
         timed("end", lambda: model.end(range(0, 1 + args.answers)))

@@ -135,3 +135,45 @@ def test_the_last_position_and_what_is_refused(gpu):
     with pytest.raises(praghip.PraghipError, match="E_PAGES_SEQUENCE"):
         m.fork(0, [0])
     assert m.held == [32, 0] == m.lengths.tolist()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 2)])
+def test_steps_of_a_captured_graph(gpu, window, sinks):
+    """Every replay against an eager model with the same tokens, with forks, ends, compactions
+    and eager extensions between them, and the last against 64 bits."""
+    print("[answers] steps", window, sinks, flush=True)
+    both = [model(torch.float16, slots=4, pages=30, capacity=128, window=window, sinks=sinks) for _ in range(2)]
+    g = torch.Generator().manual_seed(6)
+    said = {0: torch.randint(0, VOCAB, (45,), generator=g).tolist()}
+    for m in both:
+        m.extend([0], [said[0]])
+        m.fork(0, [1, 2])
+    said |= {1: list(said[0]), 2: list(said[0])}
+    m, eager = both
+    step = m.steps([2, 1])
+    assert m.lengths.tolist() == eager.lengths.tolist() and torch.equal(m.pool, eager.pool)
+    for i in range(20):
+        new = torch.randint(0, VOCAB, (2,), generator=g).tolist()
+        got = step(new if i % 2 else torch.tensor(new, device="cuda"))
+        want = eager.extend([2, 1], [[t] for t in new])
+        said[2].append(new[0]), said[1].append(new[1])
+        # (the launch's size may differ, and with it the order of a sum)
+        near(got, want.cpu().double(), torch.float16)
+        if i == 5:
+            for x in both:
+                x.end([0])
+                x.compact()
+        if i == 9:
+            for x in both:
+                x.extend([1], [[3, 4, 5]])
+            said[1] += [3, 4, 5]
+    for i, s in enumerate((2, 1)):
+        near(got[i], plain(m, said[s]), torch.float16)
+    for bad in ([], [4], [-1]):
+        with pytest.raises(ValueError):
+            m.steps(bad)
+    with pytest.raises(ValueError):
+        step([1])
+    with pytest.raises(ValueError):
+        step([1, VOCAB])
+    assert m.lengths.tolist() == eager.lengths.tolist() == m.held
