@@ -583,7 +583,7 @@ hipError_t launch_dim(const PromptArgs& a, hipStream_t s) {
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys) {
   const size_t tiles = size_t(tiles_of(max_rows, group, dim)) * seqs * kv_heads;
   // One tile alone has a CU; more than one of them there gained nothing (16 query heads of
-  // 128 over 8, 512 rows after 4000 keys: 40.5 us, with twice the splits 54.9, with none 130).
+  // 128 over 8, 512 rows after 4000 keys: 37 us, with twice the splits 14 more, with none 130).
   // Shorter stretches than 256 keys cost the join more than they save (16 rows after 300:
   // 13.4, of 128 keys 14.7), in rows of 256 values, whose tiles take longer, than 128 (64
   // rows after 1000: 25.1, of 256 keys 30.4).
