@@ -29,7 +29,7 @@
 //
 // 64 sequences of 0 to 8192 tokens, 16 heads of 128 over 8 (627 MB): 120 us, 5.2 TB/s where
 // a large copy has 5.1.  Four through a window of 32768, 32 heads of 64 over 4 (134 MB): 35.5
-// us of the copy's 26.  One of 2049 tokens (8 MB): 12.8 us, a chain of dependent reads
+// us of the copy's 26.  One of 2049 tokens (8 MB): 13.9 us, a chain of dependent reads
 // (lengths, tables, keys) in 10 us and the join's launch in 3.9.
 #include "attention.hpp"
 

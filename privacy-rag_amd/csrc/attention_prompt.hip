@@ -26,7 +26,7 @@
 // workgroups; their m, l and o go to the workspace and a second kernel joins them in
 // order.
 //
-// 8192 tokens, 16 heads of 128 over 8: 268 us, 1.0 PFLOP/s (a large bfloat16 product of the
+// 8192 tokens, 16 heads of 128 over 8: 273 us, 1.0 PFLOP/s (a large bfloat16 product of the
 // library's reaches 1.2): matrix cores and vector units are busy 45% of the time each, hardly
 // at once, with the two waves that a SIMD has registers for.  Four chunks of up to 512 tokens
 // through a window of 2048, 32 heads of 64 over 4: 54 us, with CUs busy 57% of the time, as
