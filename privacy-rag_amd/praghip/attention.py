@@ -4,6 +4,11 @@
 The reference's attention is a two-party protocol; these serve a model in the
 clear beside it, and have no counterpart there.  Tensors are on one GPU; calls
 are asynchronous on ``stream`` (the tensors' device's current stream by default).
+
+On another stream than the current one a call's workspace and the tensors that it
+returns come from that stream's memory, so they wait for nothing.  The caller orders
+the rest: ``stream`` behind the work that makes the call's inputs, the current stream
+behind ``stream`` before it reads the result, and inputs kept until the call is done.
 """
 from __future__ import annotations
 
@@ -74,9 +79,27 @@ def _starts(t, seqs: int, index: int) -> int:
     return t.data_ptr()
 
 
-def _output(q, shape, out, index: int):
+def _allocate(stream, make, *args, **kw):
+    """make(...), a tensor that a call on `stream` writes, from the memory of that stream: a
+    block of the current one's may have been freed there with work under way that uses it."""
+    if stream is None:
+        return make(*args, **kw)
+    with _torch.cuda.stream(stream):
+        return make(*args, **kw)
+
+
+def _result(stream, index: int, make, *args, **kw):
+    """The same for what a call returns: its block goes back once the current stream, where it
+    is read, is done with it too."""
+    t = _allocate(stream, make, *args, **kw)
+    if stream is not None:
+        t.record_stream(_torch.cuda.current_stream(index))
+    return t
+
+
+def _output(q, shape, out, index: int, stream):
     if out is None:
-        return _torch.empty_like(q)
+        return _result(stream, index, _torch.empty_like, q)
     if out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or \
             (shape[2] > 1 and out.stride(2) != 1):
         raise shape_error("E_ATTENTION_OUT")
@@ -84,11 +107,8 @@ def _output(q, shape, out, index: int):
 
 
 def _work(size: int, like, stream):
-    """Workspace of one call; torch's allocator keeps it until `stream` is done with it."""
-    work = _torch.empty(size, dtype=_uint8, device=like.device)
-    if stream is not None:
-        work.record_stream(stream)
-    return work
+    """Workspace of one call, which `stream` alone uses."""
+    return _allocate(stream, _torch.empty, size, dtype=_uint8, device=like.device)
 
 
 def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = None, window: int = 0, sinks: int = 0,
@@ -113,8 +133,8 @@ def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = 
     if len(shape) != 3 or shape[0] != seqs or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0:
         raise shape_error("E_ATTENTION_SHAPE")
-    out = _output(q, shape, out, index)
-    sums = _torch.empty(shape[:2], dtype=_torch.float32, device=q.device) if lse else None
+    out = _output(q, shape, out, index, stream)
+    sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
     if seqs:
         L, heads, to = lib(), shape[1], out.stride()
         size = L.praghip_paged_decode_workspace(cache, heads, max_length)
@@ -143,8 +163,8 @@ def paged_prompt(q, k_pages, v_pages, tables, lengths, starts, max_rows: int, *,
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0 or max_rows < 0:
         raise shape_error("E_ATTENTION_SHAPE")
     first = _starts(starts, seqs, index)
-    out = _output(q, shape, out, index)
-    sums = _torch.empty(shape[:2], dtype=_torch.float32, device=q.device) if lse else None
+    out = _output(q, shape, out, index, stream)
+    sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
     tokens, heads = shape[0], shape[1]
     if tokens and seqs:
         L, to = lib(), out.stride()

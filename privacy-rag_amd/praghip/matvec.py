@@ -1,11 +1,12 @@
-"""Products of a few rows with 4-bit weights and group scales."""
+"""Products of a few rows with 4-bit weights and group scales (streams as in
+:mod:`praghip.attention`)."""
 from __future__ import annotations
 
 import struct
 
 from . import attention
 from ._lib import check, lib, shape_error
-from .attention import _kind, _stream, _type_error
+from .attention import _kind, _result, _stream, _type_error
 
 _W4 = struct.Struct("PqPqPq4Qi4x").pack  # praghip_w4
 
@@ -37,7 +38,7 @@ def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, str
             raise shape_error("E_W4_SHAPE")
         zero, zs = zeros.data_ptr(), zeros.stride(0)
     if out is None:
-        out = x.new_empty((m, n))
+        out = _result(stream, index, x.new_empty, (m, n))
     elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != index or \
             (n > 1 and out.stride(1) != 1):
         raise shape_error("E_W4_OUT")

@@ -9,7 +9,8 @@ and keys or values.
 
 The lists (int32 on the GPU, each sequence at most once) are checked there: a call
 that is refused changes nothing and leaves a code in ``status`` (int32 [1], if given,
-while it is 0), which :func:`page_check` turns into an error.
+while it is 0), which :func:`page_check` turns into an error.  Streams are as in
+:mod:`praghip.attention`.
 """
 from __future__ import annotations
 
