@@ -18,6 +18,7 @@
 
 #include <algorithm>
 
+#include "page_rule.hpp"
 #include "praghip.h"
 
 namespace praghip {
@@ -49,15 +50,16 @@ __device__ __forceinline__ bool distinct(const int32_t* list, int n, int seqs, u
 
 // Sum over the workgroup of a wave's value (the same in its lanes), and the sum of
 // the waves before; all threads call it.
-__device__ __forceinline__ int waves_before(int value, int* lds, int& total) {
+template <typename T>
+__device__ __forceinline__ T waves_before(T value, T* lds, T& total) {
   const int wave = threadIdx.x >> 6;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[wave] = value;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
   for (int w = 0; w < kWaves; ++w) {
-    const int x = lds[w];
+    const T x = lds[w];
     total += x;
     if (w < wave) before += x;
   }
@@ -100,8 +102,6 @@ __device__ __forceinline__ bool give_free(const int32_t* refs, int pages, int ne
   return true;
 }
 
-__device__ __forceinline__ int pages_for(int64_t tokens, int shift) { return int((tokens + (1ll << shift) - 1) >> shift); }
-
 // ----------------------------------------------------------------- free, trim
 // Every workgroup checks the whole list and takes its share of the entries.
 __global__ void __launch_bounds__(256) page_free_kernel(TableArgs t, const int32_t* list, int n, int window, int sinks,
@@ -134,35 +134,42 @@ __global__ void __launch_bounds__(kThreads) page_reserve_kernel(TableArgs t, con
                                                                 int n) {
   __shared__ uint32_t seen[kMaxSequences / 32];
   __shared__ int start[kMaxList + 1];  // new pages before each sequence's
+  __shared__ int64_t sums[kWaves];
   __shared__ int bad, part[kWaves];
   if (!distinct(list, n, t.seqs, seen, &bad)) {
     if (threadIdx.x == 0) refuse(t.status, PRAGHIP_PAGES_SEQUENCE);
     return;
   }
   const int per = (n + kThreads - 1) / kThreads;
-  int mine = 0;
+  int64_t mine = 0;
   for (int i = threadIdx.x * per; i < min(n, int(threadIdx.x + 1) * per); ++i) {
-    const int64_t old = t.lengths[list[i]], now = old + counts[i];
-    if (old < 0 || counts[i] < 0 || now > int64_t(t.width) << t.page_shift)
+    const int64_t pages = new_pages(t.lengths[list[i]], counts[i], t.width, t.page_shift);
+    if (pages < 0)
       bad = 1;
     else
-      mine += pages_for(now, t.page_shift) - pages_for(old, t.page_shift);
+      mine += pages;
   }
-  int sum = mine;
+  int64_t sum = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(sum, d, 64);
+    const int64_t up = __shfl_up(sum, d, 64);
     if (int(threadIdx.x & 63) >= d) sum += up;
   }
-  int need, before = waves_before(__shfl(sum, 63, 64), part, need) + sum - mine;
+  int64_t all;
+  const int64_t first = waves_before(__shfl(sum, 63, 64), sums, all) + sum - mine;
   if (bad) {
     if (threadIdx.x == 0) refuse(t.status, PRAGHIP_PAGES_CAPACITY);
     return;
   }
+  if (all > t.pages) {  // (below that 32 bits hold it)
+    if (threadIdx.x == 0) refuse(t.status, PRAGHIP_PAGES_EXHAUSTED);
+    return;
+  }
+  const int need = int(all);
+  int before = int(first);
   for (int i = threadIdx.x * per; i < min(n, int(threadIdx.x + 1) * per); ++i) {
     start[i] = before;
-    const int64_t old = t.lengths[list[i]];
-    before += pages_for(old + counts[i], t.page_shift) - pages_for(old, t.page_shift);
+    before += int(new_pages(t.lengths[list[i]], counts[i], t.width, t.page_shift));
   }
   if (threadIdx.x == 0) start[n] = need;
   __syncthreads();
