@@ -652,7 +652,7 @@ int praghip_paged_prompt(int device, const praghip_cache *cache, const void *q, 
  * where status (device, or NULL) is 0, sets it to a PRAGHIP_PAGES_* code; a later call
  * does not clear it. */
 #define PRAGHIP_PAGES_SEQUENCE 1  /* a name out of range or twice; a child that is not empty or is a parent */
-#define PRAGHIP_PAGES_CAPACITY 2  /* a negative count, or more tokens than a row of the tables holds */
+#define PRAGHIP_PAGES_CAPACITY 2  /* a negative count, or more tokens than a row of the tables, or 2^31 - 1, holds */
 #define PRAGHIP_PAGES_EXHAUSTED 3 /* fewer free pages than the call needs */
 typedef struct praghip_page_table {
   int32_t *tables; /* [seqs][width] */

@@ -39,3 +39,11 @@ def test_pages_of_one_sequence(summed, shift):
 def test_what_may_not_be(summed):
     for row in ((-1, 2, 9, 4), (5, -1, 9, 4), (144, 1, 9, 4), (0, 2 ** 31 - 1, 9, 4)):
         assert summed([(0, 1, 9, 4), row, (0, 1, 9, 4)]) == "refused"
+
+
+def test_a_length_has_32_bits(summed):
+    most, width = 2 ** 31 - 1, 65600  # pages of 32768: room for more tokens than a length counts
+    assert summed([(0, most, width, 15)]) == 65536
+    assert summed([(most - 40000, 40000, width, 15)]) == 1
+    for old, more in ((most, 1), (1, most), (most - 40000, 40001), (most, most)):
+        assert summed([(old, more, width, 15)]) == "refused"
