@@ -50,6 +50,7 @@ struct PromptArgs {
   const int32_t* starts;
   int total, max_rows, splits;
   float* work;
+  float lower;  // how far a score's origin is kept below the maximum, before the scale
 };
 
 hipError_t launch_paged_decode(const DecodeArgs& a, int type, unsigned workgroups, hipStream_t s);
@@ -65,10 +66,19 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// Vectors and matrix instructions of one 16-bit type, and the power of two that P may
+// reach in it.
+//
+// P = 2^(x - m) of a score x in powers of two goes into a product in the type.  bfloat16 has
+// as many powers below 1 as 32 bits have, so m is the maximum.  float16 ends at 2^-24: keys 18
+// below the strongest in the natural exponent (2^-26) would vanish from O while l counts them,
+// 10^5 of them 2e-3 of the output, and all of it where the strongest key's value is 0.  So m
+// is kept below the maximum there and P goes up to 2^15; l, O and lse hold the same m.
 template <typename T>
-struct Half;  // vectors and matrix instructions of one 16-bit type
+struct Half;
 template <>
 struct Half<__bf16> {
+  static constexpr float most = 0;
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -80,6 +90,7 @@ struct Half<__bf16> {
 };
 template <>
 struct Half<_Float16> {
+  static constexpr float most = 15;
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {

@@ -20,7 +20,8 @@
 // * 16 query columns are the heads of one key/value head (groups above 16 take
 //   several turns), so m, l and the factor of O are one value per lane.
 // P goes into the product as a sum of two 16-bit values: 8 more of 24 products per
-// block, which the loads hide, and the rounding of P drops out of the error.
+// block, which the loads hide, and the rounding of P drops out of the error (in float16,
+// whose P is up to 2^15, it is 2^-40 of the strongest key's).
 //
 // A stretch that holds a head's blocks from first to last writes the output.
 // Else its m, l and o go to LDS, where the workgroup merges neighbours, and what a
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
           }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        top = fmaxf(m, max32(max16(top)));
+        top = fmaxf(m, max32(max16(top)) - Half<T>::most);
         if (__any(top > m)) {
           const float f = __builtin_amdgcn_exp2f(m - origin(top));
           l *= f;

@@ -76,3 +76,22 @@ def test_all_of_a_heads_keys_in_one_wave(gpu, heads):
             plain.check_lse(lse[:, at], wlse[1:])
             plain.check(both[:, at], want, size, F16, rounded=True)
             plain.check_lse(sums[:, at], wlse)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.125, 30.0])
+def test_scales(gpu, scale):
+    """float16 at scales of any size: what P's range is chosen by."""
+    print("[small] scale", scale, flush=True)
+    c = plain.make([150, 41], 8, 4, 64, 16, F16, seed=43)
+    q = (torch.randn((60, 8, 64), generator=c["g"]) * (0.01 if scale == 30.0 else 1)).to(F16)
+    on = [c[x].to("cuda") for x in ("k", "v", "tables", "lengths")]
+    starts = [0, 40, 60]
+    want, wlse, size = plain.attention(c, q, starts, scale=scale, window=50, sinks=3)
+    out, lse = praghip.paged_prompt(q.to("cuda"), *on, torch.tensor(starts, dtype=torch.int32, device="cuda"), 40,
+                                    scale=scale, window=50, sinks=3, lse=True)
+    plain.check(out, want, size, F16, rounded=True)
+    plain.check_lse(lse, wlse)
+    want, wlse, size = plain.attention(c, q[:2], [0, 1, 2], scale=scale, window=50, sinks=3)
+    out, lse = praghip.paged_decode(q[:2].to("cuda"), *on, scale=scale, window=50, sinks=3, lse=True)
+    plain.check(out, want, size, F16, rounded=False)
+    plain.check_lse(lse, wlse)
