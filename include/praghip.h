@@ -634,7 +634,9 @@ int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, 
  * already.  Causal, with window and sinks as above; a row whose position is below 0 sees
  * nothing.  max_rows is at least the longest of these stretches; rows beyond it are not
  * computed.  seqs x kv_heads x (max_rows x group / 128 + 1) is below 2^23
- * (E_ATTENTION_SHAPE).  lse: [tokens][heads]. */
+ * (E_ATTENTION_SHAPE).  lse: [tokens][heads].  work: at least the bytes that the workspace
+ * function names for the same arguments, NULL where that is 0; more rows may need less, as their
+ * tiles fill the chip without splitting their keys. */
 size_t praghip_paged_prompt_workspace(const praghip_cache *cache, size_t heads, size_t max_rows, size_t window,
                                       size_t sinks, size_t max_length);
 int praghip_paged_prompt(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,

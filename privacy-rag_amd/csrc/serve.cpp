@@ -94,6 +94,15 @@ size_t keys_of(size_t bound, size_t rows, size_t window, size_t sinks) {
   return window && window < bound ? std::min(bound, window + std::min(sinks, bound) + rows) : bound;
 }
 
+// Workgroups that share a tile's keys, by the arguments that both the call and its workspace
+// function have: with the call's smaller max_rows (no longer than its tokens) fewer tiles would
+// take more splits than the workspace has room for.
+int splits_of(const praghip_cache& c, size_t heads, size_t max_rows, size_t window, size_t sinks, size_t max_length) {
+  if (!tiles_fit(c, heads, max_rows)) return 1;
+  return prompt_splits(c.seqs, c.kv_heads, heads / c.kv_heads, c.head_dim, max_rows,
+                       keys_of(bound_of(c, max_length), max_rows, window, sinks));
+}
+
 struct DecodePlan {
   unsigned workgroups;
   size_t base_bytes, bytes;
@@ -175,10 +184,8 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
 size_t praghip_paged_prompt_workspace(const praghip_cache* c, size_t heads, size_t max_rows, size_t window, size_t sinks,
                                       size_t max_length) {
   if (!c || check_cache(c) || !heads_fit(*c, heads) || !tiles_fit(*c, heads, max_rows)) return 0;
-  const size_t group = heads / c->kv_heads;
-  const int splits = prompt_splits(c->seqs, c->kv_heads, group, c->head_dim, max_rows,
-                                   keys_of(bound_of(*c, max_length), max_rows, window, sinks));
-  return prompt_work_floats(splits, c->seqs, c->kv_heads, group, c->head_dim, max_rows) * sizeof(float);
+  const int splits = splits_of(*c, heads, max_rows, window, sinks, max_length);
+  return prompt_work_floats(splits, c->seqs, c->kv_heads, heads / c->kv_heads, c->head_dim, max_rows) * sizeof(float);
 }
 
 int praghip_paged_prompt(int device, const praghip_cache* c, const void* q, const int64_t* q_strides, size_t heads,
@@ -188,17 +195,17 @@ int praghip_paged_prompt(int device, const praghip_cache* c, const void* q, cons
   if (tokens == 0 || max_rows == 0 || (c && c->seqs == 0)) return PRAGHIP_OK;
   if (const int rc = check_cache(c)) return rc;
   if (!q || !q_strides || !starts || !out || !out_strides) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  const size_t given = max_rows;
   max_rows = std::min(max_rows, tokens);
   if (!heads_fit(*c, heads) || !tiles_fit(*c, heads, max_rows) || !std::isfinite(scale) || tokens > INT_MAX)
     return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
   if (!aligned16(q) || !aligned16(out) || !aligned16(work) || !aligned4(lse) || !aligned4(starts) || !eights(q_strides, 2) ||
       !eights(out_strides, 2))
     return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_ALIGNMENT");
-  const size_t group = heads / c->kv_heads;
   PromptArgs a{};
-  a.splits = prompt_splits(c->seqs, c->kv_heads, group, c->head_dim, max_rows,
-                           keys_of(bound_of(*c, max_length), max_rows, window, sinks));
-  const size_t need = prompt_work_floats(a.splits, c->seqs, c->kv_heads, group, c->head_dim, max_rows) * sizeof(float);
+  a.splits = splits_of(*c, heads, given, window, sinks, max_length);
+  const size_t need =
+      prompt_work_floats(a.splits, c->seqs, c->kv_heads, heads / c->kv_heads, c->head_dim, max_rows) * sizeof(float);
   if (need && (!work || work_bytes < need)) return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_WORKSPACE");
   a.c = cache_args(*c, heads, scale, window, sinks);
   a.q = q, a.q_token = q_strides[0], a.q_head = q_strides[1];
