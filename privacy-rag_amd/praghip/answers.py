@@ -127,11 +127,11 @@ class Qwen3Answers:
             page_trim(self.tables, self.lengths, self.refs, self.page_size, listed, self.window, self.sinks, self.status)
 
     def steps(self, sequences):
-        """A function that appends one token to each of these sequences, given as a list or an
-        int64 tensor (whose values outside the vocabulary count as its nearest), and returns
-        the logits after them (in the same memory each time): the layers' calls, some 30 a
-        layer, as one captured graph.  The sequences may be forked, ended and extended between
-        its calls."""
+        """A function that appends one token to each of these sequences, given as a list or a
+        tensor of whole numbers (whose values outside the vocabulary count as its nearest), and
+        returns the logits after them (in the same memory each time): the layers' calls, some
+        30 a layer, as one captured graph.  The sequences may be forked, ended and extended
+        between its calls."""
         import torch
         sequences = list(sequences)
         if not sequences or any(not 0 <= s < len(self.held) for s in sequences):
@@ -155,11 +155,15 @@ class Qwen3Answers:
         with torch.cuda.graph(graph):
             logits = forward()
 
+        whole = torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64
+
         def step(new):
             if not isinstance(new, torch.Tensor):
                 if len(new) != n or any(not 0 <= t < self.embed.shape[0] for t in new):
                     raise ValueError("one token of the vocabulary for each sequence")
                 new = torch.tensor(new)
+            if new.shape != (n,) or new.dtype not in whole:
+                raise ValueError("one whole number for each sequence")
             self._reserve(sequences, listed, ones, [1] * n)
             tokens.copy_(new)
             graph.replay()
