@@ -148,9 +148,11 @@ class Qwen3Answers:
                                              starts, 1, capacity))
 
         held = self.lengths.clone()
-        self.lengths.zero_()  # (a first time outside, which loads code and writes nothing)
-        forward()
-        self.lengths.copy_(held)
+        try:
+            self.lengths.zero_()  # (a first time outside, which loads code and writes nothing)
+            forward()
+        finally:
+            self.lengths.copy_(held)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             logits = forward()

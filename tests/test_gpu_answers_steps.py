@@ -49,3 +49,21 @@ def test_a_step_takes_one_whole_number_for_each_sequence(gpu, device):
         if dtype is torch.int64:
             assert (got.float() - want.float()).norm() <= 4 * 31 ** 0.5 * 2.0 ** -11 * want.float().norm()
     assert m.held == [7, 19, 0, 0] == m.lengths.tolist()
+
+
+def test_a_first_time_that_fails_leaves_the_lengths(gpu, monkeypatch):
+    """Memory that does not suffice for the graph's first run, say."""
+    print("[steps] a first time that fails", flush=True)
+    m = model()
+    before = state(m)
+
+    def fails(*a, **k):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(m, "_logits", fails)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        m.steps([0, 1])
+    monkeypatch.undo()
+    assert same(state(m), before)
+    m.extend([0], [[3]])
+    assert m.held == [5, 16, 0, 0] == m.lengths.tolist()
