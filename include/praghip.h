@@ -594,9 +594,11 @@ int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
  * page_size is a power of two of 16 .. 32768, head_dim a multiple of 8 up to 256 and
  * the cache's strides are below 2^31, a token's below 2^26 (E_ATTENTION_SHAPE); base
  * addresses are 16-byte aligned and strides multiples of 8 (E_ATTENTION_ALIGNMENT).  A
- * length outside 0 .. table_width * page_size is taken as the nearer end.  A key or
- * value that is not finite makes the outputs of the queries that see it NaN or
- * infinite, and no others'. */
+ * length outside 0 .. table_width * page_size is taken as the nearer end, where a row's
+ * positions count up to the whole pages within 2^31 - 64.  A value that is not finite, and
+ * a key that makes a score NaN or +infinity, make the outputs of the queries that see
+ * it NaN or infinite, and no others'.  A key whose score is -infinity has weight 0; a
+ * query that sees no other key gets what one that sees nothing gets. */
 typedef struct praghip_cache {
   void *k, *v;
   int64_t k_strides[3], v_strides[3];
@@ -632,7 +634,8 @@ int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, 
  * [tokens][heads][head_dim] (strides {token, head}) are the newest tokens of sequence
  * s, the last of them at position lengths[s] - 1; the cache holds their keys and values
  * already.  Causal, with window and sinks as above; a row whose position is below 0 sees
- * nothing.  max_rows is at least the longest of these stretches; rows beyond it are not
+ * nothing.  Each probability is rounded to the type before its product with the value, which
+ * the decode's are not; the sums are 32-bit.  max_rows is at least the longest of these stretches; rows beyond it are not
  * computed.  seqs x kv_heads x (max_rows x group / 128 + 1) is below 2^23
  * (E_ATTENTION_SHAPE).  lse: [tokens][heads].  work: at least the bytes that the workspace
  * function names for the same arguments, NULL where that is 0; more rows may need less, as their

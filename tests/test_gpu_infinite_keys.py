@@ -38,3 +38,18 @@ def test_infinite_keys_that_are_seen(gpu, type, dim, window, sinks):
     for out in (praghip.paged_prompt(q.to("cuda"), *on, starts, rows, window=window, sinks=sinks)[-rows // 2:],
                 praghip.paged_decode(q[-1:].to("cuda"), *on, window=window, sinks=sinks)):
         assert out[:, 2:].isnan().all() and torch.isfinite(out[:, :2]).all()
+
+
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [5, 100])
+def test_no_other_key_is_seen(gpu, type, n):
+    """All scores are minus infinity: zeros and minus infinity, as where nothing is seen."""
+    print("[infinite keys] all", type, n, flush=True)
+    c = plain.make([n], 4, 2, 64, 16, type, seed=n)
+    q = torch.randn((n, 4, 64), generator=c["g"]).abs().add(0.1).to(type).to("cuda")
+    k, v, tables, lengths = (c[x].to("cuda") for x in ("k", "v", "tables", "lengths"))
+    k[:, :, :, 7] = -math.inf
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for out, lse in (praghip.paged_prompt(q, k, v, tables, lengths, starts, n, lse=True),
+                     praghip.paged_decode(q[-1:], k, v, tables, lengths, lse=True)):
+        assert not out.any() and bool((lse == -math.inf).all())
