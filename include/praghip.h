@@ -711,9 +711,11 @@ int praghip_page_write(int device, const praghip_cache *cache, const void *k, co
 /* y[m][n] = sum_k x[m][k] (w[n][k] - z[n][k / group]) s[n][k / group]: x [m][k], y [m][n]
  * and scales [n][groups] of `type`, w [n][width] bytes of two 4-bit values each, the lower
  * bits first (width >= (k + 1) / 2), zeros [n][groups] bytes (NULL: 8 everywhere); groups =
- * ceil(k / group), group a multiple of 32, n up to 2^27, m up to 2^20 (E_W4_SHAPE).  Strides in elements of a row each;
- * rows at odd addresses are read as they are, more slowly.  k 0 gives zeros.  Sums are 32-bit,
- * rounded once.  An infinity or NaN in a row of x makes that row of y NaN. */
+ * ceil(k / group), group a multiple of 32, n up to 2^27, m up to 2^20 (E_W4_SHAPE).  Strides
+ * in elements of a row each; rows at odd addresses are read as they are, more slowly.  k 0
+ * gives zeros.  Sums are 32-bit (a group's of x (16 + w), less (16 + z) times that of x: off
+ * by at most group 2^-24 s sum |x| (32 + w + z)), rounded once.  An infinity or NaN in a row
+ * of x makes that row of y NaN. */
 typedef struct praghip_w4 {
   const uint8_t *w;
   int64_t w_stride;

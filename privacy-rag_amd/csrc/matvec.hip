@@ -17,8 +17,9 @@
 //   x is put into that order instead, once for all columns.
 // * With a = sum x (16 + w) and X = sum x over a group (a product with ones, exact to
 //   the accumulator's rounding), y += s (a - (16 + z) X).  16 is the smallest offset
-//   that keeps all 16 values in one binade, so the difference loses at most two bits
-//   of the 32-bit sum.
+//   that keeps all 16 values in one binade.  The two sums are 32-bit ones of up to G
+//   terms: a group's part of y is off by at most G 2^-24 s sum |x| (32 + w + z), also
+//   where w is near z and the part itself is small.
 // Waves of a workgroup take K blocks of 128 in turn and add their sums through LDS in
 // order.  1024 x 4096, one row: the kernel takes 5.3 us, the host's call 8.1.
 #include "matvec.hpp"
