@@ -89,38 +89,31 @@ __device__ __forceinline__ u32x4 load_w(const uint8_t* row, int at, int width) {
 }
 
 // The sums of the waves along K, in order, and y's values.
-template <typename T, int MT, int NT>
-__device__ __forceinline__ void finish_rows(const MatvecArgs& a, f32x4 (&y)[NT][MT], float* sums, int kw, int part, int wave,
+template <typename T, int MT>
+__device__ __forceinline__ void finish_rows(const MatvecArgs& a, f32x4 (&y)[MT], float* sums, int kw, int part, int wave,
                                             int lane, int tile, int m0) {
   const int col = lane & 15, quad = lane >> 4;
   if (kw > 1) {
-    float* mine = sums + wave * NT * MT * 256 + lane * 4;
+    float* mine = sums + wave * MT * 256 + lane * 4;
     if (part) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(mine + (t * MT + i) * 256) = y[t][i];
+      for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(mine + i * 256) = y[i];
     }
     __syncthreads();
     if (part) return;
     for (int p = 1; p < kw; ++p)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) y[t][i] += *reinterpret_cast<const f32x4*>(mine + (p * NT * MT + t * MT + i) * 256);
+      for (int i = 0; i < MT; ++i) y[i] += *reinterpret_cast<const f32x4*>(mine + (p * MT + i) * 256);
   }
+  const int n = tile * 16 + col;
+  if (n >= a.n) return;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int n = (tile + t) * 16 + col;
-    if (n >= a.n) continue;
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = m0 + 16 * i + 4 * quad + r;
-        if (m < a.m) static_cast<T*>(a.y)[m * a.y_stride + n] = T(y[t][i][r]);
-      }
-  }
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + 16 * i + 4 * quad + r;
+      if (m < a.m) static_cast<T*>(a.y)[m * a.y_stride + n] = T(y[i][r]);
+    }
 }
 
 // the words of the four lanes of a column, turned: word s of quad g is word g of quad s
@@ -140,28 +133,22 @@ __device__ __forceinline__ u32x4 turned(u32x4 w) {
   return w;
 }
 
-// MT tiles of 16 rows of x, NT tiles of 16 columns a wave, kw waves along K: any group
-template <typename T, int MT, int NT, bool ALIGNED, bool ZEROS>
+// MT tiles of 16 rows of x, one of 16 columns a wave, kw waves along K: any group
+template <typename T, int MT, bool ALIGNED, bool ZEROS>
 __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
   extern __shared__ float sums[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int part = wave % kw, tile = (blockIdx.x * (4 / kw) + wave / kw) * NT;
+  const int part = wave % kw, tile = blockIdx.x * (4 / kw) + wave / kw;
   const int m0 = blockIdx.y * 16 * MT, groups = (a.k + a.group - 1) / a.group, steps = a.group / 32;
 
-  f32x4 y[NT][MT];
-  const uint8_t* row[NT];
-  const T* scale[NT];
-  const uint8_t* zero[NT];
+  const int n = min(tile * 16 + col, a.n - 1);
+  const uint8_t* const row = a.w + n * a.w_stride;
+  const T* const scale = static_cast<const T*>(a.scales) + n * a.scale_stride;
+  const uint8_t* const zero = ZEROS ? a.zeros + n * a.zero_stride : nullptr;
+  f32x4 y[MT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int n = min((tile + t) * 16 + col, a.n - 1);
-    row[t] = a.w + n * a.w_stride;
-    scale[t] = static_cast<const T*>(a.scales) + n * a.scale_stride;
-    zero[t] = ZEROS ? a.zeros + n * a.zero_stride : nullptr;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) y[t][i] = f32x4{0, 0, 0, 0};
-  }
+  for (int i = 0; i < MT; ++i) y[i] = f32x4{0, 0, 0, 0};
   const T* x[MT];
   bool has[MT];
 #pragma unroll
@@ -170,36 +157,25 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
     has[i] = m < a.m;
     x[i] = static_cast<const T*>(a.x) + (has[i] ? m : 0) * a.x_stride;
   }
-  f32x4 acc[NT][MT], ones[MT];
+  f32x4 acc[MT], ones[MT];
   const auto clear = [&] {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      ones[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][i] = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < MT; ++i) acc[i] = ones[i] = f32x4{0, 0, 0, 0};
   };
   const auto finish = [&](int g) {
     if (g >= groups) return;
+    const float s = float(scale[g]), c = 16.f + (ZEROS ? float(zero[g]) : 8.f);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const float s = float(scale[t][g]), c = 16.f + (ZEROS ? float(zero[t][g]) : 8.f);
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[t][i][r] += s * (acc[t][i][r] - c * ones[i][r]);
-    }
+      for (int r = 0; r < 4; ++r) y[i][r] += s * (acc[i][r] - c * ones[i][r]);
     clear();
   };
   clear();
   const u32x4 one = {Nibble<T>::one, Nibble<T>::one, Nibble<T>::one, Nibble<T>::one};
   if (tile * 16 < a.n) {
     for (int kb = part * kBlockK; kb < a.k; kb += kw * kBlockK) {
-      u32x4 w[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) w[t] = load_w<ALIGNED>(row[t], kb / 2 + 16 * quad, a.width);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) w[t] = turned(w[t]);
+      const u32x4 w = turned(load_w<ALIGNED>(row, kb / 2 + 16 * quad, a.width));
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const int k = kb + 32 * st;
@@ -209,19 +185,16 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
           xf[i] = load_x<T, ALIGNED>(x[i], has[i], k + 8 * quad, a.k);
           ones[i] = Half<T>::mma16(xf[i], one, ones[i]);
         }
+        const u32x4 wf = widen<T>(w[st]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const u32x4 wf = widen<T>(w[t][st]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[t][i] = Half<T>::mma16(xf[i], wf, acc[t][i]);
-        }
+        for (int i = 0; i < MT; ++i) acc[i] = Half<T>::mma16(xf[i], wf, acc[i]);
         // a group ends here, or this wave's part of it does
         if ((k / 32 + 1) % steps == 0 || (st == 3 && kw > 1)) finish(k / a.group);
       }
     }
     if (kw == 1) finish((a.k - 1) / a.group);
   }
-  finish_rows<T, MT, NT>(a, y, sums, kw, part, wave, lane, tile, m0);
+  finish_rows<T, MT>(a, y, sums, kw, part, wave, lane, tile, m0);
 }
 
 // For groups of 32 S, S = 1, 2 or 4, many columns and whole turns.  A turn is eight groups, 2 S blocks
@@ -234,12 +207,12 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
 // are under way beside a turn's products (no load stands behind a condition: at the join the
 // compiler would wait for it).  16 rows, K = 1024, 155,648 columns: 24.8 us, 3.7 TB/s of the
 // 5.1 of a large copy.
-template <typename T, int NT, int S>
+template <int S>
 struct Turn {
-  u32x4 w[2 * S][NT], sc[NT];
-  u32x2 zc[NT];
+  u32x4 w[2 * S], sc;
+  u32x2 zc;
 };
-template <typename T, int MT, int NT, int S, bool ZEROS>
+template <typename T, int MT, int S, bool ZEROS>
 __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int part) {
   constexpr int kTurn = 256 * S;
   extern __shared__ float lds[];
@@ -247,19 +220,15 @@ __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4, row_step = part + 8;  // a row in LDS: 16 bytes more than its data
   const int m0 = blockIdx.y * 16 * MT, turns = a.k / kTurn;
-  const int sets = (a.n + 64 * NT - 1) / (64 * NT);  // of a workgroup's tiles
+  const int sets = (a.n + 63) / 64;  // of a workgroup's tiles
 
-  const auto load = [&](Turn<T, NT, S>& u, int set, int turn) {
-    const int k0 = turn * kTurn, g0 = 8 * turn;
+  const auto load = [&](Turn<S>& u, int set, int turn) {
+    const int k0 = turn * kTurn, g0 = 8 * turn, n = min((set * 4 + wave) * 16 + col, a.n - 1);
+    const uint8_t* const row = a.w + n * a.w_stride + 16 * quad + k0 / 2;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int n = min(((set * 4 + wave) * NT + t) * 16 + col, a.n - 1);
-      const uint8_t* const row = a.w + n * a.w_stride + 16 * quad + k0 / 2;
-#pragma unroll
-      for (int b = 0; b < 2 * S; ++b) u.w[b][t] = *reinterpret_cast<const u32x4*>(row + 64 * b);
-      u.sc[t] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.scales) + n * a.scale_stride + g0);
-      if (ZEROS) u.zc[t] = *reinterpret_cast<const u32x2*>(a.zeros + n * a.zero_stride + g0);
-    }
+    for (int b = 0; b < 2 * S; ++b) u.w[b] = *reinterpret_cast<const u32x4*>(row + 64 * b);
+    u.sc = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.scales) + n * a.scale_stride + g0);
+    if (ZEROS) u.zc = *reinterpret_cast<const u32x2*>(a.zeros + n * a.zero_stride + g0);
   };
   const auto stage = [&](int from) {
     const int chunks = part / 8;
@@ -271,15 +240,13 @@ __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int
     }
     __syncthreads();
   };
-  f32x4 y[NT][MT];
+  f32x4 y[MT];
   const u32x4 one = {Nibble<T>::one, Nibble<T>::one, Nibble<T>::one, Nibble<T>::one};
-  const auto multiply = [&](const Turn<T, NT, S>& u, int at) {  // `at`: the turn's place in LDS
-    f32x4 acc[NT][MT], ones[MT];
+  const auto multiply = [&](const Turn<S>& u, int at) {  // `at`: the turn's place in LDS
+    f32x4 acc[MT], ones[MT];
 #pragma unroll
     for (int b = 0; b < 2 * S; ++b) {
-      u32x4 v[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) v[t] = turned(u.w[b][t]);
+      const u32x4 v = turned(u.w[b]);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const bool first = (4 * b + st) % S == 0;
@@ -290,35 +257,27 @@ __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int
           xf[i] = *reinterpret_cast<const u32x4*>(xs + (16 * i + col) * row_step + at + kBlockK * b + 32 * st + 8 * quad);
           ones[i] = Half<T>::mma16(xf[i], one, first ? none : ones[i]);
         }
+        const u32x4 wf = widen<T>(v[st]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const u32x4 wf = widen<T>(v[t][st]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[t][i] = Half<T>::mma16(xf[i], wf, first ? none : acc[t][i]);
-        }
+        for (int i = 0; i < MT; ++i) acc[i] = Half<T>::mma16(xf[i], wf, first ? none : acc[i]);
         if ((4 * b + st + 1) % S == 0) {
           const int g = (4 * b + st) / S;
+          const float s = g & 1 ? high<T>(u.sc[g / 2]) : low<T>(u.sc[g / 2]);
+          const float c = 16.f + (ZEROS ? float(u.zc[g / 4] >> (8 * (g & 3)) & 255) : 8.f);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float s = g & 1 ? high<T>(u.sc[t][g / 2]) : low<T>(u.sc[t][g / 2]);
-            const float c = 16.f + (ZEROS ? float(u.zc[t][g / 4] >> (8 * (g & 3)) & 255) : 8.f);
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) y[t][i][r] += s * (acc[t][i][r] - c * ones[i][r]);
-          }
+            for (int r = 0; r < 4; ++r) y[i][r] += s * (acc[i][r] - c * ones[i][r]);
         }
       }
     }
   };
   const auto clear = [&] {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < MT; ++i) y[t][i] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < MT; ++i) y[i] = f32x4{0, 0, 0, 0};
   };
 
-  Turn<T, NT, S> u[2];
+  Turn<S> u[2];
   clear();
   int set = blockIdx.x, turn = 0, staged = -1;
   load(u[0], set, 0);
@@ -336,7 +295,7 @@ __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int
       }
       multiply(u[b], turn * kTurn - from);
       if (next == 0) {
-        finish_rows<T, MT, NT>(a, y, nullptr, 1, 0, wave, lane, (set * 4 + wave) * NT, m0);
+        finish_rows<T, MT>(a, y, nullptr, 1, 0, wave, lane, set * 4 + wave, m0);
         clear();
         if (next_set >= sets) return;
       }
@@ -345,27 +304,27 @@ __global__ void __launch_bounds__(256) matvec_w4_groups_kernel(MatvecArgs a, int
   }
 }
 
-template <typename T, int MT, int NT, int S>
+template <typename T, int MT, int S>
 hipError_t launch_groups(const MatvecArgs& a, hipStream_t s) {
-  const auto kernel = a.zeros ? matvec_w4_groups_kernel<T, MT, NT, S, true> : matvec_w4_groups_kernel<T, MT, NT, S, false>;
+  const auto kernel = a.zeros ? matvec_w4_groups_kernel<T, MT, S, true> : matvec_w4_groups_kernel<T, MT, S, false>;
   // x in LDS as a whole up to 64 KiB, two workgroups of a CU; three where there is room for four
   // (155,648 columns of K = 1024 and one row: 20.9 us, four 22.8)
   const int whole = a.k, part = MT * whole <= 2048 ? whole : 2048 / MT;
-  const unsigned sets = unsigned((a.n + 64 * NT - 1) / (64 * NT)), most = MT * whole <= 1024 ? 768 : 512;
+  const unsigned sets = unsigned((a.n + 63) / 64), most = MT * whole <= 1024 ? 768 : 512;
   hipLaunchKernelGGL(kernel, dim3(std::min(sets, most), (a.m + 16 * MT - 1) / (16 * MT)), dim3(256),
                      size_t(16) * MT * (part + 8) * 2, s, a, part);
   return hipGetLastError();
 }
 template <typename T, int S>
 hipError_t launch_groups(const MatvecArgs& a, hipStream_t s) {
-  return a.m <= 16 ? launch_groups<T, 1, 1, S>(a, s) : launch_groups<T, 2, 1, S>(a, s);
+  return a.m <= 16 ? launch_groups<T, 1, S>(a, s) : launch_groups<T, 2, S>(a, s);
 }
 
 template <typename T, int MT>
 hipError_t launch(const MatvecArgs& a, int kw, hipStream_t s) {
   const bool z = a.zeros != nullptr;
-  const auto kernel = a.aligned ? (z ? matvec_w4_kernel<T, MT, 1, true, true> : matvec_w4_kernel<T, MT, 1, true, false>)
-                                : (z ? matvec_w4_kernel<T, MT, 1, false, true> : matvec_w4_kernel<T, MT, 1, false, false>);
+  const auto kernel = a.aligned ? (z ? matvec_w4_kernel<T, MT, true, true> : matvec_w4_kernel<T, MT, true, false>)
+                                : (z ? matvec_w4_kernel<T, MT, false, true> : matvec_w4_kernel<T, MT, false, false>);
   const unsigned tiles = unsigned((a.n + 15) / 16), per = 4 / kw;
   hipLaunchKernelGGL(kernel, dim3((tiles + per - 1) / per, (a.m + 16 * MT - 1) / (16 * MT)), dim3(256),
                      kw > 1 ? 4 * MT * 256 * sizeof(float) : 0, s, a, kw);
