@@ -33,10 +33,10 @@ class Qwen3Answers:
                  theta: float = 1e6, eps: float = 1e-6):
         import torch
         self.shape, self.page_size, self.window, self.sinks, self.eps = shape, page_size, window, sinks, eps
-        self.group, self.embed, self.norm = group, weights["embed"], weights["norm"]
+        self.group, self.embed, self.norm = group, weights["embed"].detach(), weights["norm"].detach()
         self.device, self.type = self.embed.device, self.embed.dtype
         self.head = quantize_w4(self.embed, group, zeros=True)
-        self.layers = [{name: quantize_w4(w, group, zeros=True) if w.dim() == 2 else w for name, w in layer.items()}
+        self.layers = [{name: quantize_w4(w, group, zeros=True) if w.dim() == 2 else w.detach() for name, w in layer.items()}
                        for layer in weights["layers"]]
         self.pool = torch.zeros((shape.layers, 2, pages, shape.kv_heads, page_size, shape.head_dim), dtype=self.type,
                                 device=self.device)

@@ -9,6 +9,9 @@ On another stream than the current one a call's workspace and the tensors that i
 returns come from that stream's memory, so they wait for nothing.  The caller orders
 the rest: ``stream`` behind the work that makes the call's inputs, the current stream
 behind ``stream`` before it reads the result, and inputs kept until the call is done.
+
+The calls have no backward pass: one whose inputs require gradients is refused, unless
+gradients are off (``torch.no_grad``).
 """
 from __future__ import annotations
 
@@ -42,6 +45,13 @@ def _stream(index: int, stream):
 
 def _type_error(text: str) -> PraghipError:
     return PraghipError(E_ARGUMENT, text)
+
+
+def _no_gradients(text: str, *tensors) -> None:
+    """An output without its gradient would pass for a constant."""
+    for t in tensors:
+        if t.requires_grad and _torch.is_grad_enabled():
+            raise _type_error(text)
 
 
 def _kind(t, text: str) -> int:
@@ -133,6 +143,7 @@ def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = 
     if len(shape) != 3 or shape[0] != seqs or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0:
         raise shape_error("E_ATTENTION_SHAPE")
+    _no_gradients("E_ATTENTION_GRADIENT", q, k_pages, v_pages)
     out = _output(q, shape, out, index, stream)
     sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
     if seqs:
@@ -163,6 +174,7 @@ def paged_prompt(q, k_pages, v_pages, tables, lengths, starts, max_rows: int, *,
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0 or max_rows < 0:
         raise shape_error("E_ATTENTION_SHAPE")
     first = _starts(starts, seqs, index)
+    _no_gradients("E_ATTENTION_GRADIENT", q, k_pages, v_pages)
     out = _output(q, shape, out, index, stream)
     sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
     tokens, heads = shape[0], shape[1]
@@ -192,5 +204,6 @@ def page_write(k, v, k_pages, v_pages, tables, lengths, starts, stream=None) -> 
     ks, vs = k.stride(), v.stride()
     if len(shape) != 3 or v.shape != shape or shape[1] != pages[1] or shape[2] != pages[3] or ks[2] != 1 or vs[2] != 1:
         raise shape_error("E_ATTENTION_SHAPE")
+    _no_gradients("E_ATTENTION_GRADIENT", k, v, k_pages, v_pages)
     check(lib().praghip_page_write(index, cache, k.data_ptr(), _two(ks[0], ks[1]), v.data_ptr(), _two(vs[0], vs[1]),
                                    _starts(starts, seqs, index), shape[0], _stream(index, stream)))

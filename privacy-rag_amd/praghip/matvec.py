@@ -1,12 +1,12 @@
-"""Products of a few rows with 4-bit weights and group scales (streams as in
-:mod:`praghip.attention`)."""
+"""Products of a few rows with 4-bit weights and group scales (streams and gradients as
+in :mod:`praghip.attention`)."""
 from __future__ import annotations
 
 import struct
 
 from . import attention
 from ._lib import check, lib, shape_error
-from .attention import _kind, _result, _stream, _type_error
+from .attention import _kind, _no_gradients, _result, _stream, _type_error
 
 _W4 = struct.Struct("PqPqPq4Qi4x").pack  # praghip_w4
 
@@ -32,6 +32,7 @@ def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, str
     if group <= 0 or group % 32 or width < (k + 1) // 2 or scales.shape != (n, -(-k // group)) or \
             (xs[1] != 1 and k > 1) or (ws[1] != 1 and width > 1) or (ss[1] != 1 and k > group):
         raise shape_error("E_W4_SHAPE")
+    _no_gradients("E_W4_GRADIENT", x, scales)
     zero, zs = 0, 0
     if zeros is not None:
         if zeros.shape != scales.shape or (zeros.stride(1) != 1 and k > group):
@@ -54,12 +55,13 @@ def quantize_w4(weight, group: int = 128, *, zeros: bool = False):
     Returns (packed uint8 [n][width], scales [n][groups] of the weights' type, zeros
     uint8 or None) as :func:`matvec_w4` takes them, width a multiple of 16.  Without
     zero points a group spans -8 .. 7 times its scale, with them 0 .. 15 from its
-    smallest value on (0 included, so that a weight of 0 stays 0).
+    smallest value on (0 included, so that a weight of 0 stays 0).  No gradients pass.
     """
     import torch
     _kind(weight, "E_W4_TYPE")
     if weight.dim() != 2 or group <= 0 or group % 32:
         raise shape_error("E_W4_SHAPE")
+    weight = weight.detach()
     n, k = weight.shape
     groups, width = -(-k // group), -(-k // 32) * 16
     w = torch.zeros((n, groups * group), dtype=torch.float32, device=weight.device)
