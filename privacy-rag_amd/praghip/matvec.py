@@ -28,6 +28,8 @@ def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, str
             (zeros is not None and zeros.get_device() != index):
         raise _type_error("E_W4_DEVICE")
     xs, ws, ss = x.stride(), weights.stride(), scales.stride()
+    if not len(xs) == len(ws) == len(ss) == 2:
+        raise shape_error("E_W4_SHAPE")
     (m, k), (n, width) = x.shape, weights.shape
     if group <= 0 or group % 32 or width < (k + 1) // 2 or scales.shape != (n, -(-k // group)) or \
             (xs[1] != 1 and k > 1) or (ws[1] != 1 and width > 1) or (ss[1] != 1 and k > group):

@@ -62,12 +62,19 @@ def _list(t, n: int, index: int) -> int:
     return t.data_ptr()
 
 
+def _length(t) -> int:
+    """Entries of a call's list."""
+    if len(t.shape) != 1:
+        raise shape_error("E_PAGES_SHAPE")
+    return t.shape[0]
+
+
 def page_reserve(tables, lengths, refs, page_size: int, sequences, counts, status=None, stream=None) -> None:
     """counts[i] more tokens for sequences[i]: its new pages, and its length."""
     index = tables.get_device()
     t = _table(tables, lengths, refs, page_size, status, index)
-    n = sequences.shape[0]
-    check(lib().praghip_page_reserve(index, t, _list(sequences, sequences.shape[0], index), _list(counts, n, index), n,
+    n = _length(sequences)
+    check(lib().praghip_page_reserve(index, t, _list(sequences, n, index), _list(counts, n, index), n,
                                      _stream(index, stream)))
 
 
@@ -75,8 +82,8 @@ def page_free(tables, lengths, refs, sequences, status=None, stream=None) -> Non
     """Empties sequences: their pages lose a reference, their rows become -1, their lengths 0."""
     index = tables.get_device()
     t = _table(tables, lengths, refs, 1, status, index)
-    check(lib().praghip_page_free(index, t, _list(sequences, sequences.shape[0], index), sequences.shape[0],
-                                  _stream(index, stream)))
+    n = _length(sequences)
+    check(lib().praghip_page_free(index, t, _list(sequences, n, index), n, _stream(index, stream)))
 
 
 def page_trim(tables, lengths, refs, page_size: int, sequences, window: int, sinks: int = 0, status=None,
@@ -86,8 +93,8 @@ def page_trim(tables, lengths, refs, page_size: int, sequences, window: int, sin
     t = _table(tables, lengths, refs, page_size, status, index)
     if window < 0 or sinks < 0:
         raise shape_error("E_PAGES_WINDOW")
-    check(lib().praghip_page_trim(index, t, _list(sequences, sequences.shape[0], index), sequences.shape[0], window,
-                                  sinks, _stream(index, stream)))
+    n = _length(sequences)
+    check(lib().praghip_page_trim(index, t, _list(sequences, n, index), n, window, sinks, _stream(index, stream)))
 
 
 def page_fork(pool, tables, lengths, refs, parents, children, status=None, stream=None) -> None:
@@ -99,7 +106,7 @@ def page_fork(pool, tables, lengths, refs, parents, children, status=None, strea
     index = tables.get_device()
     p = _pool(pool, index)
     t = _table(tables, lengths, refs, pool.shape[-2], status, index)
-    n = parents.shape[0]
+    n = _length(parents)
     of, to = _list(parents, n, index), _list(children, n, index)
     if n:
         L = lib()
@@ -114,8 +121,7 @@ def page_compact(pool, tables, refs, stream=None) -> None:
     the holes below, both in rising order, and the tables follow."""
     index = tables.get_device()
     p = _pool(pool, index)
-    pages = refs.shape[0]
-    t = _table(tables, None, refs, pool.shape[-2], None, index)
+    t, pages = _table(tables, None, refs, pool.shape[-2], None, index), refs.shape[0]
     L = lib()
     size = L.praghip_page_compact_workspace(pages)
     work = _work(size, tables, stream)
@@ -128,7 +134,7 @@ def page_copy(pool, sources, targets, stream=None) -> None:
     skipped.  No page may be both a source and a target, or a target twice."""
     index = pool.get_device()
     p = _pool(pool, index)
-    n = sources.shape[0]
+    n = _length(sources)
     check(lib().praghip_page_copy(index, p, _list(sources, n, index), _list(targets, n, index), n,
                                   _stream(index, stream)))
 
