@@ -1,8 +1,8 @@
 """Attention over a paged key/value cache: one new token per sequence
 (:func:`paged_decode`) or many (:func:`paged_prompt`).
 
-The reference's attention is a two-party protocol; these serve a model in the
-clear beside it, and have no counterpart there.  Tensors are on one GPU; calls
+The reference's attention is a two-party protocol, and its float Qwen3 a transformers
+model; these serve such a model in the clear beside the protocol.  Tensors are on one GPU; calls
 are asynchronous on ``stream`` (the tensors' device's current stream by default).
 
 On another stream than the current one a call's workspace and the tensors that it
@@ -47,11 +47,10 @@ def _type_error(text: str) -> PraghipError:
     return PraghipError(E_ARGUMENT, text)
 
 
-def _no_gradients(text: str, *tensors) -> None:
-    """An output without its gradient would pass for a constant."""
-    for t in tensors:
-        if t.requires_grad and _torch.is_grad_enabled():
-            raise _type_error(text)
+def _no_gradients(text: str) -> None:
+    """A call of inputs that require gradients: its output would pass for a constant."""
+    if _torch.is_grad_enabled():
+        raise _type_error(text)
 
 
 def _kind(t, text: str) -> int:
@@ -89,11 +88,9 @@ def _starts(t, seqs: int, index: int) -> int:
     return t.data_ptr()
 
 
-def _allocate(stream, make, *args, **kw):
-    """make(...), a tensor that a call on `stream` writes, from the memory of that stream: a
-    block of the current one's may have been freed there with work under way that uses it."""
-    if stream is None:
-        return make(*args, **kw)
+def _there(stream, make, *args, **kw):
+    """make(...), a tensor that a call on another stream writes, from the memory of that stream:
+    a block of the current one's may have been freed there with work under way that uses it."""
     with _torch.cuda.stream(stream):
         return make(*args, **kw)
 
@@ -101,15 +98,19 @@ def _allocate(stream, make, *args, **kw):
 def _result(stream, index: int, make, *args, **kw):
     """The same for what a call returns: its block goes back once the current stream, where it
     is read, is done with it too."""
-    t = _allocate(stream, make, *args, **kw)
-    if stream is not None:
-        t.record_stream(_torch.cuda.current_stream(index))
+    t = _there(stream, make, *args, **kw)
+    t.record_stream(_torch.cuda.current_stream(index))
     return t
+
+
+def _lse(q, shape, index: int, stream):
+    shape, kind = shape[:2], dict(dtype=_torch.float32, device=q.device)
+    return _torch.empty(shape, **kind) if stream is None else _result(stream, index, _torch.empty, shape, **kind)
 
 
 def _output(q, shape, out, index: int, stream):
     if out is None:
-        return _result(stream, index, _torch.empty_like, q)
+        return _torch.empty_like(q) if stream is None else _result(stream, index, _torch.empty_like, q)
     if out.shape != shape or out.dtype is not q.dtype or out.get_device() != index or \
             (shape[2] > 1 and out.stride(2) != 1):
         raise shape_error("E_ATTENTION_OUT")
@@ -118,7 +119,9 @@ def _output(q, shape, out, index: int, stream):
 
 def _work(size: int, like, stream):
     """Workspace of one call, which `stream` alone uses."""
-    return _allocate(stream, _torch.empty, size, dtype=_uint8, device=like.device)
+    if stream is None:
+        return _torch.empty(size, dtype=_uint8, device=like.device)
+    return _there(stream, _torch.empty, size, dtype=_uint8, device=like.device)
 
 
 def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = None, window: int = 0, sinks: int = 0,
@@ -143,9 +146,10 @@ def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = 
     if len(shape) != 3 or shape[0] != seqs or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0:
         raise shape_error("E_ATTENTION_SHAPE")
-    _no_gradients("E_ATTENTION_GRADIENT", q, k_pages, v_pages)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_gradients("E_ATTENTION_GRADIENT")
     out = _output(q, shape, out, index, stream)
-    sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
+    sums = _lse(q, shape, index, stream) if lse else None
     if seqs:
         L, heads, to = lib(), shape[1], out.stride()
         size = L.praghip_paged_decode_workspace(cache, heads, max_length)
@@ -164,7 +168,8 @@ def paged_prompt(q, k_pages, v_pages, tables, lengths, starts, max_rows: int, *,
     q [tokens][heads][dim]: rows starts[s] .. starts[s + 1] - 1 (starts int32
     [seqs + 1]) are the newest tokens of sequence s, the last at position
     lengths[s] - 1; the cache holds their keys and values already.  max_rows is at
-    least the longest of these stretches (rows beyond it are not computed).  Token p
+    least the longest of these stretches (rows beyond it may be left unwritten, as rows
+    of no stretch are).  Token p
     sees key j where j <= p and, with a window, j > p - window or j < sinks.  The rest
     is as in :func:`paged_decode`.
     """
@@ -174,9 +179,10 @@ def paged_prompt(q, k_pages, v_pages, tables, lengths, starts, max_rows: int, *,
             shape[1] % pages[1] or window < 0 or sinks < 0 or max_length < 0 or max_rows < 0:
         raise shape_error("E_ATTENTION_SHAPE")
     first = _starts(starts, seqs, index)
-    _no_gradients("E_ATTENTION_GRADIENT", q, k_pages, v_pages)
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_gradients("E_ATTENTION_GRADIENT")
     out = _output(q, shape, out, index, stream)
-    sums = _result(stream, index, _torch.empty, shape[:2], dtype=_torch.float32, device=q.device) if lse else None
+    sums = _lse(q, shape, index, stream) if lse else None
     tokens, heads = shape[0], shape[1]
     if tokens and seqs:
         L, to = lib(), out.stride()
@@ -204,6 +210,7 @@ def page_write(k, v, k_pages, v_pages, tables, lengths, starts, stream=None) -> 
     ks, vs = k.stride(), v.stride()
     if len(shape) != 3 or v.shape != shape or shape[1] != pages[1] or shape[2] != pages[3] or ks[2] != 1 or vs[2] != 1:
         raise shape_error("E_ATTENTION_SHAPE")
-    _no_gradients("E_ATTENTION_GRADIENT", k, v, k_pages, v_pages)
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_gradients("E_ATTENTION_GRADIENT")
     check(lib().praghip_page_write(index, cache, k.data_ptr(), _two(ks[0], ks[1]), v.data_ptr(), _two(vs[0], vs[1]),
                                    _starts(starts, seqs, index), shape[0], _stream(index, stream)))

@@ -28,20 +28,22 @@ def matvec_w4(x, weights, scales, zeros=None, *, group: int = 128, out=None, str
             (zeros is not None and zeros.get_device() != index):
         raise _type_error("E_W4_DEVICE")
     xs, ws, ss = x.stride(), weights.stride(), scales.stride()
-    if not len(xs) == len(ws) == len(ss) == 2:
-        raise shape_error("E_W4_SHAPE")
-    (m, k), (n, width) = x.shape, weights.shape
+    try:
+        (m, k), (n, width) = x.shape, weights.shape
+    except ValueError:
+        raise shape_error("E_W4_SHAPE") from None
     if group <= 0 or group % 32 or width < (k + 1) // 2 or scales.shape != (n, -(-k // group)) or \
             (xs[1] != 1 and k > 1) or (ws[1] != 1 and width > 1) or (ss[1] != 1 and k > group):
         raise shape_error("E_W4_SHAPE")
-    _no_gradients("E_W4_GRADIENT", x, scales)
+    if x.requires_grad or scales.requires_grad:
+        _no_gradients("E_W4_GRADIENT")
     zero, zs = 0, 0
     if zeros is not None:
         if zeros.shape != scales.shape or (zeros.stride(1) != 1 and k > group):
             raise shape_error("E_W4_SHAPE")
         zero, zs = zeros.data_ptr(), zeros.stride(0)
     if out is None:
-        out = _result(stream, index, x.new_empty, (m, n))
+        out = x.new_empty((m, n)) if stream is None else _result(stream, index, x.new_empty, (m, n))
     elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != index or \
             (n > 1 and out.stride(1) != 1):
         raise shape_error("E_W4_OUT")
