@@ -13,7 +13,8 @@
  * [prime][N][2] (operand, quotient) NTT tables (seal_tables.cpp:22-33) and
  * [out][in] weights (bfv_matrix.inc:101-105, artifacts.hpp:86-92).  All of that is exact
  * integer arithmetic; the "serving" sections (attention over a paged cache, its pages,
- * 4-bit products) have no counterpart there and work on 16-bit floating point.
+ * 4-bit products) work on 16-bit floating point and follow no interface of the
+ * reference, whose float Qwen3 (references/) is a transformers model.
  *
  * Pointers documented "device" are HIP device pointers on the plan's device;
  * "host" pointers are ordinary host memory.  `stream` is a hipStream_t used as
@@ -578,8 +579,9 @@ int praghip_frame_decode(const uint8_t *in, praghip_frame_header *header);
 int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
 
 /* ------------------------------------------------- serving: paged attention */
-/* No counterpart in the reference, whose attention is a two-party protocol: these
- * serve a model in the clear beside it.  All pointers are device memory, all calls
+/* The reference's attention is a two-party protocol, and its float Qwen3 (references/) a
+ * transformers model without operators of its own: these serve such a model in the clear
+ * beside the protocol.  All pointers are device memory, all calls
  * asynchronous on `stream`; 16-bit data of PRAGHIP_BF16 or PRAGHIP_F16. */
 #define PRAGHIP_BF16 0
 #define PRAGHIP_F16 1
@@ -635,11 +637,12 @@ int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, 
  * s, the last of them at position lengths[s] - 1; the cache holds their keys and values
  * already.  Causal, with window and sinks as above; a row whose position is below 0 sees
  * nothing.  Each probability is rounded to the type before its product with the value, which
- * the decode's are not; the sums are 32-bit.  max_rows is at least the longest of these stretches; rows beyond it are not
- * computed.  seqs x kv_heads x (max_rows x group / 128 + 1) is below 2^23
- * (E_ATTENTION_SHAPE).  lse: [tokens][heads].  work: at least the bytes that the workspace
- * function names for the same arguments, NULL where that is 0; more rows may need less, as their
- * tiles fill the chip without splitting their keys. */
+ * the decode's are not; the sums are 32-bit.  max_rows is at least the longest of these
+ * stretches: rows beyond it may be left unwritten, as rows of no stretch are.  seqs x
+ * kv_heads x (max_rows x group / 128 + 1) is below 2^23 (E_ATTENTION_SHAPE).  lse:
+ * [tokens][heads].  work: at least the bytes that the workspace function names for the same
+ * arguments, NULL where that is 0; more rows may need less, as their tiles fill the chip
+ * without splitting their keys. */
 size_t praghip_paged_prompt_workspace(const praghip_cache *cache, size_t heads, size_t max_rows, size_t window,
                                       size_t sinks, size_t max_length);
 int praghip_paged_prompt(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,

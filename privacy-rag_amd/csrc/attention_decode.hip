@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
   __syncthreads();
 
   // key blocks before each stretch of sequences, one stretch per lane; every wave counts
-  // for itself, which takes no exchange with the others
+  // for itself, which takes no exchange with the others (for seqs / 64 reads one after the
+  // other: meant for thousands of sequences, not for the 2^20 that are allowed)
   const int per = (c.seqs + 63) >> 6;
   uint32_t mine = 0;
   for (int i = 0; i < per; ++i) {

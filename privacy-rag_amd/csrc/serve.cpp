@@ -172,7 +172,9 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
   a.work = reinterpret_cast<float*>(static_cast<char*>(work) + p.base_bytes);
   // A layer's keys and values that no cache holds until the next token are read past all of
   // them (627 MB: 119 us against 131; 134 MB: 35.5 against 37; 8 MB, which the next call finds
-  // there: 15.0 against 13.8).
+  // there: 15.0 against 13.8).  The host knows a bound of the lengths and not which pages the
+  // sequences share: where the bound is far off, or answers share their prompt, the call takes
+  // the form that finds less in the caches.
   const double keys = double(keys_of(bound_of(*c, max_length), 1, window, sinks));
   a.past = keys * double(c->seqs * c->kv_heads * c->head_dim) * 4 > double(64 << 20);
   DeviceScope scope(device);

@@ -19,10 +19,10 @@ libpraghip.so:
 * :class:`Qwen3LocalGemms` - the local products of a Qwen3 forward
   (model.hpp:66-126) as one batched call
 * :func:`paged_decode`, :func:`paged_prompt`, the ``page_*`` calls and
-  :func:`matvec_w4` - serving a model in the clear beside the protocol (no
-  counterpart in the reference): attention over a paged cache, its pages, and
-  few-row products with 4-bit weights; :class:`praghip.answers.Qwen3Answers` runs
-  them together
+  :func:`matvec_w4` - serving a model in the clear beside the protocol (the
+  reference's float Qwen3 is a transformers model): attention over a paged cache,
+  its pages, and few-row products with 4-bit weights;
+  :class:`praghip.answers.Qwen3Answers` runs them together
 
 Device data is handed over as torch tensors on the GPU (int64 or uint64 with
 u64 bit patterns); torch is used only for memory and streams.

@@ -240,7 +240,9 @@ def main() -> None:
         times.setdefault(name, []).append(time.perf_counter() - start)
         return got
 
-    for _ in range(2):  # the first time round loads code
+    for _ in range(2):  # the first time round loads code, and its capture gives torch's memory back
+        model.extend([0], [prompt])
+        model.end([0])
         times.clear()
         logits = timed("prompt", lambda: model.extend([0], [prompt]))
         answers = range(1, 1 + args.answers)
