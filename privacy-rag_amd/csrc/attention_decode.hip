@@ -30,8 +30,8 @@
 //
 // 64 sequences of 0 to 8192 tokens, 16 heads of 128 over 8 (627 MB): 120 us, 5.2 TB/s where
 // a large copy has 5.1.  Four through a window of 32768, 32 heads of 64 over 4 (134 MB): 35.5
-// us of the copy's 26.  One of 2049 tokens (8 MB): 13.9 us, a chain of dependent reads
-// (lengths, tables, keys) in 10 us and the join's launch in 3.9.
+// us of the copy's 26.  One of 2049 tokens (8 MB): 13.3 to 15 us by run, a chain of dependent
+// reads (lengths, tables, keys) in 10 us and the join's launch in 4.
 #include "attention.hpp"
 
 namespace praghip {

@@ -26,13 +26,14 @@
 // workgroups; their m, l and o go to the workspace and a second kernel joins them in
 // order.
 //
-// 8192 tokens, 16 heads of 128 over 8: 273 us, 1.0 PFLOP/s (a large bfloat16 product of the
-// library's reaches 1.2): matrix cores and vector units are busy 45% of the time each, hardly
+// 8192 tokens, 16 heads of 128 over 8: 262 to 279 us by card, 1.0 PFLOP/s (a large bfloat16
+// product of the library's reaches 1.2): matrix cores and vector units are busy 45% of the time each, hardly
 // at once, with the two waves that a SIMD has registers for.  Four chunks of up to 512 tokens
 // through a window of 2048, 32 heads of 64 over 4: 54 us, with CUs busy 57% of the time, as
 // the chunks' lengths differ (equal stretches of all tiles' keys instead, which a workgroup
-// takes across tiles: 71).  Three prompts of up to 77 tokens: 12 us, a chain of dependent
-// reads.
+// takes across tiles: 71), and twice dim 128's share of exponentials in a busy one.  Three
+// prompts of up to 77 tokens: 11 us, a chain of dependent reads.  Rows of 256 values have one
+// wave a SIMD and all of its registers: 4096 tokens of 8 heads over 4 197 us, 350 TFLOP/s.
 #include "attention.hpp"
 
 #include <type_traits>

@@ -21,7 +21,7 @@
 //   terms: a group's part of y is off by at most G 2^-24 s sum |x| (32 + w + z), also
 //   where w is near z and the part itself is small.
 // Waves of a workgroup take K blocks of 128 in turn and add their sums through LDS in
-// order.  1024 x 4096, one row: the kernel takes 5.3 us, the host's call 8.1.
+// order.  1024 x 4096, one row: the kernel takes 5.5 us, the host's call 8.0 to 8.6.
 #include "matvec.hpp"
 
 #include <algorithm>
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256) matvec_w4_kernel(MatvecArgs a, int kw) {
 // weights).  x stands in LDS, `part` values of k at a time, in the order that the weights pair
 // up in.  A workgroup stays and takes tiles of columns in turn, and the next turn's weights
 // are under way beside a turn's products (no load stands behind a condition: at the join the
-// compiler would wait for it).  16 rows, K = 1024, 155,648 columns: 24.8 us, 3.7 TB/s of the
+// compiler would wait for it).  16 rows, K = 1024, 155,648 columns: 24.6 us, 3.7 TB/s of the
 // 5.1 of a large copy.
 template <int S>
 struct Turn {

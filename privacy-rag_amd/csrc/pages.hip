@@ -13,7 +13,7 @@
 // the dirty lines of all L2s (a fork's 29 MB of copies: 8.1 us, through the caches 21).  A
 // fork takes 5 us of plan before its copies, a compaction's 92 us and 5 of plan.  New tokens
 // go through the caches, where the attention finds them: 34 MB in 12.4 us (5.4 TB/s with
-// their reads), one token of 64 sequences in 4.1 of the host's 9.9.
+// their reads), one token of 64 sequences in 4.1 of the host's 10.
 #include "pages.hpp"
 
 #include <algorithm>

@@ -104,7 +104,8 @@ class Qwen3Answers:
     def extend(self, sequences, rows):
         """Appends rows[i], a list of one token or more, to sequences[i]; returns the logits
         after each, [len(sequences)][vocab].  Raises, with nothing changed, where the pages
-        or the capacity do not suffice."""
+        or the capacity do not suffice.  (What fails later, for memory say, leaves the tokens
+        without their keys: such sequences are to be ended.)"""
         sequences, rows = list(sequences), [list(r) for r in rows]
         if len(sequences) != len(rows) or not rows or not all(rows):
             raise ValueError("each sequence takes one token or more")
