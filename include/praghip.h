@@ -732,6 +732,51 @@ typedef struct praghip_w4 {
 int praghip_matvec_w4(int device, const praghip_w4 *weights, const void *x, int64_t x_stride, size_t m, void *y,
                       int64_t y_stride, void *stream);
 
+/* --------------------------------------- serving: new tokens, rotated, into the cache */
+/* Rows starts[s] .. starts[s + 1] - 1 of q ([tokens][heads][head_dim]), k and v ([tokens]
+ * [kv_heads][head_dim]; strides {token, head}) are the newest tokens of sequence s, the last
+ * at position lengths[s] - 1.  For the token at position p, with x a head of q or of k:
+ *   x w / sqrt(mean x^2 + eps), where q_norm (k_norm) names head_dim weights w; then
+ *   (a cos[p][i] - b sin[p][i], b cos[p][i] + a sin[p][i]) for the pairs (a, b) of its first
+ *   2 half values: values i and i + half, or 2 i and 2 i + 1 where `interleaved` is not 0.
+ * Queries go to out (which may be q itself), keys and values into the cache.  All in 32
+ * bits, rounded once.  cos and sin are [positions][half] of 32 bits, rows cos_row and sin_row
+ * apart, and hold every position that a row of the tables does (positions >= table_width *
+ * page_size, or the positions that count of it: E_ROTARY_SHAPE); 2 half <= head_dim.  A
+ * token's key and value are dropped at a position below 0, beyond the tables or without a
+ * page; its query takes the nearest position there is.  Rows of no stretch stay as they are.
+ * tokens x (heads + 2 kv_heads) is below 2^31 (E_ATTENTION_SHAPE). */
+typedef struct praghip_append {
+  const void *q, *k, *v;
+  int64_t q_strides[2], k_strides[2], v_strides[2];
+  void *out;
+  int64_t out_strides[2];
+  const void *q_norm, *k_norm; /* or NULL */
+  const float *cos, *sin;
+  int64_t cos_row, sin_row;
+  size_t positions, half, heads, tokens;
+  float eps;
+  int interleaved;
+} praghip_append;
+int praghip_page_append(int device, const praghip_cache *cache, const praghip_append *args, const int32_t *starts,
+                        void *stream);
+
+/* ------------------------------------------------------------- serving: norms */
+/* total[i] = x[i] + residual[i] and out[i][j] = s w[j] / sqrt(mean s^2 + eps) with s the sum
+ * before it is rounded, for rows of n values of `type` (n up to 2^30, rows below 2^31:
+ * E_NORM_SHAPE; addresses even: E_NORM_ALIGNMENT).  residual NULL: no addition, and total is
+ * not written; total may be NULL too.  Strides of a row each, in elements.  out and total may
+ * be x or residual themselves (the same rows), not each other. */
+typedef struct praghip_norm {
+  const void *x, *residual, *weight;
+  void *out, *total;
+  int64_t x_row, residual_row, out_row, total_row;
+  size_t rows, n;
+  float eps;
+  int type;
+} praghip_norm;
+int praghip_add_norm(int device, const praghip_norm *args, void *stream);
+
 /* ------------------------------------------------------ synthetic inputs */
 /* Seeded counter-based inputs (no counterpart in the reference, whose probes
  * draw from mt19937_64, check_resident.cpp:26): element i of the buffer is

@@ -1,5 +1,6 @@
 // C ABI of the serving operators (include/praghip.h): checks of arguments, and the
-// launches of attention_decode.hip, attention_prompt.hip, pages.hip and matvec.hip.
+// launches of attention_decode.hip, attention_prompt.hip, pages.hip, matvec.hip, append.hip
+// and norm.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -7,9 +8,11 @@
 #include <cmath>
 
 #include "praghip.h"
+#include "append.hpp"
 #include "attention.hpp"
 #include "host.hpp"
 #include "matvec.hpp"
+#include "norm.hpp"
 #include "pages.hpp"
 
 using namespace praghip;
@@ -345,6 +348,55 @@ int praghip_matvec_w4(int device, const praghip_w4* w, const void* x, int64_t x_
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_matvec_w4(a, w->type, pick(stream));
   return hip_result("E_W4_HIP: ", e);
+}
+
+int praghip_page_append(int device, const praghip_cache* c, const praghip_append* p, const int32_t* starts, void* stream) {
+  if ((p && p->tokens == 0) || (c && c->seqs == 0)) return PRAGHIP_OK;
+  if (const int rc = check_cache(c)) return rc;
+  if (!p || !p->q || !p->k || !p->v || !p->out || !starts || (p->half && (!p->cos || !p->sin))) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  if (!p->heads || p->heads > 65536 || p->tokens > INT_MAX || p->tokens > INT_MAX / (p->heads + 2 * c->kv_heads))
+    return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
+  if (p->half > c->head_dim / 2 || p->positions > INT_MAX || !std::isfinite(p->eps) || p->eps < 0 ||
+      (p->half && int64_t(p->positions) < capacity_of(c->table_width, c->page_size)))
+    return fail(PRAGHIP_E_SHAPE, "E_ROTARY_SHAPE");
+  if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out) || !aligned16(p->q_norm) ||
+      !aligned16(p->k_norm) || !aligned4(p->cos) || !aligned4(p->sin) || !aligned4(starts) || !eights(p->q_strides, 2) ||
+      !eights(p->k_strides, 2) || !eights(p->v_strides, 2) || !eights(p->out_strides, 2))
+    return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_ALIGNMENT");
+  AppendArgs a{};
+  a.q = p->q, a.k = p->k, a.v = p->v, a.out = p->out;
+  a.q_token = p->q_strides[0], a.q_head = p->q_strides[1], a.k_token = p->k_strides[0], a.k_head = p->k_strides[1];
+  a.v_token = p->v_strides[0], a.v_head = p->v_strides[1], a.out_token = p->out_strides[0], a.out_head = p->out_strides[1];
+  a.q_norm = p->q_norm, a.k_norm = p->k_norm, a.eps = p->eps;
+  a.cos = p->cos, a.sin = p->sin, a.cos_row = p->cos_row, a.sin_row = p->sin_row;
+  a.positions = int(p->positions), a.half = int(p->half), a.interleaved = p->interleaved != 0;
+  a.k_pages = c->k, a.v_pages = c->v;
+  a.kp_page = c->k_strides[0], a.kp_head = c->k_strides[1], a.kp_token = c->k_strides[2];
+  a.vp_page = c->v_strides[0], a.vp_head = c->v_strides[1], a.vp_token = c->v_strides[2];
+  a.tables = c->tables, a.lengths = c->lengths, a.starts = starts, a.table_stride = c->table_stride;
+  a.width = int(c->table_width), a.seqs = int(c->seqs), a.pages = int(c->pages), a.page_shift = log2_of(c->page_size);
+  a.heads = int(p->heads), a.kv_heads = int(c->kv_heads), a.dim = int(c->head_dim), a.tokens = int(p->tokens);
+  DeviceScope scope(device);
+  hipError_t e = scope.status();
+  if (e == hipSuccess) e = launch_page_append(a, c->type, pick(stream));
+  return hip_result("E_ATTENTION_HIP: ", e);
+}
+
+int praghip_add_norm(int device, const praghip_norm* p, void* stream) {
+  if (p && (p->rows == 0 || p->n == 0)) return PRAGHIP_OK;
+  if (!p || !p->x || !p->weight || !p->out) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  if (p->type != PRAGHIP_BF16 && p->type != PRAGHIP_F16) return fail(PRAGHIP_E_ARGUMENT, "E_NORM_TYPE");
+  if (p->rows > INT_MAX || p->n > (1u << 30) || !std::isfinite(p->eps) || p->eps < 0) return fail(PRAGHIP_E_SHAPE, "E_NORM_SHAPE");
+  for (const void* at : {p->x, p->residual, p->weight, static_cast<const void*>(p->out), static_cast<const void*>(p->total)})
+    if (reinterpret_cast<uintptr_t>(at) & 1) return fail(PRAGHIP_E_ARGUMENT, "E_NORM_ALIGNMENT");
+  NormArgs a{};
+  a.x = p->x, a.residual = p->residual, a.weight = p->weight, a.out = p->out, a.total = p->residual ? p->total : nullptr;
+  a.x_row = p->x_row, a.residual_row = p->residual_row, a.out_row = p->out_row, a.total_row = p->total_row;
+  a.rows = int64_t(p->rows), a.n = int(p->n), a.eps = p->eps;
+  DeviceScope scope(device);
+  hipError_t e = scope.status();
+  if (e == hipSuccess) e = launch_add_norm(a, p->type, pick(stream));
+  return hip_result("E_NORM_HIP: ", e);
 }
 
 }  // extern "C"

@@ -43,6 +43,8 @@ from .attention import page_write, paged_decode, paged_prompt  # noqa: F401
 from .pages import (page_check, page_compact, page_copy, page_fork, page_free, page_reserve,  # noqa: F401
                     page_trim)
 from .matvec import matvec_w4, quantize_w4  # noqa: F401
+from .append import page_append, rotary_table  # noqa: F401
+from .norm import add_norm  # noqa: F401
 from . import frames, synth  # noqa: F401
 
 

@@ -94,6 +94,22 @@ class W4(ctypes.Structure):
                 ("type", i32)]
 
 
+class Append(ctypes.Structure):
+    """praghip_append: new tokens' queries, keys and values, their norms and rotations."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_strides", ctypes.c_int64 * 2), ("k_strides", ctypes.c_int64 * 2),
+                ("v_strides", ctypes.c_int64 * 2), ("out", vp), ("out_strides", ctypes.c_int64 * 2), ("q_norm", vp),
+                ("k_norm", vp), ("cos", vp), ("sin", vp), ("cos_row", ctypes.c_int64), ("sin_row", ctypes.c_int64),
+                ("positions", sz), ("half", sz), ("heads", sz), ("tokens", sz), ("eps", ctypes.c_float),
+                ("interleaved", i32)]
+
+
+class Norm(ctypes.Structure):
+    """praghip_norm: rows of a norm with the residual's addition."""
+    _fields_ = [("x", vp), ("residual", vp), ("weight", vp), ("out", vp), ("total", vp), ("x_row", ctypes.c_int64),
+                ("residual_row", ctypes.c_int64), ("out_row", ctypes.c_int64), ("total_row", ctypes.c_int64),
+                ("rows", sz), ("n", sz), ("eps", ctypes.c_float), ("type", i32)]
+
+
 pp = ctypes.POINTER(ctypes.c_void_p)
 f32, i64 = ctypes.c_float, ctypes.c_int64
 
@@ -216,6 +232,8 @@ SIGNATURES = {
     "praghip_page_copy": (i32, [i32, vp, vp, vp, sz, vp]),
     "praghip_page_write": (i32, [i32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "praghip_matvec_w4": (i32, [i32, vp, vp, i64, sz, vp, i64, vp]),
+    "praghip_page_append": (i32, [i32, vp, vp, vp, vp]),
+    "praghip_add_norm": (i32, [i32, vp, vp]),
 }
 
 _lib = None

@@ -21,16 +21,16 @@ from ._lib import E_ARGUMENT, PraghipError, check, lib, shape_error
 
 # A call's checks and packing are a few microseconds, as long as a small kernel: they
 # read each attribute of a tensor once, and structures go to the library as packed bytes.
-_torch = _int32 = _uint8 = _current = None
+_torch = _int32 = _uint8 = _float32 = _current = None
 _kinds: dict = {}                     # torch dtype -> type code
 _CACHE = struct.Struct("2P6q4Qi4xPqQPQ")  # praghip_cache
 _two = struct.Struct("2q").pack
 
 
 def _load():
-    global _torch, _int32, _uint8, _current
+    global _torch, _int32, _uint8, _float32, _current
     import torch
-    _torch, _int32, _uint8 = torch, torch.int32, torch.uint8
+    _torch, _int32, _uint8, _float32 = torch, torch.int32, torch.uint8, torch.float32
     _kinds.update({torch.bfloat16: 0, torch.float16: 1})
     _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
         (lambda index: torch.cuda.current_stream(index).cuda_stream)
