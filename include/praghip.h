@@ -632,6 +632,19 @@ int praghip_paged_decode(int device, const praghip_cache *cache, const void *q, 
                          void *out, const int64_t *out_strides, float *lse, float scale, size_t window, size_t sinks,
                          size_t max_length, void *work, size_t work_bytes, void *stream);
 
+/* praghip_paged_decode (without a window) where sequences share prefixes: those of group g,
+ * groups[g] .. groups[g + 1] - 1 (groups [count + 1], not falling, within 0 .. seqs), have
+ * their first shared[g] positions in common, whose keys and values are read once for the
+ * group, from the pages of its first sequence (and no more of them than that one is long).
+ * A sequence that is shorter than its group's prefix, and one in no group, reads all its keys
+ * from its own pages.  groups and shared are device memory; count may be 0.  The blocks of 32
+ * positions of all sequences' and groups' tables and key/value heads, times (heads / kv_heads
+ * + 31) / 16, are at most 2^31 (E_ATTENTION_SHAPE). */
+size_t praghip_paged_shared_workspace(const praghip_cache *cache, size_t heads, size_t count, size_t max_length);
+int praghip_paged_shared(int device, const praghip_cache *cache, const void *q, const int64_t *q_strides, size_t heads,
+                         const int32_t *groups, const int32_t *shared, size_t count, void *out, const int64_t *out_strides,
+                         float *lse, float scale, size_t max_length, void *work, size_t work_bytes, void *stream);
+
 /* The same for many tokens per sequence: rows starts[s] .. starts[s + 1] - 1 of q
  * [tokens][heads][head_dim] (strides {token, head}) are the newest tokens of sequence
  * s, the last of them at position lengths[s] - 1; the cache holds their keys and values

@@ -1,4 +1,4 @@
-// What the attention kernels (attention_decode.hip, attention_prompt.hip) share:
+// What the attention kernels (attention_decode.hip, attention_shared.hip, attention_prompt.hip) share:
 // the cache as a kernel sees it, which keys a query sees, 16-bit vectors of both
 // types with their matrix instructions, and reductions across a wave.
 #pragma once
@@ -40,6 +40,21 @@ struct DecodeArgs {
   bool past;       // whether keys and values are read past the caches
 };
 
+struct SharedArgs {
+  CacheArgs c;
+  const void* q;
+  int64_t q_seq, q_head;
+  void* out;
+  int64_t out_seq, out_head;
+  float* lse;             // [seqs][heads] or null
+  const int32_t* groups;  // [count + 1] first sequences
+  const int32_t* shared;  // [count] positions that a group's sequences have in common
+  int count, columns;     // columns: of a piece in the workspace
+  uint4* entries;         // [count + seqs]
+  float* rows;            // what one workgroup has of a row from first to last: [2][seqs][heads] rows
+  float* pieces;          // and in part: [workgroups][2][columns] rows
+};
+
 struct PromptArgs {
   CacheArgs c;
   const void* q;
@@ -54,9 +69,13 @@ struct PromptArgs {
 };
 
 hipError_t launch_paged_decode(const DecodeArgs& a, int type, unsigned workgroups, hipStream_t s);
+hipError_t launch_paged_shared(const SharedArgs& a, int type, unsigned workgroups, hipStream_t s);
 hipError_t launch_paged_prompt(const PromptArgs& a, int type, hipStream_t s);
 unsigned decode_workgroups(size_t seqs, size_t kv_heads, size_t group, size_t keys);
 size_t decode_work_floats(unsigned workgroups, size_t group, size_t dim);
+unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys);
+size_t shared_columns(size_t seqs, size_t group, size_t dim);  // of a piece, at most
+size_t shared_row_floats(size_t dim);
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys);
 size_t prompt_work_floats(int splits, size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows);
 

@@ -1,0 +1,433 @@
+// Attention of one new token per sequence where groups of sequences share a prefix: the
+// keys and values of the prefix are read once for the group, what follows for each
+// sequence.
+//   o = sum_j 2^(s_j - m) v_j / l over the prefix's keys and the sequence's own, as in
+//   attention_decode.hip, with the two parts' m, l and o joined at the end.
+//
+// An entry is a prefix with the heads of all its sequences as columns, or a sequence's own
+// keys with its heads of one key/value head.  4 dim bytes of K and V a key and key/value head
+// against 4 dim operations a column: reading them bounds it up to some hundred columns, and
+// what decides is again that every CU has loads under way.  The entries' blocks of 32 keys
+// stand in one row, by what they take (a block of up to 32 columns occupies one wave, one of
+// 64 two, ...), and every workgroup takes an equal stretch of it.
+//
+// Within a workgroup an entry's columns are spread over 1, 2, 4 or 8 waves of 32 columns
+// each, which read the same keys one soon after the other (a cache answers), and the others
+// take every 2nd, 4th or 8th block.  The products are attention_decode.hip's, two column
+// tiles of 16 for one load of K and V and one transposition of V.  Waves that have the same
+// columns add up through LDS; what a workgroup has of an entry in part (at most two pieces)
+// goes to the workspace, and the join kernel adds the pieces in order, so results do not
+// depend on timing.
+#include "attention.hpp"
+
+namespace praghip {
+namespace {
+
+template <int D>
+struct SharedShape {
+  static constexpr int waves = D > 128 ? 4 : 8;  // (rows of 256 values take more than 256 registers)
+  static constexpr int steps = D / 32;           // of the first product
+  static constexpr int per = D / 16;             // values of a key's row that a lane holds
+  static constexpr int words = per / 2;
+  static constexpr int row = D + 4;              // a row of o, then m and l
+};
+
+constexpr int kUnits = 4;  // a workgroup's stretch is not shorter
+
+__host__ __device__ __forceinline__ int column_waves(int columns, int waves) {
+  int n = 1;
+  while (n < waves && n * 32 < columns) n <<= 1;
+  return n;
+}
+
+// Keys lo .. hi - 1 of the pages of sequence `first`, for the heads of the sequences from
+// it on: `columns` columns of a key/value head.
+struct Entry {
+  int first, columns, lo, hi;
+  __device__ __forceinline__ int begin() const { return lo >> 5; }
+  __device__ __forceinline__ int blocks() const { return hi > lo ? ((hi + 31) >> 5) - (lo >> 5) : 0; }
+};
+
+// The prefix of a group: as long as its first sequence, whose pages it is read from, at most;
+// a group of one has none.
+__device__ __forceinline__ Entry prefix_of(const SharedArgs& a, int g) {
+  const int first = min(max(a.groups[g], 0), a.c.seqs), end = min(max(a.groups[g + 1], first), a.c.seqs);
+  Entry e{first, (end - first) * a.c.group, 0, 0};
+  if (end - first > 1) e.hi = min(max(a.shared[g], 0), length_of(a.c, first));
+  return e;
+}
+// What sequence s has of its own, and its group (-1: it takes part in none: a sequence that
+// is shorter than the prefix reads all its keys itself).
+__device__ __forceinline__ Entry own_of(const SharedArgs& a, int s, int& group) {
+  Entry e{s, a.c.group, 0, length_of(a.c, s)};
+  group = -1;
+  int lo = 0, hi = a.count - 1;  // the last group that starts at or before s
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.groups[mid] <= s)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  if (a.count > 0 && a.groups[lo] <= s && s < a.groups[lo + 1]) {
+    const int prefix = prefix_of(a, lo).hi;
+    if (prefix > 0 && e.hi >= prefix) {
+      e.lo = prefix;
+      group = lo;
+    }
+  }
+  return e;
+}
+__device__ __forceinline__ Entry entry_of(const SharedArgs& a, int e, int& group) {
+  group = -1;
+  return e < a.count ? prefix_of(a, e) : own_of(a, e - a.count, group);
+}
+// units of an entry's one key/value head: blocks times waves
+__device__ __forceinline__ uint32_t units_of(int columns, int blocks, int waves) {
+  return uint32_t(blocks) * column_waves(columns, waves) * ((columns + 32 * waves - 1) / (32 * waves));
+}
+
+// Units over the workgroups: each of the first `extra` has one more than the others.
+struct Stretches {
+  uint32_t count, each, extra;
+  __device__ __forceinline__ Stretches(uint32_t units, uint32_t most) {
+    count = max(1u, min(most, (units + kUnits - 1) / kUnits));
+    each = units / count;
+    extra = units - each * count;
+  }
+  __device__ __forceinline__ uint32_t begin(uint32_t w) const { return each * w + min(w, extra); }
+  // the workgroup whose stretch holds unit u
+  __device__ __forceinline__ uint32_t of(uint32_t u) const {
+    const uint32_t longer = extra * (each + 1);
+    return u < longer ? u / (each + 1) : extra + (u - longer) / each;
+  }
+};
+
+template <typename T, int D, bool EXACT>
+__global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kernel(SharedArgs a) {
+  using S = SharedShape<D>;
+  constexpr int W = S::waves;
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // [W][32] rows
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4, entries = a.count + c.seqs;
+
+  // units before each stretch of entries, one stretch per lane; every wave counts for itself
+  const int per = (entries + 63) >> 6;
+  uint32_t mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    if (e < entries) {
+      int group;
+      const Entry x = entry_of(a, e, group);
+      mine += units_of(x.columns, x.blocks(), W) * c.kv_heads;
+    }
+  }
+  uint32_t sum = mine;  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += up;
+  }
+  const uint32_t total = uint32_t(__builtin_amdgcn_readlane(int(sum), 63));
+  if (blockIdx.x == 0 && wave == 0) {  // for the join
+    uint32_t at = sum - mine;
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e >= entries) break;
+      int group;
+      const Entry x = entry_of(a, e, group);
+      a.entries[e] = uint4{at, uint32_t(x.blocks()), e < a.count ? uint32_t(x.first) : uint32_t(group), uint32_t(x.columns)};
+      at += units_of(x.columns, x.blocks(), W) * c.kv_heads;
+    }
+    if (lane == 0) a.entries[entries].x = total;
+  }
+  const Stretches stretches(total, gridDim.x);
+  if (blockIdx.x >= stretches.count) return;
+  const uint32_t u_begin = stretches.begin(blockIdx.x), u_end = stretches.begin(blockIdx.x + 1);
+  uint32_t u = u_begin;
+  if (u >= u_end) return;
+  const int from_lane = __popcll(__ballot(sum <= u));
+  int e = from_lane * per;
+  uint32_t base = uint32_t(__builtin_amdgcn_readlane(int(sum - mine), from_lane));
+
+  while (u < u_end && e < entries) {
+    int group;
+    const Entry x = entry_of(a, e, group);
+    const int nb = x.blocks(), cw = column_waves(x.columns, W), parts = (x.columns + 32 * W - 1) / (32 * W);
+    const uint32_t each = uint32_t(nb) * cw, all = each * parts * c.kv_heads;
+    if (u >= base + all) {
+      base += all;
+      ++e;
+      continue;
+    }
+    const int index = int((u - base) / each), h = index / parts, column0 = (index - h * parts) * 32 * W;
+    const uint32_t start = base + index * each, stop = min(u_end, start + each);
+    const int first = int(u - start + cw - 1) / cw, last = int(stop - start + cw - 1) / cw;
+    u = stop;
+    if (first >= last) continue;
+
+    const int kw = W / cw, part = wave / cw, mine0 = column0 + (wave - part * cw) * 32;
+    const bool two = mine0 + 16 < x.columns;
+    f32x4 o[2][S::per];
+    float m[2] = {kNegInf, kNegInf}, l[2] = {0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
+    if (mine0 < x.columns && first + part < last) {
+      u32x4 q[2][S::steps];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int column = mine0 + 16 * t + col, seq = x.first + column / c.group, head = h * c.group + column % c.group;
+#pragma unroll
+        for (int i = 0; i < S::steps; ++i) {
+          q[t][i] = u32x4{0, 0, 0, 0};
+          const int d = 32 * i + 8 * quad;
+          if (column < x.columns && (EXACT || d < c.dim))
+            q[t][i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + seq * a.q_seq + head * a.q_head + d);
+          q[t][i] ^= c.flip;
+        }
+      }
+      for (int i = first + part; i < last; i += kw) {
+        const int kb = (x.begin() + i) << 5;
+        u32x4 kf[2][S::steps];
+        uint32_t vr[8][S::words];
+        bool page_ok[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int at = (kb + 16 * t) >> c.page_shift;
+          int page = at < int(c.capacity >> c.page_shift) ? c.tables[x.first * c.table_stride + at] : -1;
+          page_ok[t] = page >= 0 && page < c.pages;
+          page = page_ok[t] ? page : 0;
+          const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
+          const T* kp = static_cast<const T*>(c.k) + uint64_t(page) * c.k_page + uint64_t(h) * c.k_head + uint64_t(row + col) * c.k_token + 8 * quad;
+#pragma unroll
+          for (int n = 0; n < S::steps; ++n) {
+            kf[t][n] = u32x4{0, 0, 0, 0};
+            if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
+          }
+          const T* vp = static_cast<const T*>(c.v) + uint64_t(page) * c.v_page + uint64_t(h) * c.v_head + uint64_t(row + 4 * quad) * c.v_token + S::per * col;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int w = 0; w < S::words; ++w) vr[4 * t + r][w] = 0;
+            if (EXACT || S::per * col < c.dim) {
+              if constexpr (S::words == 2) {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(vp + uint64_t(r) * c.v_token);
+                vr[4 * t + r][0] = v[0];
+                vr[4 * t + r][1] = v[1];
+              } else {
+#pragma unroll
+                for (int w = 0; w < S::words; w += 4) {
+                  if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
+                  const u32x4 v = *reinterpret_cast<const u32x4*>(vp + uint64_t(r) * c.v_token + 2 * w);
+#pragma unroll
+                  for (int b = 0; b < 4; ++b) vr[4 * t + r][w + b] = v[b];
+                }
+              }
+            }
+          }
+        }
+        const bool whole = page_ok[0] && page_ok[1] && kb >= x.lo && kb + 32 <= x.hi;
+        u32x4 ph[2], pl[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (t && !two) continue;
+          f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+          for (int n = 0; n < S::steps; ++n) {
+            st[0] = Half<T>::mma16(kf[0][n], q[t][n], st[0]);
+            st[1] = Half<T>::mma16(kf[1][n], q[t][n], st[1]);
+          }
+          float s[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) s[r] = st[r >> 2][r & 3] * c.scale;
+          if (!whole) {  // keys that are not the entry's count as nothing, whatever their page holds
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              const int at = kb + 16 * (r >> 2) + 4 * quad + (r & 3);
+              const bool sees = bool(page_ok[r >> 2]) & (at >= x.lo) & (at < x.hi);
+              s[r] = sees ? s[r] : kNegInf;
+#pragma unroll
+              for (int w = 0; w < S::words; ++w) vr[r][w] = sees ? vr[r][w] : 0;
+            }
+          }
+          float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+          top = fmaxf(m[t], max32(max16(top)) - Half<T>::most);
+          if (__any(top > m[t])) {
+            const float f = __builtin_amdgcn_exp2f(m[t] - origin(top));
+            l[t] *= f;
+#pragma unroll
+            for (int j = 0; j < S::per; ++j) o[t][j] *= f;
+            m[t] = top;
+          }
+          uint32_t hi[4], rest[4];
+#pragma unroll
+          for (int r = 0; r < 8; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(s[r] - origin(m[t])), p1 = __builtin_amdgcn_exp2f(s[r + 1] - origin(m[t]));
+            l[t] += p0 + p1;
+            hi[r / 2] = pack2<T>(p0, p1);
+            rest[r / 2] = pack2<T>(p0 - low<T>(hi[r / 2]), p1 - high<T>(hi[r / 2]));
+          }
+          ph[t] = u32x4{hi[0], hi[1], hi[2], hi[3]}, pl[t] = u32x4{rest[0], rest[1], rest[2], rest[3]};
+        }
+#pragma unroll
+        for (int j = 0; j < S::per; ++j) {
+          u32x4 vt;
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            vt[p] = __builtin_amdgcn_perm(vr[2 * p + 1][j / 2], vr[2 * p][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+          o[0][j] = Half<T>::mma16(vt, ph[0], o[0][j]);
+          o[0][j] = Half<T>::mma16(vt, pl[0], o[0][j]);
+          if (two) {
+            o[1][j] = Half<T>::mma16(vt, ph[1], o[1][j]);
+            o[1][j] = Half<T>::mma16(vt, pl[1], o[1][j]);
+          }
+        }
+      }
+    }
+    // the sums of waves that have the same columns
+    __syncthreads();  // the rows of the entry before have been read
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t && !two) continue;
+      const float sums = sum32(sum16(l[t]));
+      float* to = lds + (wave * 32 + 16 * t + col) * S::row;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < S::per; j += 4)
+          *reinterpret_cast<f32x4*>(to + (4 * quad + r) * S::per + j) = f32x4{o[t][j][r], o[t][j + 1][r], o[t][j + 2][r], o[t][j + 3][r]};
+      if (quad == 0) {
+        to[D] = m[t];
+        to[D + 1] = sums;
+      }
+    }
+    __syncthreads();
+    const int have = min(x.columns - column0, 32 * cw), waves = min(kw, last - first);
+    const bool complete = first == 0 && last == nb;
+    const int kind = e < a.count ? 0 : 1;
+    for (int i = threadIdx.x; i < have * (D / 4); i += W * 64) {
+      const int column = i / (D / 4), d = i % (D / 4) * 4, ct = column >> 5, r = column & 31;
+      float top = kNegInf;
+      for (int n = 0; n < waves; ++n) top = fmaxf(top, lds[((n * cw + ct) * 32 + r) * S::row + D]);
+      f32x4 sums = {0, 0, 0, 0};
+      float ls = 0;
+      for (int n = 0; n < waves; ++n) {
+        const float* p = lds + ((n * cw + ct) * 32 + r) * S::row;
+        const float f = __builtin_amdgcn_exp2f(p[D] - origin(top));
+        sums += f * *reinterpret_cast<const f32x4*>(p + d);
+        ls += f * p[D + 1];
+      }
+      const int seq = x.first + (column0 + column) / c.group, head = h * c.group + (column0 + column) % c.group;
+      float* to = complete ? a.rows + ((int64_t(kind) * c.seqs + seq) * (c.kv_heads * c.group) + head) * S::row
+                           : a.pieces + ((int64_t(blockIdx.x) * 2 + (start >= u_begin)) * a.columns + column) * S::row;
+      *reinterpret_cast<f32x4*>(to + d) = sums;
+      if (d == 0) {
+        to[D] = top;
+        to[D + 1] = ls;
+      }
+    }
+  }
+}
+
+// One workgroup per sequence and head: the pieces of its prefix and of its own keys, in
+// order.  Each D / 4 threads take every (1024 / D)-th piece.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned workgroups) {
+  using S = SharedShape<D>;
+  constexpr int per = D / 4, sets = 256 / per, W = S::waves;
+  __shared__ __attribute__((aligned(16))) float part[sets][D];
+  __shared__ float tops[sets], sums[sets];
+  const CacheArgs& c = a.c;
+  const int all = c.kv_heads * c.group, s = blockIdx.x / all, head = blockIdx.x - s * all, kvh = head / c.group;
+  const int set = threadIdx.x / per, d = threadIdx.x % per * 4;
+  const Stretches stretches(a.entries[a.count + c.seqs].x, workgroups);
+  const uint4 own = a.entries[a.count + s];
+  float m = kNegInf, l = 0;
+  f32x4 o = {0, 0, 0, 0};
+  int turn = 0;  // pieces before this part's
+  for (int kind = 0; kind < 2; ++kind) {
+    if (kind == 0 && int(own.z) < 0) continue;
+    const uint4 x = kind ? own : a.entries[own.z];
+    const int nb = int(x.y), columns = int(x.w), cw = column_waves(columns, W), parts = (columns + 32 * W - 1) / (32 * W);
+    if (!nb) continue;
+    const int column = (kind ? 0 : (s - int(x.z)) * c.group) + head - kvh * c.group, cut = column / (32 * W);
+    const uint32_t each = uint32_t(nb) * cw, start = x.x + (uint32_t(kvh) * parts + cut) * each;
+    const uint32_t w0 = stretches.of(start), w1 = stretches.of(start + each - 1);
+    const bool complete = (stretches.begin(w0 + 1) - start + cw - 1) / cw >= uint32_t(nb);
+    const uint32_t count = complete ? 1 : w1 - w0 + 1;
+    for (uint32_t i = (set + sets - turn % sets) % sets; i < count; i += sets) {
+      const uint32_t w = w0 + i, from = max(stretches.begin(w), start), to = min(stretches.begin(w + 1), start + each);
+      if ((from - start + cw - 1) / cw >= (to - start + cw - 1) / cw) continue;  // no block of it
+      const float* p = complete ? a.rows + ((int64_t(kind) * c.seqs + s) * all + head) * S::row
+                                : a.pieces + ((int64_t(w) * 2 + (start >= stretches.begin(w))) * a.columns + column - cut * 32 * W) * S::row;
+      const f32x4 po = *reinterpret_cast<const f32x4*>(p + d);
+      const float pm = p[D], pl = p[D + 1], top = fmaxf(m, pm);
+      const float f = __builtin_amdgcn_exp2f(m - origin(top)), pf = __builtin_amdgcn_exp2f(pm - origin(top));
+      o = o * f + po * pf;
+      l = l * f + pl * pf;
+      m = top;
+    }
+    turn += int(count);
+  }
+  *reinterpret_cast<f32x4*>(&part[set][d]) = o;
+  if (d == 0) {
+    tops[set] = m;
+    sums[set] = l;
+  }
+  __syncthreads();
+  if (int(threadIdx.x) >= D) return;
+  m = kNegInf;
+#pragma unroll
+  for (int i = 0; i < sets; ++i) m = fmaxf(m, tops[i]);
+  float sum = 0;
+  l = 0;
+#pragma unroll
+  for (int i = 0; i < sets; ++i) {
+    const float f = __builtin_amdgcn_exp2f(tops[i] - origin(m));
+    sum += f * part[i][threadIdx.x];
+    l += f * sums[i];
+  }
+  const float inv = l > 0 || l != l ? 1.f / l : 0.f;
+  if (int(threadIdx.x) < c.dim) static_cast<T*>(a.out)[s * a.out_seq + head * a.out_head + threadIdx.x] = T(sum * inv);
+  if (a.lse && threadIdx.x == 0) a.lse[int64_t(s) * all + head] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <typename T, int D>
+hipError_t launch(const SharedArgs& a, unsigned workgroups, hipStream_t s) {
+  using S = SharedShape<D>;
+  constexpr size_t lds = size_t(S::waves) * 32 * S::row * sizeof(float);
+  const auto kernel = a.c.dim == D ? paged_shared_kernel<T, D, true> : paged_shared_kernel<T, D, false>;
+  hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(S::waves * 64), lds, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((shared_join_kernel<T, D>), dim3(unsigned(a.c.seqs) * a.c.kv_heads * a.c.group), dim3(256), 0, s, a, workgroups);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_dim(const SharedArgs& a, unsigned workgroups, hipStream_t s) {
+  return a.c.dim <= 64 ? launch<T, 64>(a, workgroups, s) : a.c.dim <= 128 ? launch<T, 128>(a, workgroups, s) : launch<T, 256>(a, workgroups, s);
+}
+
+int width_of(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+}  // namespace
+
+// One workgroup a CU, and no more than there are stretches.
+unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys) {
+  const size_t units = entries * kv_heads * ((group + 31) / 32) * ((keys + 31) / 32 + 1);
+  return unsigned(std::max<size_t>(1, std::min<size_t>((units + kUnits - 1) / kUnits, 256)));
+}
+size_t shared_columns(size_t seqs, size_t group, size_t dim) {
+  return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? 4 * 32 : 8 * 32);
+}
+size_t shared_row_floats(size_t dim) { return width_of(dim) + 4; }
+
+hipError_t launch_paged_shared(const SharedArgs& a, int type, unsigned workgroups, hipStream_t s) {
+  return type == PRAGHIP_F16 ? launch_dim<_Float16>(a, workgroups, s) : launch_dim<__bf16>(a, workgroups, s);
+}
+
+}  // namespace praghip

@@ -1,6 +1,6 @@
 // C ABI of the serving operators (include/praghip.h): checks of arguments, and the
-// launches of attention_decode.hip, attention_prompt.hip, pages.hip, matvec.hip, append.hip
-// and norm.hip.
+// launches of attention_decode.hip, attention_shared.hip, attention_prompt.hip, pages.hip,
+// matvec.hip, append.hip and norm.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -120,6 +120,26 @@ DecodePlan decode_plan(const praghip_cache& c, size_t heads, size_t max_length) 
   return p;
 }
 
+struct SharedPlan {
+  unsigned workgroups;
+  size_t columns, rows, pieces, bytes;  // rows, pieces: where they begin
+};
+SharedPlan shared_plan(const praghip_cache& c, size_t heads, size_t count, size_t max_length) {
+  SharedPlan p;
+  const size_t group = heads / c.kv_heads, row = shared_row_floats(c.head_dim) * sizeof(float);
+  p.workgroups = shared_workgroups(count + c.seqs, c.kv_heads, group, bound_of(c, max_length));
+  p.columns = shared_columns(c.seqs, group, c.head_dim);
+  p.rows = (count + c.seqs + 1) * sizeof(uint4);
+  p.pieces = p.rows + 2 * c.seqs * heads * row;
+  p.bytes = p.pieces + p.workgroups * 2 * p.columns * row;
+  return p;
+}
+// units of all entries in 32 bits: a head's columns occupy no more waves than two for each 32
+bool units_fit(const praghip_cache& c, size_t heads, size_t count) {
+  const size_t blocks = size_t(capacity_of(c.table_width, c.page_size)) / 32 + 1;
+  return count <= (1u << 20) && (count + c.seqs) * c.kv_heads * ((heads / c.kv_heads + 31) / 16) <= (size_t(1) << 31) / blocks;
+}
+
 int hip_result(const char* what, hipError_t e) { return e == hipSuccess ? PRAGHIP_OK : hip_fail(what, e); }
 
 int check_table(const praghip_page_table* t, const void* a, const void* b, size_t n) {
@@ -183,6 +203,38 @@ int praghip_paged_decode(int device, const praghip_cache* c, const void* q, cons
   DeviceScope scope(device);
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_paged_decode(a, c->type, p.workgroups, pick(stream));
+  return hip_result("E_ATTENTION_HIP: ", e);
+}
+
+size_t praghip_paged_shared_workspace(const praghip_cache* c, size_t heads, size_t count, size_t max_length) {
+  if (!c || check_cache(c) || !heads_fit(*c, heads) || !units_fit(*c, heads, count)) return 0;
+  return shared_plan(*c, heads, count, max_length).bytes;
+}
+
+int praghip_paged_shared(int device, const praghip_cache* c, const void* q, const int64_t* q_strides, size_t heads,
+                         const int32_t* groups, const int32_t* shared, size_t count, void* out, const int64_t* out_strides,
+                         float* lse, float scale, size_t max_length, void* work, size_t work_bytes, void* stream) {
+  if (c && c->seqs == 0) return PRAGHIP_OK;
+  if (const int rc = check_cache(c)) return rc;
+  if (!q || !q_strides || !out || !out_strides || !work || (count && (!groups || !shared))) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  if (!heads_fit(*c, heads) || !units_fit(*c, heads, count) || !std::isfinite(scale)) return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_SHAPE");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(work) || !aligned4(lse) || !aligned4(groups) || !aligned4(shared) ||
+      !eights(q_strides, 2) || !eights(out_strides, 2))
+    return fail(PRAGHIP_E_ARGUMENT, "E_ATTENTION_ALIGNMENT");
+  const SharedPlan p = shared_plan(*c, heads, count, max_length);
+  if (work_bytes < p.bytes) return fail(PRAGHIP_E_SHAPE, "E_ATTENTION_WORKSPACE");
+  SharedArgs a{};
+  a.c = cache_args(*c, heads, scale, 0, 0);
+  a.q = q, a.q_seq = q_strides[0], a.q_head = q_strides[1];
+  a.out = out, a.out_seq = out_strides[0], a.out_head = out_strides[1];
+  a.lse = lse;
+  a.groups = groups, a.shared = shared, a.count = int(count), a.columns = int(p.columns);
+  a.entries = static_cast<uint4*>(work);
+  a.rows = reinterpret_cast<float*>(static_cast<char*>(work) + p.rows);
+  a.pieces = reinterpret_cast<float*>(static_cast<char*>(work) + p.pieces);
+  DeviceScope scope(device);
+  hipError_t e = scope.status();
+  if (e == hipSuccess) e = launch_paged_shared(a, c->type, p.workgroups, pick(stream));
   return hip_result("E_ATTENTION_HIP: ", e);
 }
 

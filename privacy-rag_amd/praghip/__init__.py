@@ -39,7 +39,7 @@ from .weights import MappedWeights  # noqa: F401
 from .qwen3 import QWEN3_0_6B, Qwen3LocalGemms, Qwen3Shape  # noqa: F401
 from .matrix import Matrix, MatrixPacking, PublicZero, matrix_packing  # noqa: F401
 from .token import DeviceCipherBatch, Packing, TokenWeights, packed_target  # noqa: F401
-from .attention import page_write, paged_decode, paged_prompt  # noqa: F401
+from .attention import page_write, paged_decode, paged_prompt, paged_shared  # noqa: F401
 from .pages import (page_check, page_compact, page_copy, page_fork, page_free, page_reserve,  # noqa: F401
                     page_trim)
 from .matvec import matvec_w4, quantize_w4  # noqa: F401

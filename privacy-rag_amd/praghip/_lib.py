@@ -220,6 +220,8 @@ SIGNATURES = {
     "praghip_share_gemm_batch": (i32, [i32, vp, sz, vp]),
     "praghip_paged_decode_workspace": (sz, [vp, sz, sz]),
     "praghip_paged_decode": (i32, [i32, vp, vp, vp, sz, vp, vp, vp, f32, sz, sz, sz, vp, sz, vp]),
+    "praghip_paged_shared_workspace": (sz, [vp, sz, sz, sz]),
+    "praghip_paged_shared": (i32, [i32, vp, vp, vp, sz, vp, vp, sz, vp, vp, vp, f32, sz, vp, sz, vp]),
     "praghip_paged_prompt_workspace": (sz, [vp, sz, sz, sz, sz, sz]),
     "praghip_paged_prompt": (i32, [i32, vp, vp, vp, sz, vp, sz, sz, vp, vp, vp, f32, sz, sz, sz, vp, sz, vp]),
     "praghip_page_reserve": (i32, [i32, vp, vp, vp, sz, vp]),

@@ -1,5 +1,6 @@
 """Attention over a paged key/value cache: one new token per sequence
-(:func:`paged_decode`) or many (:func:`paged_prompt`).
+(:func:`paged_decode`, and :func:`paged_shared` where sequences share prefixes) or many
+(:func:`paged_prompt`).
 
 The reference's attention is a two-party protocol, and its float Qwen3 a transformers
 model; these serve such a model in the clear beside the protocol.  Tensors are on one GPU; calls
@@ -158,6 +159,42 @@ def paged_decode(q, k_pages, v_pages, tables, lengths, *, scale: float | None = 
                                      _two(to[0], to[1]), sums.data_ptr() if lse else None,
                                      shape[2] ** -0.5 if scale is None else scale, window, sinks, max_length,
                                      work.data_ptr(), size, _stream(index, stream)))
+    return (out, sums) if lse else out
+
+
+def paged_shared(q, k_pages, v_pages, tables, lengths, groups, shared, *, scale: float | None = None, max_length: int = 0,
+                 lse: bool = False, out=None, stream=None):
+    """:func:`paged_decode` of sequences that share prefixes, each read once for its group.
+
+    groups int32 [count + 1], not falling: sequences groups[g] .. groups[g + 1] - 1 have their
+    first shared[g] positions (int32 [count]) in common, as :func:`page_fork` leaves a parent
+    and its children.  Those are read from the pages of the group's first sequence, as far as
+    that one is long; a sequence that is shorter, or in no group, reads its own.  There is no
+    window: one that moves on leaves the prefix.  The rest is as in :func:`paged_decode`.
+    """
+    kind, index, shape, qs = _kind(q, "E_ATTENTION_TYPE"), q.get_device(), q.shape, q.stride()
+    cache, pages, seqs = _cache(k_pages, v_pages, tables, lengths, q, kind, index)
+    if len(shape) != 3 or shape[0] != seqs or shape[2] != pages[3] or (qs[2] != 1 and shape[2] > 1) or not pages[1] or \
+            shape[1] % pages[1] or max_length < 0 or len(shared.shape) != 1:
+        raise shape_error("E_ATTENTION_SHAPE")
+    count = shared.shape[0]
+    first = _starts(groups, count, index)
+    if shared.dtype is not _int32 or shared.get_device() != index:
+        raise _type_error("E_ATTENTION_INTS")
+    if count > 1 and shared.stride(0) != 1:
+        raise shape_error("E_ATTENTION_SHAPE")
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _no_gradients("E_ATTENTION_GRADIENT")
+    out = _output(q, shape, out, index, stream)
+    sums = _lse(q, shape, index, stream) if lse else None
+    if seqs:
+        L, heads, to = lib(), shape[1], out.stride()
+        size = L.praghip_paged_shared_workspace(cache, heads, count, max_length)
+        work = _work(size, q, stream)
+        check(L.praghip_paged_shared(index, cache, q.data_ptr(), _two(qs[0], qs[1]), heads, first, shared.data_ptr(), count,
+                                     out.data_ptr(), _two(to[0], to[1]), sums.data_ptr() if lse else None,
+                                     shape[2] ** -0.5 if scale is None else scale, max_length, work.data_ptr(), size,
+                                     _stream(index, stream)))
     return (out, sums) if lse else out
 
 
