@@ -585,6 +585,7 @@ int praghip_frame_check(const uint8_t *in, const praghip_frame_header *expect);
  * asynchronous on `stream`; 16-bit data of PRAGHIP_BF16 or PRAGHIP_F16. */
 #define PRAGHIP_BF16 0
 #define PRAGHIP_F16 1
+#define PRAGHIP_F32 2 /* (logits alone) */
 
 /* One layer's keys and values in pages: position p of sequence s is token p %
  * page_size of page tables[s][p / page_size].  k and v are [pages][kv_heads]
@@ -789,6 +790,37 @@ typedef struct praghip_norm {
   int type;
 } praghip_norm;
 int praghip_add_norm(int device, const praghip_norm *args, void *stream);
+
+/* ------------------------------------------------------------ serving: draws */
+/* One token of each row of logits ([rows][vocab] of BF16, F16 or F32, rows `row` elements
+ * apart), drawn with uniform[i] of [0, 1).  With w_j = exp((x_j - max x) / temperature):
+ * of the tokens in the order of falling x (of equal ones, rising j) the first top_k stay;
+ * of those the shortest run whose sum of w reaches top_p times theirs (one token at least);
+ * of those the ones with w >= min_p.  The token is the first, by j, up to which the sum of w
+ * of what stays is above uniform[i] times the whole sum.
+ *
+ * temperature, top_k, top_p and min_p are device lists [rows], or NULL for one value of all
+ * rows.  A temperature that is not above 0 takes the largest logit's lowest index; a top_k
+ * below 1, a top_p of 1 and more and a min_p of 0 and less filter nothing (a min_p above 1
+ * counts as 1, NaN as no filter).  A logit of NaN counts as -infinity, which is never drawn,
+ * +infinity as the largest 32-bit number; a row without any other gets -1.  Weights are held
+ * in units of 2^-43 of the power of two above the largest, so that the token does not depend
+ * on an order of sums; one below 2^-44 of the largest is 0.  vocab is at most 2^20, rows at
+ * most 65535 (E_SAMPLE_SHAPE).  work: 16-byte aligned, as praghip_sample_workspace says
+ * (E_SAMPLE_WORKSPACE), not used by another call until this one is done. */
+typedef struct praghip_sample {
+  const void *logits;
+  int64_t row;
+  size_t rows, vocab;
+  const float *uniform, *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  float temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all;
+  int64_t *out;
+  int type;
+} praghip_sample;
+size_t praghip_sample_workspace(size_t rows, size_t vocab);
+int praghip_sample_tokens(int device, const praghip_sample *args, void *work, size_t work_bytes, void *stream);
 
 /* ------------------------------------------------------ synthetic inputs */
 /* Seeded counter-based inputs (no counterpart in the reference, whose probes

@@ -1,6 +1,6 @@
 // C ABI of the serving operators (include/praghip.h): checks of arguments, and the
 // launches of attention_decode.hip, attention_shared.hip, attention_prompt.hip, pages.hip,
-// matvec.hip, append.hip and norm.hip.
+// matvec.hip, append.hip, norm.hip and sample.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -14,6 +14,7 @@
 #include "matvec.hpp"
 #include "norm.hpp"
 #include "pages.hpp"
+#include "sample.hpp"
 
 using namespace praghip;
 using namespace praghip::host;
@@ -449,6 +450,33 @@ int praghip_add_norm(int device, const praghip_norm* p, void* stream) {
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_add_norm(a, p->type, pick(stream));
   return hip_result("E_NORM_HIP: ", e);
+}
+
+size_t praghip_sample_workspace(size_t rows, size_t vocab) {
+  return rows > 65535 || vocab > kSampleVocab ? 0 : sample_work_bytes(rows, vocab);
+}
+
+int praghip_sample_tokens(int device, const praghip_sample* p, void* work, size_t work_bytes, void* stream) {
+  if (p && p->rows == 0) return PRAGHIP_OK;
+  if (!p) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  const int type = p->type;
+  if (type != PRAGHIP_BF16 && type != PRAGHIP_F16 && type != PRAGHIP_F32) return fail(PRAGHIP_E_ARGUMENT, "E_SAMPLE_TYPE");
+  if (p->rows > 65535 || !p->vocab || p->vocab > kSampleVocab) return fail(PRAGHIP_E_SHAPE, "E_SAMPLE_SHAPE");
+  if (!p->logits || !p->uniform || !p->out || !work) return fail(PRAGHIP_E_ARGUMENT, "E_NULL");
+  if (reinterpret_cast<uintptr_t>(p->logits) & (type == PRAGHIP_F32 ? 3 : 1) || !aligned4(p->uniform) || !aligned4(p->temperature) ||
+      !aligned4(p->top_p) || !aligned4(p->min_p) || !aligned4(p->top_k) || !aligned8(p->out) || !aligned16(work))
+    return fail(PRAGHIP_E_ARGUMENT, "E_SAMPLE_ALIGNMENT");
+  if (work_bytes < sample_work_bytes(p->rows, p->vocab)) return fail(PRAGHIP_E_SHAPE, "E_SAMPLE_WORKSPACE");
+  SampleArgs a{};
+  a.logits = p->logits, a.row = p->row, a.rows = int(p->rows), a.vocab = int(p->vocab);
+  a.uniform = p->uniform, a.temperature = p->temperature, a.top_p = p->top_p, a.min_p = p->min_p, a.top_k = p->top_k;
+  a.temperature_all = p->temperature_all, a.top_p_all = p->top_p_all, a.min_p_all = p->min_p_all, a.top_k_all = p->top_k_all;
+  a.out = p->out;
+  sample_work(a, work);
+  DeviceScope scope(device);
+  hipError_t e = scope.status();
+  if (e == hipSuccess) e = launch_sample_tokens(a, type, pick(stream));
+  return hip_result("E_SAMPLE_HIP: ", e);
 }
 
 }  // extern "C"

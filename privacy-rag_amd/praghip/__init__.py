@@ -45,6 +45,7 @@ from .pages import (page_check, page_compact, page_copy, page_fork, page_free, p
 from .matvec import matvec_w4, quantize_w4  # noqa: F401
 from .append import page_append, rotary_table  # noqa: F401
 from .norm import add_norm  # noqa: F401
+from .sample import sample_tokens  # noqa: F401
 from . import frames, synth  # noqa: F401
 
 

@@ -110,6 +110,14 @@ class Norm(ctypes.Structure):
                 ("rows", sz), ("n", sz), ("eps", ctypes.c_float), ("type", i32)]
 
 
+class Sample(ctypes.Structure):
+    """praghip_sample: rows of logits and how to draw from them."""
+    _fields_ = [("logits", vp), ("row", ctypes.c_int64), ("rows", sz), ("vocab", sz), ("uniform", vp), ("temperature", vp),
+                ("top_p", vp), ("min_p", vp), ("top_k", vp), ("temperature_all", ctypes.c_float),
+                ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("out", vp),
+                ("type", i32)]
+
+
 pp = ctypes.POINTER(ctypes.c_void_p)
 f32, i64 = ctypes.c_float, ctypes.c_int64
 
@@ -236,6 +244,8 @@ SIGNATURES = {
     "praghip_matvec_w4": (i32, [i32, vp, vp, i64, sz, vp, i64, vp]),
     "praghip_page_append": (i32, [i32, vp, vp, vp, vp]),
     "praghip_add_norm": (i32, [i32, vp, vp]),
+    "praghip_sample_workspace": (sz, [sz, sz]),
+    "praghip_sample_tokens": (i32, [i32, vp, vp, sz, vp]),
 }
 
 _lib = None
