@@ -9,16 +9,16 @@
 //
 // Reading the logits bounds it, and beside that the weights' 64-bit instructions, some 15 a
 // token: a row is cut into parts of kPart tokens for a workgroup each.  Sorting nothing, the
-// cuts are found in bins of 1/16 of a power of two:
-// * the first kernel puts its part's counts and sums into bins (LDS, then the workspace),
-//   relative to the part's own maximum, whose bin is a whole number of powers of two from any
-//   other part's, so that parts are added by shifting;
-// * in the second every part adds the row's bins, finds those in which a cut falls, and
-//   appends its own tokens of those bins to the row's list.  The part that is done last cuts
-//   the listed bins by value and index (digits of 10 bits), adds what stays of each part,
-//   takes the part that the random number falls into and goes through that one by index.
-// No part waits for another.  The order of the list changes nothing: sums are of integers,
-// and cuts are by value and index.
+// cuts are found in bins of 1/16 of a power of two, in three kernels:
+// * bins: each part's counts and sums by bin (LDS, then the workspace), relative to the part's
+//   own maximum, whose bin is a whole number of powers of two from any other part's, so that
+//   parts are added by shifting;
+// * list: every part adds the row's bins, finds those in which a cut falls, and appends its own
+//   tokens of those bins to the row's list;
+// * draw: a workgroup a row cuts the listed bins by value and index (digits of 10 bits of both
+//   together), adds what stays of each part, takes the part that the random number falls into
+//   and goes through that one by index.
+// The order of the list changes nothing: sums are of integers, and cuts are by value and index.
 #include "sample.hpp"
 
 #include <climits>
@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kEach = 16, kPart = kThreads * kEach;  // tokens of a thread, in pieces of 8, and of a part
+constexpr int kParts = kSampleVocab / kPart > 64 ? kSampleVocab / kPart : 64;  // of a row, at most
 constexpr int kRange = 46, kBins = kRange * 16;      // powers of two that weights span, and their bins
 constexpr int kBits = 43;                            // of a weight's fraction
 constexpr int kDigit = 10, kDigits = 1 << kDigit;
@@ -137,40 +138,59 @@ __device__ __forceinline__ Filters filters_of(const SampleArgs& a, int row) {
 }
 
 // --------------------------------------------------------- over the workgroup
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
+// The lanes before and this one, by moves within rows of 16 lanes and from their last ones.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CONTROL, ROWS, 0xf, false));
 }
-__device__ __forceinline__ u64 group_sum(u64 v, u64* lds) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) v += lds[w];
-  return v;
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {
+  return u64(moved<CONTROL, ROWS>(uint32_t(v))) | u64(moved<CONTROL, ROWS>(uint32_t(v >> 32))) << 32;
 }
-// the sum of the threads before, and with this one
+template <typename V, typename F>
+__device__ __forceinline__ V wave_scan(V v, F with) {
+  v = with(v, moved<0x111, 0xf>(v));
+  v = with(v, moved<0x112, 0xf>(v));
+  v = with(v, moved<0x114, 0xf>(v));
+  v = with(v, moved<0x118, 0xf>(v));
+  v = with(v, moved<0x142, 0xa>(v));
+  return with(v, moved<0x143, 0xc>(v));
+}
+struct Sum {
+  template <typename V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Most {
+  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
+};
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), 63)); }
+__device__ __forceinline__ u64 last_lane(u64 v) { return u64(last_lane(uint32_t(v))) | u64(last_lane(uint32_t(v >> 32))) << 32; }
+
+// Sums up to each thread, and of all; all threads call it.
 template <typename V>
-__device__ __forceinline__ V group_scan(V v, V* lds) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const V up = __shfl_up(v, d, 64);
-    if (int(threadIdx.x & 63) >= d) v += up;
-  }
+__device__ __forceinline__ V group_scan(V v, V* lds, V& all) {
+  v = wave_scan(v, Sum());
   __syncthreads();
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  for (int w = 0; w < int(threadIdx.x >> 6); ++w) v += lds[w];
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const V x = lds[w];
+    v += w < int(threadIdx.x >> 6) ? x : 0;
+    all += x;
+  }
   return v;
 }
+__device__ __forceinline__ u64 group_sum(u64 v, u64* lds) {
+  u64 all;
+  group_scan(v, lds, all);
+  return all;
+}
 __device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* lds) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = max(v, uint32_t(__shfl_xor(int(v), d, 64)));
+  v = wave_scan(v, Most());
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
@@ -195,6 +215,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return v >> 31 ? ~v : v | 0x80000000u;
 }
 
+__device__ __forceinline__ float logit_of(uint32_t key) { return __builtin_bit_cast(float, key >> 31 ? key & 0x7fffffffu : ~key); }
+
 // ------------------------------------------------------------ parts into bins
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a) {
@@ -209,14 +231,13 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a) {
   for (int i = 0; i < kEach / 8; ++i) load8(logits, first + (i * kThreads + int(threadIdx.x)) * 8, a.vocab, x[i]);
   if (int(threadIdx.x) < kBins) mass[threadIdx.x] = 0, count[threadIdx.x] = 0;
   fill_table(table);
-  if (part == 0 && threadIdx.x < 2) a.state[2 * row + threadIdx.x] = 0;
+  if (part == 0 && threadIdx.x == 0) a.listed[row] = 0;
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, x[i][j]);
-  const uint32_t key = group_max(key_of(top), tops);
-  top = __builtin_bit_cast(float, key >> 31 ? key & 0x7fffffffu : ~key);
+  top = logit_of(group_max(key_of(top), tops));
   SamplePart* out = a.part + row * a.parts + part;
   if (f.greedy()) {
     uint32_t at = 0;  // the lowest index as the largest complement
@@ -257,372 +278,406 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a) {
   }
 }
 
-// ------------------------------------------------------------------- the cuts
-// The order's part that stays: logits above `key`, and those of `key` up to index `last`.
-struct Cut {
-  uint32_t key;
-  int last;
+// --------------------------------------------------------------- what a row has
+// The row's largest logit and the first part that has it, the same in all threads; every
+// wave finds them for itself.
+struct Largest {
+  float top;
+  int part;
+};
+__device__ __forceinline__ Largest largest_of(const SamplePart* parts, int count) {
+  const int lane = threadIdx.x & 63;
+  uint32_t key = 0;
+  int part = 0;
+  for (int p = lane; p < count; p += 64) {
+    const uint32_t k = key_of(parts[p].top);
+    if (k > key) key = k, part = p;
+  }
+  const uint32_t most = last_lane(wave_scan(key, Most()));
+  const uint32_t first = ~last_lane(wave_scan(key == most ? ~uint32_t(part) : 0u, Most()));
+  return {logit_of(most), int(first)};
+}
+__device__ __forceinline__ double least_of(const Filters& f, const Scale& s, const double* table) {  // of min_p
+  return double(fminf(f.min_p, 1.f)) * weight(s.from, table).units;
+}
+// what a run of a mass `of` is to reach
+__device__ __forceinline__ u64 share_of(const Filters& f, u64 of) { return max(u64(1), times(fmaxf(f.top_p, 0.f), of, true)); }
+// a part's bins below the row's, in whole powers of two (kRange: too far to count)
+__device__ __forceinline__ int away_of(const Scale& row, const SamplePart& part) {
+  const double d = row.anchor - part.anchor;
+  return d < kRange ? int(d) : kRange;
+}
+// a token in the list: its index, and its bin in the row
+constexpr int kIndex = 20;
+constexpr uint32_t kIndexes = (1u << kIndex) - 1;
+static_assert(kBins <= 1 << (32 - kIndex), "an index and a bin in 32 bits");
+
+// ---------------------------------------------------------- tokens of the cuts' bins
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a) {
+  __shared__ u64 sums[kWaves], mass_to[kBins];
+  __shared__ uint32_t words[kWaves], count_to[kBins], base;
+  __shared__ double table[256];
+  __shared__ int edges[6], aways[kParts];
+  const int part = blockIdx.x, row = blockIdx.y;
+  const T* logits = static_cast<const T*>(a.logits) + row * a.row;
+  const SamplePart* parts = a.part + row * a.parts;
+  const Filters f = filters_of(a, row);
+  if (f.greedy() || !f.any()) return;
+  const float top = largest_of(parts, a.parts).top;
+  if (top == kNegInf) return;
+  const Scale s = scale_of(top, f.temperature);
+  if (int(threadIdx.x) < a.parts) aways[threadIdx.x] = away_of(s, parts[threadIdx.x]);
+  fill_table(table);
+  if (threadIdx.x < 6) edges[threadIdx.x] = threadIdx.x & 1 ? -1 : kBins;  // empty ranges
+  __syncthreads();
+  // the row's bins: this thread's, and sums up to it
+  u64 mass = 0;
+  uint32_t count = 0;
+  {
+    const uint64_t* of = a.mass + size_t(row) * a.parts * kBins;
+    const uint32_t* many = a.count + size_t(row) * a.parts * kBins;
+    const int bin = min(int(threadIdx.x), kBins - 1);
+    const bool has = int(threadIdx.x) < kBins;
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) {  // (no load behind a condition)
+      const int away = aways[p], b = bin - 16 * away, at = p * kBins + max(b, 0);
+      const u64 v = of[at];
+      const uint32_t n = f.by_count() ? many[at] : 0;
+      const bool here = has & (b >= 0) & (away < kRange);
+      mass += here ? v >> away : 0;
+      count += here ? n : 0;
+    }
+  }
+  u64 mass_all;
+  uint32_t count_all;
+  const u64 m = group_scan(mass, sums, mass_all);
+  const uint32_t n = group_scan(count, words, count_all);
+  if (int(threadIdx.x) < kBins) mass_to[threadIdx.x] = m, count_to[threadIdx.x] = n;
+  // the bins of the cuts; that of a sum lies between two, until the cut by count is known
+  const bool counted = f.by_count() && count_all > uint32_t(f.top_k);
+  if (counted && n >= uint32_t(f.top_k) && n - count < uint32_t(f.top_k)) edges[0] = edges[1] = threadIdx.x;
+  if (f.by_weight() && threadIdx.x == 0) {  // (the logarithm is off by far less than 1/100 of a bin)
+    const double y = s.from + log2(double(fminf(f.min_p, 1.f)));
+    edges[4] = max(0, int(fmin(floor(-y * 16 - 0.51), double(kBins))));
+    edges[5] = min(kBins - 1, int(fmin(floor(-y * 16 + 0.51), double(kBins))));
+  }
+  __syncthreads();
+  if (f.by_mass()) {
+    const int kbin = counted ? edges[0] : kBins;
+    const u64 most = share_of(f, counted ? mass_to[kbin] : mass_all), fewest = share_of(f, !counted ? mass_all : kbin ? mass_to[kbin - 1] : 0);
+    if (m >= fewest && m - mass < fewest) edges[2] = threadIdx.x;
+    if (m >= most && m - mass < most) edges[3] = threadIdx.x;
+    __syncthreads();
+  }
+  const int e0 = edges[0], e1 = edges[1], e2 = edges[2], e3 = edges[3], e4 = edges[4], e5 = edges[5];
+  if (part == 0) {  // for the draw
+    if (int(threadIdx.x) < kBins) {
+      a.mass_to[size_t(row) * kBins + threadIdx.x] = m;
+      a.count_to[size_t(row) * kBins + threadIdx.x] = n;
+    }
+    if (threadIdx.x < 8) a.edges[size_t(row) * 8 + threadIdx.x] = threadIdx.x < 6 ? edges[threadIdx.x] : int(counted);
+  }
+  const int away = aways[part];
+  if (away == kRange) return;
+  // Tokens whose logit may be in one of those bins, by 32 bits and a little room on both sides
+  // (where that is no number, all of them); then, of the few, the bin that their part counted.
+  const Scale own = scale_of(parts[part].top, f.temperature);
+  const int low_bin = min(min(e0, e2), e4) - 16 * away, high_bin = max(max(e1, e3), e5) - 16 * away;
+  const double room = 1e-6 * (fabs(own.top) + 50 / own.by);
+  const float upper = float(own.top + ((-16. * low_bin + 0.5) / 256 - own.from) / own.by + room);
+  const float lower = float(own.top + ((-16. * high_bin - 15.5) / 256 - own.from) / own.by - room);
+  uint32_t maybe = 0, found = 0;
+#pragma unroll
+  for (int i = 0; i < kEach / 8; ++i) {
+    float x[8];
+    load8(logits, part * kPart + (i * kThreads + int(threadIdx.x)) * 8, a.vocab, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) maybe |= !(x[j] > upper) && !(x[j] < lower) && x[j] > kNegInf ? 1u << (8 * i + j) : 0;
+  }
+  const auto index_of = [&](int bit) { return part * kPart + ((bit >> 3) * kThreads + int(threadIdx.x)) * 8 + (bit & 7); };
+  const auto bin_of = [&](int index) {
+    const double y = exponent(own, plain(float(logits[index])));
+    return counts(y) ? int(weight(y, table).bin) + 16 * away : INT_MAX;
+  };
+  for (uint32_t left = maybe; left; left &= left - 1) {
+    const int bit = __ffs(left) - 1, b = bin_of(index_of(bit));
+    if ((b >= e0 && b <= e1) || (b >= e2 && b <= e3) || (b >= e4 && b <= e5)) found |= 1u << bit;
+  }
+  uint32_t all;
+  const uint32_t mine = __popc(found);
+  uint32_t at = group_scan(mine, words, all) - mine;
+  if (!all) return;
+  if (threadIdx.x == 0) base = atomicAdd(a.listed + row, all);
+  __syncthreads();
+  uint32_t* list = a.list + int64_t(row) * a.vocab;
+  at += base;
+  for (; found; found &= found - 1) {
+    const int index = index_of(__ffs(found) - 1);
+    list[at++] = uint32_t(index) | uint32_t(bin_of(index)) << kIndex;
+  }
+}
+
+// -------------------------------------------------------------------------- draw
+// Scratch memory of the cuts.
+struct Scratch {
+  u64 amount[kDigits];
+  uint32_t count[kDigits];
+  u64 sums[kWaves];
+  uint32_t words[2 * kWaves];
+  uint32_t digit;
+  u64 before, value;
 };
 constexpr int kHeld = 4;  // listed tokens that a thread holds (beyond them they are read again)
 
-template <typename T>
-struct Row {
-  const SampleArgs& a;
-  const T* logits;
-  const SamplePart* part;
-  Filters f;
-  Scale s;  // of the whole row
-  const double* table;
-  // a token's weight, and its bin as its own part has counted it
-  __device__ __forceinline__ float logit(int i) const { return plain(float(logits[i])); }
-  __device__ __forceinline__ int bin_of(int i, float x) const {
-    const SamplePart& p = part[i / kPart];
-    const double away = s.anchor - p.anchor;
-    if (!(away < kRange)) return INT_MAX;
-    const double y = exponent(scale_of(p.top, f.temperature), x);
-    return counts(y) ? int(weight(y, table).bin) + 16 * int(away) : INT_MAX;
-  }
+// Listed tokens: an index, the logit's key, the bin, the units.
+struct Token {
+  int index, bin;
+  uint32_t key;
+  u64 units;
 };
 
-// Scratch memory of the last part.
-struct Scratch {
-  u64 mass[kDigits];
-  uint32_t count[kDigits];
-  u64 sums[kWaves];
-  uint32_t words[kWaves];
-  uint32_t found, found_count;
-  u64 found_mass;
-};
+// The order within a bin, as one number: how far a logit's key lies below the bin's largest,
+// then the index.
+__device__ __forceinline__ u64 place_of(uint32_t most, const Token& t) { return u64(most - t.key) << kIndex | u64(t.index); }
 
-// Counts and masses of the digits that `add` gives, of which the first up to which the count
-// (the mass) is above `before`; where that is none, the last that has any, with `before` just
-// below it.
-struct Found {
-  uint32_t digit, count, own_count;  // tokens of the digits before it, and its own
-  u64 mass, own_mass;
-};
-template <typename F>
-__device__ __forceinline__ Found find_digit(Scratch& lds, bool by_count, u64& before, F add) {
-  lds.mass[threadIdx.x] = 0;
-  lds.count[threadIdx.x] = 0;
-  if (threadIdx.x == 0) lds.found = kDigits - 1, lds.found_count = 0, lds.found_mass = 0;
-  __syncthreads();
-  add([&](uint32_t digit, u64 units) {
-    atomicAdd(&lds.mass[digit], units);
-    atomicAdd(&lds.count[digit], 1u);
-  });
-  __syncthreads();
-  const u64 mass = lds.mass[threadIdx.x];
-  const uint32_t count = lds.count[threadIdx.x];
-  const u64 mass_to = group_scan<u64>(mass, lds.sums);
-  const uint32_t count_to = group_scan<uint32_t>(count, lds.words);
-  u64 all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) all += by_count ? u64(lds.words[w]) : lds.sums[w];
-  if (all) before = min(before, all - 1);
-  const bool here = by_count ? count && count_to > before && count_to - count <= before : mass && mass_to > before && mass_to - mass <= before;
-  if (here) {
-    lds.found = threadIdx.x;
-    lds.found_count = count_to - count;
-    lds.found_mass = mass_to - mass;
-  }
-  __syncthreads();
-  const Found r = {lds.found, lds.found_count, lds.count[lds.found], lds.found_mass, lds.mass[lds.found]};
-  __syncthreads();
-  return r;
-}
-
-// The cut of one listed bin after the tokens whose sum reaches `target` (by_count: after
-// `target` tokens), and the mass up to it.
-template <typename T, typename E>
-__device__ __forceinline__ Cut cut_bin(const Row<T>& row, Scratch& lds, int bin, bool by_count, u64 target, u64& mass_to, E each) {
-  uint32_t most = 0, least = 0;  // (the least as the largest complement)
-  each([&](int i, float x, int b) {
-    if (b != bin) return;
-    most = max(most, key_of(x));
-    least = max(least, ~key_of(x));
-  });
-  most = group_max(most, lds.words);
-  least = ~group_max(least, lds.words);
-  // digits of how far a logit's key lies below the largest; `target` - 1 is before the cut
-  uint32_t from = most;
-  int shift = max(0, 32 - __clz(int(most - least)) - kDigit);
-  u64 before = target - 1, mass = 0;
-  Found d;
+// The last token that stays of a bin of `each` token: the first up to which the amounts (1, or
+// units, of each) are above `before`, or the last of all.
+template <typename E>
+__device__ __forceinline__ u64 cut_bin(Scratch& lds, int bin, u64 before, bool by_count, uint32_t most, uint32_t least, E each) {
+  u64 from = 0;
+  int shift = max(0, 32 - (most > least ? __clz(int(most - least)) : 32) + kIndex - kDigit);
+#pragma unroll 1
   for (;;) {
-    d = find_digit(lds, by_count, before, [&](auto add) {
-      each([&](int i, float x, int b) {
-        if (b != bin) return;
-        const uint32_t away = from - key_of(x);  // (wraps above `from`: no digit)
-        if (away >> shift < kDigits) add(away >> shift, weight(exponent(row.s, x), row.table).whole());
-      });
+    lds.amount[threadIdx.x] = 0;
+    lds.count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) lds.digit = 0, lds.before = 0, lds.value = from;
+    __syncthreads();
+    each([&](const Token& t) {
+      const u64 digit = (place_of(most, t) - from) >> shift;  // (wraps below `from`: no digit)
+      if (t.bin == bin && digit < kDigits) {
+        atomicAdd(&lds.amount[digit], by_count ? 1 : t.units);
+        atomicAdd(&lds.count[digit], 1u);
+      }
     });
-    before -= by_count ? d.count : d.mass;
-    mass += d.mass;
-    from -= d.digit << shift;
-    if (!shift) break;
+    __syncthreads();
+    const u64 mine = lds.amount[threadIdx.x];
+    u64 all;
+    const u64 to = group_scan(mine, lds.sums, all);
+    before = min(before, max(u64(1), all) - 1);  // (changes it the first time alone)
+    if (mine && to > before && to - mine <= before) {
+      lds.digit = threadIdx.x;
+      lds.before = to - mine;
+    }
+    __syncthreads();
+    const uint32_t digit = lds.digit;
+    before -= lds.before;
+    const bool one = lds.count[digit] <= 1;
+    from += u64(digit) << shift;
+    if (one || !shift) break;
+    __syncthreads();  // all have read them
     shift = max(0, shift - kDigit);
   }
-  // tokens of one logit, and of one weight: how many of them, then up to which index
-  const u64 own = d.own_count ? d.own_mass / d.own_count : 0;
-  const u64 stay = by_count || !own ? before + 1 : before / own + 1;
-  if (stay >= d.own_count) {
-    mass_to = mass + d.own_mass;
-    return {from, INT_MAX};
-  }
-  mass_to = mass + stay * own;
-  uint32_t base = 0;
-  u64 left = stay - 1;
-  for (int s = kDigit; s >= 0; s -= kDigit) {
-    d = find_digit(lds, true, left, [&](auto add) {
-      each([&](int i, float x, int b) {
-        if (b == bin && key_of(x) == from && (uint32_t(i) - base) >> s < kDigits) add((uint32_t(i) - base) >> s, 0);
-      });
-    });
-    left -= d.count;
-    base += d.digit << s;
-  }
-  return {from, int(base)};
+  // the one token of the last digit
+  each([&](const Token& t) {
+    const u64 place = place_of(most, t);
+    if (t.bin == bin && (place - from) >> shift == 0) lds.value = place;
+  });
+  __syncthreads();
+  const u64 value = lds.value;
+  __syncthreads();
+  return value;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
   __shared__ Scratch lds;
-  __shared__ u64 mass_to[kBins], part_mass[64];
-  __shared__ uint32_t count_to[kBins];
+  __shared__ u64 part_mass[kParts];
   __shared__ double table[256];
-  __shared__ int edges[6], last_one, token;
-  const int part = blockIdx.x, row = blockIdx.y;
+  __shared__ int token, aways[kParts];
+  const int row = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const T* logits = static_cast<const T*>(a.logits) + row * a.row;
   const SamplePart* parts = a.part + row * a.parts;
   const Filters f = filters_of(a, row);
-  // the row's largest logit, the first part of those that have it
-  float top = kNegInf;
-  uint32_t at = 0;
-  for (int p = 0; p < a.parts; ++p)
-    if (parts[p].top > top) top = parts[p].top, at = parts[p].at;
-  if (top == kNegInf || f.greedy()) {
-    if (part == 0 && threadIdx.x == 0) a.out[row] = top == kNegInf ? -1 : int64_t(at);
+  const Largest largest = largest_of(parts, a.parts);
+  if (largest.top == kNegInf || f.greedy()) {
+    if (threadIdx.x == 0) a.out[row] = largest.top == kNegInf ? -1 : int64_t(parts[largest.part].at);
     return;
   }
-  if (!f.any() && part) return;
   fill_table(table);
-  if (threadIdx.x < 64) part_mass[threadIdx.x] = 0;
-  if (threadIdx.x < 6) edges[threadIdx.x] = threadIdx.x & 1 ? -1 : kBins;  // empty ranges
+  const Scale s = scale_of(largest.top, f.temperature);
+  if (int(threadIdx.x) < kParts) part_mass[threadIdx.x] = 0;
+  if (int(threadIdx.x) < a.parts) {
+    aways[threadIdx.x] = away_of(s, parts[threadIdx.x]);
+    if (!f.any()) part_mass[threadIdx.x] = aways[threadIdx.x] < kRange ? parts[threadIdx.x].mass >> aways[threadIdx.x] : 0;
+  }
+  if (threadIdx.x == 0) token = -1;
   __syncthreads();
-  const Row<T> r = {a, logits, parts, f, scale_of(top, f.temperature), table};
-  const double least = double(fminf(f.min_p, 1.f)) * weight(r.s.from, table).units;  // of min_p
-  Cut cut = {0, INT_MAX};
-  int whole = kBins;  // bins before it stay whole
+  const double least = f.by_weight() ? least_of(f, s, table) : 0;
+  // what stays: logits above `key`, and those of `key` up to index `last`
+  uint32_t key = 0;
+  int last = INT_MAX;
+  const auto stays = [&](uint32_t k, int i) { return k > key || (k == key && i <= last); };
 
   if (f.any()) {
-    // the row's bins: this thread's, and sums up to it
-    u64 mass = 0;
-    uint32_t count = 0;
-    for (int p = 0; p < a.parts; ++p) {
-      const double away = r.s.anchor - parts[p].anchor;
-      if (!(away < kRange)) continue;
-      const int b = int(threadIdx.x) - 16 * int(away);
-      if (b >= 0 && b < kBins) {
-        const size_t i = (size_t(row) * a.parts + p) * kBins + b;
-        mass += a.mass[i] >> int(away);
-        if (f.by_count()) count += a.count[i];
-      }
-    }
-    const u64 m = group_scan<u64>(mass, lds.sums);
-    const uint32_t n = group_scan<uint32_t>(count, lds.words);
-    if (int(threadIdx.x) < kBins) mass_to[threadIdx.x] = m, count_to[threadIdx.x] = n;
-    __syncthreads();
-    // the bins of the cuts: ranges of which one end may be open until a cut before is known
-    const bool counted = f.by_count() && count_to[kBins - 1] > uint32_t(f.top_k);
-    if (counted && int(threadIdx.x) < kBins && n >= uint32_t(f.top_k) && n - count < uint32_t(f.top_k)) edges[0] = edges[1] = threadIdx.x;
-    __syncthreads();
-    const int kbin = counted ? edges[0] : -1;
-    const u64 most = counted ? mass_to[kbin] : mass_to[kBins - 1], fewest = counted ? (kbin ? mass_to[kbin - 1] : 0) : most;
-    const auto share = [&](u64 of) { return max(u64(1), times(fmaxf(f.top_p, 0.f), of, true)); };  // what a run is to reach
-    if (f.by_mass() && int(threadIdx.x) < kBins) {
-      if (m >= share(fewest) && m - mass < share(fewest)) edges[2] = threadIdx.x;
-      if (m >= share(most) && m - mass < share(most)) edges[3] = threadIdx.x;
-    }
-    if (f.by_weight() && threadIdx.x == 0) {  // (the logarithm is off by far less than 1/100 of a bin)
-      const double y = r.s.from + log2(double(fminf(f.min_p, 1.f)));
-      edges[4] = max(0, int(floor(-y * 16 - 0.51)));
-      edges[5] = min(kBins - 1, int(floor(-y * 16 + 0.51)));
-    }
-    __syncthreads();
-    // this part's tokens of those bins
-    const int e0 = edges[0], e1 = edges[1], e2 = edges[2], e3 = edges[3], e4 = edges[4], e5 = edges[5];
-    const double away = r.s.anchor - parts[part].anchor;
-    if (away < kRange) {
-      const Scale own = scale_of(parts[part].top, f.temperature);
-      for (int i = 0; i < kEach / 8; ++i) {
-        const int first = part * kPart + (i * kThreads + int(threadIdx.x)) * 8;
-        float x[8];
-        load8(logits, first, a.vocab, x);
-        for (int j = 0; j < 8; ++j) {
-          const double y = exponent(own, x[j]);
-          if (!counts(y)) continue;
-          const int b = int(weight(y, table).bin) + 16 * int(away);
-          if ((b >= e0 && b <= e1) || (b >= e2 && b <= e3) || (b >= e4 && b <= e5)) {
-            const uint32_t to = atomicAdd(a.state + 2 * row + 1, 1u);
-            if (to < uint32_t(a.vocab)) a.list[int64_t(row) * a.vocab + to] = first + j;
-          }
-        }
-      }
-    }
-    // the part that is done last goes on
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last_one = atomicAdd(a.state + 2 * row, 1u) + 1 == uint32_t(a.parts);
-    __syncthreads();
-    if (!last_one) return;
-    __threadfence();
-    const int listed = int(min(__hip_atomic_load(a.state + 2 * row + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), uint32_t(a.vocab)));
+    const int* edges = a.edges + size_t(row) * 8;
+    const uint64_t* mass_to = a.mass_to + size_t(row) * kBins;
+    const int listed = int(min(a.listed[row], uint32_t(a.vocab)));
     const uint32_t* list = a.list + int64_t(row) * a.vocab;
-    int held[kHeld], held_bin[kHeld];
-    float held_x[kHeld];
+    const auto token_of = [&](uint32_t v) -> Token {
+      const int i = int(v & kIndexes);
+      const float x = plain(float(logits[i]));
+      return {i, int(v >> kIndex), key_of(x), weight(exponent(s, x), table).whole()};
+    };
+    Token held[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int n = i * kThreads + threadIdx.x;
-      held_bin[i] = -1;
-      if (n < listed) {
-        held[i] = int(list[n]);
-        held_x[i] = r.logit(held[i]);
-        held_bin[i] = r.bin_of(held[i], held_x[i]);
-      }
+      held[i].bin = -1;
+      if (n < listed) held[i] = token_of(list[n]);
     }
-    const auto each = [&](auto f) {
+    const auto each = [&](auto with) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
-        if (held_bin[i] >= 0) f(held[i], held_x[i], held_bin[i]);
-      for (int n = kHeld * kThreads + threadIdx.x; n < listed; n += kThreads) {
-        const int i = int(list[n]);
-        const float x = r.logit(i);
-        f(i, x, r.bin_of(i, x));
-      }
+        if (i * kThreads < listed && held[i].bin >= 0) with(held[i]);
+#pragma unroll 1
+      for (int n = kHeld * kThreads + threadIdx.x; n < listed; n += kThreads) with(token_of(list[n]));
     };
-    int bin = kBins;  // of the cut
-    u64 stays = mass_to[kBins - 1];
-    if (counted) {
-      bin = kbin;
-      cut = cut_bin(r, lds, kbin, true, u64(f.top_k) - (kbin ? count_to[kbin - 1] : 0), stays, each);
-      stays += kbin ? mass_to[kbin - 1] : 0;
+    const bool counted = edges[6];
+    const int kbin = counted ? edges[0] : kBins, e2 = edges[2], e3 = edges[3], e4 = edges[4];
+    int bin = kBins;
+    u64 all = mass_to[kBins - 1];
+    // the cut by count, then the one by mass of what it leaves
+#pragma unroll 1
+    for (int turn = counted ? 0 : 1; turn < (f.by_mass() ? 2 : 1); ++turn) {
+      u64 before;  // amounts, in the cut's bin, before the last that stays
+      if (turn == 0) {
+        bin = kbin;
+        before = u64(f.top_k) - 1 - (bin ? a.count_to[size_t(row) * kBins + bin - 1] : 0);
+      } else {
+        if (counted) {
+          u64 mine = 0;
+          each([&](const Token& t) {
+            if (t.bin == bin && stays(t.key, t.index)) mine += t.units;
+          });
+          all = group_sum(mine, lds.sums) + (bin ? mass_to[bin - 1] : 0);
+        }
+        const u64 target = share_of(f, all);
+        bin = e2;  // (it is one of the listed range; that is one bin, nearly always)
+        while (bin < e3 && mass_to[bin] < target) ++bin;
+        const u64 to = bin ? mass_to[bin - 1] : 0;
+        before = target > to ? target - to - 1 : 0;
+      }
+      uint32_t most = 0, complement = 0;  // of the bin's keys
+      each([&](const Token& t) {
+        if (t.bin == bin) most = max(most, t.key), complement = max(complement, ~t.key);
+      });
+      most = group_max(most, lds.words);
+      complement = group_max(complement, lds.words + kWaves);
+      const u64 place = cut_bin(lds, bin, before, turn == 0, most, ~complement, each);
+      const uint32_t new_key = most - uint32_t(place >> kIndex);
+      const int new_last = int(place & kIndexes);
+      if (stays(new_key, new_last)) key = new_key, last = new_last;
     }
-    if (f.by_mass()) {
-      const u64 target = share(stays);
-      __syncthreads();
-      if (int(threadIdx.x) < kBins && m >= target && m - mass < target) edges[0] = threadIdx.x;
-      __syncthreads();
-      // (a rounding that puts it outside the listed bins leaves the range's nearer end)
-      bin = min(max(edges[0], e2), e3);
-      const u64 before = bin ? mass_to[bin - 1] : 0;
-      u64 unused;
-      const Cut next = cut_bin(r, lds, bin, false, target > before ? target - before : 1, unused, each);
-      if (!counted || bin < kbin || next.key > cut.key || (next.key == cut.key && next.last < cut.last)) cut = next;
-    }
-    whole = min(bin, f.by_weight() ? e4 : kBins);
-    // what stays of each part: its whole bins, then the listed tokens one by one
-    for (int p = 0; p < a.parts; ++p) {
-      const double away = r.s.anchor - parts[p].anchor;
-      if (!(away < kRange)) continue;
-      const int b = int(threadIdx.x) - 16 * int(away);
+    // what stays of each part: its whole bins, a wave for a part, then the listed tokens
+    const int whole = min(bin, f.by_weight() ? e4 : kBins);
+    for (int p = wave; p < a.parts; p += kWaves) {
+      const int away = aways[p];
       u64 v = 0;
-      if (int(threadIdx.x) < whole && b >= 0 && b < kBins) v = a.mass[(size_t(row) * a.parts + p) * kBins + b] >> int(away);
-      v = wave_sum(v);
-      if ((threadIdx.x & 63) == 0 && v) atomicAdd(&part_mass[p], v);
+      for (int b = lane; b < min(whole - 16 * away, kBins); b += 64) v += a.mass[(size_t(row) * a.parts + p) * kBins + b] >> away;
+      v = wave_scan(v, Sum());
+      if (lane == 63 && v) atomicAdd(&part_mass[p], v);
     }
-    each([&](int i, float x, int b) {
-      if (b < whole || b >= kBins) return;
-      const uint32_t key = key_of(x);
-      const Weight w = weight(exponent(r.s, x), table);
-      if ((key > cut.key || (key == cut.key && i <= cut.last)) && w.units >= least) atomicAdd(&part_mass[i / kPart], w.whole());
+    each([&](const Token& t) {
+      if (t.bin < whole || !stays(t.key, t.index)) return;
+      if (f.by_weight() && weight(exponent(s, plain(float(logits[t.index]))), table).units < least) return;
+      atomicAdd(&part_mass[t.index / kPart], t.units);
     });
-  } else if (int(threadIdx.x) < a.parts) {
-    const double away = r.s.anchor - parts[threadIdx.x].anchor;
-    part_mass[threadIdx.x] = away < 64 ? parts[threadIdx.x].mass >> int(away) : 0;
+    __syncthreads();
   }
-  __syncthreads();
-  // the part that the random number falls into
-  u64 all = 0;
-  for (int p = 0; p < a.parts; ++p) all += part_mass[p];
-  u64 left = min(times(fminf(fmaxf(a.uniform[row], 0.f), 1.f), all, false), all - 1);
+  // the part that the random number falls into: the parts' masses by lanes, some each
+  u64 left;
   int mine = 0;
-  while (mine < a.parts - 1 && left >= part_mass[mine]) left -= part_mass[mine++];
-  // and its tokens by index: sums of each wave's 512, then within the one
-  u64 sums[kEach / 8];
-  float x[kEach / 8][8];
-  const auto units = [&](int i, float v) -> u64 {
-    const double y = exponent(r.s, v);
-    const uint32_t key = key_of(v);
-    if (!counts(y) || key < cut.key || (key == cut.key && i > cut.last)) return 0;
-    const Weight w = weight(y, table);
-    return f.by_weight() && w.units < least ? 0 : w.whole();
-  };
-  if (threadIdx.x == 0) token = -1;
+  {
+    constexpr int kLane = kParts / 64;
+    u64 own = 0;
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) own += part_mass[lane * kLane + i];
+    const u64 to = wave_scan(own, Sum()), all = last_lane(to);
+    left = min(times(fminf(fmaxf(a.uniform[row], 0.f), 1.f), all, false), max(u64(1), all) - 1);
+    const int from = max(0, __ffsll((long long)__ballot(to > left)) - 1);
+    left -= __shfl(to - own, from, 64);
+    mine = from * kLane;
+    while (mine < (from + 1) * kLane - 1 && left >= part_mass[mine]) left -= part_mass[mine++];
+  }
+  // and its tokens by index
+  u64 units[kEach];
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i) {
     const int first = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8;
-    load8(logits, first, a.vocab, x[i]);
-    sums[i] = 0;
+    float x[8];
+    load8(logits, first, a.vocab, x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[i] += units(first + j, x[i][j]);
+    for (int j = 0; j < 8; ++j) {
+      const double y = exponent(s, x[j]);
+      const Weight w = weight(y, table);
+      units[8 * i + j] = counts(y) && stays(key_of(x[j]), first + j) && w.units >= least ? w.whole() : 0;
+    }
   }
-  __syncthreads();
   u64 before = 0;  // of the pieces before
-  bool done = false;
+  uint32_t latest = 0;
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i) {
-    const u64 to = before + group_scan<u64>(sums[i], lds.sums), from = to - sums[i];
-    if (!done && sums[i] && from <= left && left < to) {
-      const int first = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8;
-      u64 at = from;
+    const int first = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8;
+    u64 sum = 0, all;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const u64 w = units(first + j, x[i][j]);
-        if (at <= left && left < at + w) token = first + j;
-        at += w;
-      }
+    for (int j = 0; j < 8; ++j) {
+      sum += units[8 * i + j];
+      if (units[8 * i + j]) latest = uint32_t(first + j) + 1;
     }
-    for (int w = 0; w < kWaves; ++w) before += lds.sums[w];
-    __syncthreads();
+    u64 at = before + group_scan(sum, lds.sums, all) - sum;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const u64 w = units[8 * i + j];
+      if (at <= left && left < at + w) token = first + j;
+      at += w;
+    }
+    before += all;
   }
-  // (where roundings leave the number beyond the last token: that one)
-  if (token < 0) {
-    uint32_t latest = 0;
-#pragma unroll
-    for (int i = 0; i < kEach / 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int n = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8 + j;
-        if (units(n, x[i][j])) latest = max(latest, uint32_t(n) + 1);
-      }
+  __syncthreads();
+  if (token < 0) {  // (where roundings leave the number beyond the last token: that one)
     latest = group_max(latest, lds.words);
-    if (threadIdx.x == 0) token = latest ? int(latest) - 1 : -1;
-    __syncthreads();
+    if (threadIdx.x == 0) a.out[row] = int64_t(latest) - 1;
+  } else if (threadIdx.x == 0) {
+    a.out[row] = token;
   }
-  if (threadIdx.x == 0) a.out[row] = token;
 }
 
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t s) {
   const dim3 grid(unsigned(a.parts), unsigned(a.rows));
   hipLaunchKernelGGL(sample_bins_kernel<T>, grid, dim3(kThreads), 0, s, a);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sample_draw_kernel<T>, grid, dim3(kThreads), 0, s, a);
+  if (a.top_k || a.top_p || a.min_p || a.top_k_all > 0 || a.top_p_all < 1 || a.min_p_all > 0) {
+    hipLaunchKernelGGL(sample_list_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(unsigned(a.rows)), dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 
 size_t parts_of(size_t vocab) { return (vocab + kPart - 1) / kPart; }
 size_t up(size_t bytes) { return (bytes + 15) / 16 * 16; }
-static_assert(kSampleVocab <= size_t(kPart) * 64 && kSampleVocab <= size_t(1) << (2 * kDigit), "parts, and indices, of a row");
+static_assert(kSampleVocab <= size_t(1) << kIndex && kParts <= kThreads && kParts % 64 == 0, "indexes, and parts, of a row");
 
 }  // namespace
 
 size_t sample_work_bytes(size_t rows, size_t vocab) {
   const size_t parts = parts_of(vocab);
-  return up(rows * parts * sizeof(SamplePart)) + rows * parts * kBins * (sizeof(uint64_t) + sizeof(uint32_t)) + rows * 2 * sizeof(uint32_t) +
-         rows * vocab * sizeof(uint32_t);
+  return up(rows * parts * sizeof(SamplePart)) + rows * (parts + 1) * kBins * (sizeof(uint64_t) + sizeof(uint32_t)) +
+         rows * (8 + 1 + vocab) * sizeof(uint32_t);
 }
 void sample_work(SampleArgs& a, void* work) {
   a.parts = int(parts_of(size_t(a.vocab)));
@@ -631,11 +686,12 @@ void sample_work(SampleArgs& a, void* work) {
   a.part = reinterpret_cast<SamplePart*>(at);
   at += up(items * sizeof(SamplePart));
   a.mass = reinterpret_cast<uint64_t*>(at);
-  at += items * kBins * sizeof(uint64_t);
-  a.count = reinterpret_cast<uint32_t*>(at);
-  at += items * kBins * sizeof(uint32_t);
-  a.state = reinterpret_cast<uint32_t*>(at);
-  a.list = a.state + 2 * size_t(a.rows);
+  a.mass_to = a.mass + items * kBins;
+  a.count = reinterpret_cast<uint32_t*>(a.mass_to + size_t(a.rows) * kBins);
+  a.count_to = a.count + items * kBins;
+  a.edges = reinterpret_cast<int32_t*>(a.count_to + size_t(a.rows) * kBins);
+  a.listed = reinterpret_cast<uint32_t*>(a.edges + size_t(a.rows) * 8);
+  a.list = a.listed + a.rows;
 }
 
 hipError_t launch_sample_tokens(const SampleArgs& a, int type, hipStream_t s) {

@@ -16,12 +16,13 @@ struct SampleArgs {
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   int64_t* out;
-  // the workspace, per row: what its parts hold, their bins, a list of tokens
-  struct SamplePart* part;  // [rows][parts]
-  uint64_t* mass;           // [rows][parts][bins]
-  uint32_t* count;          // [rows][parts][bins]
-  uint32_t* state;          // [rows][2]: parts that are done, tokens in the list
-  uint32_t* list;           // [rows][vocab]
+  // the workspace: what parts hold, their bins, the rows' bins with sums up to each, the bins
+  // that cuts fall in (three ranges, and whether top_k cuts), tokens of those bins
+  struct SamplePart* part;       // [rows][parts]
+  uint64_t *mass, *mass_to;      // [rows][parts][bins], [rows][bins]
+  uint32_t *count, *count_to;
+  int32_t* edges;                // [rows][8]
+  uint32_t *listed, *list;       // [rows], [rows][vocab]
 };
 
 constexpr size_t kSampleVocab = size_t(1) << 20;
