@@ -49,10 +49,12 @@ struct SharedArgs {
   float* lse;             // [seqs][heads] or null
   const int32_t* groups;  // [count + 1] first sequences
   const int32_t* shared;  // [count] positions that a group's sequences have in common
-  int count, columns;     // columns: of a piece in the workspace
-  uint4* entries;         // [count + seqs]
-  float* rows;            // what one workgroup has of a row from first to last: [2][seqs][heads] rows
-  float* pieces;          // and in part: [workgroups][2][columns] rows
+  int count;
+  // the workspace, in rows of o, m and l
+  uint4* entries;                          // [count + seqs + 1]
+  float* rows;                             // heads of one piece: [2][seqs][heads]
+  float *pieces, *own_pieces;              // in several: [workgroups][2][columns], [waves][2][own_columns]
+  int columns, own_columns;
 };
 
 struct PromptArgs {
@@ -75,6 +77,8 @@ unsigned decode_workgroups(size_t seqs, size_t kv_heads, size_t group, size_t ke
 size_t decode_work_floats(unsigned workgroups, size_t group, size_t dim);
 unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys);
 size_t shared_columns(size_t seqs, size_t group, size_t dim);  // of a piece, at most
+size_t shared_own_columns(size_t group);
+size_t shared_waves(size_t dim);  // of a workgroup
 size_t shared_row_floats(size_t dim);
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys);
 size_t prompt_work_floats(int splits, size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows);

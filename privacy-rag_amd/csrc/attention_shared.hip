@@ -4,19 +4,20 @@
 //   o = sum_j 2^(s_j - m) v_j / l over the prefix's keys and the sequence's own, as in
 //   attention_decode.hip, with the two parts' m, l and o joined at the end.
 //
-// An entry is a prefix with the heads of all its sequences as columns, or a sequence's own
-// keys with its heads of one key/value head.  4 dim bytes of K and V a key and key/value head
-// against 4 dim operations a column: reading them bounds it up to some hundred columns, and
-// what decides is again that every CU has loads under way.  The entries' blocks of 32 keys
-// stand in one row, by what they take (a block of up to 32 columns occupies one wave, one of
-// 64 two, ...), and every workgroup takes an equal stretch of it.
-//
-// Within a workgroup an entry's columns are spread over 1, 2, 4 or 8 waves of 32 columns
-// each, which read the same keys one soon after the other (a cache answers), and the others
-// take every 2nd, 4th or 8th block.  The products are attention_decode.hip's, two column
-// tiles of 16 for one load of K and V and one transposition of V.  Waves that have the same
-// columns add up through LDS; what a workgroup has of an entry in part (at most two pieces)
-// goes to the workspace, and the join kernel adds the pieces in order, so results do not
+// 4 dim bytes of K and V a key and key/value head against 4 dim operations a query: reading
+// them bounds it up to some hundred queries, and what decides is again that every CU has loads
+// under way.  A workgroup a CU works on one kind of keys, the prefixes' or the sequences' own,
+// as many on each as its share of the work, of which each takes an equal stretch, counted in
+// blocks of 32 keys that a wave takes (and some for the start of another head's keys):
+// * own keys by single waves, as in attention_decode.hip, but with no LDS: pieces of a head
+//   that several waves have part of go to the workspace;
+// * a prefix's keys by whole workgroups.  All its sequences' heads of one key/value head are
+//   columns, spread over 1, 2, 4 or 8 waves of 32 columns each, which read the same keys one
+//   soon after the other (a cache answers); the others take every 8th, 4th or 2nd block, and
+//   waves that have the same columns add up through LDS.  A workgroup has at most two pieces
+//   of heads that it shares with others.
+// The products are attention_decode.hip's, with two tiles of 16 columns for one load of K and V
+// and one transposition of V.  The join kernel adds the pieces in order, so results do not
 // depend on timing.
 #include "attention.hpp"
 
@@ -32,7 +33,9 @@ struct SharedShape {
   static constexpr int row = D + 4;              // a row of o, then m and l
 };
 
-constexpr int kUnits = 4;  // a workgroup's stretch is not shorter
+// units of a head's keys before its first block (its start takes about as long), and the
+// shortest stretch
+constexpr int kPrefixStart = 8, kOwnStart = 2, kPrefixLeast = 8, kOwnLeast = 3;
 
 __host__ __device__ __forceinline__ int column_waves(int columns, int waves) {
   int n = 1;
@@ -78,30 +81,202 @@ __device__ __forceinline__ Entry own_of(const SharedArgs& a, int s, int& group) 
   }
   return e;
 }
-__device__ __forceinline__ Entry entry_of(const SharedArgs& a, int e, int& group) {
-  group = -1;
-  return e < a.count ? prefix_of(a, e) : own_of(a, e - a.count, group);
-}
-// units of an entry's one key/value head: blocks times waves
-__device__ __forceinline__ uint32_t units_of(int columns, int blocks, int waves) {
-  return uint32_t(blocks) * column_waves(columns, waves) * ((columns + 32 * waves - 1) / (32 * waves));
-}
 
-// Units over the workgroups: each of the first `extra` has one more than the others.
+// How many parts a head's columns are cut into, waves that have the columns of one part at
+// the same time, units of one part of one head.
+struct Parts {
+  int parts, waves;
+  uint32_t units;
+  __device__ __forceinline__ Parts(bool prefix, int columns, int blocks, int group_waves) {
+    const int most = prefix ? 32 * group_waves : 32;
+    parts = (columns + most - 1) / most;
+    waves = prefix ? column_waves(columns, group_waves) : 1;
+    units = blocks ? uint32_t(blocks) * waves + (prefix ? kPrefixStart : kOwnStart) : 0;
+  }
+  __device__ __forceinline__ uint32_t all(int kv_heads) const { return units * parts * kv_heads; }
+};
+
+// Units over workgroups, or waves: each of the first `extra` has one more than the others.
 struct Stretches {
   uint32_t count, each, extra;
-  __device__ __forceinline__ Stretches(uint32_t units, uint32_t most) {
-    count = max(1u, min(most, (units + kUnits - 1) / kUnits));
+  __device__ __forceinline__ Stretches(uint32_t units, uint32_t most, uint32_t least) {
+    count = max(1u, min(most, units / least));
     each = units / count;
     extra = units - each * count;
   }
   __device__ __forceinline__ uint32_t begin(uint32_t w) const { return each * w + min(w, extra); }
-  // the workgroup whose stretch holds unit u
+  // the stretch that holds unit u
   __device__ __forceinline__ uint32_t of(uint32_t u) const {
     const uint32_t longer = extra * (each + 1);
     return u < longer ? u / (each + 1) : extra + (u - longer) / each;
   }
 };
+// blocks of a head (one of whose blocks is `waves` units, after its start) before unit u
+__device__ __forceinline__ int blocks_before(uint32_t u, uint32_t first, int waves) { return u > first ? int((u - first + waves - 1) / waves) : 0; }
+
+// The workgroups for the prefixes, as their share of the units is.
+__device__ __forceinline__ uint32_t prefix_groups(uint32_t prefix, uint32_t own, uint32_t groups) {
+  if (!prefix || !own || groups < 2) return prefix ? groups : 0;
+  const uint32_t n = uint32_t((uint64_t(groups) * prefix + (uint64_t(prefix) + own) / 2) / (uint64_t(prefix) + own));
+  return min(max(n, 1u), groups - 1);
+}
+
+// The keys of one key/value head h in an entry's blocks first, first + step .. below last,
+// for up to 32 columns from column0 on (16 unless `two`): o, m and l as of keys in powers
+// of two.
+template <typename T, int D, bool EXACT>
+__device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x, int h, int column0, bool two, int first, int last,
+                                            int step, f32x4 (&o)[2][D / 16], float (&m)[2], float (&l)[2]) {
+  using S = SharedShape<D>;
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  u32x4 q[2][S::steps];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int column = column0 + 16 * t + col, seq = x.first + column / c.group, head = h * c.group + column % c.group;
+#pragma unroll
+    for (int i = 0; i < S::steps; ++i) {
+      q[t][i] = u32x4{0, 0, 0, 0};
+      const int d = 32 * i + 8 * quad;
+      if (column < x.columns && (EXACT || d < c.dim))
+        q[t][i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + seq * a.q_seq + head * a.q_head + d);
+      q[t][i] ^= c.flip;
+    }
+  }
+  const int32_t* named = c.tables + x.first * c.table_stride;
+  const int most = int(c.capacity >> c.page_shift) - 1;
+  const auto page_at = [&](int key) { return named[min(key >> c.page_shift, most)]; };
+  int next[2] = {page_at((x.begin() + first) << 5), page_at(((x.begin() + first) << 5) + 16)};
+  for (int i = first; i < last; i += step) {
+    const int kb = (x.begin() + i) << 5;
+    u32x4 kf[2][S::steps];
+    uint32_t vr[8][S::words];
+    bool page_ok[2];
+    int pages[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      page_ok[t] = (next[t] >= 0) & (next[t] < c.pages) & ((kb + 16 * t) >> c.page_shift <= most);
+      pages[t] = page_ok[t] ? next[t] : 0;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
+      const T* kp = static_cast<const T*>(c.k) + uint64_t(pages[t]) * c.k_page + uint64_t(h) * c.k_head + uint64_t(row + col) * c.k_token + 8 * quad;
+#pragma unroll
+      for (int n = 0; n < S::steps; ++n) {
+        kf[t][n] = u32x4{0, 0, 0, 0};
+        if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
+      const T* vp = static_cast<const T*>(c.v) + uint64_t(pages[t]) * c.v_page + uint64_t(h) * c.v_head + uint64_t(row + 4 * quad) * c.v_token + S::per * col;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int w = 0; w < S::words; ++w) vr[4 * t + r][w] = 0;
+        if (EXACT || S::per * col < c.dim) {
+          if constexpr (S::words == 2) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(vp + uint64_t(r) * c.v_token);
+            vr[4 * t + r][0] = v[0];
+            vr[4 * t + r][1] = v[1];
+          } else {
+#pragma unroll
+            for (int w = 0; w < S::words; w += 4) {
+              if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
+              const u32x4 v = *reinterpret_cast<const u32x4*>(vp + uint64_t(r) * c.v_token + 2 * w);
+#pragma unroll
+              for (int b = 0; b < 4; ++b) vr[4 * t + r][w + b] = v[b];
+            }
+          }
+        }
+      }
+    }
+    // (the next block's entries, beside these loads; past the last they are the table's last)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) next[t] = page_at(((x.begin() + i + step) << 5) + 16 * t);
+    const bool whole = page_ok[0] && page_ok[1] && kb >= x.lo && kb + 32 <= x.hi;
+    u32x4 ph[2], pl[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t && !two) continue;
+      f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+      for (int n = 0; n < S::steps; ++n) {
+        st[0] = Half<T>::mma16(kf[0][n], q[t][n], st[0]);
+        st[1] = Half<T>::mma16(kf[1][n], q[t][n], st[1]);
+      }
+      float s[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] = st[r >> 2][r & 3] * c.scale;
+      if (!whole) {  // keys that are not the entry's count as nothing, whatever their page holds
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int at = kb + 16 * (r >> 2) + 4 * quad + (r & 3);
+          const bool sees = bool(page_ok[r >> 2]) & (at >= x.lo) & (at < x.hi);
+          s[r] = sees ? s[r] : kNegInf;
+#pragma unroll
+          for (int w = 0; w < S::words; ++w) vr[r][w] = sees ? vr[r][w] : 0;
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      top = fmaxf(m[t], max32(max16(top)) - Half<T>::most);
+      if (__any(top > m[t])) {
+        const float f = __builtin_amdgcn_exp2f(m[t] - origin(top));
+        l[t] *= f;
+#pragma unroll
+        for (int j = 0; j < S::per; ++j) o[t][j] *= f;
+        m[t] = top;
+      }
+      uint32_t hi[4], rest[4];
+#pragma unroll
+      for (int r = 0; r < 8; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(s[r] - origin(m[t])), p1 = __builtin_amdgcn_exp2f(s[r + 1] - origin(m[t]));
+        l[t] += p0 + p1;
+        hi[r / 2] = pack2<T>(p0, p1);
+        rest[r / 2] = pack2<T>(p0 - low<T>(hi[r / 2]), p1 - high<T>(hi[r / 2]));
+      }
+      ph[t] = u32x4{hi[0], hi[1], hi[2], hi[3]}, pl[t] = u32x4{rest[0], rest[1], rest[2], rest[3]};
+    }
+#pragma unroll
+    for (int j = 0; j < S::per; ++j) {
+      u32x4 vt;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        vt[p] = __builtin_amdgcn_perm(vr[2 * p + 1][j / 2], vr[2 * p][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+      o[0][j] = Half<T>::mma16(vt, ph[0], o[0][j]);
+      o[0][j] = Half<T>::mma16(vt, pl[0], o[0][j]);
+      if (two) {
+        o[1][j] = Half<T>::mma16(vt, ph[1], o[1][j]);
+        o[1][j] = Half<T>::mma16(vt, pl[1], o[1][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) l[t] = sum32(sum16(l[t]));
+}
+
+// A lane's rows of o, and m and l, at `to` (for the 32 columns of a wave).
+template <int D>
+__device__ __forceinline__ void store_columns(float* to, int columns, const f32x4 (&o)[2][D / 16], const float (&m)[2], const float (&l)[2]) {
+  using S = SharedShape<D>;
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if (16 * t + col >= columns) continue;
+    float* p = to + (16 * t + col) * S::row;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < S::per; j += 4)
+        *reinterpret_cast<f32x4*>(p + (4 * quad + r) * S::per + j) = f32x4{o[t][j][r], o[t][j + 1][r], o[t][j + 2][r], o[t][j + 3][r]};
+    if (quad == 0) {
+      p[D] = m[t];
+      p[D + 1] = l[t];
+    }
+  }
+}
 
 template <typename T, int D, bool EXACT>
 __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kernel(SharedArgs a) {
@@ -109,226 +284,131 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
   constexpr int W = S::waves;
   extern __shared__ __attribute__((aligned(16))) float lds[];  // [W][32] rows
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, quad = lane >> 4, entries = a.count + c.seqs;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = c.kv_heads * c.group;
 
-  // units before each stretch of entries, one stretch per lane; every wave counts for itself
-  const int per = (entries + 63) >> 6;
-  uint32_t mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int e = lane * per + i;
-    if (e < entries) {
-      int group;
-      const Entry x = entry_of(a, e, group);
-      mine += units_of(x.columns, x.blocks(), W) * c.kv_heads;
+  // units before each stretch of groups, and of sequences, one stretch per lane; every wave
+  // counts for itself
+  const int per_group = (a.count + 63) >> 6, per_seq = (c.seqs + 63) >> 6;
+  uint32_t mine_p = 0, mine_o = 0;
+  Entry last_p{0, 0, 0, 0}, last_o{0, 0, 0, 0};  // a lane's one entry, where it has one
+  int last_group = -1;
+  for (int i = 0; i < per_group; ++i)
+    if (lane * per_group + i < a.count) {
+      last_p = prefix_of(a, lane * per_group + i);
+      mine_p += Parts(true, last_p.columns, last_p.blocks(), W).all(c.kv_heads);
     }
-  }
-  uint32_t sum = mine;  // inclusive
+  for (int i = 0; i < per_seq; ++i)
+    if (lane * per_seq + i < c.seqs) {
+      last_o = own_of(a, lane * per_seq + i, last_group);
+      mine_o += Parts(false, last_o.columns, last_o.blocks(), W).all(c.kv_heads);
+    }
+  uint32_t sum_p = mine_p, sum_o = mine_o;  // inclusive
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t up = __shfl_up(sum, d, 64);
-    if (lane >= d) sum += up;
+    const uint32_t p = __shfl_up(sum_p, d, 64), o = __shfl_up(sum_o, d, 64);
+    if (lane >= d) sum_p += p, sum_o += o;
   }
-  const uint32_t total = uint32_t(__builtin_amdgcn_readlane(int(sum), 63));
+  const uint32_t total_p = uint32_t(__builtin_amdgcn_readlane(int(sum_p), 63)), total_o = uint32_t(__builtin_amdgcn_readlane(int(sum_o), 63));
   if (blockIdx.x == 0 && wave == 0) {  // for the join
-    uint32_t at = sum - mine;
-    for (int i = 0; i < per; ++i) {
-      const int e = lane * per + i;
-      if (e >= entries) break;
-      int group;
-      const Entry x = entry_of(a, e, group);
-      a.entries[e] = uint4{at, uint32_t(x.blocks()), e < a.count ? uint32_t(x.first) : uint32_t(group), uint32_t(x.columns)};
-      at += units_of(x.columns, x.blocks(), W) * c.kv_heads;
+    uint32_t at = sum_p - mine_p;
+    for (int e = lane * per_group; e < min((lane + 1) * per_group, a.count); ++e) {
+      const Entry x = per_group == 1 ? last_p : prefix_of(a, e);
+      a.entries[e] = uint4{at, uint32_t(x.blocks()), uint32_t(x.first), uint32_t(x.columns)};
+      at += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
     }
-    if (lane == 0) a.entries[entries].x = total;
+    if (lane == 0) a.entries[a.count + c.seqs] = uint4{total_p, total_o, 0, 0};
   }
-  const Stretches stretches(total, gridDim.x);
-  if (blockIdx.x >= stretches.count) return;
-  const uint32_t u_begin = stretches.begin(blockIdx.x), u_end = stretches.begin(blockIdx.x + 1);
+  if (blockIdx.x == 0 && wave == 1) {
+    uint32_t at = sum_o - mine_o;
+    for (int e = lane * per_seq; e < min((lane + 1) * per_seq, c.seqs); ++e) {
+      int group = last_group;
+      const Entry x = per_seq == 1 ? last_o : own_of(a, e, group);
+      a.entries[a.count + e] = uint4{at, uint32_t(x.blocks()), uint32_t(group), uint32_t(x.columns)};
+      at += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+    }
+  }
+  const uint32_t prefixes = prefix_groups(total_p, total_o, gridDim.x);
+  const bool kind = blockIdx.x >= prefixes;  // own keys
+  const uint32_t total = kind ? total_o : total_p;
+  const Stretches stretches(total, kind ? (gridDim.x - prefixes) * W : prefixes, kind ? kOwnLeast : kPrefixLeast);
+  // (stretch i of the own keys: waves of different workgroups first)
+  const uint32_t mine_at = kind ? (blockIdx.x - prefixes) + wave * (gridDim.x - prefixes) : blockIdx.x;
+  if (mine_at >= stretches.count || !total) return;
+  const uint32_t u_begin = stretches.begin(mine_at), u_end = stretches.begin(mine_at + 1);
   uint32_t u = u_begin;
-  if (u >= u_end) return;
-  const int from_lane = __popcll(__ballot(sum <= u));
-  int e = from_lane * per;
-  uint32_t base = uint32_t(__builtin_amdgcn_readlane(int(sum - mine), from_lane));
+  const uint32_t to_lane = kind ? sum_o : sum_p;
+  const Entry last{kind ? last_o.first : last_p.first, kind ? last_o.columns : last_p.columns, kind ? last_o.lo : last_p.lo, kind ? last_o.hi : last_p.hi};
+  const int from_lane = __popcll(__ballot(to_lane <= u)), each = kind ? per_seq : per_group, entries = kind ? c.seqs : a.count;
+  int e = from_lane * each;
+  uint32_t base = uint32_t(__builtin_amdgcn_readlane(int(to_lane - (kind ? mine_o : mine_p)), from_lane));
 
-  while (u < u_end && e < entries) {
-    int group;
-    const Entry x = entry_of(a, e, group);
-    const int nb = x.blocks(), cw = column_waves(x.columns, W), parts = (x.columns + 32 * W - 1) / (32 * W);
-    const uint32_t each = uint32_t(nb) * cw, all = each * parts * c.kv_heads;
-    if (u >= base + all) {
-      base += all;
-      ++e;
-      continue;
+  for (; u < u_end && e < entries; ++e) {
+    Entry x;
+    if (each == 1) {  // the lanes have them
+      x = {__builtin_amdgcn_readlane(last.first, e), __builtin_amdgcn_readlane(last.columns, e), __builtin_amdgcn_readlane(last.lo, e),
+           __builtin_amdgcn_readlane(last.hi, e)};
+    } else {
+      int none;
+      x = kind ? own_of(a, e, none) : prefix_of(a, e);
+      x = {__builtin_amdgcn_readfirstlane(x.first), __builtin_amdgcn_readfirstlane(x.columns), __builtin_amdgcn_readfirstlane(x.lo),
+           __builtin_amdgcn_readfirstlane(x.hi)};
     }
-    const int index = int((u - base) / each), h = index / parts, column0 = (index - h * parts) * 32 * W;
-    const uint32_t start = base + index * each, stop = min(u_end, start + each);
-    const int first = int(u - start + cw - 1) / cw, last = int(stop - start + cw - 1) / cw;
-    u = stop;
-    if (first >= last) continue;
-
-    const int kw = W / cw, part = wave / cw, mine0 = column0 + (wave - part * cw) * 32;
-    const bool two = mine0 + 16 < x.columns;
-    f32x4 o[2][S::per];
-    float m[2] = {kNegInf, kNegInf}, l[2] = {0, 0};
+    const int nb = x.blocks();
+    const Parts parts(!kind, x.columns, nb, W);
+    const uint32_t all = parts.all(c.kv_heads);
+    while (u < min(u_end, base + all)) {
+      const int index = int((u - base) / parts.units), h = index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 32 : 32 * W);
+      const uint32_t start = base + index * parts.units + (kind ? kOwnStart : kPrefixStart), stop = min(u_end, base + (index + 1) * parts.units);
+      const int first = blocks_before(u, start, parts.waves), end = blocks_before(stop, start, parts.waves);
+      u = stop;
+      if (first >= end) continue;
+      f32x4 o[2][S::per];
+      float m[2] = {kNegInf, kNegInf}, l[2] = {0, 0};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
-    if (mine0 < x.columns && first + part < last) {
-      u32x4 q[2][S::steps];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int column = mine0 + 16 * t + col, seq = x.first + column / c.group, head = h * c.group + column % c.group;
-#pragma unroll
-        for (int i = 0; i < S::steps; ++i) {
-          q[t][i] = u32x4{0, 0, 0, 0};
-          const int d = 32 * i + 8 * quad;
-          if (column < x.columns && (EXACT || d < c.dim))
-            q[t][i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + seq * a.q_seq + head * a.q_head + d);
-          q[t][i] ^= c.flip;
-        }
+        for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
+      const bool complete = first == 0 && end == nb;
+      if (kind) {
+        const int columns = min(x.columns - column0, 32);
+        take_blocks<T, D, EXACT>(a, x, h, column0, columns > 16, first, end, 1, o, m, l);
+        float* to = complete ? a.rows + ((int64_t(c.seqs) + x.first) * heads + h * c.group + column0) * S::row
+                             : a.own_pieces + (int64_t(mine_at) * 2 + (start >= u_begin)) * a.own_columns * S::row;
+        store_columns<D>(to, columns, o, m, l);
+        continue;
       }
-      for (int i = first + part; i < last; i += kw) {
-        const int kb = (x.begin() + i) << 5;
-        u32x4 kf[2][S::steps];
-        uint32_t vr[8][S::words];
-        bool page_ok[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int at = (kb + 16 * t) >> c.page_shift;
-          int page = at < int(c.capacity >> c.page_shift) ? c.tables[x.first * c.table_stride + at] : -1;
-          page_ok[t] = page >= 0 && page < c.pages;
-          page = page_ok[t] ? page : 0;
-          const int row = (kb + 16 * t) & ((1 << c.page_shift) - 1);
-          const T* kp = static_cast<const T*>(c.k) + uint64_t(page) * c.k_page + uint64_t(h) * c.k_head + uint64_t(row + col) * c.k_token + 8 * quad;
-#pragma unroll
-          for (int n = 0; n < S::steps; ++n) {
-            kf[t][n] = u32x4{0, 0, 0, 0};
-            if (EXACT || 32 * n + 8 * quad < c.dim) kf[t][n] = *reinterpret_cast<const u32x4*>(kp + 32 * n);
-          }
-          const T* vp = static_cast<const T*>(c.v) + uint64_t(page) * c.v_page + uint64_t(h) * c.v_head + uint64_t(row + 4 * quad) * c.v_token + S::per * col;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-#pragma unroll
-            for (int w = 0; w < S::words; ++w) vr[4 * t + r][w] = 0;
-            if (EXACT || S::per * col < c.dim) {
-              if constexpr (S::words == 2) {
-                const u32x2 v = *reinterpret_cast<const u32x2*>(vp + uint64_t(r) * c.v_token);
-                vr[4 * t + r][0] = v[0];
-                vr[4 * t + r][1] = v[1];
-              } else {
-#pragma unroll
-                for (int w = 0; w < S::words; w += 4) {
-                  if (!EXACT && S::per * col + 2 * w >= c.dim) continue;
-                  const u32x4 v = *reinterpret_cast<const u32x4*>(vp + uint64_t(r) * c.v_token + 2 * w);
-#pragma unroll
-                  for (int b = 0; b < 4; ++b) vr[4 * t + r][w + b] = v[b];
-                }
-              }
-            }
-          }
+      const int cw = parts.waves, kw = W / cw, part = wave / cw, mine0 = column0 + (wave - part * cw) * 32;
+      if (mine0 < x.columns && first + part < end)
+        take_blocks<T, D, EXACT>(a, x, h, mine0, mine0 + 16 < x.columns, first + part, end, kw, o, m, l);
+      // the sums of waves that have the same columns
+      __syncthreads();  // the rows of the head before have been read
+      store_columns<D>(lds + wave * 32 * S::row, x.columns - mine0, o, m, l);
+      __syncthreads();
+      const int have = min(x.columns - column0, 32 * cw), waves = min(kw, end - first);
+      for (int i = threadIdx.x; i < have * (D / 4); i += W * 64) {
+        const int column = i / (D / 4), d = i % (D / 4) * 4;
+        const float* from = lds + column * S::row;  // (32 columns a wave, one wave's after the other's)
+        float top = kNegInf;
+        for (int n = 0; n < waves; ++n) top = fmaxf(top, from[n * cw * 32 * S::row + D]);
+        f32x4 sums = {0, 0, 0, 0};
+        float ls = 0;
+        for (int n = 0; n < waves; ++n) {
+          const float* p = from + n * cw * 32 * S::row;
+          const float f = __builtin_amdgcn_exp2f(p[D] - origin(top));
+          sums += f * *reinterpret_cast<const f32x4*>(p + d);
+          ls += f * p[D + 1];
         }
-        const bool whole = page_ok[0] && page_ok[1] && kb >= x.lo && kb + 32 <= x.hi;
-        u32x4 ph[2], pl[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (t && !two) continue;
-          f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-          for (int n = 0; n < S::steps; ++n) {
-            st[0] = Half<T>::mma16(kf[0][n], q[t][n], st[0]);
-            st[1] = Half<T>::mma16(kf[1][n], q[t][n], st[1]);
-          }
-          float s[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) s[r] = st[r >> 2][r & 3] * c.scale;
-          if (!whole) {  // keys that are not the entry's count as nothing, whatever their page holds
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              const int at = kb + 16 * (r >> 2) + 4 * quad + (r & 3);
-              const bool sees = bool(page_ok[r >> 2]) & (at >= x.lo) & (at < x.hi);
-              s[r] = sees ? s[r] : kNegInf;
-#pragma unroll
-              for (int w = 0; w < S::words; ++w) vr[r][w] = sees ? vr[r][w] : 0;
-            }
-          }
-          float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-          top = fmaxf(m[t], max32(max16(top)) - Half<T>::most);
-          if (__any(top > m[t])) {
-            const float f = __builtin_amdgcn_exp2f(m[t] - origin(top));
-            l[t] *= f;
-#pragma unroll
-            for (int j = 0; j < S::per; ++j) o[t][j] *= f;
-            m[t] = top;
-          }
-          uint32_t hi[4], rest[4];
-#pragma unroll
-          for (int r = 0; r < 8; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(s[r] - origin(m[t])), p1 = __builtin_amdgcn_exp2f(s[r + 1] - origin(m[t]));
-            l[t] += p0 + p1;
-            hi[r / 2] = pack2<T>(p0, p1);
-            rest[r / 2] = pack2<T>(p0 - low<T>(hi[r / 2]), p1 - high<T>(hi[r / 2]));
-          }
-          ph[t] = u32x4{hi[0], hi[1], hi[2], hi[3]}, pl[t] = u32x4{rest[0], rest[1], rest[2], rest[3]};
-        }
-#pragma unroll
-        for (int j = 0; j < S::per; ++j) {
-          u32x4 vt;
-#pragma unroll
-          for (int p = 0; p < 4; ++p)
-            vt[p] = __builtin_amdgcn_perm(vr[2 * p + 1][j / 2], vr[2 * p][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-          o[0][j] = Half<T>::mma16(vt, ph[0], o[0][j]);
-          o[0][j] = Half<T>::mma16(vt, pl[0], o[0][j]);
-          if (two) {
-            o[1][j] = Half<T>::mma16(vt, ph[1], o[1][j]);
-            o[1][j] = Half<T>::mma16(vt, pl[1], o[1][j]);
-          }
+        const int seq = x.first + (column0 + column) / c.group, head = h * c.group + (column0 + column) % c.group;
+        float* to = complete ? a.rows + (int64_t(seq) * heads + head) * S::row
+                             : a.pieces + ((int64_t(mine_at) * 2 + (start >= u_begin)) * a.columns + column) * S::row;
+        *reinterpret_cast<f32x4*>(to + d) = sums;
+        if (d == 0) {
+          to[D] = top;
+          to[D + 1] = ls;
         }
       }
     }
-    // the sums of waves that have the same columns
-    __syncthreads();  // the rows of the entry before have been read
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t && !two) continue;
-      const float sums = sum32(sum16(l[t]));
-      float* to = lds + (wave * 32 + 16 * t + col) * S::row;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < S::per; j += 4)
-          *reinterpret_cast<f32x4*>(to + (4 * quad + r) * S::per + j) = f32x4{o[t][j][r], o[t][j + 1][r], o[t][j + 2][r], o[t][j + 3][r]};
-      if (quad == 0) {
-        to[D] = m[t];
-        to[D + 1] = sums;
-      }
-    }
-    __syncthreads();
-    const int have = min(x.columns - column0, 32 * cw), waves = min(kw, last - first);
-    const bool complete = first == 0 && last == nb;
-    const int kind = e < a.count ? 0 : 1;
-    for (int i = threadIdx.x; i < have * (D / 4); i += W * 64) {
-      const int column = i / (D / 4), d = i % (D / 4) * 4, ct = column >> 5, r = column & 31;
-      float top = kNegInf;
-      for (int n = 0; n < waves; ++n) top = fmaxf(top, lds[((n * cw + ct) * 32 + r) * S::row + D]);
-      f32x4 sums = {0, 0, 0, 0};
-      float ls = 0;
-      for (int n = 0; n < waves; ++n) {
-        const float* p = lds + ((n * cw + ct) * 32 + r) * S::row;
-        const float f = __builtin_amdgcn_exp2f(p[D] - origin(top));
-        sums += f * *reinterpret_cast<const f32x4*>(p + d);
-        ls += f * p[D + 1];
-      }
-      const int seq = x.first + (column0 + column) / c.group, head = h * c.group + (column0 + column) % c.group;
-      float* to = complete ? a.rows + ((int64_t(kind) * c.seqs + seq) * (c.kv_heads * c.group) + head) * S::row
-                           : a.pieces + ((int64_t(blockIdx.x) * 2 + (start >= u_begin)) * a.columns + column) * S::row;
-      *reinterpret_cast<f32x4*>(to + d) = sums;
-      if (d == 0) {
-        to[D] = top;
-        to[D + 1] = ls;
-      }
-    }
+    base += all;
   }
 }
 
@@ -343,26 +423,31 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned
   const CacheArgs& c = a.c;
   const int all = c.kv_heads * c.group, s = blockIdx.x / all, head = blockIdx.x - s * all, kvh = head / c.group;
   const int set = threadIdx.x / per, d = threadIdx.x % per * 4;
-  const Stretches stretches(a.entries[a.count + c.seqs].x, workgroups);
-  const uint4 own = a.entries[a.count + s];
+  const uint4 totals = a.entries[a.count + c.seqs], own = a.entries[a.count + s];
+  const uint32_t prefixes = prefix_groups(totals.x, totals.y, workgroups);
   float m = kNegInf, l = 0;
   f32x4 o = {0, 0, 0, 0};
-  int turn = 0;  // pieces before this part's
+  int turn = 0;  // pieces before this kind's
   for (int kind = 0; kind < 2; ++kind) {
     if (kind == 0 && int(own.z) < 0) continue;
     const uint4 x = kind ? own : a.entries[own.z];
-    const int nb = int(x.y), columns = int(x.w), cw = column_waves(columns, W), parts = (columns + 32 * W - 1) / (32 * W);
+    const int nb = int(x.y), columns = int(x.w), cut = kind ? 32 : 32 * W;
     if (!nb) continue;
-    const int column = (kind ? 0 : (s - int(x.z)) * c.group) + head - kvh * c.group, cut = column / (32 * W);
-    const uint32_t each = uint32_t(nb) * cw, start = x.x + (uint32_t(kvh) * parts + cut) * each;
-    const uint32_t w0 = stretches.of(start), w1 = stretches.of(start + each - 1);
-    const bool complete = (stretches.begin(w0 + 1) - start + cw - 1) / cw >= uint32_t(nb);
+    const Parts parts(!kind, columns, nb, W);
+    const Stretches stretches = kind ? Stretches(totals.y, (workgroups - prefixes) * W, kOwnLeast) : Stretches(totals.x, prefixes, kPrefixLeast);
+    const int column = (kind ? 0 : (s - int(x.z)) * c.group) + head - kvh * c.group;
+    const uint32_t start = x.x + (uint32_t(kvh) * parts.parts + column / cut) * parts.units + (kind ? kOwnStart : kPrefixStart);
+    const uint32_t stop = start + uint32_t(nb) * parts.waves;
+    const uint32_t w0 = stretches.of(start), w1 = stretches.of(stop - 1);
+    const bool complete = blocks_before(min(stop, stretches.begin(w0 + 1)), start, parts.waves) == nb;
     const uint32_t count = complete ? 1 : w1 - w0 + 1;
     for (uint32_t i = (set + sets - turn % sets) % sets; i < count; i += sets) {
-      const uint32_t w = w0 + i, from = max(stretches.begin(w), start), to = min(stretches.begin(w + 1), start + each);
-      if ((from - start + cw - 1) / cw >= (to - start + cw - 1) / cw) continue;  // no block of it
+      const uint32_t w = w0 + i, from = stretches.begin(w);
+      if (blocks_before(from, start, parts.waves) >= blocks_before(min(stop, stretches.begin(w + 1)), start, parts.waves)) continue;  // no block of it
+      const int64_t piece = int64_t(w) * 2 + (start >= from);
       const float* p = complete ? a.rows + ((int64_t(kind) * c.seqs + s) * all + head) * S::row
-                                : a.pieces + ((int64_t(w) * 2 + (start >= stretches.begin(w))) * a.columns + column - cut * 32 * W) * S::row;
+                       : kind   ? a.own_pieces + (piece * a.own_columns + column % cut) * S::row
+                                : a.pieces + (piece * a.columns + column % cut) * S::row;
       const f32x4 po = *reinterpret_cast<const f32x4*>(p + d);
       const float pm = p[D], pl = p[D + 1], top = fmaxf(m, pm);
       const float f = __builtin_amdgcn_exp2f(m - origin(top)), pf = __builtin_amdgcn_exp2f(pm - origin(top));
@@ -416,11 +501,13 @@ int width_of(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 }  // namespace
 
-// One workgroup a CU, and no more than there are stretches.
+// One workgroup a CU, and no more than there is work for.
 unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys) {
-  const size_t units = entries * kv_heads * ((group + 31) / 32) * ((keys + 31) / 32 + 1);
-  return unsigned(std::max<size_t>(1, std::min<size_t>((units + kUnits - 1) / kUnits, 256)));
+  const size_t units = entries * kv_heads * ((group + 31) / 32) * ((keys + 31) / 32 + kPrefixStart);
+  return unsigned(std::max<size_t>(2, std::min<size_t>(units / kPrefixLeast, 256)));
 }
+size_t shared_own_columns(size_t group) { return std::min<size_t>(group, 32); }
+size_t shared_waves(size_t dim) { return dim > 128 ? SharedShape<256>::waves : SharedShape<128>::waves; }
 size_t shared_columns(size_t seqs, size_t group, size_t dim) {
   return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? 4 * 32 : 8 * 32);
 }

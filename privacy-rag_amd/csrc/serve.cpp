@@ -123,7 +123,7 @@ DecodePlan decode_plan(const praghip_cache& c, size_t heads, size_t max_length) 
 
 struct SharedPlan {
   unsigned workgroups;
-  size_t columns, rows, pieces, bytes;  // rows, pieces: where they begin
+  size_t columns, own_columns, rows, pieces, own_pieces, bytes;  // rows, pieces: where they begin
 };
 SharedPlan shared_plan(const praghip_cache& c, size_t heads, size_t count, size_t max_length) {
   SharedPlan p;
@@ -131,13 +131,15 @@ SharedPlan shared_plan(const praghip_cache& c, size_t heads, size_t count, size_
   p.workgroups = shared_workgroups(count + c.seqs, c.kv_heads, group, bound_of(c, max_length));
   p.columns = shared_columns(c.seqs, group, c.head_dim);
   p.rows = (count + c.seqs + 1) * sizeof(uint4);
+  p.own_columns = shared_own_columns(group);
   p.pieces = p.rows + 2 * c.seqs * heads * row;
-  p.bytes = p.pieces + p.workgroups * 2 * p.columns * row;
+  p.own_pieces = p.pieces + p.workgroups * 2 * p.columns * row;
+  p.bytes = p.own_pieces + p.workgroups * shared_waves(c.head_dim) * 2 * p.own_columns * row;
   return p;
 }
 // units of all entries in 32 bits: a head's columns occupy no more waves than two for each 32
 bool units_fit(const praghip_cache& c, size_t heads, size_t count) {
-  const size_t blocks = size_t(capacity_of(c.table_width, c.page_size)) / 32 + 1;
+  const size_t blocks = size_t(capacity_of(c.table_width, c.page_size)) / 32 + 9;  // (a head's start counts as some)
   return count <= (1u << 20) && (count + c.seqs) * c.kv_heads * ((heads / c.kv_heads + 31) / 16) <= (size_t(1) << 31) / blocks;
 }
 
@@ -233,6 +235,7 @@ int praghip_paged_shared(int device, const praghip_cache* c, const void* q, cons
   a.entries = static_cast<uint4*>(work);
   a.rows = reinterpret_cast<float*>(static_cast<char*>(work) + p.rows);
   a.pieces = reinterpret_cast<float*>(static_cast<char*>(work) + p.pieces);
+  a.own_pieces = reinterpret_cast<float*>(static_cast<char*>(work) + p.own_pieces), a.own_columns = int(p.own_columns);
   DeviceScope scope(device);
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_paged_shared(a, c->type, p.workgroups, pick(stream));
