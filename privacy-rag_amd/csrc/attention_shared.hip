@@ -88,7 +88,7 @@ struct Parts {
   int parts, waves;
   uint32_t units;
   __device__ __forceinline__ Parts(bool prefix, int columns, int blocks, int group_waves) {
-    const int most = prefix ? 32 * group_waves : 32;
+    const int most = prefix ? 32 * group_waves : 16;
     parts = (columns + most - 1) / most;
     waves = prefix ? column_waves(columns, group_waves) : 1;
     units = blocks ? uint32_t(blocks) * waves + (prefix ? kPrefixStart : kOwnStart) : 0;
@@ -117,22 +117,22 @@ __device__ __forceinline__ int blocks_before(uint32_t u, uint32_t first, int wav
 // The workgroups for the prefixes, as their share of the units is.
 __device__ __forceinline__ uint32_t prefix_groups(uint32_t prefix, uint32_t own, uint32_t groups) {
   if (!prefix || !own || groups < 2) return prefix ? groups : 0;
-  const uint32_t n = uint32_t((uint64_t(groups) * prefix + (uint64_t(prefix) + own) / 2) / (uint64_t(prefix) + own));
+  const int less = max(0, 9 - int(__clz(prefix | own)));  // (below 2^23 each, whose products with groups 32 bits hold)
+  const uint32_t all = (prefix >> less) + (own >> less), n = (groups * (prefix >> less) + all / 2) / max(all, 1u);
   return min(max(n, 1u), groups - 1);
 }
 
 // The keys of one key/value head h in an entry's blocks first, first + step .. below last,
-// for up to 32 columns from column0 on (16 unless `two`): o, m and l as of keys in powers
-// of two.
-template <typename T, int D, bool EXACT>
-__device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x, int h, int column0, bool two, int first, int last,
-                                            int step, f32x4 (&o)[2][D / 16], float (&m)[2], float (&l)[2]) {
+// for 16 TILES columns from column0 on: o, m and l as of keys in powers of two.
+template <typename T, int D, bool EXACT, int TILES>
+__device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x, int h, int column0, int first, int last, int step,
+                                            f32x4 (&o)[2][D / 16], float (&m)[2], float (&l)[2]) {
   using S = SharedShape<D>;
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-  u32x4 q[2][S::steps];
+  u32x4 q[TILES][S::steps];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < TILES; ++t) {
     const int column = column0 + 16 * t + col, seq = x.first + column / c.group, head = h * c.group + column % c.group;
 #pragma unroll
     for (int i = 0; i < S::steps; ++i) {
@@ -197,19 +197,18 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
 #pragma unroll
     for (int t = 0; t < 2; ++t) next[t] = page_at(((x.begin() + i + step) << 5) + 16 * t);
     const bool whole = page_ok[0] && page_ok[1] && kb >= x.lo && kb + 32 <= x.hi;
-    u32x4 ph[2], pl[2];
+    u32x4 ph[TILES], pl[TILES];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t && !two) continue;
+    for (int t = 0; t < TILES; ++t) {
       f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
       for (int n = 0; n < S::steps; ++n) {
         st[0] = Half<T>::mma16(kf[0][n], q[t][n], st[0]);
         st[1] = Half<T>::mma16(kf[1][n], q[t][n], st[1]);
       }
-      float s[8];
+      float s[8];  // before the scale, which is above 0
 #pragma unroll
-      for (int r = 0; r < 8; ++r) s[r] = st[r >> 2][r & 3] * c.scale;
+      for (int r = 0; r < 8; ++r) s[r] = st[r >> 2][r & 3];
       if (!whole) {  // keys that are not the entry's count as nothing, whatever their page holds
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -221,7 +220,7 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
         }
       }
       float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      top = fmaxf(m[t], max32(max16(top)) - Half<T>::most);
+      top = fmaxf(m[t], max32(max16(top)) * c.scale - Half<T>::most);
       if (__any(top > m[t])) {
         const float f = __builtin_amdgcn_exp2f(m[t] - origin(top));
         l[t] *= f;
@@ -230,9 +229,10 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
         m[t] = top;
       }
       uint32_t hi[4], rest[4];
+      const float from = -origin(m[t]);
 #pragma unroll
       for (int r = 0; r < 8; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(s[r] - origin(m[t])), p1 = __builtin_amdgcn_exp2f(s[r + 1] - origin(m[t]));
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c.scale, from)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], c.scale, from));
         l[t] += p0 + p1;
         hi[r / 2] = pack2<T>(p0, p1);
         rest[r / 2] = pack2<T>(p0 - low<T>(hi[r / 2]), p1 - high<T>(hi[r / 2]));
@@ -245,16 +245,14 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
 #pragma unroll
       for (int p = 0; p < 4; ++p)
         vt[p] = __builtin_amdgcn_perm(vr[2 * p + 1][j / 2], vr[2 * p][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-      o[0][j] = Half<T>::mma16(vt, ph[0], o[0][j]);
-      o[0][j] = Half<T>::mma16(vt, pl[0], o[0][j]);
-      if (two) {
-        o[1][j] = Half<T>::mma16(vt, ph[1], o[1][j]);
-        o[1][j] = Half<T>::mma16(vt, pl[1], o[1][j]);
-      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[t][j] = Half<T>::mma16(vt, ph[t], o[t][j]);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[t][j] = Half<T>::mma16(vt, pl[t], o[t][j]);
     }
   }
 #pragma unroll
-  for (int t = 0; t < 2; ++t) l[t] = sum32(sum16(l[t]));
+  for (int t = 0; t < TILES; ++t) l[t] = sum32(sum16(l[t]));
 }
 
 // A lane's rows of o, and m and l, at `to` (for the 32 columns of a wave).
@@ -291,17 +289,38 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
   const int per_group = (a.count + 63) >> 6, per_seq = (c.seqs + 63) >> 6;
   uint32_t mine_p = 0, mine_o = 0;
   Entry last_p{0, 0, 0, 0}, last_o{0, 0, 0, 0};  // a lane's one entry, where it has one
-  int last_group = -1;
-  for (int i = 0; i < per_group; ++i)
-    if (lane * per_group + i < a.count) {
-      last_p = prefix_of(a, lane * per_group + i);
-      mine_p += Parts(true, last_p.columns, last_p.blocks(), W).all(c.kv_heads);
+  int group = -1;
+  const bool few = per_group <= 1 && per_seq == 1;
+  if (few) {  // all loads at once; what they depend on is in the lanes
+    const bool has = lane < a.count;
+    const int begin = has ? a.groups[lane] : 0, stop = has ? a.groups[lane + 1] : 0, shared = has ? a.shared[lane] : 0;
+    const int length = lane < c.seqs ? length_of(c, lane) : 0;
+    const int first = min(max(begin, 0), c.seqs), end = min(max(stop, first), c.seqs);
+    const int longest = __shfl(length, min(first, 63), 64);
+    last_p = {first, (end - first) * c.group, 0, end - first > 1 ? min(max(shared, 0), longest) : 0};
+    last_o = {lane, c.group, 0, length};
+    for (int g = 0; g < a.count; ++g) {
+      const int prefix = __builtin_amdgcn_readlane(last_p.hi, g);
+      if (lane >= __builtin_amdgcn_readlane(begin, g) && lane < __builtin_amdgcn_readlane(stop, g)) {
+        const bool part = prefix > 0 && length >= prefix;
+        last_o.lo = part ? prefix : 0;
+        group = part ? g : -1;
+      }
     }
-  for (int i = 0; i < per_seq; ++i)
-    if (lane * per_seq + i < c.seqs) {
-      last_o = own_of(a, lane * per_seq + i, last_group);
-      mine_o += Parts(false, last_o.columns, last_o.blocks(), W).all(c.kv_heads);
-    }
+    if (has) mine_p = Parts(true, last_p.columns, last_p.blocks(), W).all(c.kv_heads);
+    if (lane < c.seqs) mine_o = Parts(false, last_o.columns, last_o.blocks(), W).all(c.kv_heads);
+  } else {
+    for (int i = 0; i < per_group; ++i)
+      if (lane * per_group + i < a.count) {
+        const Entry x = prefix_of(a, lane * per_group + i);
+        mine_p += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
+      }
+    for (int i = 0; i < per_seq; ++i)
+      if (lane * per_seq + i < c.seqs) {
+        const Entry x = own_of(a, lane * per_seq + i, group);
+        mine_o += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+      }
+  }
   uint32_t sum_p = mine_p, sum_o = mine_o;  // inclusive
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -310,21 +329,22 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
   }
   const uint32_t total_p = uint32_t(__builtin_amdgcn_readlane(int(sum_p), 63)), total_o = uint32_t(__builtin_amdgcn_readlane(int(sum_o), 63));
   if (blockIdx.x == 0 && wave == 0) {  // for the join
-    uint32_t at = sum_p - mine_p;
-    for (int e = lane * per_group; e < min((lane + 1) * per_group, a.count); ++e) {
-      const Entry x = per_group == 1 ? last_p : prefix_of(a, e);
-      a.entries[e] = uint4{at, uint32_t(x.blocks()), uint32_t(x.first), uint32_t(x.columns)};
-      at += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
-    }
     if (lane == 0) a.entries[a.count + c.seqs] = uint4{total_p, total_o, 0, 0};
-  }
-  if (blockIdx.x == 0 && wave == 1) {
-    uint32_t at = sum_o - mine_o;
-    for (int e = lane * per_seq; e < min((lane + 1) * per_seq, c.seqs); ++e) {
-      int group = last_group;
-      const Entry x = per_seq == 1 ? last_o : own_of(a, e, group);
-      a.entries[a.count + e] = uint4{at, uint32_t(x.blocks()), uint32_t(group), uint32_t(x.columns)};
-      at += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+    uint32_t at_p = sum_p - mine_p, at_o = sum_o - mine_o;
+    if (few) {
+      if (lane < a.count) a.entries[lane] = uint4{at_p, uint32_t(last_p.blocks()), uint32_t(last_p.first), uint32_t(last_p.columns)};
+      if (lane < c.seqs) a.entries[a.count + lane] = uint4{at_o, uint32_t(last_o.blocks()), uint32_t(group), uint32_t(last_o.columns)};
+    } else {
+      for (int e = lane * per_group; e < min((lane + 1) * per_group, a.count); ++e) {
+        const Entry x = prefix_of(a, e);
+        a.entries[e] = uint4{at_p, uint32_t(x.blocks()), uint32_t(x.first), uint32_t(x.columns)};
+        at_p += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
+      }
+      for (int e = lane * per_seq; e < min((lane + 1) * per_seq, c.seqs); ++e) {
+        const Entry x = own_of(a, e, group);
+        a.entries[a.count + e] = uint4{at_o, uint32_t(x.blocks()), uint32_t(group), uint32_t(x.columns)};
+        at_o += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+      }
     }
   }
   const uint32_t prefixes = prefix_groups(total_p, total_o, gridDim.x);
@@ -344,7 +364,7 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
 
   for (; u < u_end && e < entries; ++e) {
     Entry x;
-    if (each == 1) {  // the lanes have them
+    if (few) {  // the lanes have them
       x = {__builtin_amdgcn_readlane(last.first, e), __builtin_amdgcn_readlane(last.columns, e), __builtin_amdgcn_readlane(last.lo, e),
            __builtin_amdgcn_readlane(last.hi, e)};
     } else {
@@ -357,7 +377,7 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
     const Parts parts(!kind, x.columns, nb, W);
     const uint32_t all = parts.all(c.kv_heads);
     while (u < min(u_end, base + all)) {
-      const int index = int((u - base) / parts.units), h = index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 32 : 32 * W);
+      const int index = int((u - base) / parts.units), h = index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 16 : 32 * W);
       const uint32_t start = base + index * parts.units + (kind ? kOwnStart : kPrefixStart), stop = min(u_end, base + (index + 1) * parts.units);
       const int first = blocks_before(u, start, parts.waves), end = blocks_before(stop, start, parts.waves);
       u = stop;
@@ -369,43 +389,48 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
 #pragma unroll
         for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
       const bool complete = first == 0 && end == nb;
+      const int cw = parts.waves, kw = kind ? 1 : W / cw, part = kind ? 0 : wave / cw, mine0 = kind ? column0 : column0 + (wave - part * cw) * 32;
+      if (mine0 < x.columns && first + part < end) {
+        if (kind || x.columns <= 16)
+          take_blocks<T, D, EXACT, 1>(a, x, h, mine0, first + part, end, kw, o, m, l);
+        else
+          take_blocks<T, D, EXACT, 2>(a, x, h, mine0, first + part, end, kw, o, m, l);
+      }
       if (kind) {
-        const int columns = min(x.columns - column0, 32);
-        take_blocks<T, D, EXACT>(a, x, h, column0, columns > 16, first, end, 1, o, m, l);
         float* to = complete ? a.rows + ((int64_t(c.seqs) + x.first) * heads + h * c.group + column0) * S::row
                              : a.own_pieces + (int64_t(mine_at) * 2 + (start >= u_begin)) * a.own_columns * S::row;
-        store_columns<D>(to, columns, o, m, l);
+        store_columns<D>(to, min(x.columns - column0, 16), o, m, l);
         continue;
       }
-      const int cw = parts.waves, kw = W / cw, part = wave / cw, mine0 = column0 + (wave - part * cw) * 32;
-      if (mine0 < x.columns && first + part < end)
-        take_blocks<T, D, EXACT>(a, x, h, mine0, mine0 + 16 < x.columns, first + part, end, kw, o, m, l);
       // the sums of waves that have the same columns
       __syncthreads();  // the rows of the head before have been read
       store_columns<D>(lds + wave * 32 * S::row, x.columns - mine0, o, m, l);
       __syncthreads();
       const int have = min(x.columns - column0, 32 * cw), waves = min(kw, end - first);
+      float* const to = complete ? a.rows : a.pieces + (int64_t(mine_at) * 2 + (start >= u_begin)) * a.columns * S::row;
+#pragma unroll 2
       for (int i = threadIdx.x; i < have * (D / 4); i += W * 64) {
         const int column = i / (D / 4), d = i % (D / 4) * 4;
         const float* from = lds + column * S::row;  // (32 columns a wave, one wave's after the other's)
-        float top = kNegInf;
-        for (int n = 0; n < waves; ++n) top = fmaxf(top, from[n * cw * 32 * S::row + D]);
-        f32x4 sums = {0, 0, 0, 0};
-        float ls = 0;
-        for (int n = 0; n < waves; ++n) {
+        float top = from[D], ls = from[D + 1];
+        f32x4 sums = *reinterpret_cast<const f32x4*>(from + d);
+        for (int n = 1; n < waves; ++n) {
           const float* p = from + n * cw * 32 * S::row;
-          const float f = __builtin_amdgcn_exp2f(p[D] - origin(top));
-          sums += f * *reinterpret_cast<const f32x4*>(p + d);
-          ls += f * p[D + 1];
+          const float m = p[D], l = p[D + 1], most = fmaxf(top, m);
+          const f32x4 o = *reinterpret_cast<const f32x4*>(p + d);
+          const float f0 = __builtin_amdgcn_exp2f(top - origin(most)), f1 = __builtin_amdgcn_exp2f(m - origin(most));
+          sums = sums * f0 + o * f1;
+          ls = ls * f0 + l * f1;
+          top = most;
         }
-        const int seq = x.first + (column0 + column) / c.group, head = h * c.group + (column0 + column) % c.group;
-        float* to = complete ? a.rows + (int64_t(seq) * heads + head) * S::row
-                             : a.pieces + ((int64_t(mine_at) * 2 + (start >= u_begin)) * a.columns + column) * S::row;
-        *reinterpret_cast<f32x4*>(to + d) = sums;
-        if (d == 0) {
-          to[D] = top;
-          to[D + 1] = ls;
+        int64_t row = column;
+        if (complete) {
+          const int member = (column0 + column) / c.group;
+          row = int64_t(x.first + member) * heads + h * c.group + column0 + column - member * c.group;
         }
+        // (past the caches: a kernel's end waits for the lines that they hold)
+        __builtin_nontemporal_store(sums, reinterpret_cast<f32x4*>(to + row * S::row + d));
+        if (d == 0) __builtin_nontemporal_store(f32x4{top, ls, 0, 0}, reinterpret_cast<f32x4*>(to + row * S::row + D));
       }
     }
     base += all;
@@ -431,7 +456,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned
   for (int kind = 0; kind < 2; ++kind) {
     if (kind == 0 && int(own.z) < 0) continue;
     const uint4 x = kind ? own : a.entries[own.z];
-    const int nb = int(x.y), columns = int(x.w), cut = kind ? 32 : 32 * W;
+    const int nb = int(x.y), columns = int(x.w), cut = kind ? 16 : 32 * W;
     if (!nb) continue;
     const Parts parts(!kind, columns, nb, W);
     const Stretches stretches = kind ? Stretches(totals.y, (workgroups - prefixes) * W, kOwnLeast) : Stretches(totals.x, prefixes, kPrefixLeast);
@@ -503,10 +528,10 @@ int width_of(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 // One workgroup a CU, and no more than there is work for.
 unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys) {
-  const size_t units = entries * kv_heads * ((group + 31) / 32) * ((keys + 31) / 32 + kPrefixStart);
+  const size_t units = entries * kv_heads * ((group + 15) / 16) * ((keys + 31) / 32 + kPrefixStart);
   return unsigned(std::max<size_t>(2, std::min<size_t>(units / kPrefixLeast, 256)));
 }
-size_t shared_own_columns(size_t group) { return std::min<size_t>(group, 32); }
+size_t shared_own_columns(size_t group) { return std::min<size_t>(group, 16); }
 size_t shared_waves(size_t dim) { return dim > 128 ? SharedShape<256>::waves : SharedShape<128>::waves; }
 size_t shared_columns(size_t seqs, size_t group, size_t dim) {
   return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? 4 * 32 : 8 * 32);
