@@ -55,6 +55,7 @@ struct SharedArgs {
   float* rows;                             // heads of one piece: [2][seqs][heads]
   float *pieces, *own_pieces;              // in several: [workgroups][2][columns], [waves][2][own_columns]
   int columns, own_columns;
+  uint32_t inverse;  // of the heads of a key/value head, or 0
 };
 
 struct PromptArgs {
@@ -78,6 +79,7 @@ size_t decode_work_floats(unsigned workgroups, size_t group, size_t dim);
 unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t keys);
 size_t shared_columns(size_t seqs, size_t group, size_t dim);  // of a piece, at most
 size_t shared_own_columns(size_t group);
+uint32_t shared_inverse(size_t seqs, size_t group);
 size_t shared_waves(size_t dim);  // of a workgroup
 size_t shared_row_floats(size_t dim);
 int prompt_splits(size_t seqs, size_t kv_heads, size_t group, size_t dim, size_t max_rows, size_t keys);

@@ -37,12 +37,6 @@ struct SharedShape {
 // shortest stretch
 constexpr int kPrefixStart = 8, kOwnStart = 2, kPrefixLeast = 8, kOwnLeast = 3;
 
-__host__ __device__ __forceinline__ int column_waves(int columns, int waves) {
-  int n = 1;
-  while (n < waves && n * 32 < columns) n <<= 1;
-  return n;
-}
-
 // Keys lo .. hi - 1 of the pages of sequence `first`, for the heads of the sequences from
 // it on: `columns` columns of a key/value head.
 struct Entry {
@@ -82,19 +76,32 @@ __device__ __forceinline__ Entry own_of(const SharedArgs& a, int s, int& group) 
   return e;
 }
 
-// How many parts a head's columns are cut into, waves that have the columns of one part at
-// the same time, units of one part of one head.
+// How many parts a head's columns are cut into, waves (a power of two) that have the columns
+// of one part at the same time, units of one part of one head.
 struct Parts {
-  int parts, waves;
+  int parts, shift;
   uint32_t units;
   __device__ __forceinline__ Parts(bool prefix, int columns, int blocks, int group_waves) {
-    const int most = prefix ? 32 * group_waves : 16;
-    parts = (columns + most - 1) / most;
-    waves = prefix ? column_waves(columns, group_waves) : 1;
-    units = blocks ? uint32_t(blocks) * waves + (prefix ? kPrefixStart : kOwnStart) : 0;
+    shift = prefix ? (columns > 32) + (columns > 64) + (columns > 128 && group_waves == 8) : 0;
+    parts = prefix ? (columns + 32 * group_waves - 1) / (32 * group_waves) : (columns + 15) >> 4;
+    units = blocks ? (uint32_t(blocks) << shift) + (prefix ? kPrefixStart : kOwnStart) : 0;
   }
   __device__ __forceinline__ uint32_t all(int kv_heads) const { return units * parts * kv_heads; }
 };
+
+// the sum of the lanes up to each, by moves within rows of 16 lanes and from their last ones
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CONTROL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  return v + moved<0x143, 0xc>(v);
+}
 
 // Units over workgroups, or waves: each of the first `extra` has one more than the others.
 struct Stretches {
@@ -111,8 +118,19 @@ struct Stretches {
     return u < longer ? u / (each + 1) : extra + (u - longer) / each;
   }
 };
-// blocks of a head (one of whose blocks is `waves` units, after its start) before unit u
-__device__ __forceinline__ int blocks_before(uint32_t u, uint32_t first, int waves) { return u > first ? int((u - first + waves - 1) / waves) : 0; }
+// blocks of a head (one of whose blocks is 2^shift units, after its start) before unit u
+__device__ __forceinline__ int blocks_before(uint32_t u, uint32_t first, int shift) {
+  return u > first ? int((u - first + (1u << shift) - 1) >> shift) : 0;
+}
+// A column's sequence, from the entry's first, and head of the key/value head (by a product
+// where that is exact).
+struct Column {
+  int member, head;
+  __device__ __forceinline__ Column(const SharedArgs& a, int i) {
+    member = a.inverse ? int(__umulhi(uint32_t(i), a.inverse)) : i / a.c.group;
+    head = i - member * a.c.group;
+  }
+};
 
 // The workgroups for the prefixes, as their share of the units is.
 __device__ __forceinline__ uint32_t prefix_groups(uint32_t prefix, uint32_t own, uint32_t groups) {
@@ -133,7 +151,9 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
   u32x4 q[TILES][S::steps];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
-    const int column = column0 + 16 * t + col, seq = x.first + column / c.group, head = h * c.group + column % c.group;
+    const int column = column0 + 16 * t + col;
+    const Column of(a, column);
+    const int seq = x.first + of.member, head = h * c.group + of.head;
 #pragma unroll
     for (int i = 0; i < S::steps; ++i) {
       q[t][i] = u32x4{0, 0, 0, 0};
@@ -321,12 +341,7 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
         mine_o += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
       }
   }
-  uint32_t sum_p = mine_p, sum_o = mine_o;  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t p = __shfl_up(sum_p, d, 64), o = __shfl_up(sum_o, d, 64);
-    if (lane >= d) sum_p += p, sum_o += o;
-  }
+  const uint32_t sum_p = wave_scan(mine_p), sum_o = wave_scan(mine_o);  // inclusive
   const uint32_t total_p = uint32_t(__builtin_amdgcn_readlane(int(sum_p), 63)), total_o = uint32_t(__builtin_amdgcn_readlane(int(sum_o), 63));
   if (blockIdx.x == 0 && wave == 0) {  // for the join
     if (lane == 0) a.entries[a.count + c.seqs] = uint4{total_p, total_o, 0, 0};
@@ -377,9 +392,9 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
     const Parts parts(!kind, x.columns, nb, W);
     const uint32_t all = parts.all(c.kv_heads);
     while (u < min(u_end, base + all)) {
-      const int index = int((u - base) / parts.units), h = index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 16 : 32 * W);
+      const int index = int((u - base) / parts.units), h = parts.parts == 1 ? index : index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 16 : 32 * W);
       const uint32_t start = base + index * parts.units + (kind ? kOwnStart : kPrefixStart), stop = min(u_end, base + (index + 1) * parts.units);
-      const int first = blocks_before(u, start, parts.waves), end = blocks_before(stop, start, parts.waves);
+      const int first = blocks_before(u, start, parts.shift), end = blocks_before(stop, start, parts.shift);
       u = stop;
       if (first >= end) continue;
       f32x4 o[2][S::per];
@@ -389,7 +404,8 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
 #pragma unroll
         for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
       const bool complete = first == 0 && end == nb;
-      const int cw = parts.waves, kw = kind ? 1 : W / cw, part = kind ? 0 : wave / cw, mine0 = kind ? column0 : column0 + (wave - part * cw) * 32;
+      const int cw = 1 << parts.shift, kw = kind ? 1 : W >> parts.shift, part = kind ? 0 : wave >> parts.shift;
+      const int mine0 = kind ? column0 : column0 + (wave & (cw - 1)) * 32;
       if (mine0 < x.columns && first + part < end) {
         if (kind || x.columns <= 16)
           take_blocks<T, D, EXACT, 1>(a, x, h, mine0, first + part, end, kw, o, m, l);
@@ -425,8 +441,8 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
         }
         int64_t row = column;
         if (complete) {
-          const int member = (column0 + column) / c.group;
-          row = int64_t(x.first + member) * heads + h * c.group + column0 + column - member * c.group;
+          const Column of(a, column0 + column);
+          row = int64_t(x.first + of.member) * heads + h * c.group + of.head;
         }
         // (past the caches: a kernel's end waits for the lines that they hold)
         __builtin_nontemporal_store(sums, reinterpret_cast<f32x4*>(to + row * S::row + d));
@@ -462,13 +478,13 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned
     const Stretches stretches = kind ? Stretches(totals.y, (workgroups - prefixes) * W, kOwnLeast) : Stretches(totals.x, prefixes, kPrefixLeast);
     const int column = (kind ? 0 : (s - int(x.z)) * c.group) + head - kvh * c.group;
     const uint32_t start = x.x + (uint32_t(kvh) * parts.parts + column / cut) * parts.units + (kind ? kOwnStart : kPrefixStart);
-    const uint32_t stop = start + uint32_t(nb) * parts.waves;
+    const uint32_t stop = start + (uint32_t(nb) << parts.shift);
     const uint32_t w0 = stretches.of(start), w1 = stretches.of(stop - 1);
-    const bool complete = blocks_before(min(stop, stretches.begin(w0 + 1)), start, parts.waves) == nb;
+    const bool complete = blocks_before(min(stop, stretches.begin(w0 + 1)), start, parts.shift) == nb;
     const uint32_t count = complete ? 1 : w1 - w0 + 1;
     for (uint32_t i = (set + sets - turn % sets) % sets; i < count; i += sets) {
       const uint32_t w = w0 + i, from = stretches.begin(w);
-      if (blocks_before(from, start, parts.waves) >= blocks_before(min(stop, stretches.begin(w + 1)), start, parts.waves)) continue;  // no block of it
+      if (blocks_before(from, start, parts.shift) >= blocks_before(min(stop, stretches.begin(w + 1)), start, parts.shift)) continue;  // no block of it
       const int64_t piece = int64_t(w) * 2 + (start >= from);
       const float* p = complete ? a.rows + ((int64_t(kind) * c.seqs + s) * all + head) * S::row
                        : kind   ? a.own_pieces + (piece * a.own_columns + column % cut) * S::row
@@ -535,6 +551,10 @@ size_t shared_own_columns(size_t group) { return std::min<size_t>(group, 16); }
 size_t shared_waves(size_t dim) { return dim > 128 ? SharedShape<256>::waves : SharedShape<128>::waves; }
 size_t shared_columns(size_t seqs, size_t group, size_t dim) {
   return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? 4 * 32 : 8 * 32);
+}
+// an exact i / group of i below seqs * group as a product's upper half, or 0
+uint32_t shared_inverse(size_t seqs, size_t group) {
+  return group > 1 && seqs * group * group < (uint64_t(1) << 32) ? uint32_t(((uint64_t(1) << 32) + group - 1) / group) : 0;
 }
 size_t shared_row_floats(size_t dim) { return width_of(dim) + 4; }
 

@@ -236,6 +236,7 @@ int praghip_paged_shared(int device, const praghip_cache* c, const void* q, cons
   a.rows = reinterpret_cast<float*>(static_cast<char*>(work) + p.rows);
   a.pieces = reinterpret_cast<float*>(static_cast<char*>(work) + p.pieces);
   a.own_pieces = reinterpret_cast<float*>(static_cast<char*>(work) + p.own_pieces), a.own_columns = int(p.own_columns);
+  a.inverse = shared_inverse(c->seqs, heads / c->kv_heads);
   DeviceScope scope(device);
   hipError_t e = scope.status();
   if (e == hipSuccess) e = launch_paged_shared(a, c->type, p.workgroups, pick(stream));
