@@ -13,14 +13,15 @@
 // * bins: each part's counts and sums by bin (LDS, then the workspace), relative to the part's
 //   own maximum, whose bin is a whole number of powers of two from any other part's, so that
 //   parts are added by shifting;
-// * list: every part adds the row's bins, finds those in which a cut falls, and appends its own
-//   tokens of those bins to the row's list;
+// * list: workgroups of some parts add the row's bins, find those in which a cut falls, and
+//   append their tokens of those bins to the row's list;
 // * draw: a workgroup a row cuts the listed bins by value and index (digits of 10 bits of both
 //   together), adds what stays of each part, takes the part that the random number falls into
 //   and goes through that one by index.
 // The order of the list changes nothing: sums are of integers, and cuts are by value and index.
 #include "sample.hpp"
 
+#include <algorithm>
 #include <climits>
 
 #include "attention.hpp"
@@ -29,7 +30,7 @@ namespace praghip {
 
 struct SamplePart {
   double anchor;  // the power of two at or above the part's largest weight
-  uint64_t mass;  // of all its tokens
+  uint64_t mass;  // of all its tokens (of a row without filters)
   float top;      // its largest logit
   uint32_t at;    // and the lowest index of it
 };
@@ -37,7 +38,7 @@ struct SamplePart {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kEach = 16, kPart = kThreads * kEach;  // tokens of a thread, in pieces of 8, and of a part
+constexpr int kEach = 8, kPart = kThreads * kEach;  // tokens of a thread, in pieces of 8, and of a part
 constexpr int kParts = kSampleVocab / kPart > 64 ? kSampleVocab / kPart : 64;  // of a row, at most
 constexpr int kRange = 46, kBins = kRange * 16;      // powers of two that weights span, and their bins
 constexpr int kBits = 43;                            // of a weight's fraction
@@ -93,7 +94,7 @@ __device__ __forceinline__ Scale scale_of(float top, float temperature) {
   return s;
 }
 // 2^y in units of 2^-kBits and its bin, of y in (-kRange, 0]: y in 1/256 by a table of their
-// powers, the rest by the exponential series (z^4 / 24 is below 2^-42).
+// powers, the rest by the exponential series (its fourth term is below 2^-42).
 struct Weight {
   uint32_t bin;
   double units;
@@ -107,8 +108,9 @@ __device__ __forceinline__ Weight weight(double y, const double* table) {
   constexpr double magic = 6755399441055744.0 / 256;  // 1.5 2^52 in units of 1/256
   const double moved = y + magic;
   const int n = int(uint32_t(__builtin_bit_cast(u64, moved)));
-  const double z = (y - (moved - magic)) * 0.69314718055994530942;
-  const double power = __builtin_fma(__builtin_fma(__builtin_fma(z, 1. / 6, 0.5), z, 1.), z, 1.) * table[n & 255];
+  const double z = y - (moved - magic);  // (the series' coefficients are ln 2, ln^2 2 / 2, ln^3 2 / 6)
+  const double power =
+      __builtin_fma(__builtin_fma(__builtin_fma(z, 0.055504108664821580, 0.24022650695910071), z, 0.69314718055994531), z, 1.) * table[n & 255];
   Weight w;
   w.bin = uint32_t(-n) >> 4;
   w.units = __builtin_bit_cast(double, __builtin_bit_cast(u64, power) + (u64(int64_t(n >> 8)) << 52));
@@ -166,6 +168,19 @@ struct Most {
 __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), 63)); }
 __device__ __forceinline__ u64 last_lane(u64 v) { return u64(last_lane(uint32_t(v))) | u64(last_lane(uint32_t(v >> 32))) << 32; }
 
+// The sum up to each of the waves' totals in LDS, for this wave's and of all (kWaves lanes have
+// them).
+template <typename V>
+__device__ __forceinline__ V before_wave(const V* lds, V& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const V own = lane < kWaves ? lds[lane] : 0, to = wave_scan(own, Sum());
+  all = last_lane(to);
+  const V before = to - own;
+  if constexpr (sizeof(V) == 8)
+    return u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(before)), wave))) | u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(before >> 32)), wave))) << 32;
+  else
+    return uint32_t(__builtin_amdgcn_readlane(int(before), wave));
+}
 // Sums up to each thread, and of all; all threads call it.
 template <typename V>
 __device__ __forceinline__ V group_scan(V v, V* lds, V& all) {
@@ -173,14 +188,7 @@ __device__ __forceinline__ V group_scan(V v, V* lds, V& all) {
   __syncthreads();
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const V x = lds[w];
-    v += w < int(threadIdx.x >> 6) ? x : 0;
-    all += x;
-  }
-  return v;
+  return v + before_wave(lds, all);
 }
 __device__ __forceinline__ u64 group_sum(u64 v, u64* lds) {
   u64 all;
@@ -192,10 +200,7 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* lds) {
   __syncthreads();
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = max(v, lds[w]);
-  return v;
+  return last_lane(wave_scan((threadIdx.x & 63) < kWaves ? lds[threadIdx.x & 63] : 0u, Most()));
 }
 
 // `share` (0 up to 1) times `of`, exactly, rounded down or up
@@ -261,15 +266,19 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a) {
         if (counts(y)) {
           const Weight w = weight(y, table);
           const u64 units = w.whole();
-          total += units;
           if (f.any()) {
             atomicAdd(&mass[w.bin], units);
             if (f.by_count()) atomicAdd(&count[w.bin], 1u);
+          } else {
+            total += units;
           }
         }
       }
   }
-  total = group_sum(total, sums);
+  if (f.any())
+    __syncthreads();
+  else
+    total = group_sum(total, sums);
   if (threadIdx.x == 0) *out = {s.anchor, total, top, 0};
   if (f.any() && int(threadIdx.x) < kBins) {
     const size_t at = (size_t(row) * a.parts + part) * kBins + threadIdx.x;
@@ -307,19 +316,16 @@ __device__ __forceinline__ int away_of(const Scale& row, const SamplePart& part)
   const double d = row.anchor - part.anchor;
   return d < kRange ? int(d) : kRange;
 }
-// a token in the list: its index, and its bin in the row
-constexpr int kIndex = 20;
+constexpr int kIndex = 20;  // bits of a token's index
 constexpr uint32_t kIndexes = (1u << kIndex) - 1;
-static_assert(kBins <= 1 << (32 - kIndex), "an index and a bin in 32 bits");
 
 // ---------------------------------------------------------- tokens of the cuts' bins
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, int parts_each) {
   __shared__ u64 sums[kWaves], mass_to[kBins];
   __shared__ uint32_t words[kWaves], count_to[kBins], base;
-  __shared__ double table[256];
   __shared__ int edges[6], aways[kParts];
-  const int part = blockIdx.x, row = blockIdx.y;
+  const int row = blockIdx.y;
   const T* logits = static_cast<const T*>(a.logits) + row * a.row;
   const SamplePart* parts = a.part + row * a.parts;
   const Filters f = filters_of(a, row);
@@ -328,7 +334,6 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a) {
   if (top == kNegInf) return;
   const Scale s = scale_of(top, f.temperature);
   if (int(threadIdx.x) < a.parts) aways[threadIdx.x] = away_of(s, parts[threadIdx.x]);
-  fill_table(table);
   if (threadIdx.x < 6) edges[threadIdx.x] = threadIdx.x & 1 ? -1 : kBins;  // empty ranges
   __syncthreads();
   // the row's bins: this thread's, and sums up to it
@@ -339,14 +344,24 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a) {
     const uint32_t* many = a.count + size_t(row) * a.parts * kBins;
     const int bin = min(int(threadIdx.x), kBins - 1);
     const bool has = int(threadIdx.x) < kBins;
-#pragma unroll 4
-    for (int p = 0; p < a.parts; ++p) {  // (no load behind a condition)
-      const int away = aways[p], b = bin - 16 * away, at = p * kBins + max(b, 0);
-      const u64 v = of[at];
-      const uint32_t n = f.by_count() ? many[at] : 0;
-      const bool here = has & (b >= 0) & (away < kRange);
-      mass += here ? v >> away : 0;
-      count += here ? n : 0;
+    for (int p = 0; p < a.parts; p += 4) {  // (four parts' loads at once, and none behind a condition)
+      u64 v[4];
+      uint32_t n[4];
+      int away[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int q = min(p + i, a.parts - 1);
+        away[i] = p + i < a.parts ? aways[q] : kRange;
+        b[i] = bin - 16 * away[i];
+        v[i] = of[q * kBins + max(b[i], 0)];
+        n[i] = f.by_count() ? many[q * kBins + max(b[i], 0)] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool here = has & (b[i] >= 0) & (away[i] < kRange);
+        mass += here ? v[i] >> away[i] : 0;
+        count += here ? n[i] : 0;
+      }
     }
   }
   u64 mass_all;
@@ -371,50 +386,52 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a) {
     __syncthreads();
   }
   const int e0 = edges[0], e1 = edges[1], e2 = edges[2], e3 = edges[3], e4 = edges[4], e5 = edges[5];
-  if (part == 0) {  // for the draw
+  if (blockIdx.x == 0) {  // for the draw
     if (int(threadIdx.x) < kBins) {
       a.mass_to[size_t(row) * kBins + threadIdx.x] = m;
       a.count_to[size_t(row) * kBins + threadIdx.x] = n;
     }
     if (threadIdx.x < 8) a.edges[size_t(row) * 8 + threadIdx.x] = threadIdx.x < 6 ? edges[threadIdx.x] : int(counted);
   }
-  const int away = aways[part];
-  if (away == kRange) return;
   // Tokens whose logit may be in one of those bins, by 32 bits and a little room on both sides
-  // (where that is no number, all of them); then, of the few, the bin that their part counted.
-  const Scale own = scale_of(parts[part].top, f.temperature);
-  const int low_bin = min(min(e0, e2), e4) - 16 * away, high_bin = max(max(e1, e3), e5) - 16 * away;
-  const double room = 1e-6 * (fabs(own.top) + 50 / own.by);
-  const float upper = float(own.top + ((-16. * low_bin + 0.5) / 256 - own.from) / own.by + room);
-  const float lower = float(own.top + ((-16. * high_bin - 15.5) / 256 - own.from) / own.by - room);
-  uint32_t maybe = 0, found = 0;
+  // (where that is no number, all of them): the draw looks at the few by 64.
+  const int edge[6] = {e0, e1, e2, e3, e4, e5};
+  for (int part = blockIdx.x * parts_each; part < min(int(blockIdx.x + 1) * parts_each, a.parts); ++part) {
+    const int away = aways[part];
+    if (away == kRange) continue;
+    const Scale own = scale_of(parts[part].top, f.temperature);
+    const double room = 1e-6 * (fabs(own.top) + 50 / own.by);
+    float upper[3], lower[3];
 #pragma unroll
-  for (int i = 0; i < kEach / 8; ++i) {
-    float x[8];
-    load8(logits, part * kPart + (i * kThreads + int(threadIdx.x)) * 8, a.vocab, x);
+    for (int r = 0; r < 3; ++r) {
+      upper[r] = float(own.top + ((-16. * (edge[2 * r] - 16 * away) + 0.5) / 256 - own.from) / own.by + room);
+      lower[r] = float(own.top + ((-16. * (edge[2 * r + 1] - 16 * away) - 15.5) / 256 - own.from) / own.by - room);
+      if (edge[2 * r] > edge[2 * r + 1]) upper[r] = kNegInf, lower[r] = -kNegInf;
+    }
+    uint32_t found = 0;  // a bit for each of the thread's tokens
 #pragma unroll
-    for (int j = 0; j < 8; ++j) maybe |= !(x[j] > upper) && !(x[j] < lower) && x[j] > kNegInf ? 1u << (8 * i + j) : 0;
-  }
-  const auto index_of = [&](int bit) { return part * kPart + ((bit >> 3) * kThreads + int(threadIdx.x)) * 8 + (bit & 7); };
-  const auto bin_of = [&](int index) {
-    const double y = exponent(own, plain(float(logits[index])));
-    return counts(y) ? int(weight(y, table).bin) + 16 * away : INT_MAX;
-  };
-  for (uint32_t left = maybe; left; left &= left - 1) {
-    const int bit = __ffs(left) - 1, b = bin_of(index_of(bit));
-    if ((b >= e0 && b <= e1) || (b >= e2 && b <= e3) || (b >= e4 && b <= e5)) found |= 1u << bit;
-  }
-  uint32_t all;
-  const uint32_t mine = __popc(found);
-  uint32_t at = group_scan(mine, words, all) - mine;
-  if (!all) return;
-  if (threadIdx.x == 0) base = atomicAdd(a.listed + row, all);
-  __syncthreads();
-  uint32_t* list = a.list + int64_t(row) * a.vocab;
-  at += base;
-  for (; found; found &= found - 1) {
-    const int index = index_of(__ffs(found) - 1);
-    list[at++] = uint32_t(index) | uint32_t(bin_of(index)) << kIndex;
+    for (int i = 0; i < kEach / 8; ++i) {
+      float x[8];
+      load8(logits, part * kPart + (i * kThreads + int(threadIdx.x)) * 8, a.vocab, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        bool maybe = false;
+#pragma unroll
+        for (int r = 0; r < 3; ++r) maybe |= !(x[j] > upper[r]) & !(x[j] < lower[r]);
+        if (maybe && x[j] > kNegInf) found |= 1u << (8 * i + j);
+      }
+    }
+    uint32_t all;
+    const uint32_t mine = __popc(found);
+    uint32_t at = group_scan(mine, words, all) - mine;
+    if (!all) continue;
+    if (threadIdx.x == 0) base = atomicAdd(a.listed + row, all);
+    __syncthreads();
+    uint32_t* list = a.list + int64_t(row) * a.vocab;
+    for (at += base; found; found &= found - 1) {
+      const int bit = __ffs(found) - 1;
+      list[at++] = uint32_t(part * kPart + ((bit >> 3) * kThreads + int(threadIdx.x)) * 8 + (bit & 7));
+    }
   }
 }
 
@@ -493,7 +510,8 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
   __shared__ Scratch lds;
   __shared__ u64 part_mass[kParts];
-  __shared__ double table[256];
+  __shared__ double table[256], from[kParts];
+  __shared__ float tops[kParts];
   __shared__ int token, aways[kParts];
   const int row = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const T* logits = static_cast<const T*>(a.logits) + row * a.row;
@@ -508,8 +526,12 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
   const Scale s = scale_of(largest.top, f.temperature);
   if (int(threadIdx.x) < kParts) part_mass[threadIdx.x] = 0;
   if (int(threadIdx.x) < a.parts) {
-    aways[threadIdx.x] = away_of(s, parts[threadIdx.x]);
-    if (!f.any()) part_mass[threadIdx.x] = aways[threadIdx.x] < kRange ? parts[threadIdx.x].mass >> aways[threadIdx.x] : 0;
+    const SamplePart part = parts[threadIdx.x];
+    const int away = away_of(s, part);
+    aways[threadIdx.x] = away;
+    tops[threadIdx.x] = part.top;
+    from[threadIdx.x] = scale_of(part.top, f.temperature).from;
+    if (!f.any()) part_mass[threadIdx.x] = away < kRange ? part.mass >> away : 0;
   }
   if (threadIdx.x == 0) token = -1;
   __syncthreads();
@@ -524,60 +546,116 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     const uint64_t* mass_to = a.mass_to + size_t(row) * kBins;
     const int listed = int(min(a.listed[row], uint32_t(a.vocab)));
     const uint32_t* list = a.list + int64_t(row) * a.vocab;
-    const auto token_of = [&](uint32_t v) -> Token {
-      const int i = int(v & kIndexes);
+    // a token, with the bin that its part counted it in
+    const auto token_of = [&](int i) -> Token {
       const float x = plain(float(logits[i]));
-      return {i, int(v >> kIndex), key_of(x), weight(exponent(s, x), table).whole()};
+      const int p = i / kPart;
+      const double y = __builtin_fma(double(x) - double(tops[p]), s.by, from[p]);
+      const bool has = counts(y) && aways[p] < kRange;
+      return {i, has ? int(weight(y, table).bin) + 16 * aways[p] : INT_MAX, key_of(x), weight(exponent(s, x), table).whole()};
     };
     Token held[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int n = i * kThreads + threadIdx.x;
       held[i].bin = -1;
-      if (n < listed) held[i] = token_of(list[n]);
+      if (n < listed) held[i] = token_of(int(list[n]));
     }
     const auto each = [&](auto with) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
         if (i * kThreads < listed && held[i].bin >= 0) with(held[i]);
 #pragma unroll 1
-      for (int n = kHeld * kThreads + threadIdx.x; n < listed; n += kThreads) with(token_of(list[n]));
+      for (int n = kHeld * kThreads + threadIdx.x; n < listed; n += kThreads) with(token_of(int(list[n])));
     };
     const bool counted = edges[6];
     const int kbin = counted ? edges[0] : kBins, e2 = edges[2], e3 = edges[3], e4 = edges[4];
     int bin = kBins;
     u64 all = mass_to[kBins - 1];
     // the cut by count, then the one by mass of what it leaves
-#pragma unroll 1
-    for (int turn = counted ? 0 : 1; turn < (f.by_mass() ? 2 : 1); ++turn) {
-      u64 before;  // amounts, in the cut's bin, before the last that stays
-      if (turn == 0) {
-        bin = kbin;
-        before = u64(f.top_k) - 1 - (bin ? a.count_to[size_t(row) * kBins + bin - 1] : 0);
-      } else {
-        if (counted) {
-          u64 mine = 0;
-          each([&](const Token& t) {
-            if (t.bin == bin && stays(t.key, t.index)) mine += t.units;
-          });
-          all = group_sum(mine, lds.sums) + (bin ? mass_to[bin - 1] : 0);
+    const auto count_before = [&] { return u64(f.top_k) - 1 - (kbin ? a.count_to[size_t(row) * kBins + kbin - 1] : 0); };
+    const auto mass_bin = [&](u64 target) {  // (it is one of the listed range; that is one bin, nearly always)
+      int b = e2;
+      while (b < e3 && mass_to[b] < target) ++b;
+      return b;
+    };
+    if (listed <= 64) {
+      // a wave has them all, in its lanes: each token's order in its bin by looking at every other
+      if (wave == 0) {
+        const Token& t = held[0];
+        u64 mass = 0;
+        uint32_t count = 0;
+        for (int n = 0; n < listed; ++n) {
+          const uint32_t k = uint32_t(__builtin_amdgcn_readlane(int(t.key), n));
+          const int i = __builtin_amdgcn_readlane(t.index, n), b = __builtin_amdgcn_readlane(t.bin, n);
+          const u64 units = u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.units)), n))) |
+                            u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.units >> 32)), n))) << 32;
+          if (b == t.bin && (k > t.key || (k == t.key && i <= t.index))) {
+            mass += units;
+            ++count;
+          }
         }
-        const u64 target = share_of(f, all);
-        bin = e2;  // (it is one of the listed range; that is one bin, nearly always)
-        while (bin < e3 && mass_to[bin] < target) ++bin;
-        const u64 to = bin ? mass_to[bin - 1] : 0;
-        before = target > to ? target - to - 1 : 0;
+        const auto take = [&](bool mine) {
+          const uint64_t who = __ballot(mine && lane < listed);
+          if (!who) return -1;
+          const int n = __ffsll((long long)who) - 1;
+          const uint32_t k = uint32_t(__builtin_amdgcn_readlane(int(t.key), n));
+          const int i = __builtin_amdgcn_readlane(t.index, n);
+          if (stays(k, i)) key = k, last = i;
+          return n;
+        };
+        if (counted) {
+          bin = kbin;
+          const int n = take(t.bin == bin && count == uint32_t(count_before()) + 1);
+          all = (bin ? mass_to[bin - 1] : 0) + __shfl(mass, max(n, 0), 64);
+        }
+        if (f.by_mass()) {
+          const u64 target = share_of(f, all);
+          bin = mass_bin(target);
+          const u64 to = bin ? mass_to[bin - 1] : 0, need = target > to ? target - to : 1;
+          // (the last of the bin, where roundings leave the sum below)
+          if (take(t.bin == bin && mass >= need && mass - t.units < need) < 0) {
+            uint64_t who = __ballot(t.bin == bin && lane < listed);
+            uint32_t most = 0;
+            for (uint64_t w = who; w; w &= w - 1) most = max(most, uint32_t(__builtin_amdgcn_readlane(int(count), __ffsll((long long)w) - 1)));
+            take(t.bin == bin && count == most);
+          }
+        }
+        if (lane == 0) lds.value = key, lds.before = u64(uint32_t(last)), lds.digit = uint32_t(bin);
       }
-      uint32_t most = 0, complement = 0;  // of the bin's keys
-      each([&](const Token& t) {
-        if (t.bin == bin) most = max(most, t.key), complement = max(complement, ~t.key);
-      });
-      most = group_max(most, lds.words);
-      complement = group_max(complement, lds.words + kWaves);
-      const u64 place = cut_bin(lds, bin, before, turn == 0, most, ~complement, each);
-      const uint32_t new_key = most - uint32_t(place >> kIndex);
-      const int new_last = int(place & kIndexes);
-      if (stays(new_key, new_last)) key = new_key, last = new_last;
+      __syncthreads();
+      key = uint32_t(lds.value), last = int(uint32_t(lds.before)), bin = int(lds.digit);
+    } else {
+#pragma unroll 1
+      for (int turn = counted ? 0 : 1; turn < (f.by_mass() ? 2 : 1); ++turn) {
+        u64 before;  // amounts, in the cut's bin, before the last that stays
+        if (turn == 0) {
+          bin = kbin;
+          before = count_before();
+        } else {
+          if (counted) {
+            u64 mine = 0;
+            each([&](const Token& t) {
+              if (t.bin == bin && stays(t.key, t.index)) mine += t.units;
+            });
+            all = group_sum(mine, lds.sums) + (bin ? mass_to[bin - 1] : 0);
+          }
+          const u64 target = share_of(f, all);
+          bin = mass_bin(target);
+          const u64 to = bin ? mass_to[bin - 1] : 0;
+          before = target > to ? target - to - 1 : 0;
+        }
+        uint32_t most = 0, complement = 0;  // of the bin's keys
+        each([&](const Token& t) {
+          if (t.bin == bin) most = max(most, t.key), complement = max(complement, ~t.key);
+        });
+        most = group_max(most, lds.words);
+        complement = group_max(complement, lds.words + kWaves);
+        const u64 place = cut_bin(lds, bin, before, turn == 0, most, ~complement, each);
+        const uint32_t new_key = most - uint32_t(place >> kIndex);
+        const int new_last = int(place & kIndexes);
+        if (stays(new_key, new_last)) key = new_key, last = new_last;
+      }
     }
     // what stays of each part: its whole bins, a wave for a part, then the listed tokens
     const int whole = min(bin, f.by_weight() ? e4 : kBins);
@@ -589,7 +667,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
       if (lane == 63 && v) atomicAdd(&part_mass[p], v);
     }
     each([&](const Token& t) {
-      if (t.bin < whole || !stays(t.key, t.index)) return;
+      if (t.bin < whole || t.bin >= kBins || !stays(t.key, t.index)) return;
       if (f.by_weight() && weight(exponent(s, plain(float(logits[t.index]))), table).units < least) return;
       atomicAdd(&part_mass[t.index / kPart], t.units);
     });
@@ -610,39 +688,35 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     mine = from * kLane;
     while (mine < (from + 1) * kLane - 1 && left >= part_mass[mine]) left -= part_mass[mine++];
   }
-  // and its tokens by index
-  u64 units[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach / 8; ++i) {
-    const int first = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8;
-    float x[8];
-    load8(logits, first, a.vocab, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double y = exponent(s, x[j]);
-      const Weight w = weight(y, table);
-      units[8 * i + j] = counts(y) && stays(key_of(x[j]), first + j) && w.units >= least ? w.whole() : 0;
-    }
-  }
-  u64 before = 0;  // of the pieces before
+  // and its tokens by index, kEach neighbours a thread
+  const int first = mine * kPart + int(threadIdx.x) * kEach;
+  u64 units[kEach], sum = 0;
   uint32_t latest = 0;
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i) {
-    const int first = mine * kPart + (i * kThreads + int(threadIdx.x)) * 8;
-    u64 sum = 0, all;
+    float x[8];
+    load8(logits, first + 8 * i, a.vocab, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      sum += units[8 * i + j];
-      if (units[8 * i + j]) latest = uint32_t(first + j) + 1;
+      const int n = 8 * i + j;
+      units[n] = 0;
+      const double y = exponent(s, x[j]);
+      if (stays(key_of(x[j]), first + n) && counts(y)) {
+        const Weight w = weight(y, table);
+        if (w.units >= least) units[n] = w.whole();
+      }
+      sum += units[n];
+      if (units[n]) latest = uint32_t(first + n) + 1;
     }
-    u64 at = before + group_scan(sum, lds.sums, all) - sum;
+  }
+  u64 all;
+  u64 at = group_scan(sum, lds.sums, all) - sum;
+  if (at <= left && left < at + sum) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const u64 w = units[8 * i + j];
-      if (at <= left && left < at + w) token = first + j;
-      at += w;
+    for (int n = 0; n < kEach; ++n) {
+      if (at <= left && left < at + units[n]) token = first + n;
+      at += units[n];
     }
-    before += all;
   }
   __syncthreads();
   if (token < 0) {  // (where roundings leave the number beyond the last token: that one)
@@ -660,7 +734,9 @@ hipError_t launch(const SampleArgs& a, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (a.top_k || a.top_p || a.min_p || a.top_k_all > 0 || a.top_p_all < 1 || a.min_p_all > 0) {
-    hipLaunchKernelGGL(sample_list_kernel<T>, grid, dim3(kThreads), 0, s, a);
+    // as many parts for a workgroup, which adds the row's bins first, as leave two workgroups a CU
+    const int each = std::min((a.parts * a.rows + 511) / 512, a.parts);
+    hipLaunchKernelGGL(sample_list_kernel<T>, dim3(unsigned((a.parts + each - 1) / each), unsigned(a.rows)), dim3(kThreads), 0, s, a, each);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
