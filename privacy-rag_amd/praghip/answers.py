@@ -2,19 +2,28 @@
 
 The reference computes its forward on shares; this serves the same shapes (model.hpp:63-64)
 to a party that may see the text, and shows the serving calls together: 4-bit projections
-(:func:`matvec_w4`), a prompt into the cache (:func:`page_reserve`, :func:`page_write`,
-:func:`paged_prompt`), several answers of one prompt (:func:`page_fork`), their tokens
-(:func:`paged_decode`), and their pages' way back (:func:`page_trim`, :func:`page_free`,
-:func:`page_compact`).  Norms, rotations and activations are torch's.
+(:func:`matvec_w4`), norms (:func:`add_norm`), a prompt into the cache (:func:`page_reserve`,
+:func:`page_append`, :func:`paged_prompt`), several answers of one prompt (:func:`page_fork`),
+their tokens (:func:`paged_shared` where they share enough, else :func:`paged_decode`), which
+:func:`sample_tokens` draws, and their pages' way back (:func:`page_trim`, :func:`page_free`,
+:func:`page_compact`).  Activations are torch's.
 
 ``python -m praghip.answers`` answers a synthetic prompt and prints its times.
 """
 from __future__ import annotations
 
-from .attention import page_write, paged_decode, paged_prompt
+from .append import page_append, rotary_table
+from .attention import paged_decode, paged_prompt, paged_shared
 from .matvec import matvec_w4, quantize_w4
+from .norm import add_norm
 from .pages import page_check, page_compact, page_fork, page_free, page_reserve, page_trim
 from .qwen3 import QWEN3_0_6B, Qwen3Shape
+from .sample import sample_tokens
+
+# Keys that a step reads once instead of once for each answer, from which on the attention of
+# shared prefixes is the faster one: eight answers over 256 tokens (1,792 keys) take 14 us of
+# 12, over 1,024 (7,168 keys) 14 of 15.5, over 8,192 18 of 51.
+_ENOUGH = 4096
 
 
 class Qwen3Answers:
@@ -25,18 +34,20 @@ class Qwen3Answers:
     "gate_up", "down": [out][in], "attention_norm", "mlp_norm": [hidden], "q_norm",
     "k_norm": [head_dim]}]} of one 16-bit type on one GPU; the projections are kept in
     4 bits, the output head is the embedding.  With a window every layer sees the last
-    `window` tokens and the first `sinks`, and pages that leave it are given back.
+    `window` tokens and the first `sinks`, and pages that leave it are given back.  rotary:
+    further arguments of :func:`rotary_table`, for contexts beyond those of the training.
     """
 
     def __init__(self, weights: dict, shape: Qwen3Shape = QWEN3_0_6B, *, slots: int = 16, pages: int = 1024,
                  page_size: int = 16, capacity: int = 8192, group: int = 128, window: int = 0, sinks: int = 0,
-                 theta: float = 1e6, eps: float = 1e-6):
+                 theta: float = 1e6, eps: float = 1e-6, rotary: dict | None = None):
         import torch
         self.shape, self.page_size, self.window, self.sinks, self.eps = shape, page_size, window, sinks, eps
-        self.group, self.embed, self.norm = group, weights["embed"].detach(), weights["norm"].detach()
+        self.group, self.embed = group, weights["embed"].detach()
         self.device, self.type = self.embed.device, self.embed.dtype
+        self.norm = self._norm(weights["norm"])
         self.head = quantize_w4(self.embed, group, zeros=True)
-        self.layers = [{name: quantize_w4(w, group, zeros=True) if w.dim() == 2 else w.detach() for name, w in layer.items()}
+        self.layers = [{name: quantize_w4(w, group, zeros=True) if w.dim() == 2 else self._norm(w) for name, w in layer.items()}
                        for layer in weights["layers"]]
         self.pool = torch.zeros((shape.layers, 2, pages, shape.kv_heads, page_size, shape.head_dim), dtype=self.type,
                                 device=self.device)
@@ -45,61 +56,82 @@ class Qwen3Answers:
         self.lengths, self.refs = torch.zeros(slots, **ints), torch.zeros(pages, **ints)
         self.status = torch.zeros(1, **ints)
         self.held = [0] * slots  # the lengths, as the host knows them
-        half = torch.arange(0, shape.head_dim, 2, dtype=torch.float64, device=self.device)
-        angle = torch.arange(self.tables.shape[1] * page_size, dtype=torch.float64, device=self.device)[:, None] * \
-            theta ** (-half / shape.head_dim)
-        self.cos, self.sin = angle.cos().float(), angle.sin().float()
+        # what forks have left in common: a state's number and its tokens, of which a sequence's
+        # first are the same as those of every other sequence with that number
+        self.marks, self.states, self.changes = [[] for _ in range(slots)], 0, 0
+        self.cos, self.sin = rotary_table(self.tables.shape[1] * page_size, shape.head_dim, theta=theta, device=self.device,
+                                          **(rotary or {}))
+
+    def _norm(self, weight):
+        """A norm's weights as the calls take them: of the model's type, together, aligned."""
+        w = weight.detach().to(self.type).contiguous()
+        return w if w.data_ptr() % 16 == 0 else w.clone()
 
     def _ints(self, values):
         import torch
         return torch.tensor(list(values), dtype=torch.int32).to(self.device)
 
-    def _normed(self, x, weight):
-        x = x.float()
-        return (x * (x.square().mean(-1, keepdim=True) + self.eps).rsqrt() * weight.float()).to(self.type)
-
-    def _turned(self, x, places):
-        import torch
-        a, b = x.float().chunk(2, -1)
-        cos, sin = self.cos[places][:, None], self.sin[places][:, None]
-        return torch.cat((a * cos - b * sin, b * cos + a * sin), -1).to(self.type)
-
     def _product(self, x, w):
         return matvec_w4(x, *w, group=self.group)
+
+    def _groups(self, sequences):
+        """(first of each run of neighbours that share a prefix, and the end; the tokens that
+        each shares; keys that are read once instead of for each)."""
+        groups, shared, saved, common = [0], [], 0, {}
+        for i, s in enumerate(sequences):
+            now = {state: n for state, n in common.items() if (state, n) in self.marks[s]} if i else {}
+            if i and not now:
+                groups.append(i)
+                shared.append(max(common.values(), default=0))
+            common = now or dict(self.marks[s])
+        groups.append(len(sequences))
+        shared.append(max(common.values(), default=0))
+        for a, b, n in zip(groups, groups[1:], shared):
+            saved += (b - a - 1) * n
+        return groups, shared, saved
 
     def _forward(self, sequences, rows):
         """Logits after the newest tokens, rows[i] of sequences[i], which have their pages already."""
         at = self._ints(sequences).long()
         ends = [sum(len(r) for r in rows[: i + 1]) for i in range(len(rows))]
-        places = self._ints(self.held[s] - len(r) + i for s, r in zip(sequences, rows) for i in range(len(r))).long()
-        x = self._layers(self._ints(t for r in rows for t in r).long(), places, self.tables[at], self.lengths[at],
-                         self._ints([0] + ends), max(len(r) for r in rows), max(self.held[s] for s in sequences))
+        most, together = max(len(r) for r in rows), None
+        if most == 1 and not self.window:
+            groups, shared, saved = self._groups(sequences)
+            if saved >= _ENOUGH:
+                together = self._ints(groups), self._ints(shared)
+        x = self._layers(self._ints(t for r in rows for t in r).long(), self.tables[at], self.lengths[at],
+                         self._ints([0] + ends), most, max(self.held[s] for s in sequences), together)
         return self._logits(x[self._ints(e - 1 for e in ends).long()])
 
-    def _layers(self, tokens, places, tables, lengths, starts, most: int, longest: int):
-        """The last layer's output of tokens at `places`, rows starts[s] .. of the sequences whose tables these are."""
+    def _layers(self, tokens, tables, lengths, starts, most: int, longest: int, together=None):
+        """The last layer's output, under the last norm, of the tokens that are rows starts[s] ..
+        of the sequences whose tables these are.  together: the groups and their shared tokens,
+        where single tokens' attention reads prefixes once."""
         import torch
-        shape = self.shape
+        shape, eps = self.shape, self.eps
         see = dict(window=self.window, sinks=self.sinks, max_length=longest)
-        q_out, kv_out = shape.q_heads * shape.head_dim, shape.kv_heads * shape.head_dim
+        heads = shape.q_heads, shape.kv_heads, shape.kv_heads
         x = self.embed[tokens]
-        for layer, (keys, values) in zip(self.layers, self.pool):
-            qkv = self._product(self._normed(x, layer["attention_norm"]), layer["qkv"])
-            q, k, v = (t.unflatten(1, (-1, shape.head_dim)) for t in qkv.split((q_out, kv_out, kv_out), 1))
-            q = self._turned(self._normed(q, layer["q_norm"]), places)
-            k = self._turned(self._normed(k, layer["k_norm"]), places)
-            page_write(k, v, keys, values, tables, lengths, starts)
-            if most == 1:
-                o = paged_decode(q, keys, values, tables, lengths, **see)
-            else:
+        norms = [layer["attention_norm"] for layer in self.layers] + [self.norm]
+        h = add_norm(x, norms[0], eps=eps)
+        for layer, norm, (keys, values) in zip(self.layers, norms[1:], self.pool):
+            q, k, v = self._product(h, layer["qkv"]).unflatten(1, (-1, shape.head_dim)).split(heads, 1)
+            q = page_append(q, k, v, keys, values, tables, lengths, starts, self.cos, self.sin, q_norm=layer["q_norm"],
+                            k_norm=layer["k_norm"], eps=eps)
+            if most > 1:
                 o = paged_prompt(q, keys, values, tables, lengths, starts, most, **see)
-            x = x + self._product(o.flatten(1), layer["o"])
-            gate, up = self._product(self._normed(x, layer["mlp_norm"]), layer["gate_up"]).chunk(2, 1)
-            x = x + self._product((torch.nn.functional.silu(gate.float()) * up.float()).to(self.type), layer["down"])
-        return x
+            elif together:
+                o = paged_shared(q, keys, values, tables, lengths, *together, max_length=longest)
+            else:
+                o = paged_decode(q, keys, values, tables, lengths, **see)
+            h, x = add_norm(self._product(o.flatten(1), layer["o"]), layer["mlp_norm"], x, eps=eps, total=x)
+            gate, up = self._product(h, layer["gate_up"]).chunk(2, 1)
+            h, x = add_norm(self._product((torch.nn.functional.silu(gate.float()) * up.float()).to(self.type), layer["down"]), norm,
+                            x, eps=eps, total=x)
+        return h
 
     def _logits(self, x):
-        return self._product(self._normed(x, self.norm), self.head)
+        return self._product(x, self.head)
 
     def extend(self, sequences, rows):
         """Appends rows[i], a list of one token or more, to sequences[i]; returns the logits
@@ -131,8 +163,9 @@ class Qwen3Answers:
         """A function that appends one token to each of these sequences, given as a list or a
         tensor of whole numbers (whose values outside the vocabulary count as its nearest), and
         returns the logits after them (in the same memory each time): the layers' calls, some
-        30 a layer, as one captured graph.  The sequences may be forked, ended and extended
-        between its calls."""
+        14 a layer, as one captured graph.  The sequences may be forked, ended and extended
+        between its calls.  Where they share enough when this is called, and there is no window,
+        the graph reads what neighbours in the list share once, as it is at each step."""
         import torch
         sequences = list(sequences)
         if not sequences or any(not 0 <= s < len(self.held) for s in sequences):
@@ -142,11 +175,21 @@ class Qwen3Answers:
         at, starts = listed.long(), self._ints(range(n + 1))
         tokens = torch.zeros(n, dtype=torch.int64, device=self.device)
 
+        together, changes = None, self.changes
+        if not self.window and self._groups(sequences)[2] >= _ENOUGH:
+            together = self._ints([0] * (n + 1)), self._ints([0] * n)
+
+        def share():
+            groups, shared, _ = self._groups(sequences)
+            together[0].copy_(self._ints(groups + [n] * (n + 1 - len(groups))))
+            together[1].copy_(self._ints(shared + [0] * (n - len(shared))))
+
+        if together:
+            share()
+
         def forward():
-            lengths = self.lengths[at]
-            places = (lengths - 1).clamp(min=0).long()
-            return self._logits(self._layers(tokens.clamp(0, self.embed.shape[0] - 1), places, self.tables[at], lengths,
-                                             starts, 1, capacity))
+            return self._logits(self._layers(tokens.clamp(0, self.embed.shape[0] - 1), self.tables[at], self.lengths[at], starts, 1,
+                                             capacity, together))
 
         held = self.lengths.clone()
         try:
@@ -167,13 +210,17 @@ class Qwen3Answers:
                 new = torch.tensor(new)
             if new.shape != (n,) or new.dtype not in whole:
                 raise ValueError("one whole number for each sequence")
+            nonlocal changes
             self._reserve(sequences, listed, ones, [1] * n)
             tokens.copy_(new)
+            if together and changes != self.changes:
+                share()
+                changes = self.changes
             graph.replay()
             self._trim(listed)
             return logits
 
-        step.reads = at, starts  # (the graph's addresses: they live as long as it does)
+        step.reads = at, starts, together  # (the graph's addresses: they live as long as it does)
         return step
 
     def fork(self, parent: int, children) -> None:
@@ -182,16 +229,22 @@ class Qwen3Answers:
         page_fork(self.pool, self.tables, self.lengths, self.refs, self._ints([parent] * len(children)),
                   self._ints(children), self.status)
         page_check(self.status)
+        marks = self.marks[parent]
+        if not any(n == self.held[parent] for _, n in marks):
+            marks.append((self.states, self.held[parent]))
+            self.states += 1
+        self.changes += 1
         for child in children:
-            self.held[child] = self.held[parent]
+            self.held[child], self.marks[child] = self.held[parent], list(marks)
 
     def end(self, sequences) -> None:
         """Empties sequences."""
         sequences = list(sequences)
         page_free(self.tables, self.lengths, self.refs, self._ints(sequences), self.status)
         page_check(self.status)
+        self.changes += 1
         for s in sequences:
-            self.held[s] = 0
+            self.held[s], self.marks[s] = 0, []
 
     def compact(self) -> None:
         """Moves the held pages to the pool's front."""
@@ -226,6 +279,10 @@ def main() -> None:
     parser.add_argument("--answers", type=int, default=8)
     parser.add_argument("--tokens", type=int, default=32, help="tokens of each answer")
     parser.add_argument("--window", type=int, default=0)
+    parser.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest token")
+    parser.add_argument("--top-k", type=int, default=0)
+    parser.add_argument("--top-p", type=float, default=1.0)
+    parser.add_argument("--min-p", type=float, default=0.0)
     args = parser.parse_args()
     per = -(-(args.prompt + args.tokens) // 16)
     model = Qwen3Answers(random_weights(), slots=1 + args.answers, pages=per * (1 + args.answers), window=args.window,
@@ -248,17 +305,21 @@ def main() -> None:
         logits = timed("prompt", lambda: model.extend([0], [prompt]))
         answers = range(1, 1 + args.answers)
         timed("fork", lambda: model.fork(0, answers))
-        tokens = logits[0].topk(args.answers).indices.tolist()
-        said = [[t] for t in tokens]
+        draw = dict(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
+        numbers = torch.rand((args.tokens, args.answers), generator=torch.Generator().manual_seed(2)).to("cuda")
+        if args.temperature:
+            tokens = sample_tokens(logits[:1].expand(args.answers, -1), numbers[-1], **draw)
+        else:
+            tokens = logits[0].topk(args.answers).indices
+        said = [tokens]
         step = timed("capture", lambda: model.steps(answers))
-        for _ in range(args.tokens - 1):
-            tokens = timed("token", lambda: step(tokens).argmax(-1).tolist())
-            for s, t in zip(said, tokens):
-                s.append(t)
+        for u in numbers[:-1]:
+            tokens = timed("token", lambda: sample_tokens(step(tokens), u, **draw))
+            said.append(tokens)
         timed("end", lambda: model.end(range(0, 1 + args.answers)))
     for name, t in times.items():
         print(f"{name:8s} {1e3 * sorted(t)[len(t) // 2]:8.3f} ms")
-    print("answers begin", [s[:4] for s in said])
+    print("answers begin", torch.stack(said, 1)[:, :4].tolist())
 
 
 if __name__ == "__main__":
