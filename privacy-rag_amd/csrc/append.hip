@@ -7,8 +7,15 @@
 // Bytes bound it: each value is read and written once.  A wave takes one token (whose
 // sequence and place are then the same for its lanes: scalar loads and a scalar search) and
 // `heads_each` of its heads, 16 bytes a lane: 8, 16 or 32 lanes a head, whose squares are
-// summed by lane exchanges.  The other value of a pair that is half a rotation away is read
-// a second time, which a cache answers; pairs of neighbours are in one lane.
+// summed by lane exchanges.  The other value of a pair that is half a rotation away comes from
+// its lane (read from memory a second time, 4 x 2048 tokens took 42 us instead of 34), or,
+// where the half is no multiple of eight, value by value from memory; pairs of neighbours are
+// in one lane.
+//
+// From 16 MiB of results on, half of what the L2s hold, stores pass the caches by: a kernel's
+// end waits for the dirty lines (4 x 2048 tokens of 16 heads of 128 over 8: 26 us, 5.3 TB/s,
+// where a large copy has 5.1, and 34 through the caches; with the attention after it, which then
+// reads more from memory, both take 139 us).
 #include "append.hpp"
 
 #include <algorithm>
@@ -31,7 +38,7 @@ __device__ __forceinline__ void widen8(u32x4 x, float (&s)[8]) {
 
 // LANES of a head; HALVES: 0 for pairs of neighbours, 1 for pairs half a rotation apart in
 // whole pieces of eight, 2 where the half is no multiple of eight.
-template <typename T, int LANES, int HALVES>
+template <typename T, int LANES, int HALVES, bool PAST>
 __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int waves_each, int heads_each) {
   constexpr int kHeads = 64 / LANES;  // of a wave at a time
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -71,6 +78,10 @@ __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int wave
 #pragma unroll
         for (int n = 0; n < 4; ++n) cs[j + n] = c4[n], sn[j + n] = d < a.half ? -s4[n] : s4[n];
       }
+    } else if (HALVES == 0 && d + 8 <= 2 * a.half) {
+      const f32x4 c4 = *reinterpret_cast<const f32x4_any*>(c + d / 2), s4 = *reinterpret_cast<const f32x4_any*>(s + d / 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j] = c4[j / 2], sn[j] = j & 1 ? s4[j / 2] : -s4[j / 2];
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -113,16 +124,9 @@ __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int wave
         for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
       } else if constexpr (HALVES == 1) {
         const int other = d < a.half ? d + a.half : d - a.half;
+        const int at = (lane / LANES * LANES + (d < 2 * a.half ? other >> 3 : 0)) << 2;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = 0;
-        if (d < 2 * a.half) {
-          widen8<T>(*reinterpret_cast<const u32x4*>(from + other), y);
-          if (norm) {
-            widen8<T>(*reinterpret_cast<const u32x4*>(norm + other), w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= by * w[j];
-          }
-        }
+        for (int j = 0; j < 8; ++j) y[j] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(at, __builtin_bit_cast(int, x[j])));
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -135,18 +139,32 @@ __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int wave
       for (int j = 0; j < 4; ++j)
         got[j] = pack2<T>(x[2 * j] * cs[2 * j] + y[2 * j] * sn[2 * j], x[2 * j + 1] * cs[2 * j + 1] + y[2 * j + 1] * sn[2 * j + 1]);
     }
-    if (has && (is_q || page >= 0)) *reinterpret_cast<u32x4*>(to + d) = got;
+    if (has && (is_q || page >= 0)) {
+      if constexpr (PAST)
+        __builtin_nontemporal_store(got, reinterpret_cast<u32x4*>(to + d));
+      else
+        *reinterpret_cast<u32x4*>(to + d) = got;
+    }
   }
 }
 
-template <typename T, int LANES>
-hipError_t launch(const AppendArgs& a, hipStream_t s) {
+template <typename T, int LANES, bool PAST>
+hipError_t launch_past(const AppendArgs& a, hipStream_t s) {
   const int all = a.heads + 2 * a.kv_heads, turn = 64 / LANES;
+  // Four turns a wave where there are tokens enough (one: 47 us instead of 42; eight: 47), one
+  // for short calls, whose latency counts.
   const int turns = (all + turn - 1) / turn;
   const int each = a.tokens >= 512 ? std::min(turns, 4) : 1, waves = (turns + each - 1) / each;
-  const auto kernel = a.interleaved ? page_append_kernel<T, LANES, 0> : a.half % 8 ? page_append_kernel<T, LANES, 2> : page_append_kernel<T, LANES, 1>;
+  const auto kernel = a.interleaved   ? page_append_kernel<T, LANES, 0, PAST>
+                      : a.half % 8 ? page_append_kernel<T, LANES, 2, PAST>
+                                   : page_append_kernel<T, LANES, 1, PAST>;
   hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(a.tokens) * waves + 3) / 4)), dim3(256), 0, s, a, waves, each * turn);
   return hipGetLastError();
+}
+template <typename T, int LANES>
+hipError_t launch(const AppendArgs& a, hipStream_t s) {
+  const int64_t bytes = int64_t(a.tokens) * (a.heads + 2 * a.kv_heads) * a.dim * 2;
+  return bytes >= (16 << 20) ? launch_past<T, LANES, true>(a, s) : launch_past<T, LANES, false>(a, s);
 }
 template <typename T>
 hipError_t launch_dim(const AppendArgs& a, hipStream_t s) {

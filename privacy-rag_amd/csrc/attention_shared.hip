@@ -313,8 +313,11 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
   const bool few = per_group <= 1 && per_seq == 1;
   if (few) {  // all loads at once; what they depend on is in the lanes
     const bool has = lane < a.count;
-    const int begin = has ? a.groups[lane] : 0, stop = has ? a.groups[lane + 1] : 0, shared = has ? a.shared[lane] : 0;
-    const int length = lane < c.seqs ? length_of(c, lane) : 0;
+    int begin = 0, stop = 0, shared = 0;
+    if (a.count > 0) {  // (all lanes load, as others read them)
+      begin = a.groups[min(lane, a.count)], stop = a.groups[min(lane + 1, a.count)], shared = a.shared[min(lane, a.count - 1)];
+    }
+    const int length = length_of(c, min(lane, c.seqs - 1));
     const int first = min(max(begin, 0), c.seqs), end = min(max(stop, first), c.seqs);
     const int longest = __shfl(length, min(first, 63), 64);
     last_p = {first, (end - first) * c.group, 0, end - first > 1 ? min(max(shared, 0), longest) : 0};

@@ -559,7 +559,10 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     for (int i = 0; i < kHeld; ++i) {
       const int n = i * kThreads + threadIdx.x;
       held[i].bin = -1;
-      if (n < listed) held[i] = token_of(int(list[n]));
+      if (i * kThreads < listed) {  // (all lanes load, as others read them)
+        held[i] = token_of(int(list[min(n, listed - 1)]));
+        if (n >= listed) held[i].bin = -1;
+      }
     }
     const auto each = [&](auto with) {
 #pragma unroll
