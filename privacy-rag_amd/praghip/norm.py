@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import struct
 
+from . import attention
 from ._lib import check, lib, shape_error
 from .attention import _kind, _no_gradients, _result, _stream, _type_error
 
@@ -40,7 +41,7 @@ def add_norm(x, weight, residual=None, *, eps: float = 1e-6, out=None, total=Non
     made = []
     for t in (out, total):
         if t is None:
-            t = x.new_empty(shape) if stream is None else _result(stream, index, x.new_empty, shape)
+            t = attention._torch.empty_like(x) if stream is None else _result(stream, index, attention._torch.empty_like, x)
         elif t.shape != shape or t.dtype is not type or t.get_device() != index or (n > 1 and t.stride(1) != 1):
             raise shape_error("E_NORM_OUT")
         made.append(t)
