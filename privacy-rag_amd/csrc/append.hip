@@ -121,12 +121,15 @@ __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int wave
       }
       if constexpr (HALVES == 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j ^ 1];
+        for (int j = 0; j < 8; ++j) y[j] = d + j < 2 * a.half ? x[j ^ 1] : 0.f;  // (infinite ones times 0 are NaN)
       } else if constexpr (HALVES == 1) {
         const int other = d < a.half ? d + a.half : d - a.half;
         const int at = (lane / LANES * LANES + (d < 2 * a.half ? other >> 3 : 0)) << 2;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(at, __builtin_bit_cast(int, x[j])));
+        for (int j = 0; j < 8; ++j) {
+          const float v = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(at, __builtin_bit_cast(int, x[j])));
+          y[j] = d < 2 * a.half ? v : 0.f;
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

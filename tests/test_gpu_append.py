@@ -103,6 +103,23 @@ def test_shapes(gpu, heads, kv, dim, half, interleaved):
         check(make([1, 7, 0, 20], [40, 0, 3, 13], heads, kv, dim, half, type, seed=dim + half, norms=norms), interleaved)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("half", [16, 20, 21])
+def test_infinities_stay_in_their_pairs(gpu, half, interleaved):
+    """A head's first values are turned; infinite ones reach no value behind them."""
+    m = make([4], [9], 4, 2, 64, half, BF16, seed=half, norms=(False, False))
+    finite = m["q"].clone()
+    m["q"][:, 1, 0], m["q"][:, 2, 2 * half - 1], m["k"][:, 0, 1] = float("inf"), float("-inf"), float("nan")
+    cache = [p.cuda() for p in m["pools"]]
+    rest = [m[x].cuda() for x in ("tables", "lengths", "starts", "cos", "sin")]
+    got = praghip.page_append(m["q"].cuda(), m["k"].cuda(), m["v"].cuda(), *cache, *rest, interleaved=interleaved).cpu()
+    assert torch.equal(got[..., 2 * half:], finite[..., 2 * half:])
+    place = m["tables"][0, 0]  # of positions 9 .. 12
+    assert torch.equal(cache[0][place, :, 9:13].transpose(0, 1).cpu()[..., 2 * half:], m["k"][..., 2 * half:])
+    others = [h for h in range(4) if h not in (1, 2)]
+    assert bool(got[:, others].isfinite().all())
+
+
 @pytest.mark.parametrize("norms", [(True, False), (False, True)])
 def test_one_norm(gpu, norms):
     check(make([3, 2], [5, 16], 4, 2, 64, 32, F16, seed=1, norms=norms), eps=1e-3)
