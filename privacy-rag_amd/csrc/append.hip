@@ -27,6 +27,8 @@ namespace {
 
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
+constexpr unsigned kSlab = 1 << 18;  // workgroups of a grid's row: a launch has below 2^32 threads in one dimension
+
 template <typename T>
 __device__ __forceinline__ void widen8(u32x4 x, float (&s)[8]) {
 #pragma unroll
@@ -41,8 +43,9 @@ __device__ __forceinline__ void widen8(u32x4 x, float (&s)[8]) {
 template <typename T, int LANES, int HALVES, bool PAST>
 __global__ void __launch_bounds__(256) page_append_kernel(AppendArgs a, int waves_each, int heads_each) {
   constexpr int kHeads = 64 / LANES;  // of a wave at a time
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int token = wave / waves_each, part = wave - token * waves_each;
+  const int lane = threadIdx.x & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane((blockIdx.y * kSlab + blockIdx.x) * 4 + (threadIdx.x >> 6));
+  const int token = int(wave / uint32_t(waves_each)), part = int(wave) - token * waves_each;
   if (token >= a.tokens) return;
   int lo = 0, hi = a.seqs - 1;  // the last sequence that starts at or before the token
   while (lo < hi) {
@@ -161,7 +164,8 @@ hipError_t launch_past(const AppendArgs& a, hipStream_t s) {
   const auto kernel = a.interleaved   ? page_append_kernel<T, LANES, 0, PAST>
                       : a.half % 8 ? page_append_kernel<T, LANES, 2, PAST>
                                    : page_append_kernel<T, LANES, 1, PAST>;
-  hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(a.tokens) * waves + 3) / 4)), dim3(256), 0, s, a, waves, each * turn);
+  const unsigned groups = unsigned((int64_t(a.tokens) * waves + 3) / 4);
+  hipLaunchKernelGGL(kernel, dim3(std::min(groups, kSlab), (groups + kSlab - 1) / kSlab), dim3(256), 0, s, a, waves, each * turn);
   return hipGetLastError();
 }
 template <typename T, int LANES>

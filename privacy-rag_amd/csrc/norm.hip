@@ -14,10 +14,16 @@
 // then hold counts once, and both write the same to it.
 #include "norm.hpp"
 
+#include <algorithm>
+
 #include "attention.hpp"
 
 namespace praghip {
 namespace {
+
+// Workgroups of a grid's row: a launch has below 2^32 threads in one dimension.
+constexpr int64_t kSlab = 1 << 18;
+__device__ __forceinline__ int64_t group_index() { return int64_t(blockIdx.y) * kSlab + blockIdx.x; }
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));  // 16 bytes at any address of 16-bit data
 
@@ -80,8 +86,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_norm_kernel
   __shared__ float lds[16];
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
   const int t = threadIdx.x % THREADS;
-  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / THREADS;
-  if (kRows > 1 && row >= a.rows) return;
+  const int64_t row = group_index() * kRows + threadIdx.x / THREADS;
+  if (row >= a.rows) return;  // (a whole wave's, or the workgroup's)
   const T *x = static_cast<const T*>(a.x) + row * a.x_row, *r = static_cast<const T*>(a.residual) + row * a.residual_row;
   u32x4 xs[CHUNKS], rs[CHUNKS], w[CHUNKS];
 #pragma unroll
@@ -127,7 +133,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) add_norm_kernel
 template <typename T>
 __global__ void __launch_bounds__(1024) add_norm_any_kernel(NormArgs a) {
   __shared__ float lds[16];
-  const int64_t row = blockIdx.x;
+  const int64_t row = group_index();
+  if (row >= a.rows) return;
   const T *x = static_cast<const T*>(a.x) + row * a.x_row, *r = static_cast<const T*>(a.residual) + row * a.residual_row;
   T *out = static_cast<T*>(a.out) + row * a.out_row, *total = static_cast<T*>(a.total) + row * a.total_row;
   const auto summed = [&](int i, float(&s)[8]) {
@@ -157,17 +164,19 @@ __global__ void __launch_bounds__(1024) add_norm_any_kernel(NormArgs a) {
   }
 }
 
+dim3 grid_of(int64_t groups) { return dim3(unsigned(std::min(groups, kSlab)), unsigned((groups + kSlab - 1) / kSlab)); }
+
 template <typename T, int THREADS, int CHUNKS>
 void launch_held(const NormArgs& a, hipStream_t s) {
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
   hipLaunchKernelGGL((a.residual ? add_norm_kernel<T, THREADS, CHUNKS, true> : add_norm_kernel<T, THREADS, CHUNKS, false>),
-                     dim3(unsigned((a.rows + kRows - 1) / kRows)), dim3(THREADS < 256 ? 256 : THREADS), 0, s, a);
+                     grid_of((a.rows + kRows - 1) / kRows), dim3(THREADS < 256 ? 256 : THREADS), 0, s, a);
 }
 
 template <typename T>
 hipError_t launch(const NormArgs& a, hipStream_t s) {
   if (a.n < 8 || a.n > 1024 * 32)
-    hipLaunchKernelGGL((add_norm_any_kernel<T>), dim3(unsigned(a.rows)), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((add_norm_any_kernel<T>), grid_of(a.rows), dim3(1024), 0, s, a);
   else if (a.n <= 512)
     launch_held<T, 64, 1>(a, s);
   else if (a.n <= 1024)

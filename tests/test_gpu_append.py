@@ -284,3 +284,20 @@ def test_refusals(gpu):
     refused("E_ATTENTION_GRADIENT", k_norm=w.clone().requires_grad_())
     with torch.no_grad():
         assert not praghip.page_append(q.clone().requires_grad_(), *dev[1:]).requires_grad
+
+
+def test_more_workgroups_than_a_grid_row_has_threads_for(gpu):
+    """2^24 workgroups of 256 threads; all but the last tokens stand before position 0."""
+    tokens, type = 2 ** 26 + 5, BF16
+    m = make([3], [0], 1, 1, 8, 4, type, seed=5)
+    q, k, v = (m[x][:1].cuda().expand(tokens, 1, 8) for x in ("q", "k", "v"))
+    cache = [torch.zeros_like(p).cuda() for p in m["pools"]]
+    starts = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    out = torch.full((tokens, 1, 8), 5.0, dtype=type, device="cuda")
+    praghip.page_append(q, k, v, *cache, m["tables"].cuda(), m["lengths"].cuda(), starts, m["cos"].cuda(), m["sin"].cuda(), out=out)
+    assert bool((out[:-2] == q[:-2]).all())  # (position 0 turns nothing)
+    for at in (1, 2):
+        want, size = turned(q[0].cpu(), None, m["cos"][at], m["sin"][at], False, 0)
+        assert bool(((out[at - 3].cpu().double() - want).abs() <= UNIT[type] * want.abs() + SUMS * size).all())
+    page = m["tables"][0, 0]
+    assert bool((cache[1][page, 0, :3] == v[0, 0]).all()) and not bool(cache[1][page, 0, 3:].any())

@@ -152,3 +152,15 @@ def test_refusals(gpu):
         with torch.no_grad():
             assert not F(*some)[0].requires_grad
     assert F(x[:0], w, r[:0])[0].shape == (0, 64) and F(x[:, :0], w[:0]).shape == (4, 0)
+
+
+@pytest.mark.parametrize("rows,n", [(2 ** 22 + 3, 1), (2 ** 26 + 5, 8)])
+def test_more_workgroups_than_a_grid_row_has_threads_for(gpu, rows, n):
+    """2^22 workgroups of 1024 threads, and 2^24 of 256."""
+    print("[norm]", rows, n, flush=True)
+    x, w, _ = make(1024, n, torch.bfloat16, seed=n)
+    want = praghip.add_norm(x, w)
+    check(x, w, None)
+    index = torch.arange(rows, device="cuda") % 1000
+    got = praghip.add_norm(x[index], w)
+    assert torch.equal(got, want[index])
