@@ -82,10 +82,10 @@ struct Scale {
   double top, by, from;  // w = 2^((x - top) by + from), from in [-1, 0]
   double anchor;
 };
-__device__ __forceinline__ Scale scale_of(float top, float temperature) {
+__device__ __forceinline__ Scale scale_by(float top, double by) {
   Scale s;
   s.top = top;
-  s.by = 1.4426950408889634074 / fmax(double(temperature), 1e-30);
+  s.by = by;
   // (written out as one product and one addition: both kernels are to have the same bits.  Of
   // products beyond 2^52, whose fraction is lost, any distance is right: their tokens are
   // equal or too far apart to count)
@@ -93,6 +93,8 @@ __device__ __forceinline__ Scale scale_of(float top, float temperature) {
   s.from = fmax(fmin(__builtin_fma(s.top, s.by, -s.anchor), 0.), -1.);
   return s;
 }
+__device__ __forceinline__ double degrees(float temperature) { return fmax(double(temperature), 1e-30); }
+__device__ __forceinline__ Scale scale_of(float top, float temperature) { return scale_by(top, 1.4426950408889634074 / degrees(temperature)); }
 // 2^y in units of 2^-kBits and its bin, of y in (-kRange, 0]: y in 1/256 by a table of their
 // powers, the rest by the exponential series (its fourth term is below 2^-42).
 struct Weight {
@@ -321,11 +323,16 @@ constexpr uint32_t kIndexes = (1u << kIndex) - 1;
 
 // ---------------------------------------------------------- tokens of the cuts' bins
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, int parts_each) {
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, int parts_each, int groups) {
   __shared__ u64 sums[kWaves], mass_to[kBins];
   __shared__ uint32_t words[kWaves], count_to[kBins], base;
   __shared__ int edges[6], aways[kParts];
-  const int row = blockIdx.y;
+  __shared__ float limits[3 * kParts][2];
+  // Workgroups go to the eight XCDs in turn: eight rows at a time take turns too, so that a row's
+  // are on one, whose L2 then reads the row's bins once (with rows one after the other 55 us for
+  // 53).
+  const int turn = int(blockIdx.x) / (8 * groups), within = int(blockIdx.x) - turn * 8 * groups;
+  const int some = min(a.rows - turn * 8, 8), row = turn * 8 + within % some, group = within / some;
   const T* logits = static_cast<const T*>(a.logits) + row * a.row;
   const SamplePart* parts = a.part + row * a.parts;
   const Filters f = filters_of(a, row);
@@ -385,8 +392,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, int
     if (m >= most && m - mass < most) edges[3] = threadIdx.x;
     __syncthreads();
   }
-  const int e0 = edges[0], e1 = edges[1], e2 = edges[2], e3 = edges[3], e4 = edges[4], e5 = edges[5];
-  if (blockIdx.x == 0) {  // for the draw
+  if (group == 0) {  // for the draw
     if (int(threadIdx.x) < kBins) {
       a.mass_to[size_t(row) * kBins + threadIdx.x] = m;
       a.count_to[size_t(row) * kBins + threadIdx.x] = n;
@@ -394,20 +400,24 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, int
     if (threadIdx.x < 8) a.edges[size_t(row) * 8 + threadIdx.x] = threadIdx.x < 6 ? edges[threadIdx.x] : int(counted);
   }
   // Tokens whose logit may be in one of those bins, by 32 bits and a little room on both sides
-  // (where that is no number, all of them): the draw looks at the few by 64.
-  const int edge[6] = {e0, e1, e2, e3, e4, e5};
-  for (int part = blockIdx.x * parts_each; part < min(int(blockIdx.x + 1) * parts_each, a.parts); ++part) {
-    const int away = aways[part];
-    if (away == kRange) continue;
-    const Scale own = scale_of(parts[part].top, f.temperature);
-    const double room = 1e-6 * (fabs(own.top) + 50 / own.by);
+  // (where that is no number, all of them): the draw looks at the few by 64.  The limits of this
+  // workgroup's parts are some threads' each (by all threads, 64-bit products took longer than
+  // the tokens).
+  const int begin = group * parts_each, end = min(begin + parts_each, a.parts);
+  if (int(threadIdx.x) < 3 * (end - begin)) {
+    const int part = begin + int(threadIdx.x) / 3, r = int(threadIdx.x) % 3;
+    const int first = edges[2 * r], last = edges[2 * r + 1], away = aways[part];
+    const Scale own = scale_by(parts[part].top, s.by);
+    const double each = 0.69314718055994531 * degrees(f.temperature), room = 1e-6 * (fabs(own.top) + 50 * each);
+    limits[threadIdx.x][0] = first > last ? kNegInf : float(own.top + ((-16. * (first - 16 * away) + 0.5) / 256 - own.from) * each + room);
+    limits[threadIdx.x][1] = first > last ? -kNegInf : float(own.top + ((-16. * (last - 16 * away) - 15.5) / 256 - own.from) * each - room);
+  }
+  __syncthreads();
+  for (int part = begin; part < end; ++part) {
+    if (aways[part] == kRange) continue;
     float upper[3], lower[3];
 #pragma unroll
-    for (int r = 0; r < 3; ++r) {
-      upper[r] = float(own.top + ((-16. * (edge[2 * r] - 16 * away) + 0.5) / 256 - own.from) / own.by + room);
-      lower[r] = float(own.top + ((-16. * (edge[2 * r + 1] - 16 * away) - 15.5) / 256 - own.from) / own.by - room);
-      if (edge[2 * r] > edge[2 * r + 1]) upper[r] = kNegInf, lower[r] = -kNegInf;
-    }
+    for (int r = 0; r < 3; ++r) upper[r] = limits[3 * (part - begin) + r][0], lower[r] = limits[3 * (part - begin) + r][1];
     uint32_t found = 0;  // a bit for each of the thread's tokens
 #pragma unroll
     for (int i = 0; i < kEach / 8; ++i) {
@@ -738,9 +748,9 @@ hipError_t launch(const SampleArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   if (a.top_k || a.top_p || a.min_p || a.top_k_all > 0 || a.top_p_all < 1 || a.min_p_all > 0) {
     // as many parts for a workgroup, which adds the row's bins first, as leave one workgroup a CU
-    // (64 rows of 155,648, all filters: 60 us for the call; with two a CU 63)
-    const int each = std::min((a.parts * a.rows + 255) / 256, a.parts);
-    hipLaunchKernelGGL(sample_list_kernel<T>, dim3(unsigned((a.parts + each - 1) / each), unsigned(a.rows)), dim3(kThreads), 0, s, a, each);
+    // (64 rows of 155,648, all filters: 53 us for the call; with two a CU 56)
+    const int each = std::min((a.parts * a.rows + 255) / 256, a.parts), groups = (a.parts + each - 1) / each;
+    hipLaunchKernelGGL(sample_list_kernel<T>, dim3(unsigned(groups * a.rows)), dim3(kThreads), 0, s, a, each, groups);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
