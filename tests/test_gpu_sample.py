@@ -215,6 +215,19 @@ def test_a_captured_call(gpu):
         assert got.tolist() == [plain(logits[i], f32(u[i]), f32(0.8), seed - 9, f32(0.9)) for i in range(9)]
 
 
+def test_logits_and_workspace_beyond_32_bits(gpu):
+    """2.2 x 10^9 logits, whose candidates' list is 8.7 GB: the same tokens as row by row."""
+    rows, vocab = 14000, 155648
+    g = torch.Generator(device="cuda").manual_seed(4)
+    logits = torch.empty((rows, vocab), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    uniform = torch.rand(rows, device="cuda", generator=g)
+    draw = dict(temperature=0.9, top_k=5000, top_p=0.9, min_p=1e-4)
+    got = praghip.sample_tokens(logits, uniform, **draw)
+    for first in (0, rows // 2, rows - 300):
+        some = slice(first, first + 300)
+        assert torch.equal(got[some], praghip.sample_tokens(logits[some], uniform[some], **draw))
+
+
 def test_refusals(gpu):
     logits, u = torch.zeros((3, 40), device="cuda"), torch.zeros(3, device="cuda")
 
