@@ -20,11 +20,11 @@
 // and one transposition of V.  The join kernel adds the pieces in order, so results do not
 // depend on timing.
 //
-// Measured, with the join (29 and 36 us the kernel, 6 and 7 the join): 64 sequences over one
-// prefix of 8,192 keys and up to 512 of their own, 16 heads of 128 over 8, 42 us for 103 MB,
-// where attention_decode.hip takes 310; five groups of 1 to 12 over prefixes of
-// up to 30,000, 32 heads of 64 over 4, 35 us for 114 MB (85).  The prefix of the first is 128 columns, four waves that each
-// read the same keys: its loads from the caches, and its products beside them, are what is left.
+// Measured, with the join (7 and 6 us of it): 64 sequences over one prefix of 8,192 keys and up
+// to 512 of their own, 16 heads of 128 over 8, 41 us for 103 MB, where attention_decode.hip takes
+// 310; five groups of 1 to 12 over prefixes of up to 30,000, 32 heads of 64 over 4, 34 us for
+// 114 MB (85).  The prefix of the first is 128 columns, four waves that each read the same keys:
+// its loads from the caches, and its products beside them, are what is left.
 // Columns of 64 a wave halve those loads, but leave registers for one wave a SIMD (62 us for 42),
 // and keys staged in LDS are read as often from there (no gain).
 #include "attention.hpp"
@@ -140,11 +140,16 @@ struct Column {
   }
 };
 
-// The workgroups for the prefixes, as their share of the units is.
+// The workgroups for the prefixes, as their share of the work is: a unit of theirs takes about a
+// quarter longer, most of them with two tiles of columns (groups of 5, 1, 9 and 2 over 8,192 keys,
+// 512 of their own: 29 us for 33 at the same weight; 64 over 8,192 41.6 for 42.9; 8 over 2,048,
+// one tile, and 2,048 of their own 18.9 for 18.2; at half as much again 64 over 32,768 98 for 88).
 __device__ __forceinline__ uint32_t prefix_groups(uint32_t prefix, uint32_t own, uint32_t groups) {
   if (!prefix || !own || groups < 2) return prefix ? groups : 0;
   const int less = max(0, 9 - int(__clz(prefix | own)));  // (below 2^23 each, whose products with groups 32 bits hold)
-  const uint32_t all = (prefix >> less) + (own >> less), n = (groups * (prefix >> less) + all / 2) / max(all, 1u);
+  prefix >>= less, own >>= less;
+  prefix += prefix >> 2;
+  const uint32_t all = prefix + own, n = (groups * prefix + all / 2) / max(all, 1u);
   return min(max(n, 1u), groups - 1);
 }
 
