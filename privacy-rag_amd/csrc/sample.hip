@@ -15,14 +15,14 @@
 //   parts are added by shifting;
 // * list: workgroups of some parts add the row's bins, find those in which a cut falls, and
 //   append their tokens of those bins to the row's list;
-// * draw: a workgroup a row cuts the listed bins by value and index (digits of 10 bits of both
-//   together), adds what stays of each part, takes the part that the random number falls into
+// * draw: a workgroup a row cuts the listed bins by value and index (few tokens by comparing each
+//   with every other, more by digits of 10 bits of both together), adds what stays of each part, takes the part that the random number falls into
 //   and goes through that one by index.
 // The order of the list changes nothing: sums are of integers, and cuts are by value and index.
 //
 // Measured: 64 flat rows of 155,648 logits of 32 bits, cut by their sum, 54 us (16 + 19 + 20 by
 // kernel; 16 bits without filters 22, where their bytes are 4); 8 rows of 16 bits with all
-// filters 27 to 31; one of 32,768 21 (5 + 7 + 10).  Beside the launches, the chains of a row's cuts and its last part are
+// filters 25 to 31; one of 32,768 21 (5 + 7 + 9).  Beside the launches, the chains of a row's cuts and its last part are
 // what is left, on one workgroup a row.
 #include "sample.hpp"
 
@@ -460,7 +460,11 @@ struct Scratch {
   uint32_t digit;
   u64 before, value;
 };
-constexpr int kHeld = 4;  // listed tokens that a thread holds (beyond them they are read again)
+constexpr int kHeld = 4;   // listed tokens that a thread holds (beyond them they are read again)
+// Up to so many listed tokens are compared each with every other, by all threads (8 rows of
+// 155,648 25 us for 27 by one wave's lanes, 64 rows of 16,384 24 for 33 by digits; at 256, 8 rows
+// of 16,384 cut by their sum take 27 for 24).
+constexpr int kFew = 128;
 
 // Listed tokens: an index, the logit's key, the bin, the units.
 struct Token {
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int n = i * kThreads + threadIdx.x;
-      held[i].bin = -1;
+      held[i] = {0, -1, 0, 0};
       if (i * kThreads < listed) {  // (all lanes load, as others read them)
         held[i] = token_of(int(list[min(n, listed - 1)]));
         if (n >= listed) held[i].bin = -1;
@@ -597,52 +601,64 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
       while (b < e3 && mass_to[b] < target) ++b;
       return b;
     };
-    if (listed <= 64) {
-      // a wave has them all, in its lanes: each token's order in its bin by looking at every other
-      if (wave == 0) {
-        const Token& t = held[0];
-        u64 mass = 0;
-        uint32_t count = 0;
-        for (int n = 0; n < listed; ++n) {
-          const uint32_t k = uint32_t(__builtin_amdgcn_readlane(int(t.key), n));
-          const int i = __builtin_amdgcn_readlane(t.index, n), b = __builtin_amdgcn_readlane(t.bin, n);
-          const u64 units = u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.units)), n))) |
-                            u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(t.units >> 32)), n))) << 32;
-          if (b == t.bin && (k > t.key || (k == t.key && i <= t.index))) {
-            mass += units;
-            ++count;
-          }
-        }
-        const auto take = [&](bool mine) {
-          const uint64_t who = __ballot(mine && lane < listed);
-          if (!who) return -1;
-          const int n = __ffsll((long long)who) - 1;
-          const uint32_t k = uint32_t(__builtin_amdgcn_readlane(int(t.key), n));
-          const int i = __builtin_amdgcn_readlane(t.index, n);
-          if (stays(k, i)) key = k, last = i;
-          return n;
-        };
-        if (counted) {
-          bin = kbin;
-          const int n = take(t.bin == bin && count == uint32_t(count_before()) + 1);
-          all = (bin ? mass_to[bin - 1] : 0) + __shfl(mass, max(n, 0), 64);
-        }
-        if (f.by_mass()) {
-          const u64 target = share_of(f, all);
-          bin = mass_bin(target);
-          const u64 to = bin ? mass_to[bin - 1] : 0, need = target > to ? target - to : 1;
-          // (the last of the bin, where roundings leave the sum below)
-          if (take(t.bin == bin && mass >= need && mass - t.units < need) < 0) {
-            uint64_t who = __ballot(t.bin == bin && lane < listed);
-            uint32_t most = 0;
-            for (uint64_t w = who; w; w &= w - 1) most = max(most, uint32_t(__builtin_amdgcn_readlane(int(count), __ffsll((long long)w) - 1)));
-            take(t.bin == bin && count == most);
-          }
-        }
-        if (lane == 0) lds.value = key, lds.before = u64(uint32_t(last)), lds.digit = uint32_t(bin);
+    if (listed <= kFew) {
+      // Sums up to each token in its bin: `width` threads have a token each, as have the next ones,
+      // which look at others; the order is one number, the larger first.
+      const int width = listed <= 64 ? 64 : kFew, mine = int(threadIdx.x) & (width - 1);
+      if (int(threadIdx.x) < kFew) {
+        lds.amount[threadIdx.x] = 0, lds.amount[kFew + threadIdx.x] = held[0].units;
+        lds.amount[2 * kFew + threadIdx.x] = u64(held[0].key) << 32 | ~uint32_t(held[0].index);
+        lds.count[threadIdx.x] = 0, lds.count[kFew + threadIdx.x] = uint32_t(held[0].bin);
       }
       __syncthreads();
-      key = uint32_t(lds.value), last = int(uint32_t(lds.before)), bin = int(lds.digit);
+      const u64 order = lds.amount[2 * kFew + mine], units = lds.amount[kFew + mine];
+      const int own_bin = int(lds.count[kFew + mine]);
+      if (mine < listed) {
+        u64 part = 0;
+        uint32_t some = 0;
+#pragma unroll 4
+        for (int n = int(threadIdx.x) / width; n < listed; n += kThreads / width) {
+          const bool before = (int(lds.count[kFew + n]) == own_bin) & (lds.amount[2 * kFew + n] >= order);
+          part += before ? lds.amount[kFew + n] : 0, some += before;
+        }
+        if (some) atomicAdd(&lds.amount[mine], part), atomicAdd(&lds.count[mine], some);
+      }
+      __syncthreads();
+      const bool has = int(threadIdx.x) < listed;
+      const u64 mass = has ? lds.amount[mine] : 0;  // up to it, in its bin
+      const uint32_t count = has ? lds.count[mine] : 0;
+      // cuts behind the token of the one thread whose it is; returns whether there is one
+      u64 reached = 0;
+      const auto take = [&](bool own) {
+        if (threadIdx.x == 0) lds.digit = 0;
+        __syncthreads();
+        if (own) lds.digit = 1, lds.value = order, lds.before = mass;
+        __syncthreads();
+        const bool found = lds.digit != 0;
+        if (found) {
+          const uint32_t k = uint32_t(lds.value >> 32);
+          const int i = int(~uint32_t(lds.value));
+          reached = lds.before;
+          if (stays(k, i)) key = k, last = i;
+        }
+        __syncthreads();
+        return found;
+      };
+      if (counted) {
+        bin = kbin;
+        take(has && own_bin == bin && count == uint32_t(count_before()) + 1);
+        all = (bin ? mass_to[bin - 1] : 0) + reached;
+      }
+      if (f.by_mass()) {
+        const u64 target = share_of(f, all);
+        bin = mass_bin(target);
+        const u64 to = bin ? mass_to[bin - 1] : 0, need = target > to ? target - to : 1;
+        const bool own = has && own_bin == bin;
+        if (!take(own && mass >= need && mass - units < need)) {  // (the last of the bin, where roundings leave the sum below)
+          const uint32_t most = group_max(own ? count : 0, lds.words);
+          take(own && count == most);
+        }
+      }
     } else {
 #pragma unroll 1
       for (int turn = counted ? 0 : 1; turn < (f.by_mass() ? 2 : 1); ++turn) {

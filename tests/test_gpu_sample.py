@@ -130,6 +130,21 @@ def test_few_values(gpu):
         check(logits, u, **filters)
 
 
+@pytest.mark.parametrize("near", [1, 2, 63, 64, 65, 127, 128, 129, 300, 1100, 5000])
+def test_tokens_near_a_cut(gpu, near):
+    """So many logits within 1/100, some of them equal, among lower ones: cuts fall among them."""
+    print("[sample] near a cut", near, flush=True)
+    g = torch.Generator().manual_seed(near)
+    logits = torch.randn((6, 12000), generator=g) - 9
+    for row in logits:
+        row[torch.randperm(12000, generator=g)[:near]] = 2 + torch.randint(0, 40, (near,), generator=g) / 4000
+    u = torch.rand(6, generator=g).tolist()
+    some = max(1, near // 2)
+    for filters in ({"top_k": 1}, {"top_k": some}, {"top_k": near}, {"top_k": near + 3}, {"top_p": 0.3}, {"top_p": 0.6, "top_k": some},
+                    {"top_p": 0.99, "top_k": near}, {"top_k": some, "top_p": 0.5, "min_p": f32(0.995)}):
+        check(logits, u, **filters)
+
+
 def test_masked_and_values_that_are_no_numbers(gpu):
     inf, nan, low = math.inf, math.nan, float(torch.finfo(BF16).min)
     logits, u = make(10, 20000, BF16, seed=3)
