@@ -323,6 +323,13 @@ __device__ __forceinline__ int away_of(const Scale& row, const SamplePart& part)
   const double d = row.anchor - part.anchor;
   return d < kRange ? int(d) : kRange;
 }
+// A sum of weights in units of their part's largest, as one of the row's units, in which the tokens
+// are drawn: nothing where the part's largest weight rounds to none of them (it is half a unit or
+// less, and so is the rest), and one at least where it does not, so that a part that is drawn has
+// a token with a unit, and one that has none is not drawn.
+__device__ __forceinline__ u64 of_row(const Scale& row, u64 sum, float top, int away) {
+  return sum && exponent(row, top) > -(kBits + 1) ? max(u64(1), sum >> away) : 0;
+}
 constexpr int kIndex = 20;  // bits of a token's index
 constexpr uint32_t kIndexes = (1u << kIndex) - 1;
 
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     aways[threadIdx.x] = away;
     tops[threadIdx.x] = part.top;
     from[threadIdx.x] = scale_of(part.top, f.temperature).from;
-    if (!f.any()) part_mass[threadIdx.x] = away < kRange ? part.mass >> away : 0;
+    if (!f.any()) part_mass[threadIdx.x] = of_row(s, part.mass, part.top, away);
   }
   if (threadIdx.x == 0) token = -1;
   __syncthreads();
@@ -694,11 +701,10 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     // what stays of each part: its whole bins, a wave for a part, then the listed tokens
     const int whole = min(bin, f.by_weight() ? e4 : kBins);
     for (int p = wave; p < a.parts; p += kWaves) {
-      const int away = aways[p];
       u64 v = 0;
-      for (int b = lane; b < min(whole - 16 * away, kBins); b += 64) v += a.mass[(size_t(row) * a.parts + p) * kBins + b] >> away;
+      for (int b = lane; b < min(whole - 16 * aways[p], kBins); b += 64) v += a.mass[(size_t(row) * a.parts + p) * kBins + b];
       v = wave_scan(v, Sum());
-      if (lane == 63 && v) atomicAdd(&part_mass[p], v);
+      if (lane == 63 && v) atomicAdd(&part_mass[p], of_row(s, v, tops[p], aways[p]));
     }
     each([&](const Token& t) {
       if (t.bin < whole || t.bin >= kBins || !stays(t.key, t.index)) return;
@@ -725,7 +731,6 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
   // and its tokens by index, kEach neighbours a thread
   const int first = mine * kPart + int(threadIdx.x) * kEach;
   u64 units[kEach], sum = 0;
-  uint32_t latest = 0;
 #pragma unroll
   for (int i = 0; i < kEach / 8; ++i) {
     float x[8];
@@ -740,11 +745,14 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
         if (w.units >= least) units[n] = w.whole();
       }
       sum += units[n];
-      if (units[n]) latest = uint32_t(first + n) + 1;
     }
   }
   u64 all;
   u64 at = group_scan(sum, lds.sums, all) - sum;
+  // (the part's sum and that of its tokens' rounded units differ a little: the number keeps its
+  // distance from the nearer end, so that the first and the last token are drawn at theirs)
+  const u64 behind = part_mass[mine] - left;
+  left = left < behind ? min(left, all - 1) : all - min(all, behind);
   if (at <= left && left < at + sum) {
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
@@ -753,12 +761,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a) {
     }
   }
   __syncthreads();
-  if (token < 0) {  // (where roundings leave the number beyond the last token: that one)
-    latest = group_max(latest, lds.words);
-    if (threadIdx.x == 0) a.out[row] = int64_t(latest) - 1;
-  } else if (threadIdx.x == 0) {
-    a.out[row] = token;
-  }
+  if (threadIdx.x == 0) a.out[row] = token;
 }
 
 template <typename T>
