@@ -12,8 +12,8 @@
 // * own keys by single waves, as in attention_decode.hip, but with no LDS: pieces of a head
 //   that several waves have part of go to the workspace;
 // * a prefix's keys by whole workgroups.  All its sequences' heads of one key/value head are
-//   columns, spread over 1, 2, 4 or 8 waves of 32 columns each, which read the same keys one
-//   soon after the other (a cache answers); the others take every 8th, 4th or 2nd block, and
+//   columns, spread over 1, 2, 4 or 8 waves of 32 columns each (16 in rows of more than 128 values),
+//   which read the same keys one soon after the other (a cache answers); the others take every 8th, 4th or 2nd block, and
 //   waves that have the same columns add up through LDS.  A workgroup has at most two pieces
 //   of heads that it shares with others.
 // The products are attention_decode.hip's, with two tiles of 16 columns for one load of K and V
@@ -35,6 +35,11 @@ namespace {
 template <int D>
 struct SharedShape {
   static constexpr int waves = D > 128 ? 4 : 8;  // (rows of 256 values take more than 256 registers)
+  // Tiles of 16 columns that a wave has.  Two of them in rows of 256 values take more registers
+  // than there are, so that some are kept in accumulator registers: where the compiler copies one
+  // there while only some lanes are active, the others' value is lost (tests/test_asm_spills.py).  One
+  // is faster too: 8 sequences over 4,000 keys, 8 heads of 256 over 2, 22.7 us for 27.6, 32 31 for 37.
+  static constexpr int tiles = D > 128 ? 1 : 2, columns = 16 * tiles;
   static constexpr int steps = D / 32;           // of the first product
   static constexpr int per = D / 16;             // values of a key's row that a lane holds
   static constexpr int words = per / 2;
@@ -86,12 +91,13 @@ __device__ __forceinline__ Entry own_of(const SharedArgs& a, int s, int& group) 
 
 // How many parts a head's columns are cut into, waves (a power of two) that have the columns
 // of one part at the same time, units of one part of one head.
+template <typename S>
 struct Parts {
   int parts, shift;
   uint32_t units;
-  __device__ __forceinline__ Parts(bool prefix, int columns, int blocks, int group_waves) {
-    shift = prefix ? (columns > 32) + (columns > 64) + (columns > 128 && group_waves == 8) : 0;
-    parts = prefix ? (columns + 32 * group_waves - 1) / (32 * group_waves) : (columns + 15) >> 4;
+  __device__ __forceinline__ Parts(bool prefix, int columns, int blocks) {
+    shift = prefix ? (columns > S::columns) + (columns > 2 * S::columns) + (columns > 4 * S::columns && S::waves == 8) : 0;
+    parts = prefix ? (columns + S::columns * S::waves - 1) / (S::columns * S::waves) : (columns + 15) >> 4;
     units = blocks ? (uint32_t(blocks) << shift) + (prefix ? kPrefixStart : kOwnStart) : 0;
   }
   __device__ __forceinline__ uint32_t all(int kv_heads) const { return units * parts * kv_heads; }
@@ -157,7 +163,8 @@ __device__ __forceinline__ uint32_t prefix_groups(uint32_t prefix, uint32_t own,
 // for 16 TILES columns from column0 on: o, m and l as of keys in powers of two.
 template <typename T, int D, bool EXACT, int TILES>
 __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x, int h, int column0, int first, int last, int step,
-                                            f32x4 (&o)[2][D / 16], float (&m)[2], float (&l)[2]) {
+                                            f32x4 (&o)[SharedShape<D>::tiles][D / 16], float (&m)[SharedShape<D>::tiles],
+                                            float (&l)[SharedShape<D>::tiles]) {
   using S = SharedShape<D>;
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
@@ -288,13 +295,14 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
   for (int t = 0; t < TILES; ++t) l[t] = sum32(sum16(l[t]));
 }
 
-// A lane's rows of o, and m and l, at `to` (for the 32 columns of a wave).
+// A lane's rows of o, and m and l, at `to` (for the columns of a wave).
 template <int D>
-__device__ __forceinline__ void store_columns(float* to, int columns, const f32x4 (&o)[2][D / 16], const float (&m)[2], const float (&l)[2]) {
+__device__ __forceinline__ void store_columns(float* to, int columns, const f32x4 (&o)[SharedShape<D>::tiles][D / 16],
+                                              const float (&m)[SharedShape<D>::tiles], const float (&l)[SharedShape<D>::tiles]) {
   using S = SharedShape<D>;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < S::tiles; ++t) {
     if (16 * t + col >= columns) continue;
     float* p = to + (16 * t + col) * S::row;
 #pragma unroll
@@ -313,7 +321,7 @@ template <typename T, int D, bool EXACT>
 __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kernel(SharedArgs a) {
   using S = SharedShape<D>;
   constexpr int W = S::waves;
-  extern __shared__ __attribute__((aligned(16))) float lds[];  // [W][32] rows
+  extern __shared__ __attribute__((aligned(16))) float lds[];  // [W][columns] rows
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = c.kv_heads * c.group;
 
@@ -343,18 +351,18 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
         group = part ? g : -1;
       }
     }
-    if (has) mine_p = Parts(true, last_p.columns, last_p.blocks(), W).all(c.kv_heads);
-    if (lane < c.seqs) mine_o = Parts(false, last_o.columns, last_o.blocks(), W).all(c.kv_heads);
+    if (has) mine_p = Parts<S>(true, last_p.columns, last_p.blocks()).all(c.kv_heads);
+    if (lane < c.seqs) mine_o = Parts<S>(false, last_o.columns, last_o.blocks()).all(c.kv_heads);
   } else {
     for (int i = 0; i < per_group; ++i)
       if (lane * per_group + i < a.count) {
         const Entry x = prefix_of(a, lane * per_group + i);
-        mine_p += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
+        mine_p += Parts<S>(true, x.columns, x.blocks()).all(c.kv_heads);
       }
     for (int i = 0; i < per_seq; ++i)
       if (lane * per_seq + i < c.seqs) {
         const Entry x = own_of(a, lane * per_seq + i, group);
-        mine_o += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+        mine_o += Parts<S>(false, x.columns, x.blocks()).all(c.kv_heads);
       }
   }
   const uint32_t sum_p = wave_scan(mine_p), sum_o = wave_scan(mine_o);  // inclusive
@@ -369,12 +377,12 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
       for (int e = lane * per_group; e < min((lane + 1) * per_group, a.count); ++e) {
         const Entry x = prefix_of(a, e);
         a.entries[e] = uint4{at_p, uint32_t(x.blocks()), uint32_t(x.first), uint32_t(x.columns)};
-        at_p += Parts(true, x.columns, x.blocks(), W).all(c.kv_heads);
+        at_p += Parts<S>(true, x.columns, x.blocks()).all(c.kv_heads);
       }
       for (int e = lane * per_seq; e < min((lane + 1) * per_seq, c.seqs); ++e) {
         const Entry x = own_of(a, e, group);
         a.entries[a.count + e] = uint4{at_o, uint32_t(x.blocks()), uint32_t(group), uint32_t(x.columns)};
-        at_o += Parts(false, x.columns, x.blocks(), W).all(c.kv_heads);
+        at_o += Parts<S>(false, x.columns, x.blocks()).all(c.kv_heads);
       }
     }
   }
@@ -405,28 +413,30 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
            __builtin_amdgcn_readfirstlane(x.hi)};
     }
     const int nb = x.blocks();
-    const Parts parts(!kind, x.columns, nb, W);
+    const Parts<S> parts(!kind, x.columns, nb);
     const uint32_t all = parts.all(c.kv_heads);
     while (u < min(u_end, base + all)) {
-      const int index = int((u - base) / parts.units), h = parts.parts == 1 ? index : index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 16 : 32 * W);
+      const int index = int((u - base) / parts.units), h = parts.parts == 1 ? index : index / parts.parts, column0 = (index - h * parts.parts) * (kind ? 16 : S::columns * W);
       const uint32_t start = base + index * parts.units + (kind ? kOwnStart : kPrefixStart), stop = min(u_end, base + (index + 1) * parts.units);
       const int first = blocks_before(u, start, parts.shift), end = blocks_before(stop, start, parts.shift);
       u = stop;
       if (first >= end) continue;
-      f32x4 o[2][S::per];
-      float m[2] = {kNegInf, kNegInf}, l[2] = {0, 0};
+      f32x4 o[S::tiles][S::per];
+      float m[S::tiles], l[S::tiles];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < S::tiles; ++t) {
+        m[t] = kNegInf, l[t] = 0;
 #pragma unroll
         for (int j = 0; j < S::per; ++j) o[t][j] = f32x4{0, 0, 0, 0};
+      }
       const bool complete = first == 0 && end == nb;
       const int cw = 1 << parts.shift, kw = kind ? 1 : W >> parts.shift, part = kind ? 0 : wave >> parts.shift;
-      const int mine0 = kind ? column0 : column0 + (wave & (cw - 1)) * 32;
+      const int mine0 = kind ? column0 : column0 + (wave & (cw - 1)) * S::columns;
       if (mine0 < x.columns && first + part < end) {
-        if (kind || x.columns <= 16)
+        if (S::tiles == 1 || kind || x.columns <= 16)
           take_blocks<T, D, EXACT, 1>(a, x, h, mine0, first + part, end, kw, o, m, l);
-        else
-          take_blocks<T, D, EXACT, 2>(a, x, h, mine0, first + part, end, kw, o, m, l);
+        else if constexpr (S::tiles > 1)
+          take_blocks<T, D, EXACT, S::tiles>(a, x, h, mine0, first + part, end, kw, o, m, l);
       }
       if (kind) {
         float* to = complete ? a.rows + ((int64_t(c.seqs) + x.first) * heads + h * c.group + column0) * S::row
@@ -436,18 +446,18 @@ __global__ void __launch_bounds__(SharedShape<D>::waves * 64) paged_shared_kerne
       }
       // the sums of waves that have the same columns
       __syncthreads();  // the rows of the head before have been read
-      store_columns<D>(lds + wave * 32 * S::row, x.columns - mine0, o, m, l);
+      store_columns<D>(lds + wave * S::columns * S::row, x.columns - mine0, o, m, l);
       __syncthreads();
-      const int have = min(x.columns - column0, 32 * cw), waves = min(kw, end - first);
+      const int have = min(x.columns - column0, S::columns * cw), waves = min(kw, end - first);
       float* const to = complete ? a.rows : a.pieces + (int64_t(mine_at) * 2 + (start >= u_begin)) * a.columns * S::row;
 #pragma unroll 2
       for (int i = threadIdx.x; i < have * (D / 4); i += W * 64) {
         const int column = i / (D / 4), d = i % (D / 4) * 4;
-        const float* from = lds + column * S::row;  // (32 columns a wave, one wave's after the other's)
+        const float* from = lds + column * S::row;  // (one wave's columns after the other's)
         float top = from[D], ls = from[D + 1];
         f32x4 sums = *reinterpret_cast<const f32x4*>(from + d);
         for (int n = 1; n < waves; ++n) {
-          const float* p = from + n * cw * 32 * S::row;
+          const float* p = from + n * cw * S::columns * S::row;
           const float m = p[D], l = p[D + 1], most = fmaxf(top, m);
           const f32x4 o = *reinterpret_cast<const f32x4*>(p + d);
           const float f0 = __builtin_amdgcn_exp2f(top - origin(most)), f1 = __builtin_amdgcn_exp2f(m - origin(most));
@@ -488,9 +498,9 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned
   for (int kind = 0; kind < 2; ++kind) {
     if (kind == 0 && int(own.z) < 0) continue;
     const uint4 x = kind ? own : a.entries[own.z];
-    const int nb = int(x.y), columns = int(x.w), cut = kind ? 16 : 32 * W;
+    const int nb = int(x.y), columns = int(x.w), cut = kind ? 16 : S::columns * W;
     if (!nb) continue;
-    const Parts parts(!kind, columns, nb, W);
+    const Parts<S> parts(!kind, columns, nb);
     const Stretches stretches = kind ? Stretches(totals.y, (workgroups - prefixes) * W, kOwnLeast) : Stretches(totals.x, prefixes, kPrefixLeast);
     const int column = (kind ? 0 : (s - int(x.z)) * c.group) + head - kvh * c.group;
     const uint32_t start = x.x + (uint32_t(kvh) * parts.parts + column / cut) * parts.units + (kind ? kOwnStart : kPrefixStart);
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs a, unsigned
 template <typename T, int D>
 hipError_t launch(const SharedArgs& a, unsigned workgroups, hipStream_t s) {
   using S = SharedShape<D>;
-  constexpr size_t lds = size_t(S::waves) * 32 * S::row * sizeof(float);
+  constexpr size_t lds = size_t(S::waves) * S::columns * S::row * sizeof(float);
   const auto kernel = a.c.dim == D ? paged_shared_kernel<T, D, true> : paged_shared_kernel<T, D, false>;
   hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(S::waves * 64), lds, s, a);
   hipError_t e = hipGetLastError();
@@ -566,7 +576,9 @@ unsigned shared_workgroups(size_t entries, size_t kv_heads, size_t group, size_t
 size_t shared_own_columns(size_t group) { return std::min<size_t>(group, 16); }
 size_t shared_waves(size_t dim) { return dim > 128 ? SharedShape<256>::waves : SharedShape<128>::waves; }
 size_t shared_columns(size_t seqs, size_t group, size_t dim) {
-  return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? 4 * 32 : 8 * 32);
+  using Wide = SharedShape<256>;
+  using Narrow = SharedShape<128>;
+  return std::min<size_t>((seqs * group + 31) / 32 * 32, dim > 128 ? Wide::waves * Wide::columns : Narrow::waves * Narrow::columns);
 }
 // an exact i / group of i below seqs * group as a product's upper half, or 0
 uint32_t shared_inverse(size_t seqs, size_t group) {

@@ -137,7 +137,8 @@ SharedPlan shared_plan(const praghip_cache& c, size_t heads, size_t count, size_
   p.bytes = p.own_pieces + p.workgroups * shared_waves(c.head_dim) * 2 * p.own_columns * row;
   return p;
 }
-// units of all entries in 32 bits: a head's columns occupy no more waves than two for each 32
+// units of all entries in 32 bits: a head's columns occupy no more waves than one for each 16 of
+// them, in rows of more than 128 values than one for each 8, whose units are then below 2^32
 bool units_fit(const praghip_cache& c, size_t heads, size_t count) {
   const size_t blocks = size_t(capacity_of(c.table_width, c.page_size)) / 32 + 9;  // (a head's start counts as some)
   return count <= (1u << 20) && (count + c.seqs) * c.kv_heads * ((heads / c.kv_heads + 31) / 16) <= (size_t(1) << 31) / blocks;
