@@ -28,6 +28,7 @@
 // Columns of 64 a wave halve those loads, but leave registers for one wave a SIMD (62 us for 42),
 // and keys staged in LDS are read as often from there (no gain).
 #include "attention.hpp"
+#include "shared_rule.hpp"
 
 namespace praghip {
 namespace {
@@ -185,8 +186,8 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
   }
   const int32_t* named = c.tables + x.first * c.table_stride;
   const int most = int(c.capacity >> c.page_shift) - 1;
-  const auto page_at = [&](int key) { return named[min(key >> c.page_shift, most)]; };
-  int next[2] = {page_at((x.begin() + first) << 5), page_at(((x.begin() + first) << 5) + 16)};
+  const auto page_at = [&](int block, int half) { return named[entry_at(x.begin() + block, half, c.page_shift, most)]; };
+  int next[2] = {page_at(first, 0), page_at(first, 1)};
   for (int i = first; i < last; i += step) {
     const int kb = (x.begin() + i) << 5;
     u32x4 kf[2][S::steps];
@@ -235,7 +236,7 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
     }
     // (the next block's entries, beside these loads; past the last they are the table's last)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) next[t] = page_at(((x.begin() + i + step) << 5) + 16 * t);
+    for (int t = 0; t < 2; ++t) next[t] = page_at(i + step, t);
     const bool whole = page_ok[0] && page_ok[1] && kb >= x.lo && kb + 32 <= x.hi;
     u32x4 ph[TILES], pl[TILES];
 #pragma unroll
