@@ -176,6 +176,16 @@ __device__ __forceinline__ float sum16(float x) {
   return t.a + t.b;
 }
 
+// Scores in powers of two of which 32 bits hold no fraction below 2^-3.  The exponent of one is the
+// difference of two numbers that are rounded alike (half a step of 2^24 is twice a probability,
+// half a step of 2^31 2^128 times it), and its origin the maximum itself: in float16 what it lies
+// below that could be some steps.
+constexpr float kLarge = 1 << 20;
+template <typename T>
+__device__ __forceinline__ float below_most(float top) {  // how far an origin is kept below a maximum
+  return Half<T>::most > 0 && __builtin_fabsf(top) < kLarge ? Half<T>::most : 0.f;
+}
+
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kNegInf = -__builtin_inff();
 

@@ -261,7 +261,16 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
         }
       }
       float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      top = fmaxf(m[t], max32(max16(top)) * c.scale - Half<T>::most);
+      const float most = max32(max16(top));
+      float by = c.scale;
+      top = most * c.scale - Half<T>::most;
+      if (__any(__builtin_fabsf(top) >= kLarge)) {  // scores and their maximum, rounded alike
+        by = 1, top = most * c.scale;
+        top -= below_most<T>(top);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] *= c.scale;
+      }
+      top = fmaxf(m[t], top);
       if (__any(top > m[t])) {
         const float f = __builtin_amdgcn_exp2f(m[t] - origin(top));
         l[t] *= f;
@@ -273,7 +282,7 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
       const float from = -origin(m[t]);
 #pragma unroll
       for (int r = 0; r < 8; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c.scale, from)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], c.scale, from));
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], by, from)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], by, from));
         l[t] += p0 + p1;
         hi[r / 2] = pack2<T>(p0, p1);
         rest[r / 2] = pack2<T>(p0 - low<T>(hi[r / 2]), p1 - high<T>(hi[r / 2]));
