@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_decode_kernel(DecodeArgs a)
           }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        top = fmaxf(m, max32(max16(top)) - Half<T>::most);
+        top = max32(max16(top));
+        top = fmaxf(m, top - below_most<T>(top));
         if (__any(top > m)) {
           const float f = __builtin_amdgcn_exp2f(m - origin(top));
           l *= f;

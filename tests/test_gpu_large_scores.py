@@ -84,3 +84,14 @@ def test_a_score_that_overflows_in_a_shared_prefix(gpu):
     c = make(BF16, 130, 64, 1)
     out = praghip.paged_shared(*(c[x].cuda() for x in ("q", "k", "v", "tables", "lengths", "groups", "shared")))
     assert not bool(out[:, ::2].isfinite().any()) and bool(out[:, 1::2].isfinite().all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("type,size", SIZES)
+@pytest.mark.parametrize("scale", [0.7, -0.7])
+def test_single_tokens(gpu, type, size, dim, scale):
+    print("[large] single", type, size, dim, scale, flush=True)
+    c = make(type, size, dim, 1 if scale > 0 else -1)
+    want = attention(c, c["q"], [0, 1, 2, 3], scale)
+    out, lse = praghip.paged_decode(*(c[x].cuda() for x in ("q", "k", "v", "tables", "lengths")), scale=scale, lse=True)
+    compare(out, lse, *want, type, False)
