@@ -43,7 +43,7 @@ namespace {
 
 constexpr int kRing = 4;      // tiles of K, and of V, in LDS
 constexpr int kGroups = 512;  // groups of 16 keys whose addresses are in LDS, by halves
-constexpr int kFlags = 64;    // bytes of LDS beside them
+constexpr int kFlags = 64;    // bytes of LDS beside them, and four a thread
 // keys of a tile
 template <int D>
 constexpr int tile_keys() {
@@ -89,7 +89,7 @@ __device__ __forceinline__ void raise(float top, f32x16 (&o)[B], float& m, float
   const Two both = swap32(top);
   top = __builtin_elementwise_maximum(both.a, both.b);
   if (__any((top - m) * scale > kSlack<T> + kLift<T>)) {
-    top = __builtin_elementwise_maximum(kLift<T> > 0 ? top - lower : top, m);
+    top = __builtin_elementwise_maximum(kLift<T> > 0 && !(__builtin_fabsf(top) * scale >= kLarge) ? top - lower : top, m);
     const float f = __builtin_amdgcn_exp2f((m - origin(top)) * scale);
     l *= f;
 #pragma unroll
@@ -386,18 +386,25 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
   // others' P of 0 makes NaN.  Where O is not finite it is formed again from the cache, with
   // the maximum known: 32 keys at a time, those with such values one by one, each added where
   // the row sees it.  (8192 tokens that see an infinity take 2 ms.  In the loop above the same
-  // test took 3% of every long prompt's time.)
+  // test took 3% of every long prompt's time.)  So are O and l where a score is so large that the
+  // rounded product of m and the scale, which the loop's exponents have, is no origin for them
+  // (there a test took 1% to 5%).
   bool finite = true;
 #pragma unroll
   for (int b = 0; b < blocks32; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) finite &= __builtin_fabsf(o[b][r]) < __builtin_inff();
+  finite &= !(__builtin_fabsf(origin(m)) * c.scale >= kLarge);
   if (__any(!finite)) {
+    // (l in LDS: a register for it here is one that the loop above lacks, which in rows of 256
+    // values took a fifth longer)
+    const Lds sum = flags + kFlags + 4 * (64 * wave + 32 * half + col);
+    *lds_at<float>(sum) = 0;
 #pragma unroll
     for (int b = 0; b < blocks32; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[b][r] = 0;
-    const float base = -origin(m) * c.scale;
+    const float m0 = origin(m);
 #pragma unroll 1
     for (int x = i0 * (TK / 32); x < i1 * (TK / 32); ++x) {
       const int kb = blocks.at(x / (TK / 32)) * TK + 32 * (x % (TK / 32));
@@ -430,8 +437,12 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const bool sees = seen(8 * (r >> 2) + 4 * half + (r & 3));
-        score[r] = sees ? __builtin_amdgcn_exp2f(fmaf(score[r], c.scale, base)) : 0.f;
+        score[r] = sees ? __builtin_amdgcn_exp2f((score[r] - m0) * c.scale) : 0.f;
       }
+      float some = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) some += score[r];
+      *lds_at<float>(sum) += some;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         u32x4 p;
@@ -473,6 +484,7 @@ __global__ void __launch_bounds__(NW * 64, NW / 4) paged_prompt_kernel(PromptArg
         }
       }
     }
+    l = *lds_at<float>(sum);
   }
   l = sum32(l);
   m *= c.scale;
@@ -570,7 +582,7 @@ int tiles_of(size_t max_rows, size_t group, size_t dim) {
 template <typename T, int D, int NW>
 hipError_t launch(const PromptArgs& a, hipStream_t s) {
   const int ntile = tiles_of(a.max_rows, a.c.group, a.c.dim);
-  const size_t lds = size_t(2) * kRing * tile_keys<D>() * D * sizeof(T) + 16 * kGroups + kFlags;
+  const size_t lds = size_t(2) * kRing * tile_keys<D>() * D * sizeof(T) + 16 * kGroups + kFlags + 4 * 64 * NW;
   const auto kernel = a.c.dim == D ? paged_prompt_kernel<T, D, NW, true> : paged_prompt_kernel<T, D, NW, false>;
   const unsigned groups = unsigned(ntile) * a.c.seqs * a.c.kv_heads;
   hipLaunchKernelGGL(kernel, dim3(groups * a.splits), dim3(NW * 64), lds, s, a, ntile);

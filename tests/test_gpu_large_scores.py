@@ -95,3 +95,34 @@ def test_single_tokens(gpu, type, size, dim, scale):
     want = attention(c, c["q"], [0, 1, 2, 3], scale)
     out, lse = praghip.paged_decode(*(c[x].cuda() for x in ("q", "k", "v", "tables", "lengths")), scale=scale, lse=True)
     compare(out, lse, *want, type, False)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("type,size", SIZES)
+@pytest.mark.parametrize("scale", [0.7, -0.7])
+def test_prompts(gpu, type, size, dim, scale):
+    print("[large] prompt", type, size, dim, scale, flush=True)
+    c = make(type, size, dim, 1 if scale > 0 else -1)
+    q = c["q"].repeat_interleave(20, 0)
+    starts = [0, 20, 40, 60]
+    want = attention(c, q, starts, scale)
+    first = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    out, lse = praghip.paged_prompt(q.cuda(), *(c[x].cuda() for x in ("k", "v", "tables", "lengths")), first, 20, scale=scale, lse=True)
+    compare(out, lse, *want, type, True)
+
+
+def test_a_prompt_with_an_infinity_among_large_scores(gpu):
+    """What is formed again from the cache (O that is not finite) takes the same exponents."""
+    c = make(BF16, 34, 64, 1)
+    q = c["q"].repeat_interleave(20, 0)
+    c["v"][int(c["tables"][0, 160 // 16]), 1, 0, 5] = float("inf")  # position 160 of the first sequence, as long as 190
+    starts = [0, 20, 40, 60]
+    out, _ = praghip.paged_prompt(q.cuda(), *(c[x].cuda() for x in ("k", "v", "tables", "lengths")),
+                                  torch.tensor(starts, dtype=torch.int32, device="cuda"), 20, scale=0.7, lse=True)
+    # all of its queries see that key, which the second key/value head's even queries take a share of
+    c["v"][int(c["tables"][0, 160 // 16]), 1, 0, 5] = 0
+    want, _, sums = attention(c, q, starts, 0.7)
+    held = torch.ones_like(want, dtype=torch.bool)
+    held[:20, 2:, 5] = False
+    assert not bool(out[:20, 2, 5].isfinite().any())
+    plain.check(torch.where(held, out.cpu().double(), want), want, sums, BF16, True)
