@@ -1,7 +1,7 @@
 // Rows of a root-mean-square norm, with the residual's addition before it:
 //   s = x + r,   y = s w / sqrt(mean s^2 + eps)
 // s is a 32-bit sum, rounded once where it is kept (total) and not at all where the norm
-// reads it; the mean is a 32-bit sum too.
+// reads it; the mean is a 32-bit sum too, of parts that are 64-bit ones in the widest rows.
 //
 // Bytes bound it: each of x, r, y and s moves once, so a row stays in registers between its
 // sum and its output.  A row of up to 2048 values is a wave's, whose sum takes lane
@@ -150,13 +150,17 @@ __global__ void __launch_bounds__(1024) add_norm_any_kernel(NormArgs a) {
       for (int j = 0; j < 8; ++j) s[j] += add[j];
     }
   };
-  float s[8], sum = 0;
+  // (a thread has up to 2^20 squares of a row: 32 bits lost up to 2^-6 of their sum)
+  float s[8];
+  double sum = 0;
   for (int64_t i = threadIdx.x * 8; i < a.n; i += 1024 * 8) {
     summed(int(i), s);
+    float some = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += s[j] * s[j];
+    for (int j = 0; j < 8; ++j) some += s[j] * s[j];
+    sum += some;
   }
-  const float by = factor(a, row_sum<1024>(sum, lds));
+  const float by = factor(a, row_sum<1024>(float(sum), lds));
   for (int64_t i = threadIdx.x * 8; i < a.n; i += 1024 * 8) {
     summed(int(i), s);
     float y[8];
