@@ -33,7 +33,8 @@ class Qwen3Answers:
     weights: {"embed": [vocab][hidden], "norm": [hidden], "layers": [{"qkv", "o",
     "gate_up", "down": [out][in], "attention_norm", "mlp_norm": [hidden], "q_norm",
     "k_norm": [head_dim]}]} of one 16-bit type on one GPU; the projections are kept in
-    4 bits, the output head is the embedding.  With a window every layer sees the last
+    4 bits, the output head is the embedding.  Norm weights of 32 bits that the type does not
+    hold are kept, and their norms are torch's, which are slower.  With a window every layer sees the last
     `window` tokens and the first `sinks`, and pages that leave it are given back.  rotary:
     further arguments of :func:`rotary_table`, for contexts beyond those of the training.
     """
@@ -63,9 +64,28 @@ class Qwen3Answers:
                                           **(rotary or {}))
 
     def _norm(self, weight):
-        """A norm's weights as the calls take them: of the model's type, together, aligned."""
-        w = weight.detach().to(self.type).contiguous()
+        """A norm's weights as the calls take them: of the model's type, together, aligned; in
+        32 bits (for :meth:`_normed`) where the type does not hold them."""
+        import torch
+        wide = weight.detach().float()
+        w = wide.to(self.type).contiguous()
+        if not torch.equal(w.float(), wide):
+            return wide
         return w if w.data_ptr() % 16 == 0 else w.clone()
+
+    def _held(self, weight):
+        return weight.dtype is self.type
+
+    def _normed(self, x, weight):
+        x = x.float()
+        return (x * (x.square().mean(-1, keepdim=True) + self.eps).rsqrt() * weight).to(self.type)
+
+    def _added(self, x, weight, residual):
+        """(the norm of the sum, the sum, in residual's place where that is one call)."""
+        if self._held(weight):
+            return add_norm(x, weight, residual, eps=self.eps, total=residual)
+        total = x.float() + residual.float()
+        return self._normed(total, weight), total.to(self.type)
 
     def _ints(self, values):
         import torch
@@ -108,26 +128,30 @@ class Qwen3Answers:
         of the sequences whose tables these are.  together: the groups and their shared tokens,
         where single tokens' attention reads prefixes once."""
         import torch
-        shape, eps = self.shape, self.eps
+        shape = self.shape
         see = dict(window=self.window, sinks=self.sinks, max_length=longest)
         heads = shape.q_heads, shape.kv_heads, shape.kv_heads
         x = self.embed[tokens]
         norms = [layer["attention_norm"] for layer in self.layers] + [self.norm]
-        h = add_norm(x, norms[0], eps=eps)
+        h = add_norm(x, norms[0], eps=self.eps) if self._held(norms[0]) else self._normed(x, norms[0])
         for layer, norm, (keys, values) in zip(self.layers, norms[1:], self.pool):
             q, k, v = self._product(h, layer["qkv"]).unflatten(1, (-1, shape.head_dim)).split(heads, 1)
-            q = page_append(q, k, v, keys, values, tables, lengths, starts, self.cos, self.sin, q_norm=layer["q_norm"],
-                            k_norm=layer["k_norm"], eps=eps)
+            q_norm, k_norm = layer["q_norm"], layer["k_norm"]
+            if not self._held(q_norm):
+                q, q_norm = self._normed(q, q_norm), None
+            if not self._held(k_norm):
+                k, k_norm = self._normed(k, k_norm), None
+            q = page_append(q, k, v, keys, values, tables, lengths, starts, self.cos, self.sin, q_norm=q_norm, k_norm=k_norm,
+                            eps=self.eps)
             if most > 1:
                 o = paged_prompt(q, keys, values, tables, lengths, starts, most, **see)
             elif together:
                 o = paged_shared(q, keys, values, tables, lengths, *together, max_length=longest)
             else:
                 o = paged_decode(q, keys, values, tables, lengths, **see)
-            h, x = add_norm(self._product(o.flatten(1), layer["o"]), layer["mlp_norm"], x, eps=eps, total=x)
+            h, x = self._added(self._product(o.flatten(1), layer["o"]), layer["mlp_norm"], x)
             gate, up = self._product(h, layer["gate_up"]).chunk(2, 1)
-            h, x = add_norm(self._product((torch.nn.functional.silu(gate.float()) * up.float()).to(self.type), layer["down"]), norm,
-                            x, eps=eps, total=x)
+            h, x = self._added(self._product((torch.nn.functional.silu(gate.float()) * up.float()).to(self.type), layer["down"]), norm, x)
         return h
 
     def _logits(self, x):
