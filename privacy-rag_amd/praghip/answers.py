@@ -26,6 +26,27 @@ from .sample import sample_tokens
 _ENOUGH = 4096
 
 
+def _runs(common):
+    """Where to cut a list of answers into runs that read a prefix together, its end among them:
+    common[i] tokens are the same for the i-th and the next, and for a run the fewest of its
+    pairs', which all of its members but one need not read.  The cuts that save the most."""
+    n = len(common) + 1
+    saved, first = [0] * (n + 1), [0] * (n + 1)  # by the runs of what is before i; where the last of them begins
+    for end in range(1, n + 1):
+        most, begin, fewest = saved[end - 1], end - 1, 0
+        for at in range(end - 2, -1, -1):
+            fewest = min(fewest, common[at]) if fewest else common[at]
+            if not fewest:
+                break
+            if saved[at] + (end - 1 - at) * fewest > most:
+                most, begin = saved[at] + (end - 1 - at) * fewest, at
+        saved[end], first[end] = most, begin
+    cuts = [n]
+    while cuts[-1]:
+        cuts.append(first[cuts[-1]])
+    return cuts[::-1]
+
+
 class Qwen3Answers:
     """Weights, a cache of `pages` pages for every layer, and up to `slots` sequences of
     `capacity` tokens, rounded up to whole pages.
@@ -94,21 +115,23 @@ class Qwen3Answers:
     def _product(self, x, w):
         return matvec_w4(x, *w, group=self.group)
 
+    _grouped = None  # the last list's groups, until a fork or an end
+
     def _groups(self, sequences):
         """(first of each run of neighbours that share a prefix, and the end; the tokens that
         each shares; keys that are read once instead of for each)."""
-        groups, shared, saved, common = [0], [], 0, {}
-        for i, s in enumerate(sequences):
-            now = {state: n for state, n in common.items() if (state, n) in self.marks[s]} if i else {}
-            if i and not now:
-                groups.append(i)
-                shared.append(max(common.values(), default=0))
-            common = now or dict(self.marks[s])
-        groups.append(len(sequences))
-        shared.append(max(common.values(), default=0))
-        for a, b, n in zip(groups, groups[1:], shared):
-            saved += (b - a - 1) * n
-        return groups, shared, saved
+        key = self.changes, tuple(sequences)
+        if self._grouped is None or self._grouped[0] != key:
+            # (a sequence's marks are its parent's, in order, and its own: what a run has in common
+            # is the least that two neighbours of it have)
+            marks = [self.marks[s] for s in sequences]
+            common = [max((n for state, n in a if (state, n) in b), default=0) for a, b in zip(marks, marks[1:])]
+            groups = _runs(common)
+            shared = [min(common[a: b - 1]) if b > a + 1 else max((n for _, n in marks[a]), default=0)
+                      for a, b in zip(groups, groups[1:])]
+            saved = sum((b - a - 1) * n for a, b, n in zip(groups, groups[1:], shared))
+            self._grouped = key, (groups, shared, saved)
+        return self._grouped[1]
 
     def _forward(self, sequences, rows):
         """Logits after the newest tokens, rows[i] of sequences[i], which have their pages already."""
@@ -253,6 +276,9 @@ class Qwen3Answers:
         page_fork(self.pool, self.tables, self.lengths, self.refs, self._ints([parent] * len(children)),
                   self._ints(children), self.status)
         page_check(self.status)
+        self._forked(parent, children)
+
+    def _forked(self, parent: int, children) -> None:
         marks = self.marks[parent]
         if not any(n == self.held[parent] for _, n in marks):
             marks.append((self.states, self.held[parent]))
@@ -266,6 +292,9 @@ class Qwen3Answers:
         sequences = list(sequences)
         page_free(self.tables, self.lengths, self.refs, self._ints(sequences), self.status)
         page_check(self.status)
+        self._ended(sequences)
+
+    def _ended(self, sequences) -> None:
         self.changes += 1
         for s in sequences:
             self.held[s], self.marks[s] = 0, []
