@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+import operator
 import struct
 
 from . import attention
@@ -31,6 +32,11 @@ def _each(value, rows: int, index: int, dtype, least, most):
         if value.requires_grad:
             _no_gradients("E_SAMPLE_GRADIENT")
         return value.data_ptr(), 0
+    if dtype is attention._int32:
+        try:
+            value = operator.index(value)
+        except TypeError:
+            raise shape_error("E_SAMPLE_FILTER") from None
     if not least <= value <= most:
         raise shape_error("E_SAMPLE_FILTER")
     return 0, value
@@ -41,7 +47,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
 
     logits [rows][vocab] bfloat16, float16 or float32, rows of any stride; uniform float32
     [rows] of [0, 1).  temperature, top_p and min_p are numbers or float32 [rows], top_k a
-    number or int32 [rows].  With w = exp((x - max x) / temperature): of the tokens by falling
+    whole number or int32 [rows]; numbers below 0, and a min_p above 1, are refused, in a list
+    (which is on the GPU) they count as the nearest that is not.  With w = exp((x - max x) / temperature): of the tokens by falling
     logit (of equal ones the lower index first) the first top_k stay (0: all); of those the
     shortest run whose sum of w reaches top_p times theirs; of those the ones with w >= min_p.
     The token is the first, by index, up to which the sum of w is above uniform times the sum
