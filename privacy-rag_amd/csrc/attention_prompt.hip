@@ -33,7 +33,7 @@
 // the chunks' lengths differ (equal stretches of all tiles' keys instead, which a workgroup
 // takes across tiles: 71), and twice dim 128's share of exponentials in a busy one.  Three
 // prompts of up to 77 tokens: 11 us, a chain of dependent reads.  Rows of 256 values have one
-// wave a SIMD and all of its registers: 4096 tokens of 8 heads over 4 197 us, 350 TFLOP/s.
+// wave a SIMD and all of its registers: 4096 tokens of 8 heads over 4 201 us, 340 TFLOP/s.
 #include "attention.hpp"
 
 #include <type_traits>

@@ -16,13 +16,13 @@
 //   which read the same keys one soon after the other (a cache answers); the others take every 8th, 4th or 2nd block, and
 //   waves that have the same columns add up through LDS.  A workgroup has at most two pieces
 //   of heads that it shares with others.
-// The products are attention_decode.hip's, with two tiles of 16 columns for one load of K and V
-// and one transposition of V.  The join kernel adds the pieces in order, so results do not
+// The products are attention_decode.hip's, with up to two tiles of 16 columns for one load of K and
+// V and one transposition of V.  The join kernel adds the pieces in order, so results do not
 // depend on timing.
 //
 // Measured, with the join (7 and 6 us of it): 64 sequences over one prefix of 8,192 keys and up
-// to 512 of their own, 16 heads of 128 over 8, 41 us for 103 MB, where attention_decode.hip takes
-// 310; five groups of 1 to 12 over prefixes of up to 30,000, 32 heads of 64 over 4, 34 us for
+// to 512 of their own, 16 heads of 128 over 8, 37 us for 103 MB, where attention_decode.hip takes
+// 310; five groups of 1 to 12 over prefixes of up to 30,000, 32 heads of 64 over 4, 35 us for
 // 114 MB (85).  The prefix of the first is 128 columns, four waves that each read the same keys:
 // its loads from the caches, and its products beside them, are what is left.
 // Columns of 64 a wave halve those loads, but leave registers for one wave a SIMD (62 us for 42),

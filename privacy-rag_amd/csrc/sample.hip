@@ -16,8 +16,8 @@
 // * list: workgroups of some parts add the row's bins, find those in which a cut falls, and
 //   append their tokens of those bins to the row's list;
 // * draw: a workgroup a row cuts the listed bins by value and index (few tokens by comparing each
-//   with every other, more by digits of 10 bits of both together), adds what stays of each part, takes the part that the random number falls into
-//   and goes through that one by index.
+//   with every other, more by digits of 10 bits of both together), adds what stays of each part,
+//   takes the part that the random number falls into and goes through that one by index.
 // The order of the list changes nothing: sums are of integers, and cuts are by value and index.
 //
 // Measured: 64 flat rows of 155,648 logits of 32 bits, cut by their sum, 54 us (16 + 19 + 20 by

@@ -21,8 +21,9 @@ from .qwen3 import QWEN3_0_6B, Qwen3Shape
 from .sample import sample_tokens
 
 # Keys that a step reads once instead of once for each answer, from which on the attention of
-# shared prefixes is the faster one: eight answers over 256 tokens (1,792 keys) take 14 us of
-# 12, over 1,024 (7,168 keys) 14 of 15.5, over 8,192 18 of 51.
+# shared prefixes is the faster one, at 16 heads of 128 over 8: eight answers over 256 tokens
+# (1,792 keys) take 14 us of 12, over 1,024 (7,168 keys) 14 of 15.5, over 8,192 18 of 51.  (Other
+# shapes and numbers of answers have the same bound, unmeasured.)
 _ENOUGH = 4096
 
 
