@@ -261,11 +261,11 @@ __device__ __forceinline__ void take_blocks(const SharedArgs& a, const Entry& x,
         }
       }
       float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      const float most = max32(max16(top));
+      const float peak = max32(max16(top));
       float by = c.scale;
-      top = most * c.scale - Half<T>::most;
+      top = peak * c.scale - Half<T>::most;
       if (__any(__builtin_fabsf(top) >= kLarge)) {  // scores and their maximum, rounded alike
-        by = 1, top = most * c.scale;
+        by = 1, top = peak * c.scale;
         top -= below_most<T>(top);
 #pragma unroll
         for (int r = 0; r < 8; ++r) s[r] *= c.scale;

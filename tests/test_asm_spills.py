@@ -23,19 +23,28 @@ def at(line):
     return int(m.group(1), 16), int(m.group(2), 16)
 
 
-def put_by_some(code):
-    found, regions = [], 0
+def functions(code):
+    """(name, instructions, addresses that branches on no active lanes go to) of each function."""
     start = 0
-    for end in range(1, len(code) + 1):  # a kernel's (an object's) instructions at a time
+    for end in range(1, len(code) + 1):
         if end < len(code) and code[end][0] != "FUNC":
             continue
-        part = code[start + 1: end]
-        name, start = code[start][2], end
-        meet = set()
+        part, name = code[start + 1: end], code[start][2]
+        meet, start = set(), end
         for op, _, line in part:
             if op == "s_cbranch_execz":
                 address, word = at(line)
                 meet.add(address + 4 + 4 * ((word & 0xffff) - ((word & 0x8000) << 1)))
+        yield name, part, meet
+
+
+def leaves(op, line):
+    return op.startswith("s_cbranch") or op in ("s_branch", "s_endpgm", "s_setpc_b64") or re.match(r"s_\w+ exec\b", line)
+
+
+def put_by_some(code):
+    found, regions = [], 0
+    for name, part, meet in functions(code):
         puts = None  # in the run so far, where some lanes are active
         for op, _, line in part:
             if at(line)[0] in meet:
@@ -46,7 +55,7 @@ def put_by_some(code):
                 regions += 1
                 found += [(name, x) for x in puts]
                 puts = None
-            elif op.startswith("s_cbranch") or op in ("s_branch", "s_endpgm", "s_setpc_b64") or re.match(r"s_\w+ exec\b", line):
+            elif leaves(op, line):
                 puts = None
             elif puts is not None and PUT.match(line):
                 puts.append(line)
@@ -56,4 +65,27 @@ def put_by_some(code):
 def test_nothing_is_put_away_by_some_lanes(machine_code):
     found, regions = put_by_some(machine_code)
     assert regions > 1000
+    assert not found, found[:5]
+
+
+def test_nothing_is_done_by_some_where_lanes_meet(machine_code):
+    """From the target of a branch on no active lanes to where they are active again there is no
+    vector instruction at all (but writes of a lane that is named, which need none active)."""
+    found, met = [], 0
+    for name, part, meet in functions(machine_code):
+        run = None
+        for op, _, line in part:
+            if at(line)[0] in meet:
+                run = []
+            if run is None:
+                continue
+            if RESTORED.match(line):
+                met += 1
+                found += [(name, x) for x in run]
+                run = None
+            elif leaves(op, line) or "saveexec" in op:
+                run = None
+            elif re.match(r"(v|ds|global|flat|scratch|buffer)_", op) and op not in ("v_writelane_b32", "v_readlane_b32"):
+                run.append(line)
+    assert met > 1000
     assert not found, found[:5]
